@@ -372,6 +372,81 @@ ra_status ra_tile_plan_run_lowp(ra_tile_plan* plan, const void* d_Bh, int32_t ld
 ra_status ra_tile_plan_get_info(const ra_tile_plan* plan, ra_tile_info* info);
 void ra_tile_plan_destroy(ra_tile_plan* plan);
 
+/* ------------------------------------------------------ graph attention
+ * Differential attention over the neighbour lists of a graph (no reference
+ * counterpart).  For row i, query head h with key/value head g = h / (q_heads /
+ * kv_heads), and map a = 0, 1, over the row's columns j:
+ *     s_a[j] = scale * q[i, h, a] . k[j, g, a] + bias[ij]
+ *     p_a    = softmax(s_a)
+ *     out[i, h] = sum_j (p_0 - lam[h] * p_1)[j] * v[j, g]
+ * q [M, q_heads, 2, head_dim], k [K, kv_heads, 2, head_dim] and v [K, kv_heads,
+ * value_dim] hold 32- or 16-bit floats; their rows may lie ldq, ldk, ldv elements
+ * apart (slices of one projection), everything within a row is contiguous.  out
+ * [M, q_heads, value_dim] is contiguous and of the same type.  lam [q_heads] and
+ * bias [nnz] (in CSR order, NULL = none) are fp32.  Scores, softmax statistics
+ * and sums are fp32.  What is written (and d_stats) lies on 16-byte addresses.
+ *
+ * An edge whose bias is -inf takes no part: its key and value are not used, even
+ * where they are inf or NaN.  A row without edges, or with no edge left, gives
+ * zeros.  Finite biases of any size are scores like others. */
+typedef struct ra_attn_shape {
+    int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads     */
+    int32_t head_dim;          /* 1 .. 128                           */
+    int32_t value_dim;         /* 1 .. 256                           */
+    int32_t dtype;             /* ra_dtype of q, k, v, out and grads */
+    float scale;
+    int64_t ldq, ldk, ldv;     /* elements between rows              */
+} ra_attn_shape;
+
+typedef struct ra_attn_plan ra_attn_plan;
+typedef struct ra_attn_info {
+    int32_t M, K;
+    int64_t nnz;
+    int32_t backward;                /* the transposed lists are there       */
+    int32_t num_items, num_splits;   /* row pieces of at most 256 edges,
+                                      * rows cut into several                 */
+    int32_t num_items_t, num_splits_t; /* the same of the transposed lists    */
+    int64_t num_slots, num_slots_t;  /* pieces of the cut rows                */
+    int64_t plan_bytes;
+} ra_attn_info;
+
+/* Plan of a graph: the pieces of its rows and, with backward != 0, its transposed
+ * lists, built on the GPU.  Checks rowptr (0 = rowptr[0] <= ... <= rowptr[M] = nnz)
+ * and colind (0 <= colind < K); synchronises `stream`.  The plan refers to
+ * d_rowptr and d_colind, which have to outlive it unchanged. */
+ra_status ra_attn_plan_create(const int32_t* d_rowptr, const int32_t* d_colind, int32_t M, int32_t K, int64_t nnz,
+                              int32_t backward, ra_stream_t stream, ra_attn_plan** out);
+ra_status ra_attn_plan_get_info(const ra_attn_plan* plan, ra_attn_info* info);
+/* Copy a plan array to the host: "items", "items_t" (4 int32 each: row, first
+ * edge, end, slot or -1), "splits", "splits_t" (4 int32: row, first slot, slots,
+ * 0), "rowptr_t", "row_t", "edge_t".  dst may be NULL to query *count (int32s). */
+ra_status ra_attn_plan_export(const ra_attn_plan* plan, const char* name, int32_t* dst, int64_t* count);
+void ra_attn_plan_destroy(ra_attn_plan* plan);
+/* d_stats: [M, q_heads, 2, 2] fp32 (maximum and 1/sum of every softmax, what the
+ * backward pass needs), or NULL.  Grows the plan's scratch at the first call of a
+ * larger shape. */
+ra_status ra_attn_plan_run(ra_attn_plan* plan, const ra_attn_shape* shape, const void* d_q, const void* d_k,
+                           const void* d_v, const float* d_lam, const float* d_bias, void* d_out, float* d_stats,
+                           ra_stream_t stream);
+/* Gradients of all inputs from d_grad_out [M, q_heads, value_dim] (contiguous):
+ * d_dq [M, q_heads, 2, head_dim], d_dk [K, kv_heads, 2, head_dim], d_dv [K,
+ * kv_heads, value_dim] contiguous, of the inputs' type; d_dlam [q_heads] fp32.
+ * Each is written whole, and each sum has a fixed order: equal inputs give equal
+ * bits.  Needs a plan made with backward != 0. */
+ra_status ra_attn_plan_run_backward(ra_attn_plan* plan, const ra_attn_shape* shape, const void* d_q, const void* d_k,
+                                    const void* d_v, const float* d_lam, const float* d_bias, const float* d_stats,
+                                    const void* d_grad_out, void* d_dq, void* d_dk, void* d_dv, float* d_dlam,
+                                    ra_stream_t stream);
+/* The forward pass without a plan, for lists that arrive with the call (a few new
+ * rows of a served graph).  Every row is cut into the same number of pieces, chosen
+ * from M and nnz.  As with ra_spmm_csr_direct, rowptr and colind are not checked.
+ * d_workspace: ra_attn_csr_workspace() bytes, 16-byte aligned. */
+ra_status ra_attn_csr_workspace(const ra_attn_shape* shape, int32_t M, int64_t nnz, int64_t* bytes);
+ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t M, int32_t K, int64_t nnz,
+                      const ra_attn_shape* shape, const void* d_q, const void* d_k, const void* d_v,
+                      const float* d_lam, const float* d_bias, void* d_out, void* d_workspace, int64_t bytes,
+                      ra_stream_t stream);
+
 /* ------------------------------------------------------------ utilities */
 /* fp32 -> fp16/bf16 round-to-nearest-even conversion of a [rows, cols] matrix
  * into a buffer with leading dimension ldo (columns cols..ldo-1 zero-filled).

@@ -42,6 +42,10 @@ SOURCES = {
     "zo_build_gpu.hip": [],
     "zo_noalloc.hip": [],
     "tile_f32_route.hip": [],
+    "attention_plan.hip": [],
+    "attention_fwd.hip": [],
+    "attention_bwd_rows.hip": [],
+    "attention_bwd_cols.hip": [],
 }
 LIB_NAME = "libra_spmm_hip.so"
 
@@ -109,7 +113,7 @@ def build_binding() -> Path:
             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
             "-DTORCH_API_INCLUDE_EXTENSION_H"]
            + incs + ["-I", py_inc, "-I", "/opt/rocm/include", str(CSRC / "torch_binding.cpp"),
-                     "-o", str(out), "-L", str(OUT_DIR), "-lra_spmm_hip", "-L", str(torch_lib),
+                     str(CSRC / "torch_binding_ops.cpp"), "-o", str(out), "-L", str(OUT_DIR), "-lra_spmm_hip", "-L", str(torch_lib),
                      "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-L/opt/rocm/lib", "-lamdhip64",
                      "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     _run(cmd)

@@ -1,0 +1,295 @@
+// attention.hpp — what the graph-attention kernels share: the plan, the launch
+// arguments, the lanes' layout and the row loads.
+#pragma once
+
+#include "ra_internal.hpp"
+
+namespace ra {
+
+// Edges of a piece: a row longer than this is cut into pieces that waves work on
+// in parallel; their partial results are joined in a second launch.
+constexpr int kAttnPiece = 256;
+
+// One side of a plan: the rows (or, transposed, the columns) as pieces.
+struct AttnSide {
+    const int32_t* ptr = nullptr;  // rows + 1
+    const int32_t* idx = nullptr;  // the edge's other end
+    const int32_t* edge = nullptr; // its number in CSR order (transposed side only)
+    const int4* items = nullptr;   // row, first edge, end, slot or -1
+    const int4* splits = nullptr;  // row, first slot, slots, 0
+    int32_t rows = 0, num_items = 0, num_splits = 0;
+    int64_t num_slots = 0;
+    DeviceBuffer lists;
+};
+
+}  // namespace ra
+
+struct ra_attn_plan {
+    ra_attn_info info{};
+    int device = 0;
+    ra::AttnSide side[2];       // rows, columns
+    ra::DeviceBuffer transposed;  // ptr, idx, edge of side[1]
+    ra::DeviceBuffer partial, record;
+};
+
+namespace ra {
+
+struct AttnArgs {
+    // The pieces: a list, or (items == nullptr) `pieces` equal parts of every row.
+    const int4* items;
+    const int32_t* ptr;
+    const int32_t* idx;
+    const int32_t* edge;
+    int64_t num_units;    // pieces * head blocks
+    int32_t pieces;       // per row, without a list
+    int32_t head_blocks;  // waves that share a piece
+    int32_t hb_shift;     // log2 of the heads of a wave
+    int32_t q_heads, kv_heads, group, head_dim, value_dim;
+    int32_t rows;
+    float scale;
+    int64_t ldq, ldk, ldv;
+    const void *q, *k, *v, *grad;
+    const float *lam, *bias;
+    float* stats;    // [rows, q_heads, 2] (max, 1 / sum)
+    float4* record;  // [rows, q_heads, 2] (max, 1 / sum, sum p dp, 0)
+    void *out, *out2;
+    float* partial;
+};
+
+// Lanes of a head: 2 maps x LM lanes of 8 head_dim elements each; value_dim goes
+// over all 2 * LM of them, NV elements each.
+struct AttnLayout {
+    int lm;      // 1, 2, 4, 8, 16
+    int nv;      // 4 or 8
+    bool vec;    // every lane's run is whole aligned 16-byte (value rows: NV-element) packets
+    int hb_shift;
+    int head_blocks;
+};
+
+struct AttnPtrs {
+    const void *q, *k, *v, *grad;
+    int64_t ldq, ldk, ldv, ldg;
+};
+
+AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p);
+ra_status attn_check(const ra_attn_shape* s, int32_t M, int32_t K);
+
+// Floats of a slot of partial results.
+inline int64_t attn_forward_slot(const ra_attn_shape& s) { return (int64_t)s.q_heads * (2 * s.value_dim + 4); }
+inline int64_t attn_row_slot(const ra_attn_shape& s) { return (int64_t)s.q_heads * (4 * s.head_dim + 2); }
+inline int64_t attn_col_slot(const ra_attn_shape& s) { return (int64_t)s.kv_heads * (2 * s.head_dim + s.value_dim); }
+
+ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
+ra_status attn_rows_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
+ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
+// Second launches: the cut rows' pieces (splits == nullptr: every row, a.pieces each).
+ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
+ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
+ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
+// d lam from the records; `partial` holds kLamBlocks * q_heads floats.
+constexpr int kLamBlocks = 256;
+ra_status attn_lam_launch(const float4* record, int32_t rows, int32_t q_heads, float* partial, float* dlam,
+                          hipStream_t st);
+
+// ------------------------------------------------------------- device side
+using f16_t = _Float16;
+using bf16_t = __bf16;
+
+constexpr int kAttnThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi, bf16_t) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi, f16_t) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 h = __builtin_bit_cast(h2, w);
+    lo = (float)h[0];
+    hi = (float)h[1];
+}
+
+// N (4 or 8) elements as floats.
+template <typename T, int N>
+struct Run {
+    uint32_t w[N / 2];
+    __device__ __forceinline__ void to_float(float* f) const {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) unpack2(w[i], f[2 * i], f[2 * i + 1], T());
+    }
+};
+template <int N>
+struct Run<float, N> {
+    float w[N];
+    __device__ __forceinline__ void to_float(float* f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = w[i];
+    }
+};
+
+// What lanes without an edge (or past the end of a head) load instead: zeros.
+// Never written; not const, so that both addresses of the choice are global ones.
+static __device__ uint4 kAttnZeros[2];
+
+// A lane's run of N elements, the first `count` of them in memory (the others are
+// 0).  VEC: runs are whole packets (16 bytes, or all of a shorter run) and aligned
+// to them; `count` is then 0 or covers whole packets.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_run(Run<T, N>& r, const T* p, int count) {
+    if constexpr (VEC) {
+        constexpr int kPerPacket = (int)(16 / sizeof(T)) < N ? (int)(16 / sizeof(T)) : N;
+        constexpr int kWords = kPerPacket * (int)sizeof(T) / 4;
+#pragma unroll
+        for (int i = 0; i < N / kPerPacket; ++i) {
+            const void* at = i * kPerPacket < count ? static_cast<const void*>(p + i * kPerPacket)
+                                                    : static_cast<const void*>(kAttnZeros);
+            if constexpr (kWords == 4) {
+                const uint4 x = *static_cast<const uint4*>(at);
+                __builtin_memcpy(&r.w[i * 4], &x, 16);
+            } else {
+                const uint2 x = *static_cast<const uint2*>(at);
+                __builtin_memcpy(&r.w[i * 2], &x, 8);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const T x = *(i < count ? p + i : reinterpret_cast<const T*>(kAttnZeros));
+            if constexpr (sizeof(T) == 4) {
+                r.w[i] = x;
+            } else {
+                const uint32_t b = __builtin_bit_cast(uint16_t, x);
+                if (i & 1) r.w[i / 2] |= b << 16;
+                else r.w[i / 2] = b;
+            }
+        }
+    }
+}
+
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_run(T* p, const float* f, int count) {
+    if constexpr (VEC) {
+        constexpr int kPerPacket = (int)(16 / sizeof(T)) < N ? (int)(16 / sizeof(T)) : N;
+#pragma unroll
+        for (int i = 0; i < N / kPerPacket; ++i) {
+            if (i * kPerPacket >= count) break;
+            typedef T vec __attribute__((ext_vector_type(kPerPacket)));
+            vec x;
+#pragma unroll
+            for (int e = 0; e < kPerPacket; ++e) x[e] = (T)f[i * kPerPacket + e];
+            *reinterpret_cast<vec*>(p + i * kPerPacket) = x;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < count) p[i] = (T)f[i];
+    }
+}
+
+// Sum over runs of W lanes (a power of two): every lane gets it.
+template <int W>
+__device__ __forceinline__ float lanes_sum(float x) {
+    // Within 16 lanes by data-parallel moves (quad permutes and row mirrors), the
+    // rest through the shuffle network.
+    if constexpr (W >= 2) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));
+    if constexpr (W >= 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));
+    if constexpr (W >= 8) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));
+    if constexpr (W >= 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));
+    if constexpr (W >= 32) x += __shfl_xor(x, 16, 64);
+    return x;
+}
+// The value of the lane LM away (the other map's), where all lanes of a map hold
+// the same value.
+template <int LM>
+__device__ __forceinline__ float other_map(float x) {
+    if constexpr (LM == 1) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));
+    if constexpr (LM == 2) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));
+    if constexpr (LM == 4) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));
+    if constexpr (LM == 8) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));
+    return __shfl_xor(x, LM, 64);
+}
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// Piece and heads of a wave.
+struct Unit {
+    int row, begin, end, slot;
+    int head_block;
+    bool live;
+};
+
+__device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
+    // Consecutive workgroups go to the 8 XCDs in turn: workgroup b takes the
+    // (b / 8)-th part of XCD (b % 8)'s run of the pieces, so that pieces that lie
+    // side by side (rows that share neighbours) share an L2.
+    const int64_t per = (gridDim.x + 7) / 8;
+    const int64_t full = gridDim.x - (per - 1) * 8;  // XCDs with `per` workgroups
+    const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
+    const int64_t block = x < full ? x * per + y : full * per + (x - full) * (per - 1) + y;
+    const int64_t unit = block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Unit u{};
+    u.live = unit < a.num_units;
+    if (!u.live) return u;
+    const int64_t item = a.head_blocks == 1 ? unit : unit / a.head_blocks;
+    u.head_block = static_cast<int>(unit - item * a.head_blocks);
+    if (a.items) {
+        const int4 it = a.items[item];
+        u.row = it.x, u.begin = it.y, u.end = it.z, u.slot = it.w;
+    } else {
+        u.row = static_cast<int>(item / a.pieces);
+        const int64_t part = item - (int64_t)u.row * a.pieces;
+        const int64_t b = a.ptr[u.row], n = a.ptr[u.row + 1] - b;
+        u.begin = static_cast<int>(b + n * part / a.pieces);
+        u.end = static_cast<int>(b + n * (part + 1) / a.pieces);
+        u.slot = a.pieces == 1 ? -1 : static_cast<int>(item);
+    }
+    return u;
+}
+
+// A lane's place: edge slot es of `slots`, head, map, and its runs.
+template <int LM, int NV>
+struct Place {
+    int es, slots, head, map, lm, l;
+    int kcount, vcount;  // elements of its runs that exist
+    bool live;
+    __device__ __forceinline__ Place(const AttnArgs& a, int head_block, int heads) {
+        const int lane = threadIdx.x & 63;
+        l = lane & (2 * LM - 1);
+        map = l / LM;
+        lm = l & (LM - 1);
+        const int hl = (lane / (2 * LM)) & ((1 << a.hb_shift) - 1);
+        head = (head_block << a.hb_shift) + hl;
+        slots = (32 / LM) >> a.hb_shift;
+        es = (lane / (2 * LM)) >> a.hb_shift;
+        live = head < heads;
+        kcount = live ? max(0, min(8, a.head_dim - 8 * lm)) : 0;
+        vcount = live ? max(0, min(NV, a.value_dim - NV * l)) : 0;
+        if (!live) head = 0;
+    }
+};
+
+// Calls KERNEL<T, LM, NV, VEC> for a layout.
+#define RA_ATTN_DISPATCH(KERNEL, dtype, l, grid, st, args)                                            \
+    do {                                                                                              \
+        auto by_type = [&](auto tag) {                                                                \
+            using T = decltype(tag);                                                                  \
+            auto by_lm = [&](auto lm) {                                                               \
+                constexpr int LM = decltype(lm)::value;                                               \
+                if (!(l).vec) KERNEL<T, LM, 8, false><<<grid, ra::kAttnThreads, 0, st>>>(args);       \
+                else if ((l).nv == 4) KERNEL<T, LM, 4, true><<<grid, ra::kAttnThreads, 0, st>>>(args); \
+                else KERNEL<T, LM, 8, true><<<grid, ra::kAttnThreads, 0, st>>>(args);                 \
+            };                                                                                        \
+            switch ((l).lm) {                                                                         \
+                case 1: by_lm(std::integral_constant<int, 1>()); break;                               \
+                case 2: by_lm(std::integral_constant<int, 2>()); break;                               \
+                case 4: by_lm(std::integral_constant<int, 4>()); break;                               \
+                case 8: by_lm(std::integral_constant<int, 8>()); break;                               \
+                default: by_lm(std::integral_constant<int, 16>());                                    \
+            }                                                                                         \
+        };                                                                                            \
+        if ((dtype) == RA_DTYPE_F32) by_type(float());                                                \
+        else if ((dtype) == RA_DTYPE_F16) by_type(ra::f16_t());                                       \
+        else by_type(ra::bf16_t());                                                                   \
+    } while (0)
+
+}  // namespace ra

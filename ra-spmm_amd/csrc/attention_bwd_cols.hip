@@ -1,0 +1,165 @@
+// attention_bwd_cols.hip — backward pass of the graph attention over its columns:
+// dk and dv, from the transposed lists.
+//
+// A wave works on one piece of a column's list for one block of key/value heads;
+// per edge it gathers the row's q, dout and record (maximum, 1/sum, delta of both
+// maps), and forms the weights again:
+//     dk += scale * c p (dp - delta) q,   dv += (p_0 - lam p_1) dout
+// A key/value head's query heads are taken one after another, into the same sums:
+// nothing is added atomically, and the order is fixed.
+#include <type_traits>
+
+#include "attention.hpp"
+
+namespace ra {
+namespace {
+
+constexpr int kDeep = 4;
+
+template <typename T, int LM, int NV, bool VEC>
+__device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float* dk,
+                                       const float* dv) {
+    if (p.es != 0 || !p.live) return;
+    if (u.slot >= 0) {  // [heads][2 maps][head_dim], then [heads][value_dim]
+        float* base = a.partial + (int64_t)u.slot * a.kv_heads * (2 * a.head_dim + a.value_dim);
+        float* to = base + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < p.kcount) to[i] = dk[i];
+        to = base + (int64_t)a.kv_heads * 2 * a.head_dim + (int64_t)p.head * a.value_dim + NV * p.l;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < p.vcount) to[i] = dv[i];
+        return;
+    }
+    const int64_t at = (int64_t)u.row * a.kv_heads + p.head;
+    store_run<T, 8, VEC>(static_cast<T*>(a.out) + (at * 2 + p.map) * a.head_dim + 8 * p.lm, dk, p.kcount);
+    store_run<T, NV, VEC>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, p.vcount);
+}
+
+template <typename T, int LM, int NV, bool VEC>
+__global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
+    const Unit u = unit_of(a);
+    if (!u.live) return;
+    const Place<LM, NV> p(a, u.head_block, a.kv_heads);
+    float kf[8], vf[NV], dk[8], dv[NV];
+    {
+        Run<T, 8> r;
+        load_run<T, 8, VEC>(r, static_cast<const T*>(a.k) + u.row * a.ldk + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm,
+                            p.kcount);
+        r.to_float(kf);
+        Run<T, NV> g;
+        load_run<T, NV, VEC>(g, static_cast<const T*>(a.v) + u.row * a.ldv + (int64_t)p.head * a.value_dim + NV * p.l, p.vcount);
+        g.to_float(vf);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dk[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) dv[i] = 0.f;
+
+    for (int sub = 0; sub < a.group; ++sub) {
+        const int qh = p.head * a.group + sub;
+        const T* const q = static_cast<const T*>(a.q) + (int64_t)(qh * 2 + p.map) * a.head_dim + 8 * p.lm;
+        const T* const g = static_cast<const T*>(a.grad) + (int64_t)qh * a.value_dim + NV * p.l;
+        const float4* const rec = a.record + qh * 2 + p.map;
+        const float c = p.map == 0 ? 1.f : -a.lam[qh];
+        for (int e0 = u.begin; e0 < u.end; e0 += kDeep * p.slots) {
+            Run<T, 8> qr[kDeep];
+            Run<T, NV> gr[kDeep];
+            float4 st[kDeep];
+            float add[kDeep];
+            int row[kDeep];
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                const int e = e0 + d * p.slots + p.es;
+                const bool in = e < u.end;
+                row[d] = in ? a.idx[e] : 0;
+                add[d] = in ? 0.f : -INFINITY;
+                if (a.bias && in) add[d] = a.bias[a.edge[e]];
+            }
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                const bool in = add[d] != -INFINITY;
+                load_run<T, 8, VEC>(qr[d], q + row[d] * a.ldq, in ? p.kcount : 0);
+                load_run<T, NV, VEC>(gr[d], g + (int64_t)row[d] * a.q_heads * a.value_dim, in ? p.vcount : 0);
+                st[d] = rec[(int64_t)row[d] * a.q_heads * 2];
+            }
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                float qf[8], gf[NV], t = 0.f, dp = 0.f;
+                qr[d].to_float(qf);
+                gr[d].to_float(gf);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t = fmaf(qf[i], kf[i], t);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) dp = fmaf(gf[i], vf[i], dp);
+                t = lanes_sum<LM>(t);
+                dp = lanes_sum<2 * LM>(dp);
+                const float w = add[d] == -INFINITY ? 0.f : c * exp_of(fmaf(t, a.scale, add[d]) - st[d].x) * st[d].y;
+                const float ds = add[d] == -INFINITY ? 0.f : w * (dp - st[d].z);
+                const float mix = w + other_map<LM>(w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dk[i] = fmaf(ds, qf[i], dk[i]);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) dv[i] = fmaf(mix, gf[i], dv[i]);
+            }
+        }
+    }
+    for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dk[i] += __shfl_xor(dk[i], step, 64);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) dv[i] += __shfl_xor(dv[i], step, 64);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dk[i] *= a.scale;
+    finish<T, LM, NV, VEC>(a, u, p, dk, dv);
+}
+
+// Joins a cut column's pieces: plain sums of every element, in order.  Threads are
+// four piece groups x 64 elements.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_cols_join(const AttnArgs a, const int4* __restrict__ splits, int blocks_per) {
+    __shared__ float sum[256];
+    const int4 sp = splits[blockIdx.x / blocks_per];
+    const int keys = a.kv_heads * 2 * a.head_dim, width = keys + a.kv_heads * a.value_dim;
+    const int at = (blockIdx.x % blocks_per) * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    float x = 0.f;
+    if (at < width) {
+        const float* const base = a.partial + (int64_t)sp.y * width + at;
+#pragma unroll 4
+        for (int s = part; s < sp.z; s += 4) x += base[(int64_t)s * width];
+    }
+    sum[threadIdx.x] = x;
+    __syncthreads();
+    if (part != 0 || at >= width) return;
+    x = x + sum[64 + at % 64] + sum[128 + at % 64] + sum[192 + at % 64];
+    if (at < keys) static_cast<T*>(a.out)[(int64_t)sp.x * keys + at] = (T)x;
+    else static_cast<T*>(a.out2)[(int64_t)sp.x * (width - keys) + at - keys] = (T)x;
+}
+
+}  // namespace
+
+ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
+    const int64_t blocks = (a.num_units + kAttnThreads / 64 - 1) / (kAttnThreads / 64);
+    if (blocks == 0) return RA_OK;
+    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    RA_ATTN_DISPATCH(attn_cols, dtype, l, dim3((unsigned)blocks), st, a);
+    RA_LAUNCH_CHECK("attn_cols");
+    return RA_OK;
+}
+
+ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
+    if (n == 0) return RA_OK;
+    const int per = (a.kv_heads * (2 * a.head_dim + a.value_dim) + 63) / 64;
+    const int64_t blocks = n * per;
+    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    const dim3 grid((unsigned)blocks);
+    if (dtype == RA_DTYPE_F32) attn_cols_join<float><<<grid, 256, 0, st>>>(a, splits, per);
+    else if (dtype == RA_DTYPE_F16) attn_cols_join<f16_t><<<grid, 256, 0, st>>>(a, splits, per);
+    else attn_cols_join<bf16_t><<<grid, 256, 0, st>>>(a, splits, per);
+    RA_LAUNCH_CHECK("attn_cols_join");
+    return RA_OK;
+}
+
+}  // namespace ra

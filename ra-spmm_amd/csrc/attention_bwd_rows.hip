@@ -1,0 +1,224 @@
+// attention_bwd_rows.hip — backward pass of the graph attention over its rows:
+// dq, the row sums that the column pass needs, d lam.
+//
+// With p the weights of a map, dp_j = dout . v_j and delta = sum_j p_j dp_j,
+//     ds_j = c p_j (dp_j - delta)   (c = 1 for map 0, -lam for map 1)
+//     dq   = scale * sum_j ds_j k_j = scale * c * (sum_j p_j dp_j k_j - delta sum_j p_j k_j)
+// The second form needs one pass over the edges: delta is known at its end.  The
+// weights come from the forward pass' maxima and sums.  Lanes as in the forward
+// pass; the pieces of a long row are plain sums.
+#include <type_traits>
+
+#include "attention.hpp"
+
+namespace ra {
+namespace {
+
+constexpr int kDeep = 4;
+
+// Map's gradient of q and its record.
+template <typename T, int LM, int NV, bool VEC>
+__device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float delta,
+                                       const float* pdk, const float* pk, float m, float il) {
+    if (p.es != 0 || !p.live) return;
+    if (u.slot >= 0) {  // [heads][2 maps][delta], then [heads][2 maps][2][head_dim]
+        float* base = a.partial + (int64_t)u.slot * a.q_heads * (4 * a.head_dim + 2);
+        if (p.lm == 0) base[p.head * 2 + p.map] = delta;
+        float* to = base + a.q_heads * 2 + (int64_t)(p.head * 2 + p.map) * 2 * a.head_dim + 8 * p.lm;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < p.kcount) {
+                to[i] = pdk[i];
+                to[a.head_dim + i] = pk[i];
+            }
+        return;
+    }
+    const float c = (p.map == 0 ? 1.f : -a.lam[p.head]) * a.scale;
+    float dq[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dq[i] = c * (pdk[i] - delta * pk[i]);
+    const int64_t at = ((int64_t)u.row * a.q_heads + p.head) * 2 + p.map;
+    store_run<T, 8, VEC>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, p.kcount);
+    if (p.lm == 0) a.record[at] = make_float4(m, il, delta, 0.f);
+}
+
+template <typename T, int LM, int NV, bool VEC>
+__global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
+    const Unit u = unit_of(a);
+    if (!u.live) return;
+    const Place<LM, NV> p(a, u.head_block, a.q_heads);
+    const int kv = p.head / a.group;
+    const T* const k = static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim + 8 * p.lm;
+    const T* const v = static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim + NV * p.l;
+
+    float qf[8], gf[NV];
+    {
+        Run<T, 8> r;
+        load_run<T, 8, VEC>(r, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm,
+                            p.kcount);
+        r.to_float(qf);
+        Run<T, NV> g;
+        load_run<T, NV, VEC>(g, static_cast<const T*>(a.grad) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l,
+                             p.vcount);
+        g.to_float(gf);
+    }
+    const float2 st = reinterpret_cast<const float2*>(a.stats)[((int64_t)u.row * a.q_heads + p.head) * 2 + p.map];
+    float delta = 0.f, pdk[8], pk[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pdk[i] = pk[i] = 0.f;
+
+    for (int e0 = u.begin; e0 < u.end; e0 += kDeep * p.slots) {
+        Run<T, 8> kr[kDeep];
+        Run<T, NV> vr[kDeep];
+        float add[kDeep];
+        int col[kDeep];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int e = e0 + d * p.slots + p.es;
+            const bool in = e < u.end;
+            col[d] = in ? a.idx[e] : 0;
+            add[d] = in ? 0.f : -INFINITY;
+            if (a.bias && in) add[d] = a.bias[e];
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const bool in = add[d] != -INFINITY;
+            load_run<T, 8, VEC>(kr[d], k + col[d] * a.ldk, in ? p.kcount : 0);
+            load_run<T, NV, VEC>(vr[d], v + col[d] * a.ldv, in ? p.vcount : 0);
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            float kf[8], vf[NV], t = 0.f, dp = 0.f;
+            kr[d].to_float(kf);
+            vr[d].to_float(vf);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t = fmaf(qf[i], kf[i], t);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) dp = fmaf(gf[i], vf[i], dp);
+            t = lanes_sum<LM>(t);
+            dp = lanes_sum<2 * LM>(dp);
+            const bool live = add[d] != -INFINITY;
+            const float w = live ? exp_of(fmaf(t, a.scale, add[d]) - st.x) * st.y : 0.f;
+            const float wd = live ? w * dp : 0.f;
+            delta += wd;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                pdk[i] = fmaf(wd, kf[i], pdk[i]);
+                pk[i] = fmaf(w, kf[i], pk[i]);
+            }
+        }
+    }
+    for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
+        delta += __shfl_xor(delta, step, 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            pdk[i] += __shfl_xor(pdk[i], step, 64);
+            pk[i] += __shfl_xor(pk[i], step, 64);
+        }
+    }
+    finish<T, LM, NV, VEC>(a, u, p, delta, pdk, pk, st.x, st.y);
+}
+
+// Joins a cut row's pieces: a workgroup per (row, head).  Threads are piece groups x
+// 64 .. 256 elements of the two maps' sums.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void attn_rows_join(const AttnArgs a, const int4* __restrict__ splits) {
+    __shared__ float first[kJoinThreads], second[kJoinThreads], sum[kJoinThreads];
+    const int head = blockIdx.x % a.q_heads;
+    const int4 sp = splits[blockIdx.x / a.q_heads];
+    const int64_t stride = (int64_t)a.q_heads * (4 * a.head_dim + 2);
+    const float* const base = a.partial + (int64_t)sp.y * stride;
+    int width = 64;
+    while (width < 2 * a.head_dim) width *= 2;  // at most 256
+    const int part = threadIdx.x / width, parts = kJoinThreads / width, at = threadIdx.x & (width - 1);
+    const bool live = at < 2 * a.head_dim;
+    const int map = live && at >= a.head_dim, i = at - map * a.head_dim;
+    float pdk = 0.f, pk = 0.f, delta = 0.f;
+    if (live) {
+        const float* const x = base + a.q_heads * 2 + (int64_t)(head * 2 + map) * 2 * a.head_dim + i;
+#pragma unroll 4
+        for (int s = part; s < sp.z; s += parts) {
+            pdk += x[s * stride];
+            pk += x[s * stride + a.head_dim];
+            delta += base[s * stride + head * 2 + map];
+        }
+    }
+    first[threadIdx.x] = pdk;
+    second[threadIdx.x] = pk;
+    sum[threadIdx.x] = delta;
+    __syncthreads();
+    if (part != 0 || !live) return;
+    for (int x = 1; x < parts; ++x) {
+        pdk += first[x * width + at];
+        pk += second[x * width + at];
+        delta += sum[x * width + at];
+    }
+    const int64_t to = ((int64_t)sp.x * a.q_heads + head) * 2 + map;
+    const float c = (map == 0 ? 1.f : -a.lam[head]) * a.scale;
+    static_cast<T*>(a.out)[to * a.head_dim + i] = (T)(c * (pdk - delta * pk));
+    if (i == 0) {
+        const float2 st = reinterpret_cast<const float2*>(a.stats)[to];
+        a.record[to] = make_float4(st.x, st.y, delta, 0.f);
+    }
+}
+
+// d lam[h] = -sum_i delta of map 1: a workgroup sums a run of rows for every head,
+// then one workgroup the workgroups' sums, both in a fixed order.
+__global__ __launch_bounds__(256) void attn_lam_partial(const float4* __restrict__ record, int rows, int heads,
+                                                        float* __restrict__ partial) {
+    __shared__ float part[4];
+    const int64_t per = ((int64_t)rows + gridDim.x - 1) / gridDim.x;
+    const int64_t first = blockIdx.x * per, end = min(first + per, (int64_t)rows);
+    for (int h = 0; h < heads; ++h) {
+        float x = 0.f;
+        for (int64_t i = first + threadIdx.x; i < end; i += 256) x += record[(i * heads + h) * 2 + 1].z;
+        for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+        __syncthreads();
+        if (threadIdx.x == 0) partial[(int64_t)blockIdx.x * heads + h] = part[0] + part[1] + part[2] + part[3];
+        __syncthreads();
+    }
+}
+__global__ __launch_bounds__(64) void attn_lam_final(const float* __restrict__ partial, int blocks, int heads,
+                                                     float* __restrict__ dlam) {
+    const int h = blockIdx.x;
+    float x = 0.f;
+    for (int b = threadIdx.x; b < blocks; b += 64) x += partial[(int64_t)b * heads + h];
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    if (threadIdx.x == 0) dlam[h] = -x;
+}
+
+}  // namespace
+
+ra_status attn_rows_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
+    const int64_t blocks = (a.num_units + kAttnThreads / 64 - 1) / (kAttnThreads / 64);
+    if (blocks == 0) return RA_OK;
+    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    RA_ATTN_DISPATCH(attn_rows, dtype, l, dim3((unsigned)blocks), st, a);
+    RA_LAUNCH_CHECK("attn_rows");
+    return RA_OK;
+}
+
+ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
+    if (n == 0) return RA_OK;
+    const int64_t blocks = n * a.q_heads;
+    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    const dim3 grid((unsigned)blocks);
+    if (dtype == RA_DTYPE_F32) attn_rows_join<float><<<grid, kJoinThreads, 0, st>>>(a, splits);
+    else if (dtype == RA_DTYPE_F16) attn_rows_join<f16_t><<<grid, kJoinThreads, 0, st>>>(a, splits);
+    else attn_rows_join<bf16_t><<<grid, kJoinThreads, 0, st>>>(a, splits);
+    RA_LAUNCH_CHECK("attn_rows_join");
+    return RA_OK;
+}
+
+ra_status attn_lam_launch(const float4* record, int32_t rows, int32_t q_heads, float* partial, float* dlam,
+                          hipStream_t st) {
+    attn_lam_partial<<<kLamBlocks, 256, 0, st>>>(record, rows, q_heads, partial);
+    RA_LAUNCH_CHECK("attn_lam_partial");
+    attn_lam_final<<<q_heads, 64, 0, st>>>(partial, kLamBlocks, q_heads, dlam);
+    RA_LAUNCH_CHECK("attn_lam_final");
+    return RA_OK;
+}
+
+}  // namespace ra

@@ -1,0 +1,538 @@
+// attention_plan.hip — plan of the graph attention (pieces of rows, transposed
+// lists) and the C entries that run it.
+#include <hipcub/hipcub.hpp>
+
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <string>
+
+#include "attention.hpp"
+
+namespace ra {
+namespace {
+
+constexpr int kThreads = 256;
+
+unsigned blocks_for(int64_t n) { return static_cast<unsigned>((n + kThreads - 1) / kThreads); }
+
+// What the host reads back.  bad: rowptr decreases or has wrong ends, or a column
+// is out of range.
+struct Totals {
+    unsigned long long items_slots;  // items << 32 | slots
+    int32_t splits;
+    int32_t bad;
+};
+
+__global__ __launch_bounds__(kThreads) void check_columns(const int32_t* __restrict__ idx, int64_t n, int32_t K,
+                                                          Totals* __restrict__ out) {
+    const int64_t stride = (int64_t)gridDim.x * kThreads;
+    bool bad = false;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += stride) bad |= (uint32_t)idx[i] >= (uint32_t)K;
+    if (bad) out->bad = 1;
+}
+
+// Pieces, slots and cuts of every row; entry `rows` gets zeros, so that the
+// exclusive sums end with the totals.
+__global__ __launch_bounds__(kThreads) void count_pieces(const int32_t* __restrict__ ptr, int32_t rows, int64_t nnz,
+                                                         unsigned long long* __restrict__ items_slots,
+                                                         int32_t* __restrict__ splits, Totals* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i > rows) return;
+    int64_t n = 0;
+    if (i < rows) {
+        n = (int64_t)ptr[i + 1] - ptr[i];
+        if (n < 0 || (i == 0 && ptr[0] != 0) || (i == rows - 1 && ptr[rows] != nnz)) out->bad = 1;
+        n = max(n, (int64_t)0);
+    }
+    const unsigned long long pieces = i == rows ? 0 : n == 0 ? 1 : (n + kAttnPiece - 1) / kAttnPiece;
+    items_slots[i] = pieces << 32 | (pieces > 1 ? pieces : 0);
+    splits[i] = pieces > 1;
+}
+
+__global__ __launch_bounds__(kThreads) void place_pieces(const int32_t* __restrict__ ptr, int32_t rows,
+                                                         const unsigned long long* __restrict__ items_slots,
+                                                         const int32_t* __restrict__ splits, int4* __restrict__ items,
+                                                         int4* __restrict__ split_rows) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= rows) return;
+    const int begin = ptr[i], end = ptr[i + 1];
+    const int64_t item = items_slots[i] >> 32;
+    const int slot = static_cast<int>(items_slots[i] & 0xFFFFFFFFu);
+    const int pieces = static_cast<int>((items_slots[i + 1] >> 32) - item);
+    if (pieces == 1) {
+        items[item] = make_int4(static_cast<int>(i), begin, end, -1);
+        return;
+    }
+    for (int k = 0; k < pieces; ++k) {
+        const int64_t b = (int64_t)begin + (int64_t)k * kAttnPiece;
+        items[item + k] = make_int4(static_cast<int>(i), static_cast<int>(b),
+                                    static_cast<int>(min(b + kAttnPiece, (int64_t)end)), slot + k);
+    }
+    split_rows[splits[i]] = make_int4(static_cast<int>(i), slot, pieces, 0);
+}
+
+__global__ __launch_bounds__(kThreads) void read_totals(const unsigned long long* __restrict__ items_slots,
+                                                        const int32_t* __restrict__ splits, int32_t rows,
+                                                        Totals* __restrict__ out) {
+    out->items_slots = items_slots[rows];
+    out->splits = splits[rows];
+}
+
+// Row of every edge: the edges of 256 consecutive ones lie in few rows, found by
+// bisection.
+__global__ __launch_bounds__(kThreads) void edge_numbers(int64_t n, int32_t* __restrict__ out) {
+    const int64_t stride = (int64_t)gridDim.x * kThreads;
+    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < n; e += stride) out[e] = static_cast<int32_t>(e);
+}
+
+// Last row whose first edge is at most e.
+__device__ __forceinline__ int32_t row_of(const int32_t* __restrict__ ptr, int32_t rows, int32_t e) {
+    int32_t lo = 0, hi = rows;  // ptr[lo] <= e < ptr[hi]
+    while (hi - lo > 1) {
+        const int32_t mid = lo + (hi - lo) / 2;
+        if (ptr[mid] <= e) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(kThreads) void transposed_rows(const int32_t* __restrict__ ptr, int32_t rows, int64_t n,
+                                                            const int32_t* __restrict__ edge, int32_t* __restrict__ out) {
+    const int64_t stride = (int64_t)gridDim.x * kThreads;
+    for (int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x; t < n; t += stride) out[t] = row_of(ptr, rows, edge[t]);
+}
+
+// First sorted key that is at least i, for i = 0 .. K.
+__global__ __launch_bounds__(kThreads) void transposed_ptr(const int32_t* __restrict__ keys, int64_t n, int32_t K,
+                                                           int32_t* __restrict__ ptr) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i > K) return;
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (keys[mid] < i) lo = mid + 1;
+        else hi = mid;
+    }
+    ptr[i] = static_cast<int32_t>(lo);
+}
+
+// Pieces of one side.  `tot`: device totals, with the checks of the columns done.
+ra_status cut(AttnSide& s, int64_t nnz, Totals* tot, hipStream_t st) {
+    const int64_t n = (int64_t)s.rows + 1;
+    DeviceBuffer work;
+    size_t scan_a = 0, scan_b = 0;
+    RA_HIP_TRY(hipcub::DeviceScan::ExclusiveSum(nullptr, scan_a, (unsigned long long*)nullptr, (unsigned long long*)nullptr,
+                                                static_cast<int>(n), st));
+    RA_HIP_TRY(hipcub::DeviceScan::ExclusiveSum(nullptr, scan_b, (int32_t*)nullptr, (int32_t*)nullptr, static_cast<int>(n), st));
+    const size_t scan = (std::max(scan_a, scan_b) + 15) / 16 * 16;
+    RA_TRY(work.allocate(scan + n * 12 + 16));
+    void* tmp = work.get();
+    auto* items_slots = reinterpret_cast<unsigned long long*>(work.get<char>() + scan);
+    auto* splits = reinterpret_cast<int32_t*>(items_slots + n);
+    count_pieces<<<blocks_for(n), kThreads, 0, st>>>(s.ptr, s.rows, nnz, items_slots, splits, tot);
+    RA_LAUNCH_CHECK("count_pieces");
+    RA_HIP_TRY(hipcub::DeviceScan::ExclusiveSum(tmp, scan_a, items_slots, items_slots, static_cast<int>(n), st));
+    RA_HIP_TRY(hipcub::DeviceScan::ExclusiveSum(tmp, scan_b, splits, splits, static_cast<int>(n), st));
+    read_totals<<<1, 1, 0, st>>>(items_slots, splits, s.rows, tot);
+    RA_LAUNCH_CHECK("read_totals");
+    Totals t;
+    RA_HIP_TRY(hipMemcpyAsync(&t, tot, sizeof(t), hipMemcpyDeviceToHost, st));
+    RA_HIP_TRY(hipStreamSynchronize(st));
+    if (t.bad)
+        return fail(RA_ERR_INVALID_ARGUMENT,
+                    "attention plan: rowptr must run from 0 to nnz without decreasing, and colind lie in [0, K)");
+    const int64_t items = static_cast<int64_t>(t.items_slots >> 32);
+    s.num_items = static_cast<int32_t>(items);
+    s.num_slots = static_cast<int64_t>(t.items_slots & 0xFFFFFFFFu);
+    s.num_splits = t.splits;
+    RA_TRY(s.lists.allocate((items + s.num_splits) * sizeof(int4)));
+    auto* list = s.lists.get<int4>();
+    s.items = list;
+    s.splits = list + items;
+    place_pieces<<<blocks_for(s.rows), kThreads, 0, st>>>(s.ptr, s.rows, items_slots, splits, list, list + items);
+    RA_LAUNCH_CHECK("place_pieces");
+    RA_HIP_TRY(hipStreamSynchronize(st));
+    work.reset_idle();
+    return RA_OK;
+}
+
+ra_status transpose(ra_attn_plan* p, hipStream_t st) {
+    const AttnSide& r = p->side[0];
+    AttnSide& c = p->side[1];
+    const int64_t nnz = p->info.nnz, K = p->info.K;
+    c.rows = p->info.K;
+    // ptr [K + 1], row [nnz], edge [nnz], each 16-byte aligned
+    const int64_t a = (K + 4) / 4 * 4, b = (nnz + 3) / 4 * 4;
+    RA_TRY(p->transposed.allocate((a + 2 * b) * sizeof(int32_t)));
+    auto* ptr = p->transposed.get<int32_t>();
+    int32_t *row = ptr + a, *edge = row + b;
+    c.ptr = ptr;
+    c.idx = row;
+    c.edge = edge;
+    DeviceBuffer work;
+    int bits = 1;
+    while (bits < 31 && (int64_t{1} << bits) < K) ++bits;
+    size_t sort = 0;
+    RA_HIP_TRY(hipcub::DeviceRadixSort::SortPairs(nullptr, sort, (const int32_t*)nullptr, (int32_t*)nullptr,
+                                                  (const int32_t*)nullptr, (int32_t*)nullptr, static_cast<int>(nnz), 0,
+                                                  bits, st));
+    sort = (sort + 15) / 16 * 16;
+    RA_TRY(work.allocate(sort + 2 * b * sizeof(int32_t)));
+    auto* keys = reinterpret_cast<int32_t*>(work.get<char>() + sort);
+    int32_t* numbers = keys + b;
+    const unsigned grid = std::min(blocks_for(nnz), 65536u);
+    if (nnz > 0) {
+        edge_numbers<<<grid, kThreads, 0, st>>>(nnz, numbers);
+        RA_LAUNCH_CHECK("edge_numbers");
+        // Stable: a column's rows stay in ascending order.
+        RA_HIP_TRY(hipcub::DeviceRadixSort::SortPairs(work.get(), sort, r.idx, keys, numbers, edge,
+                                                      static_cast<int>(nnz), 0, bits, st));
+        transposed_rows<<<grid, kThreads, 0, st>>>(r.ptr, r.rows, nnz, edge, row);
+        RA_LAUNCH_CHECK("transposed_rows");
+    }
+    transposed_ptr<<<blocks_for(K + 1), kThreads, 0, st>>>(keys, nnz, p->info.K, ptr);
+    RA_LAUNCH_CHECK("transposed_ptr");
+    RA_HIP_TRY(hipStreamSynchronize(st));
+    work.reset_idle();
+    return RA_OK;
+}
+
+ra_status build(ra_attn_plan* p, const int32_t* rowptr, const int32_t* colind, bool backward, hipStream_t st) {
+    RA_HIP_TRY(hipGetDevice(&p->device));
+    AttnSide& r = p->side[0];
+    r.ptr = rowptr;
+    r.idx = colind;
+    r.rows = p->info.M;
+    if (p->info.M > 0) {
+        DeviceBuffer totals;
+        RA_TRY(totals.allocate(sizeof(Totals)));
+        auto* tot = totals.get<Totals>();
+        const Totals zero{};
+        RA_HIP_TRY(hipMemcpyAsync(tot, &zero, sizeof(zero), hipMemcpyHostToDevice, st));
+        if (p->info.nnz > 0) {
+            check_columns<<<std::min(blocks_for(p->info.nnz), 4096u), kThreads, 0, st>>>(colind, p->info.nnz, p->info.K, tot);
+            RA_LAUNCH_CHECK("check_columns");
+        }
+        RA_TRY(cut(r, p->info.nnz, tot, st));
+        if (backward && p->info.K > 0) {
+            RA_TRY(transpose(p, st));
+            RA_TRY(cut(p->side[1], p->info.nnz, tot, st));
+        }
+    } else if (backward && p->info.K > 0) {
+        // No rows: the columns' lists are empty, their gradients zero.
+        RA_TRY(transpose(p, st));
+        DeviceBuffer totals;
+        RA_TRY(totals.allocate(sizeof(Totals)));
+        const Totals zero{};
+        RA_HIP_TRY(hipMemcpyAsync(totals.get(), &zero, sizeof(zero), hipMemcpyHostToDevice, st));
+        RA_TRY(cut(p->side[1], 0, totals.get<Totals>(), st));
+    }
+    const AttnSide& c = p->side[1];
+    ra_attn_info& i = p->info;
+    i.backward = backward;
+    i.num_items = r.num_items;
+    i.num_splits = r.num_splits;
+    i.num_slots = r.num_slots;
+    i.num_items_t = c.num_items;
+    i.num_splits_t = c.num_splits;
+    i.num_slots_t = c.num_slots;
+    i.plan_bytes = (int64_t)(r.lists.bytes() + c.lists.bytes() + p->transposed.bytes());
+    return RA_OK;
+}
+
+int log2_up(int64_t n) {
+    int b = 0;
+    while ((int64_t{1} << b) < n) ++b;
+    return b;
+}
+
+AttnArgs args_of(const ra_attn_shape& s, const AttnLayout& l) {
+    AttnArgs a{};
+    a.q_heads = s.q_heads;
+    a.kv_heads = s.kv_heads;
+    a.group = s.q_heads / s.kv_heads;
+    a.head_dim = s.head_dim;
+    a.value_dim = s.value_dim;
+    a.scale = s.scale;
+    a.ldq = s.ldq;
+    a.ldk = s.ldk;
+    a.ldv = s.ldv;
+    a.head_blocks = l.head_blocks;
+    a.hb_shift = l.hb_shift;
+    a.pieces = 1;
+    return a;
+}
+
+void side_of(AttnArgs& a, const AttnSide& s) {
+    a.items = s.items;
+    a.ptr = s.ptr;
+    a.idx = s.idx;
+    a.edge = s.edge;
+    a.rows = s.rows;
+    a.num_units = (int64_t)s.num_items * a.head_blocks;
+}
+
+// Pieces of every row of a plan-free call: about kAttnPiece edges, fewer where that
+// leaves most of the GPU's wave slots empty, but at least 32.
+int plan_free_pieces(const ra_attn_shape& s, int32_t M, int64_t nnz) {
+    if (M <= 0 || nnz <= 0) return 1;
+    const int64_t mean = (nnz + M - 1) / M;
+    const int64_t waves = (int64_t)M * s.q_heads;  // a wave holds one head or more
+    int64_t piece = kAttnPiece;
+    while (piece > 32 && waves * ((mean + piece - 1) / piece) < 2048) piece /= 2;
+    return static_cast<int>(std::min<int64_t>((mean + piece - 1) / piece, 4096));
+}
+
+bool same_device(const ra_attn_plan* p) {
+    int d = -1;
+    return hipGetDevice(&d) == hipSuccess && d == p->device;
+}
+
+}  // namespace
+
+AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p) {
+    AttnLayout l{};
+    l.lm = 1;
+    while (l.lm * 8 < s.head_dim || l.lm * 16 < s.value_dim) l.lm *= 2;
+    l.nv = s.value_dim <= 8 * l.lm ? 4 : 8;
+    const int64_t size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
+    const int64_t key = 16, value = std::min<int64_t>(16, l.nv * size);  // bytes of a packet
+    auto whole = [](const void* ptr, int64_t ld_bytes, int64_t run_bytes, int64_t packet) {
+        return reinterpret_cast<uintptr_t>(ptr) % packet == 0 && ld_bytes % packet == 0 && run_bytes % packet == 0;
+    };
+    l.vec = whole(p.q, p.ldq * size, s.head_dim * size, key) && whole(p.k, p.ldk * size, s.head_dim * size, key) &&
+            whole(p.v, p.ldv * size, s.value_dim * size, value) && whole(p.grad, p.ldg * size, s.value_dim * size, value);
+    if (!l.vec) l.nv = 8;
+    // Heads of a wave: as many as leave the fewest lanes without a head.
+    const int most = log2_up(32 / l.lm);
+    int best = 0;
+    int64_t best_lanes = INT64_MAX;
+    for (int b = most; b >= 0; --b) {
+        const int64_t blocks = (heads + (1 << b) - 1) >> b;
+        if ((blocks << b) < best_lanes) {
+            best_lanes = blocks << b;
+            best = b;
+        }
+    }
+    l.hb_shift = best;
+    l.head_blocks = (heads + (1 << best) - 1) >> best;
+    return l;
+}
+
+ra_status attn_check(const ra_attn_shape* s, int32_t M, int32_t K) {
+    if (!s) return fail(RA_ERR_INVALID_ARGUMENT, "attention: shape is NULL");
+    if (s->dtype != RA_DTYPE_F32 && s->dtype != RA_DTYPE_F16 && s->dtype != RA_DTYPE_BF16)
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: unknown dtype");
+    if (s->q_heads < 1 || s->kv_heads < 1 || s->q_heads % s->kv_heads != 0)
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: q_heads must be a positive multiple of kv_heads");
+    if (s->head_dim < 1 || s->value_dim < 1) return fail(RA_ERR_INVALID_ARGUMENT, "attention: empty heads");
+    if (s->head_dim > 128 || s->value_dim > 256 || s->q_heads > 1024)
+        return fail(RA_ERR_UNSUPPORTED, "attention: head_dim is at most 128, value_dim at most 256, q_heads at most 1024");
+    if ((M > 0 && s->ldq < (int64_t)s->q_heads * 2 * s->head_dim) ||
+        (K > 0 && (s->ldk < (int64_t)s->kv_heads * 2 * s->head_dim || s->ldv < (int64_t)s->kv_heads * s->value_dim)))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: rows overlap (a leading dimension is too small)");
+    return RA_OK;
+}
+
+}  // namespace ra
+
+using ra::fail;
+
+namespace {
+
+// The pool's lists and the messages take host memory: no exception leaves a C entry.
+template <typename F>
+ra_status guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return RA_ERR_OUT_OF_MEMORY;
+    }
+}
+
+ra_status check_output(const void* p, const char* what) {
+    return ra::aligned16(p) ? RA_OK : fail(RA_ERR_INVALID_ARGUMENT, std::string("attention: ") + what + " is not 16-byte aligned");
+}
+
+}  // namespace
+
+extern "C" {
+
+ra_status ra_attn_plan_create(const int32_t* d_rowptr, const int32_t* d_colind, int32_t M, int32_t K, int64_t nnz,
+                              int32_t backward, ra_stream_t stream, ra_attn_plan** out) {
+    if (!out) return fail(RA_ERR_INVALID_ARGUMENT, "attention plan: out is NULL");
+    *out = nullptr;
+    if (M < 0 || K < 0 || nnz < 0) return fail(RA_ERR_INVALID_ARGUMENT, "attention plan: negative size");
+    if (nnz > INT32_MAX || M == INT32_MAX || K == INT32_MAX)
+        return fail(RA_ERR_UNSUPPORTED, "attention plan: int32 lists hold at most 2^31 - 1 edges");
+    if ((M > 0 && !d_rowptr) || (nnz > 0 && !d_colind))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention plan: NULL rowptr or colind");
+    if (M == 0 && nnz > 0) return fail(RA_ERR_INVALID_ARGUMENT, "attention plan: edges without rows");
+    std::unique_ptr<ra_attn_plan> p(new (std::nothrow) ra_attn_plan());
+    if (!p) return fail(RA_ERR_OUT_OF_MEMORY, "attention plan allocation");
+    p->info.M = M;
+    p->info.K = K;
+    p->info.nnz = nnz;
+    RA_TRY(guarded([&] { return ra::build(p.get(), d_rowptr, d_colind, backward != 0, reinterpret_cast<hipStream_t>(stream)); }));
+    *out = p.release();
+    return RA_OK;
+}
+
+ra_status ra_attn_plan_get_info(const ra_attn_plan* p, ra_attn_info* info) {
+    if (!p || !info) return fail(RA_ERR_INVALID_ARGUMENT, "attention plan info: NULL argument");
+    *info = p->info;
+    return RA_OK;
+}
+
+ra_status ra_attn_plan_export(const ra_attn_plan* p, const char* name, int32_t* dst, int64_t* count) {
+    if (!p || !name || !count) return fail(RA_ERR_INVALID_ARGUMENT, "attention plan export: NULL argument");
+    const std::string n(name);
+    const ra::AttnSide &r = p->side[0], &c = p->side[1];
+    const void* from = nullptr;
+    int64_t k = 0;
+    if (n == "items") { from = r.items; k = 4LL * r.num_items; }
+    else if (n == "items_t") { from = c.items; k = 4LL * c.num_items; }
+    else if (n == "splits") { from = r.splits; k = 4LL * r.num_splits; }
+    else if (n == "splits_t") { from = c.splits; k = 4LL * c.num_splits; }
+    else if (n == "rowptr_t") { from = c.ptr; k = c.ptr ? c.rows + 1LL : 0; }
+    else if (n == "row_t") { from = c.idx; k = c.idx ? p->info.nnz : 0; }
+    else if (n == "edge_t") { from = c.edge; k = c.edge ? p->info.nnz : 0; }
+    else return fail(RA_ERR_INVALID_ARGUMENT, "attention plan export: unknown array '" + n + "'");
+    *count = k;
+    if (dst && k > 0) RA_HIP_TRY(hipMemcpy(dst, from, k * sizeof(int32_t), hipMemcpyDeviceToHost));
+    return RA_OK;
+}
+
+void ra_attn_plan_destroy(ra_attn_plan* p) { delete p; }
+
+ra_status ra_attn_plan_run(ra_attn_plan* p, const ra_attn_shape* shape, const void* d_q, const void* d_k,
+                           const void* d_v, const float* d_lam, const float* d_bias, void* d_out, float* d_stats,
+                           ra_stream_t stream) {
+    if (!p) return fail(RA_ERR_INVALID_ARGUMENT, "attention: plan is NULL");
+    RA_TRY(ra::attn_check(shape, p->info.M, p->info.K));
+    if (p->info.M == 0) return RA_OK;
+    if (!d_q || !d_lam || !d_out || (p->info.nnz > 0 && (!d_k || !d_v)))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: NULL tensor");
+    if (!ra::same_device(p)) return fail(RA_ERR_INVALID_ARGUMENT, "attention: the plan was built on another GPU");
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const ra_attn_shape& s = *shape;
+    const ra::AttnLayout l = ra::attn_layout(
+        s, s.q_heads, {d_q, d_k, d_v, d_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim});
+    ra::AttnArgs a = ra::args_of(s, l);
+    ra::side_of(a, p->side[0]);
+    RA_TRY(check_output(d_out, "out"));
+    RA_TRY(check_output(d_stats, "stats"));
+    RA_TRY(guarded([&] { return p->partial.ensure(p->side[0].num_slots * ra::attn_forward_slot(s) * sizeof(float), st); }));
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.lam = d_lam;
+    a.bias = d_bias;
+    a.out = d_out;
+    a.stats = d_stats;
+    a.partial = p->partial.get<float>();
+    RA_TRY(ra::attn_forward_launch(s.dtype, l, a, st));
+    return ra::attn_forward_join_launch(s.dtype, a, p->side[0].splits, p->side[0].num_splits, st);
+}
+
+ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape, const void* d_q, const void* d_k,
+                                    const void* d_v, const float* d_lam, const float* d_bias, const float* d_stats,
+                                    const void* d_grad_out, void* d_dq, void* d_dk, void* d_dv, float* d_dlam,
+                                    ra_stream_t stream) {
+    if (!p) return fail(RA_ERR_INVALID_ARGUMENT, "attention: plan is NULL");
+    if (!p->info.backward)
+        return fail(RA_ERR_INACTIVE_PLAN, "attention: the plan was built without the backward pass' lists");
+    RA_TRY(ra::attn_check(shape, p->info.M, p->info.K));
+    const int32_t M = p->info.M, K = p->info.K;
+    if (!d_dlam || !d_lam || (M > 0 && (!d_q || !d_stats || !d_grad_out || !d_dq)) || (K > 0 && (!d_k || !d_v || !d_dk || !d_dv)))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: NULL tensor");
+    if (!ra::same_device(p)) return fail(RA_ERR_INVALID_ARGUMENT, "attention: the plan was built on another GPU");
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const ra_attn_shape& s = *shape;
+    const ra::AttnPtrs ptrs{d_q, d_k, d_v, d_grad_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim};
+    const ra::AttnSide &rows = p->side[0], &cols = p->side[1];
+    const int64_t partial = std::max({rows.num_slots * ra::attn_row_slot(s), cols.num_slots * ra::attn_col_slot(s),
+                                      (int64_t)ra::kLamBlocks * s.q_heads});
+    RA_TRY(check_output(d_dq, "dq"));
+    RA_TRY(check_output(d_dk, "dk"));
+    RA_TRY(check_output(d_dv, "dv"));
+    RA_TRY(check_output(d_stats, "stats"));
+    RA_TRY(guarded([&] { return p->partial.ensure(partial * sizeof(float), st); }));
+    RA_TRY(guarded([&] { return p->record.ensure((int64_t)M * s.q_heads * 2 * sizeof(float4), st); }));
+    ra::AttnLayout l = ra::attn_layout(s, s.q_heads, ptrs);
+    ra::AttnArgs a = ra::args_of(s, l);
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.grad = d_grad_out;
+    a.lam = d_lam;
+    a.bias = d_bias;
+    a.stats = const_cast<float*>(d_stats);
+    a.record = p->record.get<float4>();
+    a.partial = p->partial.get<float>();
+    if (M > 0) {
+        ra::side_of(a, rows);
+        a.out = d_dq;
+        RA_TRY(ra::attn_rows_launch(s.dtype, l, a, st));
+        RA_TRY(ra::attn_rows_join_launch(s.dtype, a, rows.splits, rows.num_splits, st));
+    }
+    RA_TRY(ra::attn_lam_launch(a.record, M, s.q_heads, a.partial, d_dlam, st));
+    if (K > 0) {
+        l = ra::attn_layout(s, s.kv_heads, ptrs);
+        a.head_blocks = l.head_blocks;
+        a.hb_shift = l.hb_shift;
+        ra::side_of(a, cols);
+        a.out = d_dk;
+        a.out2 = d_dv;
+        RA_TRY(ra::attn_cols_launch(s.dtype, l, a, st));
+        RA_TRY(ra::attn_cols_join_launch(s.dtype, a, cols.splits, cols.num_splits, st));
+    }
+    return RA_OK;
+}
+
+ra_status ra_attn_csr_workspace(const ra_attn_shape* shape, int32_t M, int64_t nnz, int64_t* bytes) {
+    if (!bytes) return fail(RA_ERR_INVALID_ARGUMENT, "attention: bytes is NULL");
+    RA_TRY(ra::attn_check(shape, 0, 0));
+    if (M < 0 || nnz < 0) return fail(RA_ERR_INVALID_ARGUMENT, "attention: negative size");
+    const int pieces = ra::plan_free_pieces(*shape, M, nnz);
+    *bytes = pieces == 1 ? 0 : (int64_t)M * pieces * ra::attn_forward_slot(*shape) * (int64_t)sizeof(float);
+    return RA_OK;
+}
+
+ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t M, int32_t K, int64_t nnz,
+                      const ra_attn_shape* shape, const void* d_q, const void* d_k, const void* d_v,
+                      const float* d_lam, const float* d_bias, void* d_out, void* d_workspace, int64_t bytes,
+                      ra_stream_t stream) {
+    if (M < 0 || K < 0 || nnz < 0 || nnz > INT32_MAX) return fail(RA_ERR_INVALID_ARGUMENT, "attention: bad size");
+    RA_TRY(ra::attn_check(shape, M, K));
+    if (M == 0) return RA_OK;
+    if (!d_rowptr || !d_q || !d_lam || !d_out || (nnz > 0 && (!d_colind || !d_k || !d_v)))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: NULL tensor");
+    int64_t need = 0;
+    RA_TRY(ra_attn_csr_workspace(shape, M, nnz, &need));
+    if (bytes < need || (need > 0 && (!d_workspace || !ra::aligned16(d_workspace))))
+        return fail(RA_ERR_INVALID_ARGUMENT, "attention: the workspace is too small or not 16-byte aligned");
+    RA_TRY(check_output(d_out, "out"));
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const ra_attn_shape& s = *shape;
+    const ra::AttnLayout l = ra::attn_layout(
+        s, s.q_heads, {d_q, d_k, d_v, d_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim});
+    ra::AttnArgs a = ra::args_of(s, l);
+    a.ptr = d_rowptr;
+    a.idx = d_colind;
+    a.rows = M;
+    a.pieces = ra::plan_free_pieces(s, M, nnz);
+    a.num_units = (int64_t)M * a.pieces * a.head_blocks;
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.lam = d_lam;
+    a.bias = d_bias;
+    a.out = d_out;
+    a.partial = static_cast<float*>(d_workspace);
+    RA_TRY(ra::attn_forward_launch(s.dtype, l, a, st));
+    return a.pieces == 1 ? RA_OK : ra::attn_forward_join_launch(s.dtype, a, nullptr, M, st);
+}
+
+}  // extern "C"

@@ -21,6 +21,8 @@
 
 #include "../../include/ra_spmm.h"
 
+void bind_operators(pybind11::module_& m);  // torch_binding_ops.cpp
+
 namespace {
 
 ra_stream_t current_stream() {
@@ -808,6 +810,7 @@ PYBIND11_MODULE(_C, m) {
     m.def("analyze_matrix", &analyze_matrix,
           "Diagnostic structural features of a CSR matrix (host computation)", pybind11::arg("rowptr"),
           pybind11::arg("colind"), pybind11::arg("M"), pybind11::arg("K"), pybind11::arg("N"));
+    bind_operators(m);
     m.def("abi_version", &ra_abi_version);
     m.def("release_memory", &ra_release_memory,
           "Give the device memory kept from destroyed plans back to the driver");

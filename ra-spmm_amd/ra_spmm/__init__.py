@@ -25,7 +25,10 @@ from ._C import (  # noqa: F401
     run_segment_hybrid_plan, run_segment_hybrid_plan_tf32, run_tc_direct_plan,
     run_tc_direct_plan_tf32, run_tile_plan_route, run_zero_overhead_plan, spmm_csr_baseline,
     spmm_csr_baseline_f16, spmm_csr_direct, spmm_cusparse,
+    RAAttentionPlan, diff_attention_csr, export_attention_plan, make_attention_plan, run_attention_plan,
+    run_attention_plan_backward, run_attention_plan_train,
 )
+from .attention import diff_attention  # noqa: F401
 from .dispatch import (  # noqa: F401
     BASE_ATOL, COLD_ITERS, COLD_ZO_MIN_CV, DEPLOYED_KERNELS, HARD_FAIL_THRESHOLD, TC_EXTRA_FACTOR, TILE_KERNELS, TIMED_ITERS,
     WARMUP, benchmark_cusparse, benchmark_cusparse_cold, benchmark_cusparse_fp16, benchmark_cusparse_fp16_cold,

@@ -28,6 +28,8 @@ EXPORTED = [
     "ra_tile_plan_create", "ra_tile_plan_create_device", "ra_tile_plan_export",
     "ra_tile_plan_run", "ra_tile_plan_run_lowp",
     "ra_tile_plan_get_info", "ra_tile_plan_destroy", "ra_convert_f32",
+    "ra_attn_plan_create", "ra_attn_plan_get_info", "ra_attn_plan_export", "ra_attn_plan_destroy", "ra_attn_plan_run",
+    "ra_attn_plan_run_backward", "ra_attn_csr_workspace", "ra_attn_csr",
 ]
 
 
@@ -109,6 +111,17 @@ class TileInfo(ctypes.Structure):
         ("col_parts", ctypes.c_int32), ("pad3_", ctypes.c_int32)]
 
 
+class AttnShape(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("q_heads", "kv_heads", "head_dim", "value_dim", "dtype")] +
+                [("scale", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("ldq", "ldk", "ldv")])
+
+
+class AttnInfo(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int32), ("K", ctypes.c_int32), ("nnz", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("backward", "num_items", "num_splits", "num_items_t", "num_splits_t")] + [
+        (n, ctypes.c_int64) for n in ("num_slots", "num_slots_t", "plan_bytes")]
+
+
 _lib = None
 
 
@@ -161,6 +174,14 @@ def load():
         "ra_tile_plan_run_lowp": (ctypes.c_int, [P, P, I32, I32, P, I32, P]),
         "ra_tile_plan_get_info": (ctypes.c_int, [P, ctypes.POINTER(TileInfo)]),
         "ra_tile_plan_destroy": (None, [P]),
+        "ra_attn_plan_create": (ctypes.c_int, [P, P, I32, I32, I64, I32, P, ctypes.POINTER(P)]),
+        "ra_attn_plan_get_info": (ctypes.c_int, [P, ctypes.POINTER(AttnInfo)]),
+        "ra_attn_plan_export": (ctypes.c_int, [P, ctypes.c_char_p, P, ctypes.POINTER(I64)]),
+        "ra_attn_plan_destroy": (None, [P]),
+        "ra_attn_plan_run": (ctypes.c_int, [P, ctypes.POINTER(AttnShape)] + [P] * 8),
+        "ra_attn_plan_run_backward": (ctypes.c_int, [P, ctypes.POINTER(AttnShape)] + [P] * 12),
+        "ra_attn_csr_workspace": (ctypes.c_int, [ctypes.POINTER(AttnShape), I32, I64, ctypes.POINTER(I64)]),
+        "ra_attn_csr": (ctypes.c_int, [P, P, I32, I32, I64, ctypes.POINTER(AttnShape)] + [P] * 7 + [I64, P]),
         "ra_convert_f32": (ctypes.c_int, [P, P, I64, I32, I32, I32, P]),
     }
     for name, (res, args) in sig.items():
