@@ -447,6 +447,74 @@ ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t 
                       const float* d_lam, const float* d_bias, void* d_out, void* d_workspace, int64_t bytes,
                       ra_stream_t stream);
 
+/* ------------------------------------------------- head norms and rotation
+ * RMS norm of every head of q [rows, q_heads, head_dim] and k [rows, k_heads,
+ * head_dim], its weight, and the rotation of the first rot_dim coordinates by the
+ * row's position, in one pass (no reference counterpart):
+ *     y = R(position) (w * x / sqrt(mean(x^2) + eps))
+ * d_table [positions, rot_dim / 2, 2] fp32 holds (cos, sin) of every pair's angle;
+ * pairs are (i, i + rot_dim / 2) in the half layout, (2 i, 2 i + 1) in the
+ * interleaved one.  d_positions [rows] int32, NULL = the row numbers; a position
+ * outside of the table gives NaN.  rot_dim may be 0 (table and positions are not
+ * used), and one of q_heads and k_heads may be 0.  Weights are fp32 [head_dim].
+ * Rows of q and k may lie ldq, ldk elements apart; outputs and gradients are
+ * contiguous.  Sums are fp32, and those of the weights' gradients have a fixed
+ * order. */
+typedef enum ra_rotation { RA_ROTATION_HALF = 0, RA_ROTATION_INTERLEAVED = 1 } ra_rotation;
+typedef struct ra_norm_shape {
+    int32_t rows, q_heads, k_heads;
+    int32_t head_dim;  /* 1 .. 256                  */
+    int32_t rot_dim;   /* even, at most head_dim    */
+    int32_t positions; /* rows of the table         */
+    int32_t layout;    /* ra_rotation               */
+    int32_t dtype;     /* ra_dtype                  */
+    float eps;
+    int64_t ldq, ldk;  /* elements between rows     */
+} ra_norm_shape;
+ra_status ra_head_norm(const ra_norm_shape* shape, const void* d_q, const void* d_k, const float* d_wq,
+                       const float* d_wk, const float* d_table, const int32_t* d_positions, void* d_out_q,
+                       void* d_out_k, ra_stream_t stream);
+/* d_workspace: ra_head_norm_workspace() bytes. */
+ra_status ra_head_norm_workspace(const ra_norm_shape* shape, int64_t* bytes);
+ra_status ra_head_norm_backward(const ra_norm_shape* shape, const void* d_q, const void* d_k, const float* d_wq,
+                                const float* d_wk, const float* d_table, const int32_t* d_positions,
+                                const void* d_grad_q, const void* d_grad_k, void* d_dq, void* d_dk, float* d_dwq,
+                                float* d_dwk, void* d_workspace, int64_t bytes, ra_stream_t stream);
+
+/* ------------------------------------------------- activations kept in 8 bits
+ * A [rows, cols] matrix kept as one byte per element and one scale per 32
+ * consecutive columns of a row (no reference counterpart).  The scale is the power
+ * of two that puts the group's largest magnitude into [64, 128), or [128, 256) in
+ * the unsigned form, so that code * scale has at most 8 significant bits: it is
+ * exact in bf16, and products with it on the matrix cores are exact.
+ *   signed    code = round(x / scale), -127 .. 127 (two's complement)
+ *   unsigned  of max(x, 0): 0 .. 255, and at least 1 where x > 0, so that the codes
+ *             also hold the ReLU's mask exactly
+ * Codes lie in rows of ldc = cols rounded up to 32 bytes (the padding is 0), scales
+ * as their exponent + 127 in one byte, [rows, ldc / 32]; 255 marks a group that
+ * holds an inf or NaN: all of it reads back as NaN, and its unsigned codes are the
+ * mask (1 where x > 0 or NaN).  d_codes and d_scales lie on 16-byte addresses. */
+ra_status ra_pack8(const void* d_x, int64_t rows, int32_t cols, int64_t ldx, int32_t dtype, uint8_t* d_codes,
+                   uint8_t* d_scales, ra_stream_t stream);
+/* y = max(x, 0) (contiguous; NaN stays) and its unsigned codes in one pass. */
+ra_status ra_relu_pack8(const void* d_x, int64_t rows, int32_t cols, int64_t ldx, int32_t dtype, void* d_y,
+                        uint8_t* d_codes, uint8_t* d_scales, ra_stream_t stream);
+/* code * scale in dtype (contiguous). */
+ra_status ra_unpack8(const uint8_t* d_codes, const uint8_t* d_scales, int64_t rows, int32_t cols, int32_t is_signed,
+                     int32_t dtype, void* d_out, ra_stream_t stream);
+/* Gradient of the ReLU from its unsigned codes: grad where code > 0, else 0. */
+ra_status ra_relu_grad8(const void* d_grad, const uint8_t* d_codes, int64_t rows, int32_t cols, int64_t ldg,
+                        int32_t dtype, void* d_out, ra_stream_t stream);
+/* The weight gradient of y = x W^T from the kept x: d_out [out, cols] fp32 =
+ * grad^T (code * scale), grad [rows, out].  On the matrix cores in bf16 with fp32
+ * sums; a grad of more bits is cut into bf16 pieces that add up to it exactly (three
+ * for fp32, two for fp16), so no product is rounded.  The sums have a fixed order.
+ * d_workspace: ra_weight_grad8_workspace() bytes, 16-byte aligned. */
+ra_status ra_weight_grad8_workspace(int64_t rows, int32_t out, int32_t cols, int64_t* bytes);
+ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint8_t* d_scales, int64_t rows,
+                          int32_t out, int32_t cols, int64_t ldg, int32_t is_signed, int32_t dtype, float* d_out,
+                          void* d_workspace, int64_t bytes, ra_stream_t stream);
+
 /* ------------------------------------------------------------ utilities */
 /* fp32 -> fp16/bf16 round-to-nearest-even conversion of a [rows, cols] matrix
  * into a buffer with leading dimension ldo (columns cols..ldo-1 zero-filled).

@@ -46,6 +46,9 @@ SOURCES = {
     "attention_fwd.hip": [],
     "attention_bwd_rows.hip": [],
     "attention_bwd_cols.hip": [],
+    "head_norm.hip": [],
+    "pack8.hip": [],
+    "weight_grad8.hip": [],
 }
 LIB_NAME = "libra_spmm_hip.so"
 

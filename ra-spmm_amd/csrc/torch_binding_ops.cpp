@@ -216,6 +216,203 @@ Tensor diff_attention_csr(Tensor rowptr, Tensor colind, Tensor q, Tensor k, Tens
     return out;
 }
 
+// ------------------------------------------------- head norms and rotation
+// q and k: [rows, ..., head_dim]; the dimensions between are heads.
+struct NormCall {
+    ra_norm_shape shape{};
+    const float *wq = nullptr, *wk = nullptr, *table = nullptr;
+    const int32_t* positions = nullptr;
+};
+
+int64_t heads_of(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.dim() >= 2 && t.size(-1) > 0, name, " must have shape [rows, heads.., head_dim], has ", t.sizes());
+    int64_t n = 1;
+    for (int64_t d = 1; d + 1 < t.dim(); ++d) n *= t.size(d);
+    TORCH_CHECK(n > 0, name, " has no heads");
+    return n;
+}
+
+NormCall norm_call(const Tensor& q, const OptTensor& k, const Tensor& wq, const OptTensor& wk, const OptTensor& table,
+                   const OptTensor& positions, double eps, const std::string& layout) {
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    const auto dev = q.device();
+    NormCall c;
+    ra_norm_shape& s = c.shape;
+    const int64_t hq = heads_of(q, "q"), hk = k.has_value() ? heads_of(*k, "k") : 0, D = q.size(-1);
+    TORCH_CHECK(q.size(0) < INT32_MAX && hq < INT32_MAX && hk < INT32_MAX && D < INT32_MAX, "q or k is too large");
+    s.rows = static_cast<int32_t>(q.size(0));
+    s.q_heads = static_cast<int32_t>(hq);
+    s.k_heads = static_cast<int32_t>(hk);
+    s.head_dim = static_cast<int32_t>(D);
+    s.dtype = dtype_of(q, "q and k");
+    s.eps = static_cast<float>(eps);
+    s.ldq = row_stride(q, "q");
+    c.wq = f32_vector(wq, "wq", D, dev);
+    TORCH_CHECK(k.has_value() == wk.has_value(), "k and wk go together");
+    if (k.has_value()) {
+        check_on(*k, "k", dev);
+        TORCH_CHECK(k->scalar_type() == q.scalar_type(), "q and k must have one dtype");
+        TORCH_CHECK(k->size(0) == q.size(0) && k->size(-1) == D, "q and k must have the same rows and head_dim");
+        s.ldk = row_stride(*k, "k");
+        c.wk = f32_vector(*wk, "wk", D, dev);
+    }
+    if (layout == "half") s.layout = RA_ROTATION_HALF;
+    else if (layout == "interleaved") s.layout = RA_ROTATION_INTERLEAVED;
+    else TORCH_CHECK(false, "layout must be 'half' or 'interleaved', got '", layout, "'");
+    if (table.has_value()) {
+        check_on(*table, "table", dev);
+        TORCH_CHECK(table->scalar_type() == torch::kFloat32 && table->is_contiguous() && table->dim() == 3 && table->size(2) == 2,
+                    "table must be contiguous float32 [positions, rot_dim / 2, 2], has ", table->sizes());
+        TORCH_CHECK(2 * table->size(1) <= D, "the table's rot_dim ", 2 * table->size(1), " passes head_dim ", D);
+        TORCH_CHECK(table->size(0) < INT32_MAX, "the table is too long");
+        s.positions = static_cast<int32_t>(table->size(0));
+        s.rot_dim = static_cast<int32_t>(2 * table->size(1));
+        c.table = table->data_ptr<float>();
+    }
+    if (positions.has_value()) {
+        check_on(*positions, "positions", dev);
+        TORCH_CHECK(table.has_value(), "positions need a table");
+        TORCH_CHECK(positions->scalar_type() == torch::kInt32 && positions->is_contiguous() && positions->dim() == 1 &&
+                        positions->numel() == q.size(0),
+                    "positions must be contiguous int32 [rows]");
+        c.positions = positions->data_ptr<int32_t>();
+    }
+    return c;
+}
+
+std::tuple<Tensor, OptTensor> run_head_norm(Tensor q, OptTensor k, Tensor wq, OptTensor wk, OptTensor table,
+                                            OptTensor positions, double eps, std::string layout) {
+    const NormCall c = norm_call(q, k, wq, wk, table, positions, eps, layout);
+    const c10::DeviceGuard guard(q.device());
+    auto yq = torch::empty(q.sizes(), q.options());
+    OptTensor yk;
+    if (k.has_value()) yk = torch::empty(k->sizes(), k->options());
+    check(ra_head_norm(&c.shape, q.data_ptr(), k.has_value() ? k->data_ptr() : nullptr, c.wq, c.wk, c.table, c.positions,
+                       yq.data_ptr(), yk.has_value() ? yk->data_ptr() : nullptr, current_stream()),
+          "head_norm_rotate");
+    return {yq, yk};
+}
+
+std::tuple<Tensor, OptTensor, Tensor, OptTensor> run_head_norm_backward(Tensor q, OptTensor k, Tensor wq, OptTensor wk,
+                                                                        OptTensor table, OptTensor positions, double eps,
+                                                                        std::string layout, Tensor gq, OptTensor gk) {
+    const NormCall c = norm_call(q, k, wq, wk, table, positions, eps, layout);
+    auto check_grad = [&](const Tensor& g, const Tensor& x, const char* name) {
+        check_on(g, name, q.device());
+        TORCH_CHECK(g.scalar_type() == x.scalar_type() && g.is_contiguous() && g.sizes() == x.sizes(), name,
+                    " must be contiguous, of the output's shape and dtype");
+    };
+    check_grad(gq, q, "grad_q");
+    TORCH_CHECK(k.has_value() == gk.has_value(), "k and grad_k go together");
+    if (k.has_value()) check_grad(*gk, *k, "grad_k");
+    const c10::DeviceGuard guard(q.device());
+    auto dq = torch::empty(q.sizes(), q.options());
+    auto dwq = torch::empty(wq.sizes(), wq.options());
+    OptTensor dk, dwk;
+    if (k.has_value()) {
+        dk = torch::empty(k->sizes(), k->options());
+        dwk = torch::empty(wk->sizes(), wk->options());
+    }
+    int64_t bytes = 0;
+    check(ra_head_norm_workspace(&c.shape, &bytes), "head_norm_rotate backward");
+    auto work = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+    check(ra_head_norm_backward(&c.shape, q.data_ptr(), k.has_value() ? k->data_ptr() : nullptr, c.wq, c.wk, c.table,
+                                c.positions, gq.data_ptr(), gk.has_value() ? gk->data_ptr() : nullptr, dq.data_ptr(),
+                                dk.has_value() ? dk->data_ptr() : nullptr, dwq.data_ptr<float>(),
+                                dwk.has_value() ? dwk->data_ptr<float>() : nullptr, work.data_ptr(), bytes, current_stream()),
+          "head_norm_rotate backward");
+    return {dq, dk, dwq, dwk};
+}
+
+// ------------------------------------------------- activations kept in 8 bits
+int64_t packed_width(int64_t cols) { return (cols + 31) / 32 * 32; }
+
+int64_t check_matrix(const Tensor& x, const char* name) {
+    TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) < INT32_MAX - 64, name, " must be [rows, cols], has ", x.sizes());
+    dtype_of(x, name);
+    return row_stride(x, name);
+}
+
+void check_packed(const Tensor& codes, const Tensor& scales, int64_t cols) {
+    TORCH_CHECK(codes.is_cuda() && scales.is_cuda() && codes.device() == scales.device(),
+                "codes and scales must be CUDA tensors on the same device");
+    TORCH_CHECK(codes.scalar_type() == torch::kUInt8 && codes.is_contiguous() && codes.dim() == 2 && cols > 0 &&
+                    codes.size(1) == packed_width(cols),
+                "codes must be contiguous uint8 [rows, cols rounded up to 32]");
+    TORCH_CHECK(scales.scalar_type() == torch::kUInt8 && scales.is_contiguous() && scales.dim() == 2 &&
+                    scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1) / 32,
+                "scales must be contiguous uint8 [rows, groups]");
+}
+
+std::tuple<Tensor, Tensor> pack8(Tensor x) {
+    const int64_t ld = check_matrix(x, "x");
+    const c10::DeviceGuard guard(x.device());
+    const auto bytes = x.options().dtype(torch::kUInt8);
+    auto codes = torch::empty({x.size(0), packed_width(x.size(1))}, bytes);
+    auto scales = torch::empty({x.size(0), packed_width(x.size(1)) / 32}, bytes);
+    check(ra_pack8(x.data_ptr(), x.size(0), static_cast<int32_t>(x.size(1)), ld, dtype_of(x, "x"),
+                   codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), current_stream()),
+          "pack8");
+    return {codes, scales};
+}
+
+std::tuple<Tensor, Tensor, Tensor> relu_pack8(Tensor x) {
+    const int64_t ld = check_matrix(x, "x");
+    const c10::DeviceGuard guard(x.device());
+    const auto bytes = x.options().dtype(torch::kUInt8);
+    auto y = torch::empty(x.sizes(), x.options());
+    auto codes = torch::empty({x.size(0), packed_width(x.size(1))}, bytes);
+    auto scales = torch::empty({x.size(0), packed_width(x.size(1)) / 32}, bytes);
+    check(ra_relu_pack8(x.data_ptr(), x.size(0), static_cast<int32_t>(x.size(1)), ld, dtype_of(x, "x"), y.data_ptr(),
+                        codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), current_stream()),
+          "relu_pack8");
+    return {y, codes, scales};
+}
+
+Tensor unpack8(Tensor codes, Tensor scales, int64_t cols, bool is_signed, torch::ScalarType dtype) {
+    check_packed(codes, scales, cols);
+    TORCH_CHECK(dtype == torch::kFloat32 || dtype == torch::kFloat16 || dtype == torch::kBFloat16,
+                "dtype must be float32, float16 or bfloat16");
+    const c10::DeviceGuard guard(codes.device());
+    auto out = torch::empty({codes.size(0), cols}, codes.options().dtype(dtype));
+    check(ra_unpack8(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), codes.size(0), static_cast<int32_t>(cols),
+                     is_signed, dtype_of(out, "dtype"), out.data_ptr(), current_stream()),
+          "unpack8");
+    return out;
+}
+
+Tensor relu_grad8(Tensor grad, Tensor codes, Tensor scales, int64_t cols) {
+    check_packed(codes, scales, cols);
+    check_on(grad, "grad", codes.device());
+    const int64_t ld = check_matrix(grad, "grad");
+    TORCH_CHECK(grad.size(0) == codes.size(0) && grad.size(1) == cols, "grad must have the packed shape [", codes.size(0),
+                ", ", cols, "], has ", grad.sizes());
+    const c10::DeviceGuard guard(codes.device());
+    auto out = torch::empty(grad.sizes(), grad.options());
+    check(ra_relu_grad8(grad.data_ptr(), codes.data_ptr<uint8_t>(), grad.size(0), static_cast<int32_t>(cols), ld,
+                        dtype_of(grad, "grad"), out.data_ptr(), current_stream()),
+          "relu_grad8");
+    return out;
+}
+
+Tensor weight_grad8(Tensor grad, Tensor codes, Tensor scales, int64_t cols, bool is_signed) {
+    check_packed(codes, scales, cols);
+    check_on(grad, "grad", codes.device());
+    const int64_t ld = check_matrix(grad, "grad");
+    TORCH_CHECK(grad.size(0) == codes.size(0), "grad has ", grad.size(0), " rows, the packed activation ", codes.size(0));
+    const c10::DeviceGuard guard(codes.device());
+    const auto O = static_cast<int32_t>(grad.size(1)), C = static_cast<int32_t>(cols);
+    auto out = torch::empty({grad.size(1), cols}, grad.options().dtype(torch::kFloat32));
+    int64_t bytes = 0;
+    check(ra_weight_grad8_workspace(grad.size(0), O, C, &bytes), "weight_grad8");
+    auto work = torch::empty({bytes}, codes.options());
+    check(ra_weight_grad8(grad.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), grad.size(0), O, C, ld,
+                          is_signed, dtype_of(grad, "grad"), out.data_ptr<float>(), work.data_ptr(), bytes, current_stream()),
+          "weight_grad8");
+    return out;
+}
+
 }  // namespace
 
 void bind_operators(pybind11::module_& m) {
@@ -256,4 +453,22 @@ void bind_operators(pybind11::module_& m) {
           },
           "Copy a plan array to the host (items, splits, rowptr_t, row_t, edge_t, items_t, splits_t)", py::arg("plan"),
           py::arg("name"));
+
+    m.def("run_head_norm", &run_head_norm, "RMS norm of every head and rotation: (q, k)", py::arg("q"), py::arg("k"),
+          py::arg("wq"), py::arg("wk"), py::arg("table"), py::arg("positions"), py::arg("eps"), py::arg("layout"));
+    m.def("run_head_norm_backward", &run_head_norm_backward, "(dq, dk, dwq, dwk) of run_head_norm", py::arg("q"),
+          py::arg("k"), py::arg("wq"), py::arg("wk"), py::arg("table"), py::arg("positions"), py::arg("eps"),
+          py::arg("layout"), py::arg("grad_q"), py::arg("grad_k"));
+
+    m.def("pack8", &pack8, "(codes, scales) of a matrix in 8 bits", py::arg("x"));
+    m.def("relu_pack8", &relu_pack8, "(relu(x), codes, scales)", py::arg("x"));
+    m.def("unpack8",
+          [](Tensor codes, Tensor scales, int64_t cols, bool is_signed, py::object dtype) {
+              return unpack8(codes, scales, cols, is_signed, torch::python::detail::py_object_to_dtype(dtype));
+          },
+          "code * scale", py::arg("codes"), py::arg("scales"), py::arg("cols"), py::arg("signed"), py::arg("dtype"));
+    m.def("relu_grad8", &relu_grad8, "grad where the unsigned code is positive", py::arg("grad"), py::arg("codes"),
+          py::arg("scales"), py::arg("cols"));
+    m.def("weight_grad8", &weight_grad8, "grad^T (code * scale), float32", py::arg("grad"), py::arg("codes"),
+          py::arg("scales"), py::arg("cols"), py::arg("signed"));
 }

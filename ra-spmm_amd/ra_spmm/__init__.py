@@ -28,7 +28,10 @@ from ._C import (  # noqa: F401
     RAAttentionPlan, diff_attention_csr, export_attention_plan, make_attention_plan, run_attention_plan,
     run_attention_plan_backward, run_attention_plan_train,
 )
-from .attention import diff_attention  # noqa: F401
+from .attention import diff_attention, head_norm_rotate, rotation_table  # noqa: F401
+from .checkpoint8 import (  # noqa: F401
+    Packed8, linear8, pack8, relu8, relu_grad8, relu_pack8, unpack8, weight_grad8,
+)
 from .dispatch import (  # noqa: F401
     BASE_ATOL, COLD_ITERS, COLD_ZO_MIN_CV, DEPLOYED_KERNELS, HARD_FAIL_THRESHOLD, TC_EXTRA_FACTOR, TILE_KERNELS, TIMED_ITERS,
     WARMUP, benchmark_cusparse, benchmark_cusparse_cold, benchmark_cusparse_fp16, benchmark_cusparse_fp16_cold,

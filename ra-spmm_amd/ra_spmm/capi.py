@@ -30,6 +30,8 @@ EXPORTED = [
     "ra_tile_plan_get_info", "ra_tile_plan_destroy", "ra_convert_f32",
     "ra_attn_plan_create", "ra_attn_plan_get_info", "ra_attn_plan_export", "ra_attn_plan_destroy", "ra_attn_plan_run",
     "ra_attn_plan_run_backward", "ra_attn_csr_workspace", "ra_attn_csr",
+    "ra_head_norm", "ra_head_norm_workspace", "ra_head_norm_backward",
+    "ra_pack8", "ra_relu_pack8", "ra_unpack8", "ra_relu_grad8", "ra_weight_grad8_workspace", "ra_weight_grad8",
 ]
 
 
@@ -122,6 +124,12 @@ class AttnInfo(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("num_slots", "num_slots_t", "plan_bytes")]
 
 
+class NormShape(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("rows", "q_heads", "k_heads", "head_dim", "rot_dim", "positions",
+                                               "layout", "dtype")] +
+                [("eps", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("ldq", "ldk")])
+
+
 _lib = None
 
 
@@ -182,6 +190,15 @@ def load():
         "ra_attn_plan_run_backward": (ctypes.c_int, [P, ctypes.POINTER(AttnShape)] + [P] * 12),
         "ra_attn_csr_workspace": (ctypes.c_int, [ctypes.POINTER(AttnShape), I32, I64, ctypes.POINTER(I64)]),
         "ra_attn_csr": (ctypes.c_int, [P, P, I32, I32, I64, ctypes.POINTER(AttnShape)] + [P] * 7 + [I64, P]),
+        "ra_head_norm": (ctypes.c_int, [ctypes.POINTER(NormShape)] + [P] * 9),
+        "ra_head_norm_workspace": (ctypes.c_int, [ctypes.POINTER(NormShape), ctypes.POINTER(I64)]),
+        "ra_head_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormShape)] + [P] * 13 + [I64, P]),
+        "ra_pack8": (ctypes.c_int, [P, I64, I32, I64, I32, P, P, P]),
+        "ra_relu_pack8": (ctypes.c_int, [P, I64, I32, I64, I32, P, P, P, P]),
+        "ra_unpack8": (ctypes.c_int, [P, P, I64, I32, I32, I32, P, P]),
+        "ra_relu_grad8": (ctypes.c_int, [P, P, I64, I32, I64, I32, P, P]),
+        "ra_weight_grad8_workspace": (ctypes.c_int, [I64, I32, I32, ctypes.POINTER(I64)]),
+        "ra_weight_grad8": (ctypes.c_int, [P, P, P, I64, I32, I32, I64, I32, I32, P, P, I64, P]),
         "ra_convert_f32": (ctypes.c_int, [P, P, I64, I32, I32, I32, P]),
     }
     for name, (res, args) in sig.items():
