@@ -395,7 +395,7 @@ typedef struct ra_attn_shape {
     int32_t value_dim;         /* 1 .. 256                           */
     int32_t dtype;             /* ra_dtype of q, k, v, out and grads */
     float scale;
-    int64_t ldq, ldk, ldv;     /* elements between rows              */
+    int64_t ldq, ldk, ldv;     /* elements between rows, below 2^30  */
 } ra_attn_shape;
 
 typedef struct ra_attn_plan ra_attn_plan;

@@ -49,6 +49,8 @@ struct AttnArgs {
     int32_t rows;
     float scale;
     int64_t ldq, ldk, ldv;
+    uint32_t q_pitch, k_pitch, v_pitch, g_pitch;  // bytes between rows
+    bool ragged;          // some lane's run is not whole: loaded words are masked
     const void *q, *k, *v, *grad;
     const float *lam, *bias;
     float* stats;    // [rows, q_heads, 2] (max, 1 / sum)
@@ -62,7 +64,8 @@ struct AttnArgs {
 struct AttnLayout {
     int lm;      // 1, 2, 4, 8, 16
     int nv;      // 4 or 8
-    bool vec;    // every lane's run is whole aligned 16-byte (value rows: NV-element) packets
+    int packet;  // bytes that a lane loads at once: 16 (value rows of NV = 4: 4 elements), 4 or 2
+    bool ragged;
     int hb_shift;
     int head_blocks;
 };
@@ -80,6 +83,12 @@ inline int64_t attn_forward_slot(const ra_attn_shape& s) { return (int64_t)s.q_h
 inline int64_t attn_row_slot(const ra_attn_shape& s) { return (int64_t)s.q_heads * (4 * s.head_dim + 2); }
 inline int64_t attn_col_slot(const ra_attn_shape& s) { return (int64_t)s.kv_heads * (2 * s.head_dim + s.value_dim); }
 
+// Workgroups of a launch, 0 where there is nothing to do.
+inline ra_status attn_grid(const AttnArgs& a, unsigned& blocks) {
+    if (a.num_units > (int64_t{1} << 32) - 1024) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads");
+    blocks = static_cast<unsigned>((a.num_units + 3) / 4);
+    return RA_OK;
+}
 ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
 ra_status attn_rows_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
 ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
@@ -136,22 +145,26 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
     const int64_t full = gridDim.x - (per - 1) * 8;  // XCDs with `per` workgroups
     const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
     const int64_t block = x < full ? x * per + y : full * per + (x - full) * (per - 1) + y;
-    const int64_t unit = block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // At most 2^32 units (attn_*_launch): 32-bit divisions.
+    const uint64_t at = block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Unit u{};
-    u.live = unit < a.num_units;
+    u.live = at < static_cast<uint64_t>(a.num_units);
     if (!u.live) return u;
-    const int64_t item = a.head_blocks == 1 ? unit : unit / a.head_blocks;
-    u.head_block = static_cast<int>(unit - item * a.head_blocks);
+    const uint32_t unit = static_cast<uint32_t>(at), blocks = a.head_blocks;
+    const uint32_t item = blocks == 1 ? unit : unit / blocks;
+    u.head_block = static_cast<int>(unit - item * blocks);
     if (a.items) {
         const int4 it = a.items[item];
         u.row = it.x, u.begin = it.y, u.end = it.z, u.slot = it.w;
     } else {
-        u.row = static_cast<int>(item / a.pieces);
-        const int64_t part = item - (int64_t)u.row * a.pieces;
-        const int64_t b = a.ptr[u.row], n = a.ptr[u.row + 1] - b;
-        u.begin = static_cast<int>(b + n * part / a.pieces);
-        u.end = static_cast<int>(b + n * (part + 1) / a.pieces);
-        u.slot = a.pieces == 1 ? -1 : static_cast<int>(item);
+        const uint32_t pieces = a.pieces, row = pieces == 1 ? item : item / pieces, part = item - row * pieces;
+        const int64_t b = a.ptr[row], n = a.ptr[row + 1] - b;
+        u.row = static_cast<int>(row);
+        // Whole multiples of the first part's length, rounded up.
+        const int64_t each = pieces == 1 ? n : (int64_t)(((uint32_t)n + pieces - 1) / pieces);
+        u.begin = static_cast<int>(b + min(n, each * part));
+        u.end = static_cast<int>(b + min(n, each * (part + 1)));
+        u.slot = pieces == 1 ? -1 : static_cast<int>(item);
     }
     return u;
 }
@@ -178,28 +191,147 @@ struct Place {
     }
 };
 
-// Calls KERNEL<T, LM, NV, VEC> for a layout.
-#define RA_ATTN_DISPATCH(KERNEL, dtype, l, grid, st, args)                                            \
-    do {                                                                                              \
-        auto by_type = [&](auto tag) {                                                                \
-            using T = decltype(tag);                                                                  \
-            auto by_lm = [&](auto lm) {                                                               \
-                constexpr int LM = decltype(lm)::value;                                               \
-                if (!(l).vec) KERNEL<T, LM, 8, false><<<grid, ra::kAttnThreads, 0, st>>>(args);       \
-                else if ((l).nv == 4) KERNEL<T, LM, 4, true><<<grid, ra::kAttnThreads, 0, st>>>(args); \
-                else KERNEL<T, LM, 8, true><<<grid, ra::kAttnThreads, 0, st>>>(args);                 \
-            };                                                                                        \
-            switch ((l).lm) {                                                                         \
-                case 1: by_lm(std::integral_constant<int, 1>()); break;                               \
-                case 2: by_lm(std::integral_constant<int, 2>()); break;                               \
-                case 4: by_lm(std::integral_constant<int, 4>()); break;                               \
-                case 8: by_lm(std::integral_constant<int, 8>()); break;                               \
-                default: by_lm(std::integral_constant<int, 16>());                                    \
-            }                                                                                         \
-        };                                                                                            \
-        if ((dtype) == RA_DTYPE_F32) by_type(float());                                                \
-        else if ((dtype) == RA_DTYPE_F16) by_type(ra::f16_t());                                       \
-        else by_type(ra::bf16_t());                                                                   \
+// Edges in flight per slot: their loads are all issued before the first is used
+// (the scheduler would otherwise wait for each in turn to save registers).
+constexpr int kDeep = 4;
+
+// The next kDeep edges of every slot.  Past the end the last edge again, not live.
+struct Edges {
+    int other[kDeep];
+    float add[kDeep];
+};
+
+template <bool TRANSPOSED>
+__device__ __forceinline__ void load_edges(const AttnArgs& a, Edges& x, int e0, int end, int es, int slots) {
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+        const int e = min(e0 + d * slots + es, end - 1);
+        x.other[d] = a.idx[e];
+        x.add[d] = 0.f;
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int e = min(e0 + d * slots + es, end - 1);
+            x.add[d] = a.bias[TRANSPOSED ? a.edge[e] : e];
+        }
+    }
+}
+// Edges past the end, and left out by their bias, get -inf.
+__device__ __forceinline__ void close_edges(Edges& x, int e0, int end, int es, int slots) {
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+        if (e0 + d * slots + es >= end) x.add[d] = -INFINITY;
+}
+
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, f16_t) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), c, false);
+}
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, bf16_t) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, a), __builtin_bit_cast(b2, b), c, false);
+}
+// Products of two runs, summed in fp32 (16-bit pairs by the two-term instruction).
+template <typename T, int N>
+__device__ __forceinline__ float dot(const Run<T, N>& a, const Run<T, N>& b) {
+    float t = 0.f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) t = fmaf(a.w[i], b.w[i], t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) t = dot2(a.w[i], b.w[i], t, T());
+    }
+    return t;
+}
+
+// A lane's run in the rows of a gathered matrix, in packets of PB bytes.  Packets
+// that do not exist are loaded from the start of the row's part instead, and masked.
+template <typename T, int N, int PB>
+struct Gather {
+    static constexpr int kBytes = N * (int)sizeof(T);
+    static constexpr int kPacket = PB < kBytes ? PB : kBytes;
+    static constexpr int kPackets = kBytes / kPacket;
+    const char* base;
+    uint32_t delta[kPackets];
+    bool there[kPackets];
+    // part: the head's elements in row 0; the run starts `first` elements into them.
+    __device__ __forceinline__ Gather(const T* part, int first, int count) {
+        there[0] = count > 0;
+        base = reinterpret_cast<const char*>(there[0] ? part + first : part);
+        delta[0] = 0;
+#pragma unroll
+        for (int i = 1; i < kPackets; ++i) {
+            there[i] = i * (kPacket / (int)sizeof(T)) < count;
+            delta[i] = there[i] ? i * kPacket : 0;
+        }
+    }
+    __device__ __forceinline__ void load(Run<T, N>& r, int row, uint32_t pitch) const {
+        const char* const at = base + static_cast<uint64_t>(static_cast<uint32_t>(row)) * pitch;
+        uint32_t* const w = reinterpret_cast<uint32_t*>(r.w);
+#pragma unroll
+        for (int i = 0; i < kPackets; ++i) {
+            const char* const p = at + delta[i];
+            if constexpr (kPacket == 16) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p);
+                w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+            } else if constexpr (kPacket == 8) {
+                const uint2 x = *reinterpret_cast<const uint2*>(p);
+                w[2 * i] = x.x, w[2 * i + 1] = x.y;
+            } else if constexpr (kPacket == 4) {
+                w[i] = *reinterpret_cast<const uint32_t*>(p);
+            } else {
+                const uint32_t x = *reinterpret_cast<const uint16_t*>(p);
+                w[i / 2] = i & 1 ? w[i / 2] | (x << 16) : x;
+            }
+        }
+    }
+    __device__ __forceinline__ void mask(Run<T, N>& r, bool live) const {
+        uint32_t* const w = reinterpret_cast<uint32_t*>(r.w);
+        if constexpr (kPacket == 2) {
+#pragma unroll
+            for (int i = 0; i < kPackets / 2; ++i) {
+                const uint32_t low = live && there[2 * i] ? 0xFFFFu : 0u, high = live && there[2 * i + 1] ? 0xFFFF0000u : 0u;
+                w[i] &= low | high;
+            }
+        } else {
+            constexpr int kWords = kPacket / 4;
+#pragma unroll
+            for (int i = 0; i < kPackets; ++i)
+#pragma unroll
+                for (int j = 0; j < kWords; ++j) w[kWords * i + j] = live && there[i] ? w[kWords * i + j] : 0u;
+        }
+    }
+};
+
+// Calls KERNEL<T, LM, NV, PB> for a layout.
+#define RA_ATTN_DISPATCH(KERNEL, dtype, l, grid, st, args)                                                  \
+    do {                                                                                                    \
+        auto by_type = [&](auto tag) {                                                                      \
+            using T = decltype(tag);                                                                        \
+            auto by_lm = [&](auto lm) {                                                                     \
+                constexpr int LM = decltype(lm)::value;                                                     \
+                if ((l).packet == 16) {                                                                     \
+                    if ((l).nv == 4) KERNEL<T, LM, 4, 16><<<grid, ra::kAttnThreads, 0, st>>>(args);         \
+                    else KERNEL<T, LM, 8, 16><<<grid, ra::kAttnThreads, 0, st>>>(args);                     \
+                } else if (sizeof(T) == 4 || (l).packet == 4) {                                             \
+                    KERNEL<T, LM, 8, 4><<<grid, ra::kAttnThreads, 0, st>>>(args);                           \
+                } else if constexpr (sizeof(T) == 2) {                                                      \
+                    KERNEL<T, LM, 8, 2><<<grid, ra::kAttnThreads, 0, st>>>(args);                           \
+                }                                                                                           \
+            };                                                                                              \
+            switch ((l).lm) {                                                                               \
+                case 1: by_lm(std::integral_constant<int, 1>()); break;                                     \
+                case 2: by_lm(std::integral_constant<int, 2>()); break;                                     \
+                case 4: by_lm(std::integral_constant<int, 4>()); break;                                     \
+                case 8: by_lm(std::integral_constant<int, 8>()); break;                                     \
+                default: by_lm(std::integral_constant<int, 16>());                                          \
+            }                                                                                               \
+        };                                                                                                  \
+        if ((dtype) == RA_DTYPE_F32) by_type(float());                                                      \
+        else if ((dtype) == RA_DTYPE_F16) by_type(ra::f16_t());                                             \
+        else by_type(ra::bf16_t());                                                                         \
     } while (0)
 
 }  // namespace ra

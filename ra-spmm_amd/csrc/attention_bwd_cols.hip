@@ -14,9 +14,7 @@
 namespace ra {
 namespace {
 
-constexpr int kDeep = 4;
-
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float* dk,
                                        const float* dv) {
     if (p.es != 0 || !p.live) return;
@@ -33,76 +31,73 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const P
         return;
     }
     const int64_t at = (int64_t)u.row * a.kv_heads + p.head;
-    store_run<T, 8, VEC>(static_cast<T*>(a.out) + (at * 2 + p.map) * a.head_dim + 8 * p.lm, dk, p.kcount);
-    store_run<T, NV, VEC>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, p.vcount);
+    store_run<T, 8, PB == 16>(static_cast<T*>(a.out) + (at * 2 + p.map) * a.head_dim + 8 * p.lm, dk, p.kcount);
+    store_run<T, NV, PB == 16>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, p.vcount);
 }
 
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.kv_heads);
-    float kf[8], vf[NV], dk[8], dv[NV];
-    {
-        Run<T, 8> r;
-        load_run<T, 8, VEC>(r, static_cast<const T*>(a.k) + u.row * a.ldk + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm,
-                            p.kcount);
-        r.to_float(kf);
-        Run<T, NV> g;
-        load_run<T, NV, VEC>(g, static_cast<const T*>(a.v) + u.row * a.ldv + (int64_t)p.head * a.value_dim + NV * p.l, p.vcount);
-        g.to_float(vf);
-    }
+    float dk[8], dv[NV];
+    Run<T, 8> k;
+    load_run<T, 8, PB == 16>(
+        k, static_cast<const T*>(a.k) + u.row * a.ldk + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
+    Run<T, NV> v;
+    load_run<T, NV, PB == 16>(v, static_cast<const T*>(a.v) + u.row * a.ldv + (int64_t)p.head * a.value_dim + NV * p.l,
+                              p.vcount);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dk[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) dv[i] = 0.f;
 
+    const int step_edges = kDeep * p.slots;
     for (int sub = 0; sub < a.group; ++sub) {
         const int qh = p.head * a.group + sub;
-        const T* const q = static_cast<const T*>(a.q) + (int64_t)(qh * 2 + p.map) * a.head_dim + 8 * p.lm;
-        const T* const g = static_cast<const T*>(a.grad) + (int64_t)qh * a.value_dim + NV * p.l;
+        const Gather<T, 8, PB> q(static_cast<const T*>(a.q) + (int64_t)(qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+        const Gather<T, NV, PB> g(static_cast<const T*>(a.grad) + (int64_t)qh * a.value_dim, NV * p.l, p.vcount);
         const float4* const rec = a.record + qh * 2 + p.map;
         const float c = p.map == 0 ? 1.f : -a.lam[qh];
-        for (int e0 = u.begin; e0 < u.end; e0 += kDeep * p.slots) {
+        Edges now, next;
+        if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, p.slots);
+        for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
             Run<T, 8> qr[kDeep];
             Run<T, NV> gr[kDeep];
             float4 st[kDeep];
-            float add[kDeep];
-            int row[kDeep];
+            const bool last = e0 + step_edges >= u.end;
 #pragma unroll
             for (int d = 0; d < kDeep; ++d) {
-                const int e = e0 + d * p.slots + p.es;
-                const bool in = e < u.end;
-                row[d] = in ? a.idx[e] : 0;
-                add[d] = in ? 0.f : -INFINITY;
-                if (a.bias && in) add[d] = a.bias[a.edge[e]];
+                st[d] = rec[static_cast<uint64_t>(static_cast<uint32_t>(now.other[d])) * static_cast<uint32_t>(a.q_heads * 2)];
+                q.load(qr[d], now.other[d], a.q_pitch);
+                g.load(gr[d], now.other[d], a.g_pitch);
+            }
+            if (!last) load_edges<true>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+            __builtin_amdgcn_sched_barrier(0);
+            if (last) close_edges(now, e0, u.end, p.es, p.slots);
+            if (last || a.ragged || a.bias) {
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d) {
+                    q.mask(qr[d], now.add[d] != -INFINITY);
+                    g.mask(gr[d], now.add[d] != -INFINITY);
+                }
             }
 #pragma unroll
             for (int d = 0; d < kDeep; ++d) {
-                const bool in = add[d] != -INFINITY;
-                load_run<T, 8, VEC>(qr[d], q + row[d] * a.ldq, in ? p.kcount : 0);
-                load_run<T, NV, VEC>(gr[d], g + (int64_t)row[d] * a.q_heads * a.value_dim, in ? p.vcount : 0);
-                st[d] = rec[(int64_t)row[d] * a.q_heads * 2];
-            }
-#pragma unroll
-            for (int d = 0; d < kDeep; ++d) {
-                float qf[8], gf[NV], t = 0.f, dp = 0.f;
+                const float t = lanes_sum<LM>(dot(k, qr[d])), dp = lanes_sum<2 * LM>(dot(v, gr[d]));
+                const bool live = now.add[d] != -INFINITY;
+                const float w = live ? c * exp_of(fmaf(t, a.scale, now.add[d]) - st[d].x) * st[d].y : 0.f;
+                const float ds = live ? w * (dp - st[d].z) : 0.f;
+                const float mix = w + other_map<LM>(w);
+                float qf[8], gf[NV];
                 qr[d].to_float(qf);
                 gr[d].to_float(gf);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t = fmaf(qf[i], kf[i], t);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) dp = fmaf(gf[i], vf[i], dp);
-                t = lanes_sum<LM>(t);
-                dp = lanes_sum<2 * LM>(dp);
-                const float w = add[d] == -INFINITY ? 0.f : c * exp_of(fmaf(t, a.scale, add[d]) - st[d].x) * st[d].y;
-                const float ds = add[d] == -INFINITY ? 0.f : w * (dp - st[d].z);
-                const float mix = w + other_map<LM>(w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) dk[i] = fmaf(ds, qf[i], dk[i]);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) dv[i] = fmaf(mix, gf[i], dv[i]);
             }
+            now = next;
         }
     }
     for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
@@ -113,7 +108,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) dk[i] *= a.scale;
-    finish<T, LM, NV, VEC>(a, u, p, dk, dv);
+    finish<T, LM, NV, PB>(a, u, p, dk, dv);
 }
 
 // Joins a cut column's pieces: plain sums of every element, in order.  Threads are
@@ -141,10 +136,10 @@ __global__ __launch_bounds__(256) void attn_cols_join(const AttnArgs a, const in
 }  // namespace
 
 ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    const int64_t blocks = (a.num_units + kAttnThreads / 64 - 1) / (kAttnThreads / 64);
+    unsigned blocks = 0;
+    RA_TRY(attn_grid(a, blocks));
     if (blocks == 0) return RA_OK;
-    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    RA_ATTN_DISPATCH(attn_cols, dtype, l, dim3((unsigned)blocks), st, a);
+    RA_ATTN_DISPATCH(attn_cols, dtype, l, dim3(blocks), st, a);
     RA_LAUNCH_CHECK("attn_cols");
     return RA_OK;
 }

@@ -14,10 +14,8 @@
 namespace ra {
 namespace {
 
-constexpr int kDeep = 4;
-
 // Map's gradient of q and its record.
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float delta,
                                        const float* pdk, const float* pk, float m, float il) {
     if (p.es != 0 || !p.live) return;
@@ -38,75 +36,68 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const P
 #pragma unroll
     for (int i = 0; i < 8; ++i) dq[i] = c * (pdk[i] - delta * pk[i]);
     const int64_t at = ((int64_t)u.row * a.q_heads + p.head) * 2 + p.map;
-    store_run<T, 8, VEC>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, p.kcount);
+    store_run<T, 8, PB == 16>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, p.kcount);
     if (p.lm == 0) a.record[at] = make_float4(m, il, delta, 0.f);
 }
 
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);
     const int kv = p.head / a.group;
-    const T* const k = static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim + 8 * p.lm;
-    const T* const v = static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim + NV * p.l;
+    const Gather<T, 8, PB> k(static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+    const Gather<T, NV, PB> v(static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim, NV * p.l, p.vcount);
 
-    float qf[8], gf[NV];
-    {
-        Run<T, 8> r;
-        load_run<T, 8, VEC>(r, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm,
-                            p.kcount);
-        r.to_float(qf);
-        Run<T, NV> g;
-        load_run<T, NV, VEC>(g, static_cast<const T*>(a.grad) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l,
-                             p.vcount);
-        g.to_float(gf);
-    }
+    Run<T, 8> q;
+    load_run<T, 8, PB == 16>(
+        q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
+    Run<T, NV> g;
+    load_run<T, NV, PB == 16>(
+        g, static_cast<const T*>(a.grad) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, p.vcount);
     const float2 st = reinterpret_cast<const float2*>(a.stats)[((int64_t)u.row * a.q_heads + p.head) * 2 + p.map];
     float delta = 0.f, pdk[8], pk[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) pdk[i] = pk[i] = 0.f;
 
-    for (int e0 = u.begin; e0 < u.end; e0 += kDeep * p.slots) {
+    Edges now, next;
+    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, p.slots);
+    const int step_edges = kDeep * p.slots;
+    for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
         Run<T, 8> kr[kDeep];
         Run<T, NV> vr[kDeep];
-        float add[kDeep];
-        int col[kDeep];
+        const bool last = e0 + step_edges >= u.end;
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const int e = e0 + d * p.slots + p.es;
-            const bool in = e < u.end;
-            col[d] = in ? a.idx[e] : 0;
-            add[d] = in ? 0.f : -INFINITY;
-            if (a.bias && in) add[d] = a.bias[e];
+            k.load(kr[d], now.other[d], a.k_pitch);
+            v.load(vr[d], now.other[d], a.v_pitch);
+        }
+        if (!last) load_edges<false>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last) close_edges(now, e0, u.end, p.es, p.slots);
+        if (last || a.ragged || a.bias) {
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                k.mask(kr[d], now.add[d] != -INFINITY);
+                v.mask(vr[d], now.add[d] != -INFINITY);
+            }
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const bool in = add[d] != -INFINITY;
-            load_run<T, 8, VEC>(kr[d], k + col[d] * a.ldk, in ? p.kcount : 0);
-            load_run<T, NV, VEC>(vr[d], v + col[d] * a.ldv, in ? p.vcount : 0);
-        }
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            float kf[8], vf[NV], t = 0.f, dp = 0.f;
-            kr[d].to_float(kf);
-            vr[d].to_float(vf);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t = fmaf(qf[i], kf[i], t);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) dp = fmaf(gf[i], vf[i], dp);
-            t = lanes_sum<LM>(t);
-            dp = lanes_sum<2 * LM>(dp);
-            const bool live = add[d] != -INFINITY;
-            const float w = live ? exp_of(fmaf(t, a.scale, add[d]) - st.x) * st.y : 0.f;
+            const float t = lanes_sum<LM>(dot(q, kr[d])), dp = lanes_sum<2 * LM>(dot(g, vr[d]));
+            const bool live = now.add[d] != -INFINITY;
+            const float w = live ? exp_of(fmaf(t, a.scale, now.add[d]) - st.x) * st.y : 0.f;
             const float wd = live ? w * dp : 0.f;
             delta += wd;
+            float kf[8];
+            kr[d].to_float(kf);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 pdk[i] = fmaf(wd, kf[i], pdk[i]);
                 pk[i] = fmaf(w, kf[i], pk[i]);
             }
         }
+        now = next;
     }
     for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
         delta += __shfl_xor(delta, step, 64);
@@ -116,7 +107,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
             pk[i] += __shfl_xor(pk[i], step, 64);
         }
     }
-    finish<T, LM, NV, VEC>(a, u, p, delta, pdk, pk, st.x, st.y);
+    finish<T, LM, NV, PB>(a, u, p, delta, pdk, pk, st.x, st.y);
 }
 
 // Joins a cut row's pieces: a workgroup per (row, head).  Threads are piece groups x
@@ -192,10 +183,10 @@ __global__ __launch_bounds__(64) void attn_lam_final(const float* __restrict__ p
 }  // namespace
 
 ra_status attn_rows_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    const int64_t blocks = (a.num_units + kAttnThreads / 64 - 1) / (kAttnThreads / 64);
+    unsigned blocks = 0;
+    RA_TRY(attn_grid(a, blocks));
     if (blocks == 0) return RA_OK;
-    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    RA_ATTN_DISPATCH(attn_rows, dtype, l, dim3((unsigned)blocks), st, a);
+    RA_ATTN_DISPATCH(attn_rows, dtype, l, dim3(blocks), st, a);
     RA_LAUNCH_CHECK("attn_rows");
     return RA_OK;
 }

@@ -14,8 +14,6 @@
 namespace ra {
 namespace {
 
-constexpr int kDeep = 4;  // edges in flight per slot
-
 // Softmax state of a (slot, head): of the lane's own map, and v sums of both.
 template <int NV>
 struct State {
@@ -25,7 +23,7 @@ struct State {
 
 // Writes a finished row, or a piece's state to its slot:
 // [heads][2 maps][max, sum], then [heads][2 maps][value_dim].
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, const State<NV>& s) {
     if (p.es != 0 || !p.live) return;
     if (u.slot >= 0) {
@@ -53,64 +51,58 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const P
     // No edge left: zeros, whatever lam is.
 #pragma unroll
     for (int i = 0; i < NV; ++i) o[i] = s.l == 0.f ? 0.f : s.own[i] * w + s.other[i] * wx;
-    store_run<T, NV, VEC>(static_cast<T*>(a.out) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, o,
+    store_run<T, NV, PB == 16>(static_cast<T*>(a.out) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, o,
                           p.vcount);
     if (a.stats && p.lm == 0)
         reinterpret_cast<float2*>(a.stats)[((int64_t)u.row * a.q_heads + p.head) * 2 + p.map] =
             make_float2(s.m == -INFINITY ? 0.f : s.m, il);
 }
 
-template <typename T, int LM, int NV, bool VEC>
+template <typename T, int LM, int NV, int PB>
 __global__ __launch_bounds__(kAttnThreads) void attn_forward(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);
     const int kv = p.head / a.group;
-    const T* const q = static_cast<const T*>(a.q);
-    const T* const k = static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim + 8 * p.lm;
-    const T* const v = static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim + NV * p.l;
+    const Gather<T, 8, PB> k(static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+    const Gather<T, NV, PB> v(static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim, NV * p.l, p.vcount);
 
-    float qf[8];
-    {
-        Run<T, 8> r;
-        load_run<T, 8, VEC>(r, q + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
-        r.to_float(qf);
-    }
+    Run<T, 8> q;
+    load_run<T, 8, PB == 16>(
+        q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
     State<NV> s;
     s.m = -INFINITY;
     s.l = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) s.own[i] = s.other[i] = 0.f;
 
-    for (int e0 = u.begin; e0 < u.end; e0 += kDeep * p.slots) {
+    Edges now, next;
+    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, p.slots);
+    const int step_edges = kDeep * p.slots;
+    for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
         Run<T, 8> kr[kDeep];
         Run<T, NV> vr[kDeep];
-        float add[kDeep];
-        int col[kDeep];
+        const bool last = e0 + step_edges >= u.end;
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const int e = e0 + d * p.slots + p.es;
-            const bool in = e < u.end;
-            col[d] = in ? a.idx[e] : 0;
-            add[d] = in ? 0.f : -INFINITY;
-            if (a.bias && in) add[d] = a.bias[e];
+            k.load(kr[d], now.other[d], a.k_pitch);
+            v.load(vr[d], now.other[d], a.v_pitch);
         }
+        if (!last) load_edges<false>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last) close_edges(now, e0, u.end, p.es, p.slots);
+        if (last || a.ragged || a.bias) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const bool in = add[d] != -INFINITY;
-            load_run<T, 8, VEC>(kr[d], k + col[d] * a.ldk, in ? p.kcount : 0);
-            load_run<T, NV, VEC>(vr[d], v + col[d] * a.ldv, in ? p.vcount : 0);
+            for (int d = 0; d < kDeep; ++d) {
+                k.mask(kr[d], now.add[d] != -INFINITY);
+                v.mask(vr[d], now.add[d] != -INFINITY);
+            }
         }
         float score[kDeep], top = s.m;
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            float kf[8], t = 0.f;
-            kr[d].to_float(kf);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t = fmaf(qf[i], kf[i], t);
-            t = lanes_sum<LM>(t);
-            score[d] = fmaf(t, a.scale, add[d]);
-            if (add[d] == -INFINITY) score[d] = -INFINITY;
+            score[d] = fmaf(lanes_sum<LM>(dot(q, kr[d])), a.scale, now.add[d]);
+            if (now.add[d] == -INFINITY) score[d] = -INFINITY;
             top = score[d] > top || score[d] != score[d] ? score[d] : top;  // a NaN stays
         }
         // All edges so far left out: every weight is 0, not exp(-inf + inf).
@@ -135,6 +127,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward(const AttnArgs a) {
                 s.other[i] = fmaf(wx, vf[i], s.other[i]);
             }
         }
+        now = next;
     }
     for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
         const float m2 = __shfl_xor(s.m, step, 64);
@@ -150,7 +143,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward(const AttnArgs a) {
         }
         s.m = top;
     }
-    finish<T, LM, NV, VEC>(a, u, p, s);
+    finish<T, LM, NV, PB>(a, u, p, s);
 }
 
 // Joins the pieces of a cut row: a workgroup per (row, head).  Its threads are
@@ -241,10 +234,10 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
 }  // namespace
 
 ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    const int64_t blocks = (a.num_units + kAttnThreads / 64 - 1) / (kAttnThreads / 64);
+    unsigned blocks = 0;
+    RA_TRY(attn_grid(a, blocks));
     if (blocks == 0) return RA_OK;
-    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    RA_ATTN_DISPATCH(attn_forward, dtype, l, dim3((unsigned)blocks), st, a);
+    RA_ATTN_DISPATCH(attn_forward, dtype, l, dim3(blocks), st, a);
     RA_LAUNCH_CHECK("attn_forward");
     return RA_OK;
 }

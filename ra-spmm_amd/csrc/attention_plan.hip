@@ -258,6 +258,12 @@ AttnArgs args_of(const ra_attn_shape& s, const AttnLayout& l) {
     a.ldq = s.ldq;
     a.ldk = s.ldk;
     a.ldv = s.ldv;
+    const uint32_t size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
+    a.q_pitch = static_cast<uint32_t>(s.ldq) * size;
+    a.k_pitch = static_cast<uint32_t>(s.ldk) * size;
+    a.v_pitch = static_cast<uint32_t>(s.ldv) * size;
+    a.g_pitch = static_cast<uint32_t>(s.q_heads * s.value_dim) * size;
+    a.ragged = l.ragged;
     a.head_blocks = l.head_blocks;
     a.hb_shift = l.hb_shift;
     a.pieces = 1;
@@ -297,13 +303,16 @@ AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p) {
     while (l.lm * 8 < s.head_dim || l.lm * 16 < s.value_dim) l.lm *= 2;
     l.nv = s.value_dim <= 8 * l.lm ? 4 : 8;
     const int64_t size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
-    const int64_t key = 16, value = std::min<int64_t>(16, l.nv * size);  // bytes of a packet
-    auto whole = [](const void* ptr, int64_t ld_bytes, int64_t run_bytes, int64_t packet) {
-        return reinterpret_cast<uintptr_t>(ptr) % packet == 0 && ld_bytes % packet == 0 && run_bytes % packet == 0;
+    // Whole packets: every matrix' address, pitch and head width are multiples of them.
+    auto whole = [&](int64_t key, int64_t value) {
+        auto fits = [](const void* ptr, int64_t pitch, int64_t run, int64_t packet) {
+            return reinterpret_cast<uintptr_t>(ptr) % packet == 0 && pitch % packet == 0 && run % packet == 0;
+        };
+        return fits(p.q, p.ldq * size, s.head_dim * size, key) && fits(p.k, p.ldk * size, s.head_dim * size, key) &&
+               fits(p.v, p.ldv * size, s.value_dim * size, value) && fits(p.grad, p.ldg * size, s.value_dim * size, value);
     };
-    l.vec = whole(p.q, p.ldq * size, s.head_dim * size, key) && whole(p.k, p.ldk * size, s.head_dim * size, key) &&
-            whole(p.v, p.ldv * size, s.value_dim * size, value) && whole(p.grad, p.ldg * size, s.value_dim * size, value);
-    if (!l.vec) l.nv = 8;
+    l.packet = whole(16, std::min<int64_t>(16, l.nv * size)) ? 16 : whole(4, 4) ? 4 : 2;
+    if (l.packet != 16) l.nv = 8;
     // Heads of a wave: as many as leave the fewest lanes without a head.
     const int most = log2_up(32 / l.lm);
     int best = 0;
@@ -317,6 +326,7 @@ AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p) {
     }
     l.hb_shift = best;
     l.head_blocks = (heads + (1 << best) - 1) >> best;
+    l.ragged = s.head_dim != 8 * l.lm || s.value_dim != 2 * l.lm * l.nv || heads != l.head_blocks << best;
     return l;
 }
 
@@ -329,6 +339,8 @@ ra_status attn_check(const ra_attn_shape* s, int32_t M, int32_t K) {
     if (s->head_dim < 1 || s->value_dim < 1) return fail(RA_ERR_INVALID_ARGUMENT, "attention: empty heads");
     if (s->head_dim > 128 || s->value_dim > 256 || s->q_heads > 1024)
         return fail(RA_ERR_UNSUPPORTED, "attention: head_dim is at most 128, value_dim at most 256, q_heads at most 1024");
+    if (std::max({s->ldq, s->ldk, s->ldv}) >= int64_t{1} << 30)
+        return fail(RA_ERR_UNSUPPORTED, "attention: rows lie at most 2^30 elements apart");
     if ((M > 0 && s->ldq < (int64_t)s->q_heads * 2 * s->head_dim) ||
         (K > 0 && (s->ldk < (int64_t)s->kv_heads * 2 * s->head_dim || s->ldv < (int64_t)s->kv_heads * s->value_dim)))
         return fail(RA_ERR_INVALID_ARGUMENT, "attention: rows overlap (a leading dimension is too small)");
@@ -482,6 +494,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
         l = ra::attn_layout(s, s.kv_heads, ptrs);
         a.head_blocks = l.head_blocks;
         a.hb_shift = l.hb_shift;
+        a.ragged = l.ragged;
         ra::side_of(a, cols);
         a.out = d_dk;
         a.out2 = d_dv;
