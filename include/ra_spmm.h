@@ -422,8 +422,8 @@ ra_status ra_attn_plan_get_info(const ra_attn_plan* plan, ra_attn_info* info);
  * 0), "rowptr_t", "row_t", "edge_t".  dst may be NULL to query *count (int32s). */
 ra_status ra_attn_plan_export(const ra_attn_plan* plan, const char* name, int32_t* dst, int64_t* count);
 void ra_attn_plan_destroy(ra_attn_plan* plan);
-/* d_stats: [M, q_heads, 2, 2] fp32 (maximum and 1/sum of every softmax, what the
- * backward pass needs), or NULL.  Grows the plan's scratch at the first call of a
+/* d_stats: [M, q_heads, 2, 2] fp32, what the backward pass needs (maximum in powers
+ * of two and 1/sum of every softmax), or NULL.  Grows the plan's scratch at the first call of a
  * larger shape. */
 ra_status ra_attn_plan_run(ra_attn_plan* plan, const ra_attn_shape* shape, const void* d_q, const void* d_k,
                            const void* d_v, const float* d_lam, const float* d_bias, void* d_out, float* d_stats,

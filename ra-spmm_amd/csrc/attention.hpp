@@ -2,6 +2,8 @@
 // arguments, the lanes' layout and the row loads.
 #pragma once
 
+#include <type_traits>
+
 #include "ra_internal.hpp"
 #include "vector_run.hpp"
 
@@ -47,14 +49,15 @@ struct AttnArgs {
     int32_t hb_shift;     // log2 of the heads of a wave
     int32_t q_heads, kv_heads, group, head_dim, value_dim;
     int32_t rows;
-    float scale;
+    float scale, scale2;  // scale2 = scale * log2(e): scores are held in powers of two
     int64_t ldq, ldk, ldv;
     uint32_t q_pitch, k_pitch, v_pitch, g_pitch;  // bytes between rows
     bool ragged;          // some lane's run is not whole: loaded words are masked
+    bool wide;            // gathered offsets need 64 bits
     const void *q, *k, *v, *grad;
     const float *lam, *bias;
-    float* stats;    // [rows, q_heads, 2] (max, 1 / sum)
-    float4* record;  // [rows, q_heads, 2] (max, 1 / sum, sum p dp, 0)
+    float* stats;    // [rows, q_heads, 2] (max in powers of two, 1 / sum)
+    float4* record;  // [rows, q_heads, 2] (the same, sum p dp, 0)
     void *out, *out2;
     float* partial;
 };
@@ -104,31 +107,155 @@ ra_status attn_lam_launch(const float4* record, int32_t rows, int32_t q_heads, f
 // ------------------------------------------------------------- device side
 constexpr int kAttnThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBiasMost = 2e38f;
+
+// Lane moves.  Within a row of 16 lanes by data-parallel moves, between rows and
+// halves by the swaps of two registers' rows and halves.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kRotate = 0x120;
+
+struct Pair {
+    float a, b;
+};
+// (x of the even rows, y of the even rows), (x of the odd rows, y of the odd rows).
+__device__ __forceinline__ Pair swap_rows(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+// The same of the lower and the upper half.
+__device__ __forceinline__ Pair swap_halves(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
 
 // Sum over runs of W lanes (a power of two): every lane gets it.
 template <int W>
 __device__ __forceinline__ float lanes_sum(float x) {
-    // Within 16 lanes by data-parallel moves (quad permutes and row mirrors), the
-    // rest through the shuffle network.
-    if constexpr (W >= 2) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));
-    if constexpr (W >= 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));
-    if constexpr (W >= 8) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));
-    if constexpr (W >= 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));
-    if constexpr (W >= 32) x += __shfl_xor(x, 16, 64);
+    if constexpr (W >= 2) x += dpp<kXor1>(x);
+    if constexpr (W >= 4) x += dpp<kXor2>(x);
+    if constexpr (W >= 8) x += dpp<kHalfMirror>(x);
+    if constexpr (W >= 16) x += dpp<kMirror>(x);
+    if constexpr (W >= 32) {
+        const Pair p = swap_rows(x, x);
+        x = p.a + p.b;
+    }
     return x;
 }
 // The value of the lane LM away (the other map's), where all lanes of a map hold
 // the same value.
 template <int LM>
 __device__ __forceinline__ float other_map(float x) {
-    if constexpr (LM == 1) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));
-    if constexpr (LM == 2) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));
-    if constexpr (LM == 4) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));
-    if constexpr (LM == 8) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));
-    return __shfl_xor(x, LM, 64);
+    if constexpr (LM == 1) return dpp<kXor1>(x);
+    if constexpr (LM == 2) return dpp<kXor2>(x);
+    if constexpr (LM == 4) return dpp<kHalfMirror>(x);
+    if constexpr (LM == 8) return dpp<kMirror>(x);
+    const Pair p = swap_rows(x, x);
+    return threadIdx.x & 16 ? p.a : p.b;
+}
+// Over the edge slots, which lie 64 / slots lanes apart: every lane gets it.
+template <typename F>
+__device__ __forceinline__ float over_slots(float x, int slots, F f) {
+    if (slots >= 8) x = f(x, dpp<kRotate + 8>(x));
+    if (slots >= 16) x = f(x, dpp<kRotate + 4>(x));
+    if (slots >= 32) x = f(x, dpp<kRotate + 2>(x));
+    if (slots >= 4) {
+        const Pair p = swap_rows(x, x);
+        x = f(p.a, p.b);
+    }
+    if (slots >= 2) {
+        const Pair p = swap_halves(x, x);
+        x = f(p.a, p.b);
+    }
+    return x;
+}
+__device__ __forceinline__ float slots_sum(float x, int slots) {
+    return over_slots(x, slots, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float slots_max(float x, int slots) {
+    return over_slots(x, slots, [](float a, float b) { return fmaxf(a, b); });
 }
 
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// Sums of N values over the edge slots.  With two slots a lane ends with half of
+// them, with more with a quarter, starting at scattered_first(): x[0 ..].
+template <int N>
+__device__ __forceinline__ void scatter_sum(float* x, int slots) {
+    if (slots >= 8) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += dpp<kRotate + 8>(x[i]);
+    }
+    if (slots >= 16) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += dpp<kRotate + 4>(x[i]);
+    }
+    if (slots >= 32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += dpp<kRotate + 2>(x[i]);
+    }
+    if (slots >= 2) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const Pair p = swap_halves(x[i], x[i + N / 2]);
+            x[i] = p.a + p.b;
+        }
+    }
+    if (slots >= 4) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const Pair p = swap_rows(x[i], x[i + N / 4]);
+            x[i] = p.a + p.b;
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ int scattered_first(int slots) {
+    const int lane = threadIdx.x & 63;
+    return (slots >= 2 && lane & 32 ? N / 2 : 0) + (slots >= 4 && lane & 16 ? N / 4 : 0);
+}
+// Of the lanes that hold the same sums, the one that stores them.
+__device__ __forceinline__ bool scattered_stores(int slots) {
+    return slots <= 4 || (int)(threadIdx.x & 15) < 64 / slots;
+}
+// Stores what scatter_sum left, of a run at p of which `count` elements exist.
+// WHOLE: the run is whole packets.
+template <typename T, int N, bool WHOLE>
+__device__ __forceinline__ void store_scattered(T* p, const float* sums, int slots, int count) {
+    // In a vector: the compiler would merge the branches' stores into one of a
+    // variable element and move the array to LDS.
+    typedef float values __attribute__((ext_vector_type(N)));
+    values x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = sums[i];
+    if (!scattered_stores(slots)) return;
+    const int first = scattered_first<N>(slots);
+    auto put = [&](auto n) {
+        constexpr int kN = decltype(n)::value;
+        if constexpr (WHOLE) {
+            if (first >= count) return;
+            constexpr int kMost = (int)(16 / sizeof(T)) < kN ? (int)(16 / sizeof(T)) : kN;
+            typedef T part __attribute__((ext_vector_type(kMost)));
+#pragma unroll
+            for (int j = 0; j < kN / kMost; ++j) {
+                if (first + j * kMost >= count) break;
+                part v;
+#pragma unroll
+                for (int i = 0; i < kMost; ++i) v[i] = (T)x[j * kMost + i];
+                *reinterpret_cast<part*>(p + first + j * kMost) = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (first + i < count) p[first + i] = (T)x[i];
+        }
+    };
+    if (slots == 1) put(std::integral_constant<int, N>());
+    else if (slots == 2) put(std::integral_constant<int, N / 2>());
+    else put(std::integral_constant<int, N / 4>());
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Piece and heads of a wave.
 struct Unit {
@@ -195,20 +322,16 @@ struct Place {
 // (the scheduler would otherwise wait for each in turn to save registers).
 constexpr int kDeep = 4;
 
-// The next kDeep edges of every slot.  Past the end the last edge again, not live.
+// The next kDeep edges of every slot.  Past the end the last edge again.
 struct Edges {
-    int other[kDeep];
-    float add[kDeep];
+    uint32_t other[kDeep];
+    float add[kDeep];  // bias in powers of two, where there is one
 };
 
 template <bool TRANSPOSED>
 __device__ __forceinline__ void load_edges(const AttnArgs& a, Edges& x, int e0, int end, int es, int slots) {
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
-        const int e = min(e0 + d * slots + es, end - 1);
-        x.other[d] = a.idx[e];
-        x.add[d] = 0.f;
-    }
+    for (int d = 0; d < kDeep; ++d) x.other[d] = a.idx[min(e0 + d * slots + es, end - 1)];
     if (a.bias) {
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
@@ -217,11 +340,37 @@ __device__ __forceinline__ void load_edges(const AttnArgs& a, Edges& x, int e0, 
         }
     }
 }
-// Edges past the end, and left out by their bias, get -inf.
-__device__ __forceinline__ void close_edges(Edges& x, int e0, int end, int es, int slots) {
+// Live edges of a step: in the list (a LAST step only may pass its end), and not
+// left out by their bias, which becomes powers of two here.  A finite bias is kept
+// finite: beyond +-2e38 all are equal.
+template <int DEEP, bool LAST>
+__device__ __forceinline__ void close_edges(const AttnArgs& a, Edges& x, bool* live, int e0, int end, int es, int slots) {
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d)
-        if (e0 + d * slots + es >= end) x.add[d] = -INFINITY;
+    for (int d = 0; d < DEEP; ++d) {
+        live[d] = !LAST || e0 + d * slots + es < end;
+        if (!a.bias) x.add[d] = 0.f;
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const float b = x.add[d];
+            live[d] = live[d] && b != -INFINITY;
+            x.add[d] = (b < -kBiasMost ? -kBiasMost : b > kBiasMost ? kBiasMost : b) * kLog2e;
+        }
+    }
+}
+
+// Runs step(DEEP, LAST, first edge) over a wave's edges: whole steps of kDeep edges a
+// slot, then one of as few as hold the rest.  Straight-line bodies: conditions on
+// single edges would have each load waited for on its own.
+template <typename F>
+__device__ __forceinline__ void over_edges(int begin, int end, int slots, F step) {
+    if (begin >= end) return;
+    int e0 = begin;
+    for (; end - e0 > kDeep * slots; e0 += kDeep * slots) step(std::integral_constant<int, kDeep>(), std::false_type(), e0);
+    if (end - e0 <= slots) step(std::integral_constant<int, 1>(), std::true_type(), e0);
+    else if (end - e0 <= 2 * slots) step(std::integral_constant<int, 2>(), std::true_type(), e0);
+    else step(std::integral_constant<int, kDeep>(), std::true_type(), e0);
 }
 
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, f16_t) {
@@ -248,18 +397,23 @@ __device__ __forceinline__ float dot(const Run<T, N>& a, const Run<T, N>& b) {
 
 // A lane's run in the rows of a gathered matrix, in packets of PB bytes.  Packets
 // that do not exist are loaded from the start of the row's part instead, and masked.
-template <typename T, int N, int PB>
+// WIDE: offsets of 64 bits; else of 32, from 24-bit factors (one full-rate
+// instruction, and half of the address registers).
+template <typename T, int N, int PB, bool WIDE>
 struct Gather {
     static constexpr int kBytes = N * (int)sizeof(T);
     static constexpr int kPacket = PB < kBytes ? PB : kBytes;
     static constexpr int kPackets = kBytes / kPacket;
-    const char* base;
+    const char* base;  // of the matrix
+    uint32_t offset;   // of the run in row 0
     uint32_t delta[kPackets];
     bool there[kPackets];
-    // part: the head's elements in row 0; the run starts `first` elements into them.
-    __device__ __forceinline__ Gather(const T* part, int first, int count) {
+    // part: first element of the head's part of a row; the run starts `first`
+    // elements into it.
+    __device__ __forceinline__ Gather(const void* matrix, int part, int first, int count) {
         there[0] = count > 0;
-        base = reinterpret_cast<const char*>(there[0] ? part + first : part);
+        base = static_cast<const char*>(matrix);
+        offset = static_cast<uint32_t>(there[0] ? part + first : part) * sizeof(T);
         delta[0] = 0;
 #pragma unroll
         for (int i = 1; i < kPackets; ++i) {
@@ -267,12 +421,13 @@ struct Gather {
             delta[i] = there[i] ? i * kPacket : 0;
         }
     }
-    __device__ __forceinline__ void load(Run<T, N>& r, int row, uint32_t pitch) const {
-        const char* const at = base + static_cast<uint64_t>(static_cast<uint32_t>(row)) * pitch;
+    __device__ __forceinline__ void load(Run<T, N>& r, uint32_t row, uint32_t pitch) const {
         uint32_t* const w = reinterpret_cast<uint32_t*>(r.w);
 #pragma unroll
         for (int i = 0; i < kPackets; ++i) {
-            const char* const p = at + delta[i];
+            const char* p;
+            if constexpr (WIDE) p = base + (static_cast<uint64_t>(row) * pitch + (offset + delta[i]));
+            else p = base + (__umul24(row, pitch) + (offset + delta[i]));
             if constexpr (kPacket == 16) {
                 const uint4 x = *reinterpret_cast<const uint4*>(p);
                 w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
@@ -305,20 +460,23 @@ struct Gather {
     }
 };
 
-// Calls KERNEL<T, LM, NV, PB> for a layout.
+// Calls KERNEL<T, LM, NV, PB, WIDE> for a layout.
 #define RA_ATTN_DISPATCH(KERNEL, dtype, l, grid, st, args)                                                  \
     do {                                                                                                    \
         auto by_type = [&](auto tag) {                                                                      \
             using T = decltype(tag);                                                                        \
             auto by_lm = [&](auto lm) {                                                                     \
                 constexpr int LM = decltype(lm)::value;                                                     \
-                if ((l).packet == 16) {                                                                     \
-                    if ((l).nv == 4) KERNEL<T, LM, 4, 16><<<grid, ra::kAttnThreads, 0, st>>>(args);         \
-                    else KERNEL<T, LM, 8, 16><<<grid, ra::kAttnThreads, 0, st>>>(args);                     \
+                if ((l).packet == 16 && !(args).wide) {                                                     \
+                    if ((l).nv == 4) KERNEL<T, LM, 4, 16, false><<<grid, ra::kAttnThreads, 0, st>>>(args);  \
+                    else KERNEL<T, LM, 8, 16, false><<<grid, ra::kAttnThreads, 0, st>>>(args);              \
+                } else if ((l).packet == 16) {                                                              \
+                    if ((l).nv == 4) KERNEL<T, LM, 4, 16, true><<<grid, ra::kAttnThreads, 0, st>>>(args);   \
+                    else KERNEL<T, LM, 8, 16, true><<<grid, ra::kAttnThreads, 0, st>>>(args);               \
                 } else if (sizeof(T) == 4 || (l).packet == 4) {                                             \
-                    KERNEL<T, LM, 8, 4><<<grid, ra::kAttnThreads, 0, st>>>(args);                           \
+                    KERNEL<T, LM, 8, 4, true><<<grid, ra::kAttnThreads, 0, st>>>(args);                     \
                 } else if constexpr (sizeof(T) == 2) {                                                      \
-                    KERNEL<T, LM, 8, 2><<<grid, ra::kAttnThreads, 0, st>>>(args);                           \
+                    KERNEL<T, LM, 8, 2, true><<<grid, ra::kAttnThreads, 0, st>>>(args);                     \
                 }                                                                                           \
             };                                                                                              \
             switch ((l).lm) {                                                                               \

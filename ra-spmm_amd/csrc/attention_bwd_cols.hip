@@ -14,32 +14,12 @@
 namespace ra {
 namespace {
 
-template <typename T, int LM, int NV, int PB>
-__device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float* dk,
-                                       const float* dv) {
-    if (p.es != 0 || !p.live) return;
-    if (u.slot >= 0) {  // [heads][2 maps][head_dim], then [heads][value_dim]
-        float* base = a.partial + (int64_t)u.slot * a.kv_heads * (2 * a.head_dim + a.value_dim);
-        float* to = base + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < p.kcount) to[i] = dk[i];
-        to = base + (int64_t)a.kv_heads * 2 * a.head_dim + (int64_t)p.head * a.value_dim + NV * p.l;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < p.vcount) to[i] = dv[i];
-        return;
-    }
-    const int64_t at = (int64_t)u.row * a.kv_heads + p.head;
-    store_run<T, 8, PB == 16>(static_cast<T*>(a.out) + (at * 2 + p.map) * a.head_dim + 8 * p.lm, dk, p.kcount);
-    store_run<T, NV, PB == 16>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, p.vcount);
-}
-
-template <typename T, int LM, int NV, int PB>
+template <typename T, int LM, int NV, int PB, bool WIDE>
 __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.kv_heads);
+    const int slots = p.slots;
     float dk[8], dv[NV];
     Run<T, 8> k;
     load_run<T, 8, PB == 16>(
@@ -52,42 +32,44 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) dv[i] = 0.f;
 
-    const int step_edges = kDeep * p.slots;
+    const uint32_t record_pitch = a.q_heads * 2 * sizeof(float4);
     for (int sub = 0; sub < a.group; ++sub) {
         const int qh = p.head * a.group + sub;
-        const Gather<T, 8, PB> q(static_cast<const T*>(a.q) + (int64_t)(qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
-        const Gather<T, NV, PB> g(static_cast<const T*>(a.grad) + (int64_t)qh * a.value_dim, NV * p.l, p.vcount);
-        const float4* const rec = a.record + qh * 2 + p.map;
+        const Gather<T, 8, PB, WIDE> q(a.q, (qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+        const Gather<T, NV, PB, WIDE> g(a.grad, qh * a.value_dim, NV * p.l, p.vcount);
+        const Gather<float, 4, 16, WIDE> rec(a.record, (qh * 2 + p.map) * 4, 0, 4);
         const float c = p.map == 0 ? 1.f : -a.lam[qh];
         Edges now, next;
-        if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, p.slots);
-        for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
-            Run<T, 8> qr[kDeep];
-            Run<T, NV> gr[kDeep];
-            float4 st[kDeep];
-            const bool last = e0 + step_edges >= u.end;
+        if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, slots);
+        over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
+            constexpr int DEEP = decltype(deep)::value;
+            constexpr bool LAST = decltype(is_last)::value;
+            Run<T, 8> qr[DEEP];
+            Run<T, NV> gr[DEEP];
+            Run<float, 4> st[DEEP];  // maximum, 1 / sum, delta
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d) {
-                st[d] = rec[static_cast<uint64_t>(static_cast<uint32_t>(now.other[d])) * static_cast<uint32_t>(a.q_heads * 2)];
+            for (int d = 0; d < DEEP; ++d) {
                 q.load(qr[d], now.other[d], a.q_pitch);
                 g.load(gr[d], now.other[d], a.g_pitch);
+                rec.load(st[d], now.other[d], record_pitch);
             }
-            if (!last) load_edges<true>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+            if constexpr (!LAST) load_edges<true>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
             __builtin_amdgcn_sched_barrier(0);
-            if (last) close_edges(now, e0, u.end, p.es, p.slots);
-            if (last || a.ragged || a.bias) {
+            bool live[DEEP];
+            close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
+            if (LAST || a.ragged || a.bias) {
 #pragma unroll
-                for (int d = 0; d < kDeep; ++d) {
-                    q.mask(qr[d], now.add[d] != -INFINITY);
-                    g.mask(gr[d], now.add[d] != -INFINITY);
+                for (int d = 0; d < DEEP; ++d) {
+                    q.mask(qr[d], live[d]);
+                    g.mask(gr[d], live[d]);
                 }
             }
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d) {
+            for (int d = 0; d < DEEP; ++d) {
                 const float t = lanes_sum<LM>(dot(k, qr[d])), dp = lanes_sum<2 * LM>(dot(v, gr[d]));
-                const bool live = now.add[d] != -INFINITY;
-                const float w = live ? c * exp_of(fmaf(t, a.scale, now.add[d]) - st[d].x) * st[d].y : 0.f;
-                const float ds = live ? w * (dp - st[d].z) : 0.f;
+                float w = c * exp2_of(fmaf(t, a.scale2, now.add[d]) - st[d].w[0]) * st[d].w[1];
+                float ds = w * (dp - st[d].w[2]);
+                if (!live[d]) w = ds = 0.f;
                 const float mix = w + other_map<LM>(w);
                 float qf[8], gf[NV];
                 qr[d].to_float(qf);
@@ -97,18 +79,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) dv[i] = fmaf(mix, gf[i], dv[i]);
             }
-            now = next;
-        }
+            if constexpr (!LAST) now = next;
+        });
     }
-    for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dk[i] += __shfl_xor(dk[i], step, 64);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) dv[i] += __shfl_xor(dv[i], step, 64);
-    }
+    scatter_sum<8>(dk, slots);
+    scatter_sum<NV>(dv, slots);
+    if (!p.live) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) dk[i] *= a.scale;
-    finish<T, LM, NV, PB>(a, u, p, dk, dv);
+    if (u.slot >= 0) {  // [heads][2 maps][head_dim], then [heads][value_dim]
+        float* const base = a.partial + (int64_t)u.slot * a.kv_heads * (2 * a.head_dim + a.value_dim);
+        store_scattered<float, 8, false>(base + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, dk, slots, p.kcount);
+        store_scattered<float, NV, false>(
+            base + (int64_t)a.kv_heads * 2 * a.head_dim + (int64_t)p.head * a.value_dim + NV * p.l, dv, slots, p.vcount);
+        return;
+    }
+    const int64_t at = (int64_t)u.row * a.kv_heads + p.head;
+    store_scattered<T, 8, PB == 16>(static_cast<T*>(a.out) + (at * 2 + p.map) * a.head_dim + 8 * p.lm, dk, slots, p.kcount);
+    store_scattered<T, NV, PB == 16>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, slots, p.vcount);
 }
 
 // Joins a cut column's pieces: plain sums of every element, in order.  Threads are

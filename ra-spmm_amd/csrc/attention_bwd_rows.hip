@@ -4,9 +4,10 @@
 // With p the weights of a map, dp_j = dout . v_j and delta = sum_j p_j dp_j,
 //     ds_j = c p_j (dp_j - delta)   (c = 1 for map 0, -lam for map 1)
 //     dq   = scale * sum_j ds_j k_j = scale * c * (sum_j p_j dp_j k_j - delta sum_j p_j k_j)
-// The second form needs one pass over the edges: delta is known at its end.  The
-// weights come from the forward pass' maxima and sums.  Lanes as in the forward
-// pass; the pieces of a long row are plain sums.
+// The second form needs one pass over the edges: delta is known at its end.  In a
+// row's last step (most rows' only one) it is known before k is added, and the first
+// form is used.  The weights come from the forward pass' maxima and sums.  Lanes as
+// in the forward pass; the pieces of a long row are plain sums.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -14,100 +15,108 @@
 namespace ra {
 namespace {
 
-// Map's gradient of q and its record.
-template <typename T, int LM, int NV, int PB>
-__device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, float delta,
-                                       const float* pdk, const float* pk, float m, float il) {
-    if (p.es != 0 || !p.live) return;
-    if (u.slot >= 0) {  // [heads][2 maps][delta], then [heads][2 maps][2][head_dim]
-        float* base = a.partial + (int64_t)u.slot * a.q_heads * (4 * a.head_dim + 2);
-        if (p.lm == 0) base[p.head * 2 + p.map] = delta;
-        float* to = base + a.q_heads * 2 + (int64_t)(p.head * 2 + p.map) * 2 * a.head_dim + 8 * p.lm;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < p.kcount) {
-                to[i] = pdk[i];
-                to[a.head_dim + i] = pk[i];
-            }
-        return;
-    }
-    const float c = (p.map == 0 ? 1.f : -a.lam[p.head]) * a.scale;
-    float dq[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dq[i] = c * (pdk[i] - delta * pk[i]);
-    const int64_t at = ((int64_t)u.row * a.q_heads + p.head) * 2 + p.map;
-    store_run<T, 8, PB == 16>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, p.kcount);
-    if (p.lm == 0) a.record[at] = make_float4(m, il, delta, 0.f);
-}
-
-template <typename T, int LM, int NV, int PB>
+template <typename T, int LM, int NV, int PB, bool WIDE>
 __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);
-    const int kv = p.head / a.group;
-    const Gather<T, 8, PB> k(static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
-    const Gather<T, NV, PB> v(static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim, NV * p.l, p.vcount);
+    const int kv = p.head / a.group, slots = p.slots;
+    const Gather<T, 8, PB, WIDE> k(a.k, (kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+    const Gather<T, NV, PB, WIDE> v(a.v, kv * a.value_dim, NV * p.l, p.vcount);
 
+    Edges now, next;
+    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, slots);
     Run<T, 8> q;
     load_run<T, 8, PB == 16>(
         q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
     Run<T, NV> g;
     load_run<T, NV, PB == 16>(
         g, static_cast<const T*>(a.grad) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, p.vcount);
-    const float2 st = reinterpret_cast<const float2*>(a.stats)[((int64_t)u.row * a.q_heads + p.head) * 2 + p.map];
-    float delta = 0.f, pdk[8], pk[8];
+    const int64_t at = ((int64_t)u.row * a.q_heads + p.head) * 2 + p.map;
+    const float2 st = reinterpret_cast<const float2*>(a.stats)[at];
+    const bool whole = u.slot < 0;
+    float delta = 0.f, pdk[8], pk[8], dq[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) pdk[i] = pk[i] = 0.f;
+    for (int i = 0; i < 8; ++i) pdk[i] = pk[i] = dq[i] = 0.f;
 
-    Edges now, next;
-    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, p.slots);
-    const int step_edges = kDeep * p.slots;
-    for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
-        Run<T, 8> kr[kDeep];
-        Run<T, NV> vr[kDeep];
-        const bool last = e0 + step_edges >= u.end;
+    over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
+        constexpr int DEEP = decltype(deep)::value;
+        constexpr bool LAST = decltype(is_last)::value;
+        Run<T, 8> kr[DEEP];
+        Run<T, NV> vr[DEEP];
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
+        for (int d = 0; d < DEEP; ++d) {
             k.load(kr[d], now.other[d], a.k_pitch);
             v.load(vr[d], now.other[d], a.v_pitch);
         }
-        if (!last) load_edges<false>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+        if constexpr (!LAST) load_edges<false>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
         __builtin_amdgcn_sched_barrier(0);
-        if (last) close_edges(now, e0, u.end, p.es, p.slots);
-        if (last || a.ragged || a.bias) {
+        bool live[DEEP];
+        close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
+        if (LAST || a.ragged || a.bias) {
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d) {
-                k.mask(kr[d], now.add[d] != -INFINITY);
-                v.mask(vr[d], now.add[d] != -INFINITY);
+            for (int d = 0; d < DEEP; ++d) {
+                k.mask(kr[d], live[d]);
+                v.mask(vr[d], live[d]);
             }
         }
+        float w[DEEP], dp[DEEP];
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const float t = lanes_sum<LM>(dot(q, kr[d])), dp = lanes_sum<2 * LM>(dot(g, vr[d]));
-            const bool live = now.add[d] != -INFINITY;
-            const float w = live ? exp_of(fmaf(t, a.scale, now.add[d]) - st.x) * st.y : 0.f;
-            const float wd = live ? w * dp : 0.f;
-            delta += wd;
+        for (int d = 0; d < DEEP; ++d) {
+            w[d] = exp2_of(fmaf(lanes_sum<LM>(dot(q, kr[d])), a.scale2, now.add[d]) - st.x) * st.y;
+            dp[d] = lanes_sum<2 * LM>(dot(g, vr[d]));
+            if (!live[d]) w[d] = dp[d] = 0.f;
+            delta = fmaf(w[d], dp[d], delta);
+        }
+        if (LAST && whole) {
+            delta = slots_sum(delta, slots);
+            if (e0 != u.begin) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dq[i] = fmaf(-delta, pk[i], pdk[i]);
+            }
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+                const float ds = w[d] * (dp[d] - delta);
+                float kf[8];
+                kr[d].to_float(kf);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dq[i] = fmaf(ds, kf[i], dq[i]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const float wd = w[d] * dp[d];
             float kf[8];
             kr[d].to_float(kf);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 pdk[i] = fmaf(wd, kf[i], pdk[i]);
-                pk[i] = fmaf(w, kf[i], pk[i]);
+                pk[i] = fmaf(w[d], kf[i], pk[i]);
             }
         }
-        now = next;
-    }
-    for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
-        delta += __shfl_xor(delta, step, 64);
+        if constexpr (!LAST) now = next;
+    });
+    if (whole) {
+        scatter_sum<8>(dq, slots);
+        if (!p.live) return;
+        const float c = (p.map == 0 ? 1.f : -a.lam[p.head]) * a.scale;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            pdk[i] += __shfl_xor(pdk[i], step, 64);
-            pk[i] += __shfl_xor(pk[i], step, 64);
-        }
+        for (int i = 0; i < 8; ++i) dq[i] *= c;
+        store_scattered<T, 8, PB == 16>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, slots, p.kcount);
+        if (p.lm == 0 && p.es == 0) a.record[at] = make_float4(st.x, st.y, delta, 0.f);
+        return;
     }
-    finish<T, LM, NV, PB>(a, u, p, delta, pdk, pk, st.x, st.y);
+    // A piece: [heads][2 maps][delta], then [heads][2 maps][2][head_dim].
+    delta = slots_sum(delta, slots);
+    scatter_sum<8>(pdk, slots);
+    scatter_sum<8>(pk, slots);
+    if (!p.live) return;
+    float* const base = a.partial + (int64_t)u.slot * a.q_heads * (4 * a.head_dim + 2);
+    if (p.lm == 0 && p.es == 0) base[p.head * 2 + p.map] = delta;
+    float* const to = base + a.q_heads * 2 + (int64_t)(p.head * 2 + p.map) * 2 * a.head_dim + 8 * p.lm;
+    store_scattered<float, 8, false>(to, pdk, slots, p.kcount);
+    store_scattered<float, 8, false>(to + a.head_dim, pk, slots, p.kcount);
 }
 
 // Joins a cut row's pieces: a workgroup per (row, head).  Threads are piece groups x

@@ -4,9 +4,11 @@
 // heads.  Its lanes are edge slots x heads x 2 maps x LM lanes, so that a load
 // instruction takes whole runs of the gathered k and v rows: a lane holds 8
 // elements of its map's half of a key and NV of the head's value row.  One pass
-// over the edges with a running maximum and sum per (edge slot, head, map); the
-// two maps' sums of v are kept apart, because their weights are only known at the
-// end.  The slots are joined by shuffles, pieces of a long row by a second launch.
+// over the edges, four a slot at a time, with a running maximum and sum per (edge
+// slot, head, map).  Until the last step of a row its final weights are not known, so
+// the two maps' sums of v are kept apart; in the last step (most rows' only one) the
+// slots' maxima and sums are joined first, and v is added once with its final weight
+// p_0 / l_0 - lam p_1 / l_1.  Pieces of a long row are joined by a second launch.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -21,129 +23,152 @@ struct State {
     float own[NV], other[NV];
 };
 
-// Writes a finished row, or a piece's state to its slot:
-// [heads][2 maps][max, sum], then [heads][2 maps][value_dim].
-template <typename T, int LM, int NV, int PB>
-__device__ __forceinline__ void finish(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, const State<NV>& s) {
-    if (p.es != 0 || !p.live) return;
-    if (u.slot >= 0) {
-        float* base = a.partial + (int64_t)u.slot * a.q_heads * (2 * a.value_dim + 4);
-        if (p.lm == 0) {
-            float* ml = base + (p.head * 2 + p.map) * 2;
-            ml[0] = s.m;
-            ml[1] = s.l;
-        }
-        // Map 0's lanes hold map 0's sums in `own`.
-        float* acc = base + a.q_heads * 4 + (int64_t)p.head * 2 * a.value_dim + NV * p.l;
-        const bool first = p.map == 0;
+// Joins the slots of a piece and writes its state: [heads][2 maps][max, sum], then
+// [heads][2 maps][value_dim].
+template <int LM, int NV>
+__device__ __forceinline__ void store_piece(const AttnArgs& a, const Unit& u, const Place<LM, NV>& p, State<NV>& s) {
+    const float top = slots_max(s.m, p.slots);
+    const float keep = s.m == -INFINITY ? 0.f : exp2_of(s.m - top), keep_x = other_map<LM>(keep);
+    const float sum = slots_sum(s.l * keep, p.slots);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < p.vcount) {
-                acc[i] = first ? s.own[i] : s.other[i];
-                acc[a.value_dim + i] = first ? s.other[i] : s.own[i];
-            }
-        return;
+    for (int i = 0; i < NV; ++i) {
+        s.own[i] *= keep;
+        s.other[i] *= keep_x;
     }
-    const float il = s.l > 0.f ? 1.f / s.l : s.l == 0.f ? 0.f : s.l;  // NaN stays
-    const float w = p.map == 0 ? il : -a.lam[p.head] * il;
-    const float wx = other_map<LM>(w);
-    float o[NV];
-    // No edge left: zeros, whatever lam is.
-#pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = s.l == 0.f ? 0.f : s.own[i] * w + s.other[i] * wx;
-    store_run<T, NV, PB == 16>(static_cast<T*>(a.out) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, o,
-                          p.vcount);
-    if (a.stats && p.lm == 0)
-        reinterpret_cast<float2*>(a.stats)[((int64_t)u.row * a.q_heads + p.head) * 2 + p.map] =
-            make_float2(s.m == -INFINITY ? 0.f : s.m, il);
+    scatter_sum<NV>(s.own, p.slots);
+    scatter_sum<NV>(s.other, p.slots);
+    if (!p.live) return;
+    float* base = a.partial + (int64_t)u.slot * a.q_heads * (2 * a.value_dim + 4);
+    if (p.lm == 0 && p.es == 0) {
+        float* ml = base + (p.head * 2 + p.map) * 2;
+        ml[0] = top;
+        ml[1] = sum;
+    }
+    float* acc = base + a.q_heads * 4 + (int64_t)p.head * 2 * a.value_dim + NV * p.l;
+    store_scattered<float, NV, false>(acc + (p.map ? a.value_dim : 0), s.own, p.slots, p.vcount);
+    store_scattered<float, NV, false>(acc + (p.map ? 0 : a.value_dim), s.other, p.slots, p.vcount);
 }
 
-template <typename T, int LM, int NV, int PB>
+template <typename T, int LM, int NV, int PB, bool WIDE>
 __global__ __launch_bounds__(kAttnThreads) void attn_forward(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);
-    const int kv = p.head / a.group;
-    const Gather<T, 8, PB> k(static_cast<const T*>(a.k) + (int64_t)(kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
-    const Gather<T, NV, PB> v(static_cast<const T*>(a.v) + (int64_t)kv * a.value_dim, NV * p.l, p.vcount);
+    const int kv = p.head / a.group, slots = p.slots;
+    const Gather<T, 8, PB, WIDE> k(a.k, (kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+    const Gather<T, NV, PB, WIDE> v(a.v, kv * a.value_dim, NV * p.l, p.vcount);
 
-    Run<T, 8> q;
-    load_run<T, 8, PB == 16>(
-        q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
+    const bool whole = u.slot < 0;
+    const int64_t at = (int64_t)u.row * a.q_heads + p.head;
+    T* const out = static_cast<T*>(a.out) + at * a.value_dim + NV * p.l;
     State<NV> s;
     s.m = -INFINITY;
     s.l = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) s.own[i] = s.other[i] = 0.f;
-
+    if (u.begin == u.end && whole) {
+        if (!p.live) return;
+        store_scattered<T, NV, PB == 16>(out, s.own, slots, p.vcount);
+        if (a.stats && p.lm == 0 && p.es == 0) reinterpret_cast<float2*>(a.stats)[at * 2 + p.map] = make_float2(0.f, 0.f);
+        return;
+    }
     Edges now, next;
-    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, p.slots);
-    const int step_edges = kDeep * p.slots;
-    for (int e0 = u.begin; e0 < u.end; e0 += step_edges) {
-        Run<T, 8> kr[kDeep];
-        Run<T, NV> vr[kDeep];
-        const bool last = e0 + step_edges >= u.end;
+    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, slots);
+    Run<T, 8> q;
+    load_run<T, 8, PB == 16>(
+        q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
+    over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
+        constexpr int DEEP = decltype(deep)::value;
+        constexpr bool LAST = decltype(is_last)::value;
+        Run<T, 8> kr[DEEP];
+        Run<T, NV> vr[DEEP];
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
+        for (int d = 0; d < DEEP; ++d) {
             k.load(kr[d], now.other[d], a.k_pitch);
             v.load(vr[d], now.other[d], a.v_pitch);
         }
-        if (!last) load_edges<false>(a, next, e0 + step_edges, u.end, p.es, p.slots);
+        if constexpr (!LAST) load_edges<false>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
         __builtin_amdgcn_sched_barrier(0);
-        if (last) close_edges(now, e0, u.end, p.es, p.slots);
-        if (last || a.ragged || a.bias) {
+        bool live[DEEP];
+        close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
+        if (LAST || a.ragged || a.bias) {
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d) {
-                k.mask(kr[d], now.add[d] != -INFINITY);
-                v.mask(vr[d], now.add[d] != -INFINITY);
+            for (int d = 0; d < DEEP; ++d) {
+                k.mask(kr[d], live[d]);
+                v.mask(vr[d], live[d]);
             }
         }
-        float score[kDeep], top = s.m;
+        float score[DEEP], top = s.m;
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            score[d] = fmaf(lanes_sum<LM>(dot(q, kr[d])), a.scale, now.add[d]);
-            if (now.add[d] == -INFINITY) score[d] = -INFINITY;
-            top = score[d] > top || score[d] != score[d] ? score[d] : top;  // a NaN stays
+        for (int d = 0; d < DEEP; ++d) {
+            score[d] = fmaf(lanes_sum<LM>(dot(q, kr[d])), a.scale2, now.add[d]);
+            if (!live[d]) score[d] = -INFINITY;
+            top = fmaxf(top, score[d]);  // a NaN score makes its weight NaN below
         }
-        // All edges so far left out: every weight is 0, not exp(-inf + inf).
+        // No live edge so far: every weight is exp2(-inf) = 0.
         const float ref = top == -INFINITY ? 0.f : top;
-        const float keep = exp_of(s.m - ref), keep_x = other_map<LM>(keep);
-        s.m = top;
-        s.l *= keep;
+        const float keep = exp2_of(s.m - ref);
+        float w[DEEP], sum = s.l * keep;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            s.own[i] *= keep;
-            s.other[i] *= keep_x;
+        for (int d = 0; d < DEEP; ++d) {
+            w[d] = exp2_of(score[d] - ref);
+            sum += w[d];
+        }
+        if (LAST && whole) {
+            const float all = slots_max(top, slots);
+            const float part = top == -INFINITY ? (sum == 0.f ? 0.f : sum) : exp2_of(top - all);
+            const float total = slots_sum(sum * part, slots);
+            const float il = total > 0.f ? 1.f / total : total;  // 0, or a NaN that stays
+            const float f = (p.map == 0 ? il : -a.lam[p.head] * il) * part;
+            float o[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) o[i] = 0.f;
+            if (e0 != u.begin) {
+                const float c = f * keep, cx = other_map<LM>(c);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) o[i] = fmaf(s.own[i], c, s.other[i] * cx);
+            }
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+                const float wf = w[d] * f, mix = wf + other_map<LM>(wf);
+                float vf[NV];
+                vr[d].to_float(vf);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) o[i] = fmaf(mix, vf[i], o[i]);
+            }
+            scatter_sum<NV>(o, slots);
+            if (p.live) {
+                store_scattered<T, NV, PB == 16>(out, o, slots, p.vcount);
+                if (a.stats && p.lm == 0 && p.es == 0)
+                    reinterpret_cast<float2*>(a.stats)[at * 2 + p.map] = make_float2(all == -INFINITY ? 0.f : all, il);
+            }
+            return;
+        }
+        s.m = top;
+        s.l = sum;
+        if (e0 != u.begin) {
+            const float keep_x = other_map<LM>(keep);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                s.own[i] *= keep;
+                s.other[i] *= keep_x;
+            }
         }
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const float w = exp_of(score[d] - ref), wx = other_map<LM>(w);
-            s.l += w;
+        for (int d = 0; d < DEEP; ++d) {
+            const float wx = other_map<LM>(w[d]);
             float vf[NV];
             vr[d].to_float(vf);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                s.own[i] = fmaf(w, vf[i], s.own[i]);
+                s.own[i] = fmaf(w[d], vf[i], s.own[i]);
                 s.other[i] = fmaf(wx, vf[i], s.other[i]);
             }
         }
-        now = next;
-    }
-    for (int step = 32 / p.slots * 2; step < 64; step <<= 1) {
-        const float m2 = __shfl_xor(s.m, step, 64);
-        const float top = m2 > s.m || m2 != m2 ? m2 : s.m;
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float keep = exp_of(s.m - ref), keep2 = exp_of(m2 - ref);
-        const float keep_x = other_map<LM>(keep), keep2_x = other_map<LM>(keep2);
-        s.l = s.l * keep + __shfl_xor(s.l, step, 64) * keep2;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            s.own[i] = s.own[i] * keep + __shfl_xor(s.own[i], step, 64) * keep2;
-            s.other[i] = s.other[i] * keep_x + __shfl_xor(s.other[i], step, 64) * keep2_x;
-        }
-        s.m = top;
-    }
-    finish<T, LM, NV, PB>(a, u, p, s);
+        if constexpr (!LAST) now = next;
+    });
+    if (whole) return;
+    store_piece(a, u, p, s);
 }
 
 // Joins the pieces of a cut row: a workgroup per (row, head).  Its threads are
@@ -193,7 +218,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
     float sum[2] = {0.f, 0.f};
     for (int i = threadIdx.x; i < n; i += kJoinThreads)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) sum[m] += ml[i * stride + 2 * m + 1] * exp_of(ml[i * stride + 2 * m] - ref[m]);
+        for (int m = 0; m < 2; ++m) sum[m] += ml[i * stride + 2 * m + 1] * exp2_of(ml[i * stride + 2 * m] - ref[m]);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         for (int off = 32; off > 0; off >>= 1) sum[m] += __shfl_xor(sum[m], off, 64);
@@ -210,7 +235,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
         for (int i = part; i < n; i += parts)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-                acc[m] = fmaf(v[i * stride + m * a.value_dim], exp_of(ml[i * stride + 2 * m] - ref[m]), acc[m]);
+                acc[m] = fmaf(v[i * stride + m * a.value_dim], exp2_of(ml[i * stride + 2 * m] - ref[m]), acc[m]);
     }
     acc_of[0][threadIdx.x] = acc[0];
     acc_of[1][threadIdx.x] = acc[1];

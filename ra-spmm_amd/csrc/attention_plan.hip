@@ -255,6 +255,7 @@ AttnArgs args_of(const ra_attn_shape& s, const AttnLayout& l) {
     a.head_dim = s.head_dim;
     a.value_dim = s.value_dim;
     a.scale = s.scale;
+    a.scale2 = s.scale * ra::kLog2e;
     a.ldq = s.ldq;
     a.ldk = s.ldk;
     a.ldv = s.ldv;
@@ -268,6 +269,13 @@ AttnArgs args_of(const ra_attn_shape& s, const AttnLayout& l) {
     a.hb_shift = l.hb_shift;
     a.pieces = 1;
     return a;
+}
+
+// 32-bit offsets reach the gathered matrices: 24-bit factors, less than 4 GiB.
+bool narrow(int64_t rows, std::initializer_list<uint32_t> pitches) {
+    for (const uint32_t p : pitches)
+        if (rows >= (1 << 24) || p >= (1u << 24) || rows * (int64_t)p >= (int64_t{1} << 32)) return false;
+    return true;
 }
 
 void side_of(AttnArgs& a, const AttnSide& s) {
@@ -433,6 +441,7 @@ ra_status ra_attn_plan_run(ra_attn_plan* p, const ra_attn_shape* shape, const vo
         s, s.q_heads, {d_q, d_k, d_v, d_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim});
     ra::AttnArgs a = ra::args_of(s, l);
     ra::side_of(a, p->side[0]);
+    a.wide = !ra::narrow(p->info.K, {a.k_pitch, a.v_pitch});
     RA_TRY(check_output(d_out, "out"));
     RA_TRY(check_output(d_stats, "stats"));
     RA_TRY(guarded([&] { return p->partial.ensure(p->side[0].num_slots * ra::attn_forward_slot(s) * sizeof(float), st); }));
@@ -485,6 +494,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
     a.partial = p->partial.get<float>();
     if (M > 0) {
         ra::side_of(a, rows);
+        a.wide = !ra::narrow(K, {a.k_pitch, a.v_pitch});
         a.out = d_dq;
         RA_TRY(ra::attn_rows_launch(s.dtype, l, a, st));
         RA_TRY(ra::attn_rows_join_launch(s.dtype, a, rows.splits, rows.num_splits, st));
@@ -496,6 +506,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
         a.hb_shift = l.hb_shift;
         a.ragged = l.ragged;
         ra::side_of(a, cols);
+        a.wide = !ra::narrow(M, {a.q_pitch, a.g_pitch, static_cast<uint32_t>(s.q_heads * 2 * sizeof(float4))});
         a.out = d_dk;
         a.out2 = d_dv;
         RA_TRY(ra::attn_cols_launch(s.dtype, l, a, st));
@@ -537,6 +548,7 @@ ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t 
     a.rows = M;
     a.pieces = ra::plan_free_pieces(s, M, nnz);
     a.num_units = (int64_t)M * a.pieces * a.head_blocks;
+    a.wide = !ra::narrow(K, {a.k_pitch, a.v_pitch});
     a.q = d_q;
     a.k = d_k;
     a.v = d_v;
