@@ -46,6 +46,7 @@ struct AttnArgs {
     int64_t num_units;    // pieces * head blocks
     int32_t pieces;       // per row, without a list
     int32_t head_blocks;  // waves that share a piece
+    int32_t head_items;   // 0: a piece's waves are neighbours; else pieces, all of one head block's first
     int32_t hb_shift;     // log2 of the heads of a wave
     int32_t q_heads, kv_heads, group, head_dim, value_dim;
     int32_t rows;
@@ -57,7 +58,10 @@ struct AttnArgs {
     const void *q, *k, *v, *grad;
     const float *lam, *bias;
     float* stats;    // [rows, q_heads, 2] (max in powers of two, 1 / sum)
-    float4* record;  // [rows, q_heads, 2] (the same, sum p dp, 0)
+    // What the column pass takes of a row and head: per map (max, 1 / sum, sum p dp, 0).
+    float4* record;
+    uint32_t record_row;  // distances in bytes: [rows][q_heads] or [q_heads][rows]
+    int64_t record_head;
     void *out, *out2;
     float* partial;
 };
@@ -78,7 +82,9 @@ struct AttnPtrs {
     int64_t ldq, ldk, ldv, ldg;
 };
 
-AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p);
+// pieces: of the launch; by_head: attn_by_head.
+AttnLayout attn_layout(const ra_attn_shape& s, int heads, const AttnPtrs& p, int64_t pieces, bool by_head);
+bool attn_by_head(const ra_attn_shape& s, int64_t rows, int64_t gathered, int64_t nnz);
 ra_status attn_check(const ra_attn_shape* s, int32_t M, int32_t K);
 
 // Floats of a slot of partial results.
@@ -100,9 +106,8 @@ ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4*
 ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
 ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
 // d lam from the records; `partial` holds kLamBlocks * q_heads floats.
-constexpr int kLamBlocks = 256;
-ra_status attn_lam_launch(const float4* record, int32_t rows, int32_t q_heads, float* partial, float* dlam,
-                          hipStream_t st);
+constexpr int kLamBlocks = 128;
+ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStream_t st);
 
 // ------------------------------------------------------------- device side
 constexpr int kAttnThreads = 256;
@@ -257,6 +262,9 @@ __device__ __forceinline__ void store_scattered(T* p, const float* sums, int slo
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+__device__ __forceinline__ float4* record_at(const AttnArgs& a, int64_t row, int head) {
+    return reinterpret_cast<float4*>(reinterpret_cast<char*>(a.record) + row * a.record_row + head * a.record_head);
+}
 // Piece and heads of a wave.
 struct Unit {
     int row, begin, end, slot;
@@ -278,8 +286,16 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
     u.live = at < static_cast<uint64_t>(a.num_units);
     if (!u.live) return u;
     const uint32_t unit = static_cast<uint32_t>(at), blocks = a.head_blocks;
-    const uint32_t item = blocks == 1 ? unit : unit / blocks;
-    u.head_block = static_cast<int>(unit - item * blocks);
+    uint32_t item = unit;
+    if (blocks != 1) {
+        if (a.head_items) {
+            u.head_block = static_cast<int>(unit / static_cast<uint32_t>(a.head_items));
+            item = unit - static_cast<uint32_t>(u.head_block) * static_cast<uint32_t>(a.head_items);
+        } else {
+            item = unit / blocks;
+            u.head_block = static_cast<int>(unit - item * blocks);
+        }
+    }
     if (a.items) {
         const int4 it = a.items[item];
         u.row = it.x, u.begin = it.y, u.end = it.z, u.slot = it.w;
@@ -319,8 +335,10 @@ struct Place {
 };
 
 // Edges in flight per slot: their loads are all issued before the first is used
-// (the scheduler would otherwise wait for each in turn to save registers).
-constexpr int kDeep = 4;
+// (the scheduler would otherwise wait for each in turn to save registers).  Two
+// leave registers for 5 or 6 waves a SIMD, four for 4 (power-law graph of 1e6 rows,
+// forward: 1.66 against 1.81 ms; skewed fp32 rows 0.50 against 0.61).
+constexpr int kDeep = 2;
 
 // The next kDeep edges of every slot.  Past the end the last edge again.
 struct Edges {
@@ -369,7 +387,6 @@ __device__ __forceinline__ void over_edges(int begin, int end, int slots, F step
     int e0 = begin;
     for (; end - e0 > kDeep * slots; e0 += kDeep * slots) step(std::integral_constant<int, kDeep>(), std::false_type(), e0);
     if (end - e0 <= slots) step(std::integral_constant<int, 1>(), std::true_type(), e0);
-    else if (end - e0 <= 2 * slots) step(std::integral_constant<int, 2>(), std::true_type(), e0);
     else step(std::integral_constant<int, kDeep>(), std::true_type(), e0);
 }
 

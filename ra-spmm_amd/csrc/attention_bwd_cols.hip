@@ -2,7 +2,7 @@
 // dk and dv, from the transposed lists.
 //
 // A wave works on one piece of a column's list for one block of key/value heads;
-// per edge it gathers the row's q, dout and record (maximum, 1/sum, delta of both
+// per edge it gathers the row's q, dout and record (maximum, 1/sum and delta of both
 // maps), and forms the weights again:
 //     dk += scale * c p (dp - delta) q,   dv += (p_0 - lam p_1) dout
 // A key/value head's query heads are taken one after another, into the same sums:
@@ -32,31 +32,31 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) dv[i] = 0.f;
 
-    const uint32_t record_pitch = a.q_heads * 2 * sizeof(float4);
-    for (int sub = 0; sub < a.group; ++sub) {
-        const int qh = p.head * a.group + sub;
-        const Gather<T, 8, PB, WIDE> q(a.q, (qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
-        const Gather<T, NV, PB, WIDE> g(a.grad, qh * a.value_dim, NV * p.l, p.vcount);
-        const Gather<float, 4, 16, WIDE> rec(a.record, (qh * 2 + p.map) * 4, 0, 4);
-        const float c = p.map == 0 ? 1.f : -a.lam[qh];
-        Edges now, next;
-        if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, slots);
-        over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
-            constexpr int DEEP = decltype(deep)::value;
-            constexpr bool LAST = decltype(is_last)::value;
+    Edges now, next;
+    if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, slots);
+    over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
+        constexpr int DEEP = decltype(deep)::value;
+        constexpr bool LAST = decltype(is_last)::value;
+        if constexpr (!LAST) load_edges<true>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
+        bool live[DEEP];
+        close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
+        for (int sub = 0; sub < a.group; ++sub) {
+            const int qh = p.head * a.group + sub;
+            const Gather<T, 8, PB, WIDE> q(a.q, (qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+            const Gather<T, NV, PB, WIDE> g(a.grad, qh * a.value_dim, NV * p.l, p.vcount);
+            const char* const record = reinterpret_cast<const char*>(a.record) + qh * a.record_head + p.map * sizeof(float4);
+            const float c = p.map == 0 ? 1.f : -a.lam[qh];
             Run<T, 8> qr[DEEP];
             Run<T, NV> gr[DEEP];
-            Run<float, 4> st[DEEP];  // maximum, 1 / sum, delta
+            float4 st[DEEP];  // maximum, 1 / sum, delta
 #pragma unroll
             for (int d = 0; d < DEEP; ++d) {
                 q.load(qr[d], now.other[d], a.q_pitch);
                 g.load(gr[d], now.other[d], a.g_pitch);
-                rec.load(st[d], now.other[d], record_pitch);
+                const uint64_t at = WIDE ? static_cast<uint64_t>(now.other[d]) * a.record_row : __umul24(now.other[d], a.record_row);
+                st[d] = *reinterpret_cast<const float4*>(record + at);
             }
-            if constexpr (!LAST) load_edges<true>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
             __builtin_amdgcn_sched_barrier(0);
-            bool live[DEEP];
-            close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
             if (LAST || a.ragged || a.bias) {
 #pragma unroll
                 for (int d = 0; d < DEEP; ++d) {
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < DEEP; ++d) {
                 const float t = lanes_sum<LM>(dot(k, qr[d])), dp = lanes_sum<2 * LM>(dot(v, gr[d]));
-                float w = c * exp2_of(fmaf(t, a.scale2, now.add[d]) - st[d].w[0]) * st[d].w[1];
-                float ds = w * (dp - st[d].w[2]);
+                float w = c * exp2_of(fmaf(t, a.scale2, now.add[d]) - st[d].x) * st[d].y;
+                float ds = w * (dp - st[d].z);
                 if (!live[d]) w = ds = 0.f;
                 const float mix = w + other_map<LM>(w);
                 float qf[8], gf[NV];
@@ -79,9 +79,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) dv[i] = fmaf(mix, gf[i], dv[i]);
             }
-            if constexpr (!LAST) now = next;
-        });
-    }
+        }
+        if constexpr (!LAST) now = next;
+    });
     scatter_sum<8>(dk, slots);
     scatter_sum<NV>(dv, slots);
     if (!p.live) return;

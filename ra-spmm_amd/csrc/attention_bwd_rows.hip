@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) dq[i] *= c;
         store_scattered<T, 8, PB == 16>(static_cast<T*>(a.out) + at * a.head_dim + 8 * p.lm, dq, slots, p.kcount);
-        if (p.lm == 0 && p.es == 0) a.record[at] = make_float4(st.x, st.y, delta, 0.f);
+        if (p.lm == 0 && p.es == 0) record_at(a, u.row, p.head)[p.map] = make_float4(st.x, st.y, delta, 0.f);
         return;
     }
     // A piece: [heads][2 maps][delta], then [heads][2 maps][2][head_dim].
@@ -159,26 +159,24 @@ __global__ __launch_bounds__(kJoinThreads) void attn_rows_join(const AttnArgs a,
     static_cast<T*>(a.out)[to * a.head_dim + i] = (T)(c * (pdk - delta * pk));
     if (i == 0) {
         const float2 st = reinterpret_cast<const float2*>(a.stats)[to];
-        a.record[to] = make_float4(st.x, st.y, delta, 0.f);
+        record_at(a, sp.x, head)[map] = make_float4(st.x, st.y, delta, 0.f);
     }
 }
 
-// d lam[h] = -sum_i delta of map 1: a workgroup sums a run of rows for every head,
-// then one workgroup the workgroups' sums, both in a fixed order.
-__global__ __launch_bounds__(256) void attn_lam_partial(const float4* __restrict__ record, int rows, int heads,
-                                                        float* __restrict__ partial) {
+// d lam[h] = -sum_i delta of map 1: a workgroup sums a run of rows for one head, then
+// one workgroup the workgroups' sums, both in a fixed order.
+__global__ __launch_bounds__(256) void attn_lam_partial(const AttnArgs a, float* __restrict__ partial) {
     __shared__ float part[4];
-    const int64_t per = ((int64_t)rows + gridDim.x - 1) / gridDim.x;
-    const int64_t first = blockIdx.x * per, end = min(first + per, (int64_t)rows);
-    for (int h = 0; h < heads; ++h) {
-        float x = 0.f;
-        for (int64_t i = first + threadIdx.x; i < end; i += 256) x += record[(i * heads + h) * 2 + 1].z;
-        for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
-        __syncthreads();
-        if (threadIdx.x == 0) partial[(int64_t)blockIdx.x * heads + h] = part[0] + part[1] + part[2] + part[3];
-        __syncthreads();
-    }
+    const int64_t per = ((int64_t)a.rows + gridDim.x - 1) / gridDim.x;
+    const int64_t first = blockIdx.x * per, end = min(first + per, (int64_t)a.rows);
+    const int h = blockIdx.y;
+    float x = 0.f;
+#pragma unroll 4
+    for (int64_t i = first + threadIdx.x; i < end; i += 256) x += record_at(a, i, h)[1].z;
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[(int64_t)blockIdx.x * a.q_heads + h] = part[0] + part[1] + part[2] + part[3];
 }
 __global__ __launch_bounds__(64) void attn_lam_final(const float* __restrict__ partial, int blocks, int heads,
                                                      float* __restrict__ dlam) {
@@ -212,11 +210,10 @@ ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* sp
     return RA_OK;
 }
 
-ra_status attn_lam_launch(const float4* record, int32_t rows, int32_t q_heads, float* partial, float* dlam,
-                          hipStream_t st) {
-    attn_lam_partial<<<kLamBlocks, 256, 0, st>>>(record, rows, q_heads, partial);
+ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStream_t st) {
+    attn_lam_partial<<<dim3(kLamBlocks, a.q_heads), 256, 0, st>>>(a, partial);
     RA_LAUNCH_CHECK("attn_lam_partial");
-    attn_lam_final<<<q_heads, 64, 0, st>>>(partial, kLamBlocks, q_heads, dlam);
+    attn_lam_final<<<a.q_heads, 64, 0, st>>>(partial, kLamBlocks, a.q_heads, dlam);
     RA_LAUNCH_CHECK("attn_lam_final");
     return RA_OK;
 }

@@ -171,89 +171,98 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward(const AttnArgs a) {
     store_piece(a, u, p, s);
 }
 
-// Joins the pieces of a cut row: a workgroup per (row, head).  Its threads are
-// piece groups x value_dim (padded to 64 at least); each group runs over its share
-// of the pieces.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of a cut row: a workgroup per (row, head).  The pieces' weights
+// are formed once, in LDS, for up to kJoinPieces of them at a time (a running maximum
+// over those steps); the v sums then go over piece groups x value_dim threads.
+constexpr int kJoinThreads = 256, kJoinPieces = 1024;
+
+// A pair over the workgroup; `lds` is not read by others any more.
+template <typename F>
+__device__ __forceinline__ void join_reduce(float* x, float2* lds, F f) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        x[0] = f(x[0], __shfl_xor(x[0], off, 64));
+        x[1] = f(x[1], __shfl_xor(x[1], off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(x[0], x[1]);
+    __syncthreads();
+    const float2 a = lds[0], b = lds[1], c = lds[2], d = lds[3];
+    x[0] = f(f(a.x, b.x), f(c.x, d.x));
+    x[1] = f(f(a.y, b.y), f(c.y, d.y));
+}
+
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs a, const int4* __restrict__ splits) {
-    __shared__ float top_of[2][kJoinThreads / 64], sum_of[2][kJoinThreads / 64], acc_of[2][kJoinThreads];
-    const int head = blockIdx.x % a.q_heads;
-    int4 sp;
-    if (splits) sp = splits[blockIdx.x / a.q_heads];
-    else {
-        const int row = blockIdx.x / a.q_heads;
-        sp = make_int4(row, 0, a.pieces, 0);
-    }
-    const int64_t slot0 = splits ? sp.y : (int64_t)sp.x * a.pieces;
-    const int n = sp.z;
+    __shared__ float weight[2][kJoinPieces], sums[2][kJoinThreads];
+    __shared__ float2 tops[kJoinThreads / 64], totals[kJoinThreads / 64];
+    const int head = blockIdx.x % a.q_heads, which = blockIdx.x / a.q_heads;
+    const int4 sp = splits ? splits[which] : make_int4(which, 0, a.pieces, 0);
+    const int64_t slot0 = splits ? sp.y : (int64_t)which * a.pieces;
     const int64_t stride = (int64_t)a.q_heads * (2 * a.value_dim + 4);
-    const float* const ml = a.partial + slot0 * stride + head * 4;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-
-    float top[2] = {-INFINITY, -INFINITY};
-    for (int i = threadIdx.x; i < n; i += kJoinThreads)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const float x = ml[i * stride + 2 * m];
-            top[m] = x > top[m] || x != x ? x : top[m];
-        }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        for (int off = 32; off > 0; off >>= 1) {
-            const float x = __shfl_xor(top[m], off, 64);
-            top[m] = x > top[m] || x != x ? x : top[m];
-        }
-        if (lane == 0) top_of[m][wave] = top[m];
-    }
-    __syncthreads();
-    float ref[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        top[m] = top_of[m][0];
-        for (int w = 1; w < kJoinThreads / 64; ++w)
-            top[m] = top_of[m][w] > top[m] || top_of[m][w] != top_of[m][w] ? top_of[m][w] : top[m];
-        ref[m] = top[m] == -INFINITY ? 0.f : top[m];
-    }
-    float sum[2] = {0.f, 0.f};
-    for (int i = threadIdx.x; i < n; i += kJoinThreads)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) sum[m] += ml[i * stride + 2 * m + 1] * exp2_of(ml[i * stride + 2 * m] - ref[m]);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        for (int off = 32; off > 0; off >>= 1) sum[m] += __shfl_xor(sum[m], off, 64);
-        if (lane == 0) sum_of[m][wave] = sum[m];
-    }
-    // The v sums.
-    int width = 64;
+    const float* const first = a.partial + slot0 * stride;
+    int width = 16;
     while (width < a.value_dim) width *= 2;  // at most 256
     const int part = threadIdx.x / width, parts = kJoinThreads / width, at = threadIdx.x & (width - 1);
-    float acc[2] = {0.f, 0.f};
-    if (at < a.value_dim) {
-        const float* const v = a.partial + slot0 * stride + a.q_heads * 4 + (int64_t)head * 2 * a.value_dim + at;
-#pragma unroll 4
-        for (int i = part; i < n; i += parts)
+
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2] = {0.f, 0.f};
+    for (int i0 = 0; i0 < sp.z; i0 += kJoinPieces) {
+        const int n = min(kJoinPieces, sp.z - i0);
+        constexpr int kEach = kJoinPieces / kJoinThreads;
+        float4 ml[kEach];  // max, sum of both maps
+        float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-                acc[m] = fmaf(v[i * stride + m * a.value_dim], exp2_of(ml[i * stride + 2 * m] - ref[m]), acc[m]);
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * kJoinThreads;
+            ml[j] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            if (i < n) {
+                const float* const x = first + (i0 + i) * stride + head * 4;
+                ml[j] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+            most[0] = fmaxf(most[0], ml[j].x);
+            most[1] = fmaxf(most[1], ml[j].z);
+        }
+        join_reduce(most, tops, [](float x, float y) { return fmaxf(x, y); });
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float now = fmaxf(top[m], most[m]);
+            const float ref = now == -INFINITY ? 0.f : now, keep = exp2_of(top[m] - ref);
+            sum[m] *= keep;  // of the thread's pieces
+            acc[m] *= keep;
+            top[m] = now;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const float w = exp2_of((m == 0 ? ml[j].x : ml[j].z) - ref);
+                weight[m][threadIdx.x + j * kJoinThreads] = w;
+                sum[m] = fmaf(m == 0 ? ml[j].y : ml[j].w, w, sum[m]);
+            }
+        }
+        __syncthreads();
+        if (at < a.value_dim) {
+            const float* const v = first + i0 * stride + a.q_heads * 4 + (int64_t)head * 2 * a.value_dim + at;
+#pragma unroll 8
+            for (int i = part; i < n; i += parts) {
+                acc[0] = fmaf(v[i * stride], weight[0][i], acc[0]);
+                acc[1] = fmaf(v[i * stride + a.value_dim], weight[1][i], acc[1]);
+            }
+        }
+        __syncthreads();  // before the next step's weights
     }
-    acc_of[0][threadIdx.x] = acc[0];
-    acc_of[1][threadIdx.x] = acc[1];
-    __syncthreads();
+    sums[0][threadIdx.x] = acc[0];
+    sums[1][threadIdx.x] = acc[1];
+    join_reduce(sum, totals, [](float x, float y) { return x + y; });
     if (part != 0 || at >= a.value_dim) return;
     float il[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        sum[m] = sum_of[m][0];
-        for (int w = 1; w < kJoinThreads / 64; ++w) sum[m] += sum_of[m][w];
-        for (int x = 1; x < parts; ++x) acc[m] += acc_of[m][x * width + at];
-        il[m] = sum[m] > 0.f ? 1.f / sum[m] : sum[m] == 0.f ? 0.f : sum[m];
+        for (int x = 1; x < parts; ++x) acc[m] += sums[m][x * width + at];
+        il[m] = sum[m] > 0.f ? 1.f / sum[m] : sum[m];  // 0, or a NaN that stays
     }
     const int64_t to = (int64_t)sp.x * a.q_heads + head;
     const float o = sum[0] == 0.f ? 0.f : acc[0] * il[0] - a.lam[head] * il[1] * acc[1];
     static_cast<T*>(a.out)[to * a.value_dim + at] = (T)o;
     if (a.stats && at == 0)
-        reinterpret_cast<float4*>(a.stats)[to] = make_float4(ref[0], il[0], ref[1], il[1]);
+        reinterpret_cast<float4*>(a.stats)[to] =
+            make_float4(top[0] == -INFINITY ? 0.f : top[0], il[0], top[1] == -INFINITY ? 0.f : top[1], il[1]);
 }
 
 }  // namespace

@@ -454,3 +454,17 @@ def test_refusals(case, name):
         fn(case)
     torch.cuda.synchronize()
     assert _run(case).shape == (4, 4, 32)
+
+
+@pytest.mark.parametrize("side", ["rows", "columns"])
+def test_heads_kept_apart(side):
+    """Long lists over gathered rows past the L2s: each XCD takes a part of the heads, on either side."""
+    few, many = 300, 70_000
+    rng = np.random.default_rng(1)
+    if side == "rows":
+        rowptr, colind = lists(rng.integers(0, 160, few), many, 5)
+        M, K = few, many
+    else:
+        rowptr, colind = lists(rng.integers(0, 3, many), few, 5)
+        M, K = many, few
+    check(rowptr, colind, inputs(M, K, 4, 4, 32, 64, torch.bfloat16, 6))
