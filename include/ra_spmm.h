@@ -491,8 +491,9 @@ ra_status ra_head_norm_backward(const ra_norm_shape* shape, const void* d_q, con
  *   unsigned  of max(x, 0): 0 .. 255, and at least 1 where x > 0, so that the codes
  *             also hold the ReLU's mask exactly
  * Codes lie in rows of ldc = cols rounded up to 32 bytes (the padding is 0), scales
- * as their exponent + 127 in one byte, [rows, ldc / 32]; 255 marks a group that
- * holds an inf or NaN: all of it reads back as NaN, and its unsigned codes are the
+ * as their exponent + 127 in one byte, the rows of a group together: [ldc / 32, rows
+ * rounded up to 8] (what the weight gradient, a sum over rows, loads at once; the
+ * padding is not written); 255 marks a group that holds an inf or NaN: all of it reads back as NaN, and its unsigned codes are the
  * mask (1 where x > 0 or NaN).  d_codes and d_scales lie on 16-byte addresses. */
 ra_status ra_pack8(const void* d_x, int64_t rows, int32_t cols, int64_t ldx, int32_t dtype, uint8_t* d_codes,
                    uint8_t* d_scales, ra_stream_t stream);

@@ -34,6 +34,7 @@ struct NormArgs {
     int32_t blocks_q;
     int32_t dim, rot, positions, lanes_shift;
     bool half;
+    bool table_packets;  // rows of the table are whole aligned 16-byte packets
     float eps, inv_dim;
 };
 
@@ -61,26 +62,40 @@ struct Runs {
     }
 };
 
-// Angles of a lane's pairs; pairs past the rotated part stay as they are.  A
+// Row of the table, -1 outside of it.
+__device__ __forceinline__ int64_t table_row(const NormArgs& n, int64_t position) {
+    return position >= 0 && position < n.positions ? position : -1;
+}
+// The table's entries for a lane's pairs (those past the rotated part are not used).
+// Two pairs a load where rows of the table are whole 16-byte packets.
+template <int P>
+__device__ __forceinline__ void load_angles(const NormArgs& n, const Runs<P>& r, int64_t at, float2* turn) {
+    const float2* const t = n.table + max(at, (int64_t)0) * (n.rot / 2);
+    const int last = n.rot / 2 - 1;
+    if (n.table_packets) {
+        const float4* const t4 = reinterpret_cast<const float4*>(t);
+#pragma unroll
+        for (int i = 0; i < P; i += 2) {
+            const float4 x = t4[min(r.pair + i, last) / 2];
+            turn[i] = make_float2(x.x, x.y);
+            turn[i + 1] = make_float2(x.z, x.w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) turn[i] = t[min(r.pair + i, last)];
+    }
+}
+// Their cosines and sines; pairs past the rotated part stay as they are, and a
 // position outside of the table gives NaN.
 template <int P>
-__device__ __forceinline__ void angles(const NormArgs& n, const Runs<P>& r, uint32_t row, float* c, float* s) {
+__device__ __forceinline__ void angles(const NormArgs& n, const Runs<P>& r, const float2* turn, bool inside, float* c,
+                                       float* s) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        c[i] = 1.f;
-        s[i] = 0.f;
+        const bool rotated = r.pair + i < n.rot / 2;
+        c[i] = !rotated ? 1.f : inside ? turn[i].x : __builtin_nanf("");
+        s[i] = !rotated ? 0.f : inside ? turn[i].y : __builtin_nanf("");
     }
-    if (r.pair >= n.rot / 2) return;
-    const int64_t at = n.pos ? n.pos[row] : row;
-    const bool inside = at >= 0 && at < n.positions;
-    const float2* const t = n.table + (inside ? at * (n.rot / 2) : 0) + r.pair;
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-        if (r.pair + i < n.rot / 2) {
-            const float2 x = t[i];
-            c[i] = inside ? x.x : __builtin_nanf("");
-            s[i] = inside ? x.y : __builtin_nanf("");
-        }
 }
 
 // (f, s) -> (f c - s si, f si + s c) for the pairs of two runs.
@@ -127,6 +142,8 @@ __global__ __launch_bounds__(kThreads) void head_norm(const NormArgs n) {
     }
     for (uint32_t unit = thread >> n.lanes_shift; unit < units; unit += step) {
         const uint32_t row = unit / heads, head = unit - row * heads;
+        int64_t at = row;
+        if (n.rot && n.pos) at = n.pos[row];
         const T* const x = static_cast<const T*>(n.x[side]) + row * n.ld[side] + (int64_t)head * n.dim;
         const int64_t out = (int64_t)unit * n.dim;
         Run<T, P> ra, rb, ga, gb;
@@ -137,15 +154,18 @@ __global__ __launch_bounds__(kThreads) void head_norm(const NormArgs n) {
             load_run<T, P, VEC>(ga, g + r.a, r.na);
             load_run<T, P, VEC>(gb, g + r.b, r.nb);
         }
+        float2 turn[P];
+        at = table_row(n, at);
+        if (n.rot) load_angles<P>(n, r, at, turn);
+        __builtin_amdgcn_sched_barrier(0);  // all loads before the first use
         float c[P], s[P], a[P], b[P];
-        angles<P>(n, r, row, c, s);
+        angles<P>(n, r, turn, at >= 0, c, s);
         ra.to_float(a);
         rb.to_float(b);
         float square = 0.f;
 #pragma unroll
         for (int i = 0; i < P; ++i) square = fmaf(a[i], a[i], fmaf(b[i], b[i], square));
         const float rms = rsqrtf(fmaf(head_sum(square, lanes), n.inv_dim, n.eps));
-        T* const y = static_cast<T*>(n.y[side]) + out;
         if constexpr (!BACK) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -175,6 +195,7 @@ __global__ __launch_bounds__(kThreads) void head_norm(const NormArgs n) {
                 b[i] = rms * (fb[i] - b[i] * inner);
             }
         }
+        T* const y = static_cast<T*>(n.y[side]) + out;
         store_run<T, P, VEC>(y + r.a, a, r.na);
         store_run<T, P, VEC>(y + r.b, b, r.nb);
     }
@@ -286,6 +307,7 @@ Launch launch_of(const ra_norm_shape& s, const void* const x[2], const void* con
     a.rot = s.rot_dim;
     a.positions = s.positions;
     a.half = s.layout == RA_ROTATION_HALF;
+    a.table_packets = aligned16(table) && s.rot_dim % 4 == 0;
     a.eps = s.eps;
     a.inv_dim = 1.f / static_cast<float>(s.head_dim);
     return l;

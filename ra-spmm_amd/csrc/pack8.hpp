@@ -11,6 +11,9 @@ constexpr int kPackGroup = 32;  // columns of a scale
 
 inline int32_t pack8_groups(int32_t cols) { return static_cast<int32_t>(((int64_t)cols + kPackGroup - 1) / kPackGroup); }
 
+// Bytes between the groups' scales: one per row, padded to 8.
+inline int64_t pack8_scale_pitch(int64_t rows) { return (rows + 7) / 8 * 8; }
+
 // Scale of a byte: 2^(byte - 127), NaN for 255.
 __device__ __forceinline__ float pack8_scale(uint32_t byte) {
     return __uint_as_float(byte << 23 | (byte == 255u ? 0x400000u : 0u));

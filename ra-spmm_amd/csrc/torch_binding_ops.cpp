@@ -327,6 +327,10 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor> run_head_norm_backward(Tensor q
 // ------------------------------------------------- activations kept in 8 bits
 int64_t packed_width(int64_t cols) { return (cols + 31) / 32 * 32; }
 
+Tensor empty_scales(const Tensor& x) {
+    return torch::empty({packed_width(x.size(1)) / 32, (x.size(0) + 7) / 8 * 8}, x.options().dtype(torch::kUInt8));
+}
+
 int64_t check_matrix(const Tensor& x, const char* name) {
     TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) < INT32_MAX - 64, name, " must be [rows, cols], has ", x.sizes());
@@ -341,8 +345,8 @@ void check_packed(const Tensor& codes, const Tensor& scales, int64_t cols) {
                     codes.size(1) == packed_width(cols),
                 "codes must be contiguous uint8 [rows, cols rounded up to 32]");
     TORCH_CHECK(scales.scalar_type() == torch::kUInt8 && scales.is_contiguous() && scales.dim() == 2 &&
-                    scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1) / 32,
-                "scales must be contiguous uint8 [rows, groups]");
+                    scales.size(0) == codes.size(1) / 32 && scales.size(1) == (codes.size(0) + 7) / 8 * 8,
+                "scales must be contiguous uint8 [groups, rows rounded up to 8]");
 }
 
 std::tuple<Tensor, Tensor> pack8(Tensor x) {
@@ -350,7 +354,7 @@ std::tuple<Tensor, Tensor> pack8(Tensor x) {
     const c10::DeviceGuard guard(x.device());
     const auto bytes = x.options().dtype(torch::kUInt8);
     auto codes = torch::empty({x.size(0), packed_width(x.size(1))}, bytes);
-    auto scales = torch::empty({x.size(0), packed_width(x.size(1)) / 32}, bytes);
+    auto scales = empty_scales(x);
     check(ra_pack8(x.data_ptr(), x.size(0), static_cast<int32_t>(x.size(1)), ld, dtype_of(x, "x"),
                    codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), current_stream()),
           "pack8");
@@ -363,7 +367,7 @@ std::tuple<Tensor, Tensor, Tensor> relu_pack8(Tensor x) {
     const auto bytes = x.options().dtype(torch::kUInt8);
     auto y = torch::empty(x.sizes(), x.options());
     auto codes = torch::empty({x.size(0), packed_width(x.size(1))}, bytes);
-    auto scales = torch::empty({x.size(0), packed_width(x.size(1)) / 32}, bytes);
+    auto scales = empty_scales(x);
     check(ra_relu_pack8(x.data_ptr(), x.size(0), static_cast<int32_t>(x.size(1)), ld, dtype_of(x, "x"), y.data_ptr(),
                         codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), current_stream()),
           "relu_pack8");

@@ -26,12 +26,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRows = 32;  // rows of a stage
 constexpr int kTile = 64;  // a wave's part of the output, both ways
+constexpr int kWavesPerSimd = 2;
 
 struct GradArgs {
     const void* grad;
     const uint8_t *codes, *scales;
     float* out;  // the result, or the workgroups' parts [splits][O][C]
-    int64_t rows, ldg, rows_per_split;
+    int64_t rows, ldg, rows_per_split, scale_pitch;
     int32_t O, C, groups, tiles_o, tiles_c, splits;
     bool even;  // pairs of 16-bit columns lie on 4-byte addresses
 };
@@ -67,8 +68,8 @@ __device__ __forceinline__ void cut(const float* x, uint4* piece) {
 }
 
 // WO x WI waves.
-template <typename T, int WO, int WI, bool SIGNED>
-__global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
+template <typename T, int WO, int WI, bool SIGNED, bool FEW>
+__global__ __launch_bounds__(64 * WO * WI, kWavesPerSimd) void weight_grad8(const GradArgs a) {
     constexpr int PIECES = kPieces<T>, BO = WO * kTile, BI = WI * kTile, NT = 64 * WO * WI, KB = kRows / 8;
     constexpr bool PAIRS = sizeof(T) == 2;
     // Staging work: (8 rows, column or pair of columns) of grad, (8 rows, 4 columns)
@@ -77,6 +78,11 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
     constexpr int C_ITEMS = KB * BI / 4, C_EACH = (C_ITEMS + NT - 1) / NT;
     __shared__ uint4 gs[2][PIECES][KB][BO];
     __shared__ uint4 cs[2][KB][BI];
+    // A thread's neighbouring columns lie BO / 2 and BI / 4 vectors apart, so that the
+    // lanes of a write lie side by side; the output's rows and columns come in that
+    // order.
+    auto o_of = [](int slot) { return PAIRS ? slot % (BO / 2) * 2 + slot / (BO / 2) : slot; };
+    auto c_of = [](int slot) { return slot % (BI / 4) * 4 + slot / (BI / 4); };
 
     const int tiles = a.tiles_o * a.tiles_c;
     const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
@@ -84,46 +90,84 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
     const int64_t first = split * a.rows_per_split, end = min(first + a.rows_per_split, a.rows);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 
-    uint32_t graw[G_EACH][8], craw[C_EACH][8], sraw[C_EACH][8];
-    auto load = [&](int64_t m0) {
+    // Where a thread's parts lie: rows of 8 and the first column.  Columns past the
+    // output's give results that are not stored; they load the last ones.
+    int g_row[G_EACH], g_col[G_EACH], c_row[C_EACH], c_col[C_EACH];
 #pragma unroll
-        for (int e = 0; e < G_EACH; ++e) {
-            const int item = tid + e * NT;
-            const int kb = item / (G_ITEMS / KB), o = o0 + item % (G_ITEMS / KB) * (PAIRS ? 2 : 1);
-            const bool in = (G_ITEMS % NT == 0 || item < G_ITEMS) && o < a.O;
-            const T* const p = static_cast<const T*>(a.grad) + (m0 + kb * 8) * a.ldg + o;
+    for (int e = 0; e < G_EACH; ++e) {
+        const int item = tid + e * NT, o = o0 + item % (G_ITEMS / KB) * (PAIRS ? 2 : 1);
+        g_row[e] = item / (G_ITEMS / KB) * 8 % kRows;
+        g_col[e] = min(o, PAIRS && a.even ? a.O - 2 : a.O - 1);
+    }
+#pragma unroll
+    for (int e = 0; e < C_EACH; ++e) {
+        const int item = tid + e * NT;
+        c_row[e] = item / (BI / 4) * 8 % kRows;
+        c_col[e] = min(c0 + item % (BI / 4) * 4, a.groups * kPackGroup - 4);
+    }
+    // Two stages' loads are in flight: one stage's products take a tenth of the time
+    // of a load.
+    struct Raw {
+        uint32_t g[G_EACH][8], c[C_EACH][8];
+        uint2 s[C_EACH];  // scales of the 8 rows
+    } raw[2];
+    const int64_t pitch = (int64_t)a.groups * kPackGroup;
+    // Every stage loads kRows whole rows, without a condition that the wait for the
+    // stage before would have to allow for: the last one starts early enough, and the
+    // rows that were counted before are masked.  FEW: fewer rows than a stage in all;
+    // the last one stands in for those that do not exist.
+    auto base_of = [&](int64_t m0) { return FEW ? m0 : min(m0, end - kRows); };
+    auto load = [&](Raw& r, int64_t m0) {
+        const int64_t base = base_of(m0);
+        const int last = FEW ? static_cast<int>(end - base) - 1 : kRows - 1;
+#pragma unroll
+        for (int e = 0; e < G_EACH; ++e)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                uint32_t x = 0;
-                if (in && m0 + kb * 8 + i < end) {
-                    if constexpr (!PAIRS) {
-                        x = __float_as_uint(p[i * a.ldg]);
-                    } else if (a.even) {
-                        x = *reinterpret_cast<const uint32_t*>(p + i * a.ldg);
-                    } else {
-                        const uint16_t* const h = reinterpret_cast<const uint16_t*>(p + i * a.ldg);
-                        x = h[0];
-                        if (o + 1 < a.O) x |= static_cast<uint32_t>(h[1]) << 16;
-                    }
+                // A uniform row and a 32-bit offset.
+                const T* const p = FEW ? static_cast<const T*>(a.grad) + (base + min(g_row[e] + i, last)) * a.ldg + g_col[e]
+                                       : static_cast<const T*>(a.grad) + (base + i) * a.ldg +
+                                             static_cast<uint32_t>(g_row[e] * static_cast<int>(a.ldg) + g_col[e]);
+                if constexpr (!PAIRS) {
+                    r.g[e][i] = __builtin_bit_cast(uint32_t, *p);
+                } else if (a.even) {
+                    r.g[e][i] = *reinterpret_cast<const uint32_t*>(p);
+                } else {
+                    const uint16_t* const h = reinterpret_cast<const uint16_t*>(p);
+                    r.g[e][i] = h[0] | static_cast<uint32_t>(h[g_col[e] + 1 < a.O ? 1 : 0]) << 16;
                 }
-                graw[e][i] = x;
             }
-        }
 #pragma unroll
         for (int e = 0; e < C_EACH; ++e) {
-            const int item = tid + e * NT;
-            const int kb = item / (BI / 4), c = c0 + item % (BI / 4) * 4;
-            const bool in = (C_ITEMS % NT == 0 || item < C_ITEMS) && c < a.groups * kPackGroup;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int64_t m = m0 + kb * 8 + i;
-                const bool live = in && m < end;
-                craw[e][i] = live ? *reinterpret_cast<const uint32_t*>(a.codes + m * a.groups * kPackGroup + c) : 0u;
-                sraw[e][i] = live ? a.scales[m * a.groups + c / kPackGroup] : 127u;
+                const uint8_t* const p = FEW ? a.codes + (base + min(c_row[e] + i, last)) * pitch + c_col[e]
+                                             : a.codes + (base + i) * pitch +
+                                                   static_cast<uint32_t>(c_row[e] * static_cast<int>(pitch) + c_col[e]);
+                r.c[e][i] = *reinterpret_cast<const uint32_t*>(p);
+            }
+            const uint8_t* const p = a.scales + (c_col[e] / kPackGroup) * a.scale_pitch + base;
+            if constexpr (FEW) {
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i / 4] |= static_cast<uint32_t>(p[min(c_row[e] + i, last)]) << (8 * (i & 3));
+                r.s[e] = make_uint2(w[0], w[1]);
+            } else {
+                __builtin_memcpy(&r.s[e], p + c_row[e], 8);  // of any alignment in the last stage
             }
         }
     };
-    auto store = [&](int stage) {
+    auto store = [&](Raw& r, int stage, int64_t m0) {
+        const int counted = static_cast<int>(m0 - base_of(m0)), rows = static_cast<int>(min(end - m0, (int64_t)kRows));
+        if (counted > 0 || (FEW && rows < kRows)) {
+#pragma unroll
+            for (int e = 0; e < G_EACH; ++e)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = g_row[e] + i;
+                    r.g[e][i] = row >= counted && (!FEW || row < rows) ? r.g[e][i] : 0u;
+                }
+        }
 #pragma unroll
         for (int e = 0; e < G_EACH; ++e) {
             const int item = tid + e * NT;
@@ -132,15 +176,15 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
             float x[2][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if constexpr (PAIRS) unpack2(graw[e][i], x[0][i], x[1][i], T());
-                else x[0][i] = __uint_as_float(graw[e][i]);
+                if constexpr (PAIRS) unpack2(r.g[e][i], x[0][i], x[1][i], T());
+                else x[0][i] = __uint_as_float(r.g[e][i]);
             }
 #pragma unroll
             for (int h = 0; h < (PAIRS ? 2 : 1); ++h) {
                 uint4 piece[PIECES];
                 cut<PIECES>(x[h], piece);
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p) gs[stage][p][kb][o + h] = piece[p];
+                for (int p = 0; p < PIECES; ++p) gs[stage][p][kb][o / (PAIRS ? 2 : 1) + h * (BO / 2)] = piece[p];
             }
         }
 #pragma unroll
@@ -152,12 +196,12 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float v[4];
-                pack8_values<SIGNED>(craw[e][i], pack8_scale(sraw[e][i]), v);
+                pack8_values<SIGNED>(r.c[e][i], pack8_scale((i < 4 ? r.s[e].x : r.s[e].y) >> (8 * (i & 3)) & 0xFFu), v);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j][i] = v[j];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) cut<1>(x[j], &cs[stage][kb][c + j]);
+            for (int j = 0; j < 4; ++j) cut<1>(x[j], &cs[stage][kb][c / 4 + j * (BI / 4)]);
         }
     };
 
@@ -170,15 +214,12 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const int wo = wave / WI * kTile, wi = wave % WI * kTile, col = lane & 31, half = lane >> 5;
 
-    if (first < end) {
-        load(first);
-        store(0);
-    }
-    __syncthreads();
-    int stage = 0;
-    for (int64_t m0 = first; m0 < end; m0 += kRows, stage ^= 1) {
-        const bool more = m0 + kRows < end;
-        if (more) load(m0 + kRows);
+    // A stage is written while slower waves may still
+    // read the other one; the barrier keeps them at most one apart.
+    auto step = [&](Raw& r, int stage, int64_t m0) {
+        store(r, stage, m0);
+        if constexpr (!FEW) load(r, m0 + 2 * kRows);
+        __syncthreads();
 #pragma unroll
         for (int kk = 0; kk < kRows / 16; ++kk) {
             bf16x8 b[2];
@@ -193,8 +234,17 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
                     for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, b[j], acc[i][j], 0, 0, 0);
                 }
         }
-        if (more) store(stage ^ 1);
-        __syncthreads();
+    };
+    if (first < end) {
+        load(raw[0], first);
+        load(raw[1], FEW ? first : first + kRows);
+        int64_t m0 = first;
+        if constexpr (!FEW)
+            for (; m0 + kRows < end; m0 += 2 * kRows) {
+                step(raw[0], 0, m0);
+                step(raw[1], 1, m0 + kRows);
+            }
+        if (m0 < end) step(raw[0], 0, m0);
     }
 
     float* const out = a.out + (int64_t)split * a.O * a.C;
@@ -202,10 +252,10 @@ __global__ __launch_bounds__(64 * WO * WI) void weight_grad8(const GradArgs a) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int c = c0 + wi + 32 * j + col;
+            const int c = c0 + c_of(wi + 32 * j + col);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int o = o0 + wo + 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+                const int o = o0 + o_of(wo + 32 * i + 8 * (e / 4) + 4 * half + e % 4);
                 if (o < a.O && c < a.C) out[(int64_t)o * a.C + c] = acc[i][j][e];
             }
         }
@@ -237,8 +287,8 @@ struct Split {
     int64_t rows_per_split;
 };
 
-// As many splits as give every CU its workgroups (16 waves of them), of at least 128
-// rows.  A workgroup has 8 waves at most (more spill their sums): where both sides
+// As many splits as give every CU its workgroups (8 waves of them, what their
+// registers allow), of at least 128 rows.  A workgroup has 8 waves at most (more spill their sums): where both sides
 // of the output are wide, it covers the columns first, because a second pass over
 // grad costs up to four times a second pass over the codes.
 Split split_of(int64_t rows, int32_t O, int32_t C) {
@@ -246,10 +296,11 @@ Split split_of(int64_t rows, int32_t O, int32_t C) {
     s.wo = waves_for(O);
     s.wi = waves_for(C);
     if (s.wo * s.wi > 8) s.wo = 2;
+    if (rows < kRows) s.wo = s.wi = 1;
     s.tiles_o = (O + s.wo * kTile - 1) / (s.wo * kTile);
     s.tiles_c = (C + s.wi * kTile - 1) / (s.wi * kTile);
     const int64_t tiles = (int64_t)s.tiles_o * s.tiles_c;
-    const int64_t wanted = std::max<int64_t>(1, 256 * std::min(4, 16 / (s.wo * s.wi)) / tiles);
+    const int64_t wanted = std::max<int64_t>(1, 256 * std::min(4, 8 / (s.wo * s.wi)) / tiles);
     const int64_t per = std::max<int64_t>(128, (rows + wanted - 1) / wanted);
     s.rows_per_split = (per + kRows - 1) / kRows * kRows;
     s.splits = static_cast<int>(std::max<int64_t>(1, (rows + s.rows_per_split - 1) / s.rows_per_split));
@@ -261,8 +312,12 @@ void launch(const Split& s, const GradArgs& a, hipStream_t st) {
     const unsigned grid = static_cast<unsigned>(s.splits) * s.tiles_o * s.tiles_c;
     auto go = [&](auto wo, auto wi) {
         constexpr int WO = decltype(wo)::value, WI = decltype(wi)::value;
-        weight_grad8<T, WO, WI, SIGNED><<<grid, 64 * WO * WI, 0, st>>>(a);
+        weight_grad8<T, WO, WI, SIGNED, false><<<grid, 64 * WO * WI, 0, st>>>(a);
     };
+    if (a.rows < kRows) {
+        weight_grad8<T, 1, 1, SIGNED, true><<<grid, 64, 0, st>>>(a);
+        return;
+    }
     auto by_wi = [&](auto wo) {
         if (s.wi == 1) go(wo, std::integral_constant<int, 1>());
         else if (s.wi == 2) go(wo, std::integral_constant<int, 2>());
@@ -275,7 +330,7 @@ void launch(const Split& s, const GradArgs& a, hipStream_t st) {
 
 ra_status check(int64_t rows, int32_t O, int32_t C) {
     if (rows < 0 || O < 1 || C < 1) return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: bad sizes");
-    if (rows > INT64_MAX / 8 / ((int64_t)C + 64) || (int64_t)O * C > INT32_MAX)
+    if (rows > INT64_MAX / 8 / ((int64_t)C + 64) || (int64_t)O * C > INT32_MAX || C > (1 << 26))
         return fail(RA_ERR_UNSUPPORTED, "weight_grad8: too large");
     return RA_OK;
 }
@@ -304,9 +359,10 @@ ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint
         return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: unknown dtype");
     if (!d_out || (rows > 0 && (!d_grad || !d_codes || !d_scales)))
         return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: NULL tensor");
+    if (ldg >= int64_t{1} << 26) return fail(RA_ERR_UNSUPPORTED, "weight_grad8: rows lie at most 2^26 elements apart");
     if (rows > 1 && ldg < out) return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: rows overlap (a leading dimension is too small)");
-    if (!ra::aligned16(d_codes) || !ra::aligned16(d_workspace) || bytes < need || (need && !d_workspace))
-        return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: the workspace is too small, or it or the codes are not 16-byte aligned");
+    if (!ra::aligned16(d_codes) || !ra::aligned16(d_scales) || !ra::aligned16(d_workspace) || bytes < need || (need && !d_workspace))
+        return fail(RA_ERR_INVALID_ARGUMENT, "weight_grad8: the workspace is too small, or it, the codes or the scales are not 16-byte aligned");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const ra::Split s = ra::split_of(rows, out, cols);
     ra::GradArgs a{};
@@ -320,6 +376,7 @@ ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint
     a.O = out;
     a.C = cols;
     a.groups = ra::pack8_groups(cols);
+    a.scale_pitch = ra::pack8_scale_pitch(rows);
     a.tiles_o = s.tiles_o;
     a.tiles_c = s.tiles_c;
     a.splits = s.splits;

@@ -27,7 +27,7 @@ from .attention import _rows
 
 class Packed8(NamedTuple):
     codes: torch.Tensor   # uint8 [rows, cols rounded up to 32]
-    scales: torch.Tensor  # uint8 [rows, groups]: exponent + 127, 255 for a group that was not finite
+    scales: torch.Tensor  # uint8 [groups, rows rounded up to 8]: exponent + 127, 255 for a group that was not finite
     cols: int
     signed: bool
 
