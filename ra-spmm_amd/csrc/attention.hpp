@@ -340,32 +340,41 @@ struct Place {
 // forward: 1.66 against 1.81 ms; skewed fp32 rows 0.50 against 0.61).
 constexpr int kDeep = 2;
 
-// The next kDeep edges of every slot.  Past the end the last edge again.
+// The next DEEP edges of every slot.  Past the end the last edge again.
+template <int DEEP>
 struct Edges {
-    uint32_t other[kDeep];
-    float add[kDeep];  // bias in powers of two, where there is one
+    uint32_t other[DEEP];
+    float add[DEEP];  // bias in powers of two, where there is one
 };
 
-template <bool TRANSPOSED>
-__device__ __forceinline__ void load_edges(const AttnArgs& a, Edges& x, int e0, int end, int es, int slots) {
+// left: edges from e0 on, at least 1.  A uniform address and a lane's offset (opaque
+// to the compiler, which would widen it to 64 bits).
+template <bool TRANSPOSED, int DEEP>
+__device__ __forceinline__ void load_edges(const AttnArgs& a, Edges<DEEP>& x, int e0, int left, int es, int slots) {
+    const uint32_t last = static_cast<uint32_t>(min(left - 1, 255)) * 4;  // a step has at most 64 edges
+    auto take = [](const auto* p, uint32_t bytes) {
+        return *reinterpret_cast<decltype(p)>(reinterpret_cast<const char*>(p) + bytes);
+    };
+    uint32_t at[DEEP];
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) x.other[d] = a.idx[min(e0 + d * slots + es, end - 1)];
+    for (int d = 0; d < DEEP; ++d) {
+        at[d] = min(static_cast<uint32_t>(d * slots + es) * 4, last);
+        asm("" : "+v"(at[d]));
+        x.other[d] = take(a.idx + e0, at[d]);
+    }
     if (a.bias) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const int e = min(e0 + d * slots + es, end - 1);
-            x.add[d] = a.bias[TRANSPOSED ? a.edge[e] : e];
-        }
+        for (int d = 0; d < DEEP; ++d) x.add[d] = TRANSPOSED ? a.bias[take(a.edge + e0, at[d])] : take(a.bias + e0, at[d]);
     }
 }
 // Live edges of a step: in the list (a LAST step only may pass its end), and not
 // left out by their bias, which becomes powers of two here.  A finite bias is kept
 // finite: beyond +-2e38 all are equal.
-template <int DEEP, bool LAST>
-__device__ __forceinline__ void close_edges(const AttnArgs& a, Edges& x, bool* live, int e0, int end, int es, int slots) {
+template <int DEEP, bool LAST, int N>
+__device__ __forceinline__ void close_edges(const AttnArgs& a, Edges<N>& x, bool* live, int left, int es, int slots) {
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
-        live[d] = !LAST || e0 + d * slots + es < end;
+        live[d] = !LAST || d * slots + es < left;
         if (!a.bias) x.add[d] = 0.f;
     }
     if (a.bias) {
@@ -438,7 +447,9 @@ struct Gather {
             delta[i] = there[i] ? i * kPacket : 0;
         }
     }
-    __device__ __forceinline__ void load(Run<T, N>& r, uint32_t row, uint32_t pitch) const {
+    // further: bytes from the run, the same in all lanes.
+    __device__ __forceinline__ void load(Run<T, N>& r, uint32_t row, uint32_t pitch, int further = 0) const {
+        const char* const base = this->base + further;
         uint32_t* const w = reinterpret_cast<uint32_t*>(r.w);
 #pragma unroll
         for (int i = 0; i < kPackets; ++i) {

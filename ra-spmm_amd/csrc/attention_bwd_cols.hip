@@ -14,8 +14,9 @@
 namespace ra {
 namespace {
 
-template <typename T, int LM, int NV, int PB, bool WIDE>
-__global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
+// ONE: a key/value head has one query head.
+template <typename T, int LM, int NV, int PB, bool WIDE, bool ONE>
+__device__ __forceinline__ void attn_cols(const AttnArgs& a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.kv_heads);
@@ -32,30 +33,38 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) dv[i] = 0.f;
 
-    Edges now, next;
-    if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end, p.es, slots);
+    // Of the first of the head's query heads; the others lie `sub` strides further on.
+    const int first = ONE ? p.head : p.head * a.group;
+    const Gather<T, 8, PB, WIDE> q(a.q, (first * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
+    const Gather<T, NV, PB, WIDE> g(a.grad, first * a.value_dim, NV * p.l, p.vcount);
+    const uint64_t record_first = first * a.record_head + p.map * sizeof(float4);
+    const float lam = a.lam[first];
+
+    Edges<kDeep> now, next;
+    if (u.begin < u.end) load_edges<true>(a, now, u.begin, u.end - u.begin, p.es, slots);
     over_edges(u.begin, u.end, slots, [&](auto deep, auto is_last, int e0) {
         constexpr int DEEP = decltype(deep)::value;
         constexpr bool LAST = decltype(is_last)::value;
-        if constexpr (!LAST) load_edges<true>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
+        if constexpr (!LAST) load_edges<true>(a, next, e0 + kDeep * slots, u.end - e0 - kDeep * slots, p.es, slots);
         bool live[DEEP];
-        close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
-        for (int sub = 0; sub < a.group; ++sub) {
-            const int qh = p.head * a.group + sub;
-            const Gather<T, 8, PB, WIDE> q(a.q, (qh * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
-            const Gather<T, NV, PB, WIDE> g(a.grad, qh * a.value_dim, NV * p.l, p.vcount);
-            const char* const record = reinterpret_cast<const char*>(a.record) + qh * a.record_head + p.map * sizeof(float4);
-            const float c = p.map == 0 ? 1.f : -a.lam[qh];
+        close_edges<DEEP, LAST>(a, now, live, u.end - e0, p.es, slots);
+        for (int sub = 0; sub < (ONE ? 1 : a.group); ++sub) {
+            const char* const record = reinterpret_cast<const char*>(a.record) + sub * a.record_head;
             Run<T, 8> qr[DEEP];
             Run<T, NV> gr[DEEP];
             float4 st[DEEP];  // maximum, 1 / sum, delta
 #pragma unroll
             for (int d = 0; d < DEEP; ++d) {
-                q.load(qr[d], now.other[d], a.q_pitch);
-                g.load(gr[d], now.other[d], a.g_pitch);
-                const uint64_t at = WIDE ? static_cast<uint64_t>(now.other[d]) * a.record_row : __umul24(now.other[d], a.record_row);
-                st[d] = *reinterpret_cast<const float4*>(record + at);
+                q.load(qr[d], now.other[d], a.q_pitch, sub * 2 * a.head_dim * (int)sizeof(T));
+                g.load(gr[d], now.other[d], a.g_pitch, sub * a.value_dim * (int)sizeof(T));
+                if constexpr (WIDE)
+                    st[d] = *reinterpret_cast<const float4*>(record + (uint64_t)now.other[d] * a.record_row + record_first);
+                else
+                    st[d] = *reinterpret_cast<const float4*>(record + (__umul24(now.other[d], a.record_row) +
+                                                                       static_cast<uint32_t>(record_first)));
             }
+            float c = p.map == 0 ? 1.f : -lam;
+            if (sub > 0) c = p.map == 0 ? 1.f : -a.lam[first + sub];
             __builtin_amdgcn_sched_barrier(0);
             if (LAST || a.ragged || a.bias) {
 #pragma unroll
@@ -99,6 +108,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_cols(const AttnArgs a) {
     store_scattered<T, NV, PB == 16>(static_cast<T*>(a.out2) + at * a.value_dim + NV * p.l, dv, slots, p.vcount);
 }
 
+template <typename T, int LM, int NV, int PB, bool WIDE>
+__global__ __launch_bounds__(kAttnThreads) void attn_cols_one(const AttnArgs a) {
+    attn_cols<T, LM, NV, PB, WIDE, true>(a);
+}
+template <typename T, int LM, int NV, int PB, bool WIDE>
+__global__ __launch_bounds__(kAttnThreads) void attn_cols_many(const AttnArgs a) {
+    attn_cols<T, LM, NV, PB, WIDE, false>(a);
+}
+
 // Joins a cut column's pieces: plain sums of every element, in order.  Threads are
 // four piece groups x 64 elements.
 template <typename T>
@@ -127,7 +145,8 @@ ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a
     unsigned blocks = 0;
     RA_TRY(attn_grid(a, blocks));
     if (blocks == 0) return RA_OK;
-    RA_ATTN_DISPATCH(attn_cols, dtype, l, dim3(blocks), st, a);
+    if (a.group == 1) RA_ATTN_DISPATCH(attn_cols_one, dtype, l, dim3(blocks), st, a);
+    else RA_ATTN_DISPATCH(attn_cols_many, dtype, l, dim3(blocks), st, a);
     RA_LAUNCH_CHECK("attn_cols");
     return RA_OK;
 }

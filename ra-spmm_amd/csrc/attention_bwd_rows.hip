@@ -15,8 +15,10 @@
 namespace ra {
 namespace {
 
+// Six waves a SIMD for 16-bit types (82 registers without the bound; power-law graph
+// of 1e6 rows: 1.73 against 1.83 ms).
 template <typename T, int LM, int NV, int PB, bool WIDE>
-__global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 6 : 4) void attn_rows(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);
@@ -24,8 +26,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
     const Gather<T, 8, PB, WIDE> k(a.k, (kv * 2 + p.map) * a.head_dim, 8 * p.lm, p.kcount);
     const Gather<T, NV, PB, WIDE> v(a.v, kv * a.value_dim, NV * p.l, p.vcount);
 
-    Edges now, next;
-    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end, p.es, slots);
+    Edges<kDeep> now, next;
+    if (u.begin < u.end) load_edges<false>(a, now, u.begin, u.end - u.begin, p.es, slots);
     Run<T, 8> q;
     load_run<T, 8, PB == 16>(
         q, static_cast<const T*>(a.q) + u.row * a.ldq + (int64_t)(p.head * 2 + p.map) * a.head_dim + 8 * p.lm, p.kcount);
@@ -49,10 +51,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows(const AttnArgs a) {
             k.load(kr[d], now.other[d], a.k_pitch);
             v.load(vr[d], now.other[d], a.v_pitch);
         }
-        if constexpr (!LAST) load_edges<false>(a, next, e0 + kDeep * slots, u.end, p.es, slots);
+        if constexpr (!LAST) load_edges<false>(a, next, e0 + kDeep * slots, u.end - e0 - kDeep * slots, p.es, slots);
         __builtin_amdgcn_sched_barrier(0);
         bool live[DEEP];
-        close_edges<DEEP, LAST>(a, now, live, e0, u.end, p.es, slots);
+        close_edges<DEEP, LAST>(a, now, live, u.end - e0, p.es, slots);
         if (LAST || a.ragged || a.bias) {
 #pragma unroll
             for (int d = 0; d < DEEP; ++d) {

@@ -533,7 +533,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
         a.hb_shift = l.hb_shift;
         a.ragged = l.ragged;
         ra::side_of(a, cols, cols_by_head);
-        a.wide = !ra::narrow(M, {a.q_pitch, a.g_pitch, a.record_row});
+        a.wide = !ra::narrow(M, {a.q_pitch, a.g_pitch, static_cast<uint32_t>(s.q_heads * 2 * sizeof(float4))});
         a.out = d_dk;
         a.out2 = d_dv;
         RA_TRY(ra::attn_cols_launch(s.dtype, l, a, st));

@@ -137,7 +137,8 @@ def test_heads_and_types(heads, dtype):
 
 
 @pytest.mark.parametrize("lengths,K", [([0], 1), ([1], 1), ([1, 0, 1], 2), ([257], 300), ([256, 255, 512, 513], 600),
-                                       ([3000, 0, 2, 777], 3000), ([40] * 300, 7), ([2] * 700, 3), ([0] * 9, 5)], ids=str)
+                                       ([3000, 0, 2, 777], 3000), ([40] * 300, 7), ([2] * 700, 3), ([0] * 9, 5),
+                                       ([127, 128, 129, 130, 15, 16, 17, 64, 65], 200), ([3] * 3000 + [2000], 2500)], ids=lambda x: str(x)[:40])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_lengths_and_hubs(lengths, K, dtype):
     """Rows and columns of no, one and thousands of edges, cut and joined on both sides; duplicate edges."""
@@ -270,9 +271,9 @@ def test_equal_inputs_give_equal_bits():
 
 
 def test_plan_arrays():
-    lengths, K = [0, 1, 256, 257, 700, 3], 50
+    lengths, K = [0, 1, 128, 129, 256, 257, 700, 3], 50
     rowptr, colind = lists(lengths, K, 3)
-    plan = ra_spmm.make_attention_plan(rowptr.cuda(), colind.cuda(), 6, K)
+    plan = ra_spmm.make_attention_plan(rowptr.cuda(), colind.cuda(), 8, K)
     for side, ptr in (("", rowptr.numpy()), ("_t", ra_spmm.export_attention_plan(plan, "rowptr_t").numpy())):
         want, splits, slot = [], [], 0
         for r in range(len(ptr) - 1):
@@ -286,7 +287,7 @@ def test_plan_arrays():
         assert ra_spmm.export_attention_plan(plan, "items" + side).view(-1, 4).tolist() == [list(x) for x in want]
         assert ra_spmm.export_attention_plan(plan, "splits" + side).view(-1, 4).tolist() == [list(x) for x in splits]
     order = np.argsort(colind.numpy(), kind="stable")
-    rows = np.repeat(np.arange(6), lengths)
+    rows = np.repeat(np.arange(8), lengths)
     assert (ra_spmm.export_attention_plan(plan, "edge_t").numpy() == order).all()
     assert (ra_spmm.export_attention_plan(plan, "row_t").numpy() == rows[order]).all()
     counts = np.bincount(colind.numpy(), minlength=K)
