@@ -15,10 +15,10 @@
 namespace ra {
 namespace {
 
-// Six waves a SIMD for 16-bit types (82 registers without the bound; power-law graph
+// Six waves a SIMD for whole packets of 16-bit types (82 registers without the bound; power-law graph
 // of 1e6 rows: 1.73 against 1.83 ms).
 template <typename T, int LM, int NV, int PB, bool WIDE>
-__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 6 : 4) void attn_rows(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, PB == 16 ? (sizeof(T) == 2 ? 6 : 4) : 1) void attn_rows(const AttnArgs a) {
     const Unit u = unit_of(a);
     if (!u.live) return;
     const Place<LM, NV> p(a, u.head_block, a.q_heads);

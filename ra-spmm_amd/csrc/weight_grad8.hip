@@ -26,7 +26,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRows = 32;  // rows of a stage
 constexpr int kTile = 64;  // a wave's part of the output, both ways
-constexpr int kWavesPerSimd = 2;
 
 struct GradArgs {
     const void* grad;
@@ -67,9 +66,13 @@ __device__ __forceinline__ void cut(const float* x, uint4* piece) {
                               high_halves(word[p][4], word[p][5]), high_halves(word[p][6], word[p][7]));
 }
 
+// Waves a SIMD that shared memory leaves room for: the three pieces of float32 take 24 KB for every wave of WO.
+template <typename T, int WO, int WI>
+constexpr int kWavesPerSimd = kPieces<T> == 3 && WO > 1 && WI == 1 ? 1 : 2;
+
 // WO x WI waves.
 template <typename T, int WO, int WI, bool SIGNED, bool FEW>
-__global__ __launch_bounds__(64 * WO * WI, kWavesPerSimd) void weight_grad8(const GradArgs a) {
+__global__ __launch_bounds__(64 * WO * WI, (kWavesPerSimd<T, WO, WI>)) void weight_grad8(const GradArgs a) {
     constexpr int PIECES = kPieces<T>, BO = WO * kTile, BI = WI * kTile, NT = 64 * WO * WI, KB = kRows / 8;
     constexpr bool PAIRS = sizeof(T) == 2;
     // Staging work: (8 rows, column or pair of columns) of grad, (8 rows, 4 columns)
