@@ -110,8 +110,10 @@ class _Linear8(torch.autograd.Function):
 def linear8(x: torch.Tensor, weight: torch.Tensor, packed: Optional[Packed8] = None) -> torch.Tensor:
     """x W^T that keeps its input in 8 bits: in `packed` where the caller has it (relu8), else packed here.  The weight
     gradient is that of the kept values."""
+    if packed is not None and (packed.cols != x.size(1) or packed.codes.size(0) != x.size(0)):
+        raise RuntimeError(f"linear8: packed holds [{packed.codes.size(0)}, {packed.cols}], x is {tuple(x.shape)}")
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        return F.linear(x, weight)  # nothing to keep
     if packed is None:
         return _Linear8.apply(_rows(x), weight, None, None, True)
-    if packed.cols != x.size(1) or packed.codes.size(0) != x.size(0):
-        raise RuntimeError(f"linear8: packed holds [{packed.codes.size(0)}, {packed.cols}], x is {tuple(x.shape)}")
     return _Linear8.apply(x, weight, packed.codes, packed.scales, packed.signed)
