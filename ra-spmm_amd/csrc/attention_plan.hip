@@ -79,28 +79,25 @@ __global__ __launch_bounds__(kThreads) void read_totals(const unsigned long long
     out->splits = splits[rows];
 }
 
-// Row of every edge: the edges of 256 consecutive ones lie in few rows, found by
-// bisection.
 __global__ __launch_bounds__(kThreads) void edge_numbers(int64_t n, int32_t* __restrict__ out) {
     const int64_t stride = (int64_t)gridDim.x * kThreads;
     for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < n; e += stride) out[e] = static_cast<int32_t>(e);
 }
 
-// Last row whose first edge is at most e.
-__device__ __forceinline__ int32_t row_of(const int32_t* __restrict__ ptr, int32_t rows, int32_t e) {
-    int32_t lo = 0, hi = rows;  // ptr[lo] <= e < ptr[hi]
-    while (hi - lo > 1) {
-        const int32_t mid = lo + (hi - lo) / 2;
-        if (ptr[mid] <= e) lo = mid;
-        else hi = mid;
+// Row of every edge in CSR order, a wave for each piece.
+__global__ __launch_bounds__(kThreads) void edge_rows(const int4* __restrict__ items, int32_t num_items,
+                                                      int32_t* __restrict__ out) {
+    const int64_t waves = (int64_t)gridDim.x * (kThreads / 64);
+    for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 6; i < num_items; i += waves) {
+        const int4 it = items[i];
+        for (int64_t e = (int64_t)it.y + (threadIdx.x & 63); e < it.z; e += 64) out[e] = it.x;
     }
-    return lo;
 }
 
-__global__ __launch_bounds__(kThreads) void transposed_rows(const int32_t* __restrict__ ptr, int32_t rows, int64_t n,
+__global__ __launch_bounds__(kThreads) void transposed_rows(const int32_t* __restrict__ rows, int64_t n,
                                                             const int32_t* __restrict__ edge, int32_t* __restrict__ out) {
     const int64_t stride = (int64_t)gridDim.x * kThreads;
-    for (int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x; t < n; t += stride) out[t] = row_of(ptr, rows, edge[t]);
+    for (int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x; t < n; t += stride) out[t] = rows[edge[t]];
 }
 
 // First sorted key that is at least i, for i = 0 .. K.
@@ -188,7 +185,10 @@ ra_status transpose(ra_attn_plan* p, hipStream_t st) {
         // Stable: a column's rows stay in ascending order.
         RA_HIP_TRY(hipcub::DeviceRadixSort::SortPairs(work.get(), sort, r.idx, keys, numbers, edge,
                                                       static_cast<int>(nnz), 0, bits, st));
-        transposed_rows<<<grid, kThreads, 0, st>>>(r.ptr, r.rows, nnz, edge, row);
+        // The rows are written in order and gathered once; 0.49 ms at 23e6 edges, each found by bisection 1.25.
+        edge_rows<<<std::min(blocks_for((int64_t)r.num_items * 64), 1u << 20), kThreads, 0, st>>>(r.items, r.num_items, numbers);
+        RA_LAUNCH_CHECK("edge_rows");
+        transposed_rows<<<grid, kThreads, 0, st>>>(numbers, nnz, edge, row);
         RA_LAUNCH_CHECK("transposed_rows");
     }
     transposed_ptr<<<blocks_for(K + 1), kThreads, 0, st>>>(keys, nnz, p->info.K, ptr);
