@@ -469,3 +469,11 @@ def test_heads_kept_apart(side):
         rowptr, colind = lists(rng.integers(0, 3, many), few, 5)
         M, K = many, few
     check(rowptr, colind, inputs(M, K, 4, 4, 32, 64, torch.bfloat16, 6))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_many_cut_rows(dtype):
+    """More joining workgroups than are resident at once; the lists' rows hold 2 and 3 pieces."""
+    print(f"[attention] cut rows {dtype}", flush=True)
+    rowptr, colind = lists([260, 600] * 300, 500, 12)
+    check(rowptr, colind, inputs(600, 500, 4, 4, 16, 32, dtype, 13))
