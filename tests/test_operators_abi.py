@@ -68,6 +68,8 @@ def test_attention_arguments_are_refused():
     assert call(q=None) == INVALID and call(lam=None) == INVALID and call(M=-1) == INVALID and call(nnz=1 << 40) == INVALID
     assert call(out=odd) == INVALID and b"aligned" in lib.ra_last_error()
     assert call(M=0, nnz=0) == OK  # nothing to do
+    # a wave for every row at least: a launch holds fewer than 2^32 threads
+    assert call(M=1 << 26, nnz=0) == UNSUPPORTED and b"too many" in lib.ra_last_error()
     p = ctypes.c_void_p()
     assert lib.ra_attn_plan_create(None, None, 3, 3, 5, 1, None, ctypes.byref(p)) == INVALID
     assert lib.ra_attn_plan_create(fake, fake, 3, 3, 1 << 32, 1, None, ctypes.byref(p)) == UNSUPPORTED
