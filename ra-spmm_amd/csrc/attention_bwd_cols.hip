@@ -146,6 +146,8 @@ ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a
     unsigned blocks = 0;
     RA_TRY(attn_grid(a, blocks));
     if (blocks == 0) return RA_OK;
+    // Without the loop over a head's query heads: power-law graph of 1e6 rows 1.88 against 2.04 ms, social graph of
+    // 50,000 rows of 80 472 against 504 us.
     if (a.group == 1) RA_ATTN_DISPATCH(attn_cols_one, dtype, l, dim3(blocks), st, a);
     else RA_ATTN_DISPATCH(attn_cols_many, dtype, l, dim3(blocks), st, a);
     RA_LAUNCH_CHECK("attn_cols");

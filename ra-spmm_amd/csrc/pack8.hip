@@ -5,8 +5,8 @@
 // run in whole packets, the group's largest magnitude takes two exchanges within the
 // four lanes, and the codes go out as 8 bytes a lane.  The scale is a power of two,
 // so code * scale and x / scale are exact and rounding happens once.  Measured: ReLU and
-// pack of 1e6 x 256 fp32 428 us (2.31 GB, 5.4 TB/s), the ReLU's gradient 432 (5.3); 512,000 x
-// 128 in bf16 51 and 55 us (6.5 and 6.0 TB/s, partly from the last-level cache); a large copy
+// pack of 1e6 x 256 fp32 428 us (2.31 GB, 5.4 TB/s), the ReLU's gradient 424 (5.4); 512,000 x
+// 128 in bf16 51 and 53 us (6.5 and 6.2 TB/s, partly from the last-level cache); a large copy
 // reaches 5.1.
 #include <type_traits>
 
@@ -29,7 +29,8 @@ struct PackArgs {
 
 // A wave takes 16 * STEPS consecutive (row, group) pairs, 16 at a time, with all
 // steps' loads in flight together: 4 steps where that leaves enough waves (a wave for
-// every slot of the GPU), else 1 (10,000 rows of 2 groups: 3.5 against 5 us).
+// every slot of the GPU; pack of 512,000 x 128 bf16 53 against 63 us, of 1e6 x 256 fp32 436
+// against 448), else 1 (10,000 rows of 2 groups: 3.5 against 5 us).
 constexpr int64_t kManyPairs = 64 * 8192;
 struct Spot {
     int64_t row;
@@ -150,34 +151,27 @@ __global__ __launch_bounds__(kThreads) void unpack8(const PackArgs a) {
     }
 }
 
-template <typename T, bool VEC, int STEPS>
+// One step a wave: it has two loads in flight already (1e6 x 256 fp32: 424 against 431 us with
+// four steps, 512,000 x 128 bf16: 53 against 55).
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void relu_grad8(const PackArgs a) {
     const int lane = threadIdx.x & 63;
-    for (int64_t first = first_pair<STEPS>(); first < a.rows * a.groups; first += pair_step<STEPS>()) {
-        Spot at[STEPS];
-        uint2 w[STEPS];
-        Run<T, 8> r[STEPS];
+    for (int64_t first = first_pair<1>(); first < a.rows * a.groups; first += pair_step<1>()) {
+        const Spot at(first + (lane >> 2), a);
+        Run<T, 8> r;
+        const uint2 w = *reinterpret_cast<const uint2*>(a.codes + at.code(a));
+        load_run<T, 8, VEC>(r, static_cast<const T*>(a.x) + at.row * a.ld + at.col, at.count);
+        float x[8];
+        r.to_float(x);
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            at[i] = Spot(first + 16 * i + (lane >> 2), a);
-            w[i] = *reinterpret_cast<const uint2*>(a.codes + at[i].code(a));
-            load_run<T, 8, VEC>(r[i], static_cast<const T*>(a.x) + at[i].row * a.ld + at[i].col, at[i].count);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            float x[8];
-            r[s].to_float(x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = (i < 4 ? w[s].x : w[s].y) >> (8 * (i & 3)) & 0xFFu ? x[i] : 0.f;
-            if (at[s].live) store_run<T, 8, VEC>(static_cast<T*>(a.y) + at[s].row * a.cols + at[s].col, x, at[s].count);
-        }
+        for (int i = 0; i < 8; ++i) x[i] = (i < 4 ? w.x : w.y) >> (8 * (i & 3)) & 0xFFu ? x[i] : 0.f;
+        if (at.live) store_run<T, 8, VEC>(static_cast<T*>(a.y) + at.row * a.cols + at.col, x, at.count);
     }
 }
 
 int steps_for(const PackArgs& a) { return a.rows * a.groups >= kManyPairs ? 4 : 1; }
-unsigned grid_for(const PackArgs& a) {
-    const int64_t per = kThreads / 64 * 16 * steps_for(a);
+unsigned grid_for(const PackArgs& a, int steps) {
+    const int64_t per = kThreads / 64 * 16 * steps;
     return static_cast<unsigned>(std::min<int64_t>((a.rows * a.groups + per - 1) / per, 65536));
 }
 
@@ -243,7 +237,7 @@ ra_status ra_pack8(const void* d_x, int64_t rows, int32_t cols, int64_t ldx, int
     const ra::PackArgs a = ra::args_of(d_x, nullptr, d_codes, d_scales, rows, cols, ldx);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::by_type(dtype, a, [&](auto tag, auto vec, auto steps) {
-        ra::pack8<decltype(tag), decltype(vec)::value, false, decltype(steps)::value><<<ra::grid_for(a), ra::kThreads, 0, st>>>(a);
+        ra::pack8<decltype(tag), decltype(vec)::value, false, decltype(steps)::value><<<ra::grid_for(a, steps), ra::kThreads, 0, st>>>(a);
     });
     RA_LAUNCH_CHECK("pack8");
     return RA_OK;
@@ -257,7 +251,7 @@ ra_status ra_relu_pack8(const void* d_x, int64_t rows, int32_t cols, int64_t ldx
     const ra::PackArgs a = ra::args_of(d_x, d_y, d_codes, d_scales, rows, cols, ldx);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::by_type(dtype, a, [&](auto tag, auto vec, auto steps) {
-        ra::pack8<decltype(tag), decltype(vec)::value, true, decltype(steps)::value><<<ra::grid_for(a), ra::kThreads, 0, st>>>(a);
+        ra::pack8<decltype(tag), decltype(vec)::value, true, decltype(steps)::value><<<ra::grid_for(a, steps), ra::kThreads, 0, st>>>(a);
     });
     RA_LAUNCH_CHECK("relu_pack8");
     return RA_OK;
@@ -272,8 +266,8 @@ ra_status ra_unpack8(const uint8_t* d_codes, const uint8_t* d_scales, int64_t ro
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::by_type(dtype, a, [&](auto tag, auto vec, auto steps) {
         using T = decltype(tag);
-        if (is_signed) ra::unpack8<T, decltype(vec)::value, true, decltype(steps)::value><<<ra::grid_for(a), ra::kThreads, 0, st>>>(a);
-        else ra::unpack8<T, decltype(vec)::value, false, decltype(steps)::value><<<ra::grid_for(a), ra::kThreads, 0, st>>>(a);
+        if (is_signed) ra::unpack8<T, decltype(vec)::value, true, decltype(steps)::value><<<ra::grid_for(a, steps), ra::kThreads, 0, st>>>(a);
+        else ra::unpack8<T, decltype(vec)::value, false, decltype(steps)::value><<<ra::grid_for(a, steps), ra::kThreads, 0, st>>>(a);
     });
     RA_LAUNCH_CHECK("unpack8");
     return RA_OK;
@@ -286,8 +280,8 @@ ra_status ra_relu_grad8(const void* d_grad, const uint8_t* d_codes, int64_t rows
     if (!d_grad || !d_out) return fail(RA_ERR_INVALID_ARGUMENT, "relu_grad8: NULL tensor");
     const ra::PackArgs a = ra::args_of(d_grad, d_out, d_codes, nullptr, rows, cols, ldg);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    ra::by_type(dtype, a, [&](auto tag, auto vec, auto steps) {
-        ra::relu_grad8<decltype(tag), decltype(vec)::value, decltype(steps)::value><<<ra::grid_for(a), ra::kThreads, 0, st>>>(a);
+    ra::by_type(dtype, a, [&](auto tag, auto vec, auto) {
+        ra::relu_grad8<decltype(tag), decltype(vec)::value><<<ra::grid_for(a, 1), ra::kThreads, 0, st>>>(a);
     });
     RA_LAUNCH_CHECK("relu_grad8");
     return RA_OK;
