@@ -306,7 +306,7 @@ bool same_device(const ra_attn_plan* p) {
 
 }  // namespace
 
-// Waves of one round: 4 for each of the 1024 SIMDs.  Below it one head a wave: 4 new rows of 6,000 edges,
+// Waves that run at once: 4 for each of the 1024 SIMDs.  Below it one head a wave: 4 new rows of 6,000 edges,
 // 8 heads: 9.7 us, 16.3 with all heads in a wave.
 constexpr int64_t kFewWaves = 4096;
 
