@@ -17,12 +17,8 @@ s_a[j] = scale * q_a[i, h] . k_a[j, g] + bias[ij] over the row's columns j; p_a 
 sum_j (p_1 - lam[h] * p_2)[j] * v[j, g].  An edge with bias -inf takes no part; a row without edges gives zeros.
 """
 import math
-import os
-import sys
 
 import torch
-
-sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ra-spmm_amd"))
 
 own = False
 
