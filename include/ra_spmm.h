@@ -424,7 +424,8 @@ ra_status ra_attn_plan_export(const ra_attn_plan* plan, const char* name, int32_
 void ra_attn_plan_destroy(ra_attn_plan* plan);
 /* d_stats: [M, q_heads, 2, 2] fp32, what the backward pass needs (maximum in powers
  * of two and 1/sum of every softmax), or NULL.  Grows the plan's scratch at the first call of a
- * larger shape. */
+ * larger shape, which a stream capture refuses; a captured run keeps the scratch that it has, whatever
+ * runs later, and needs the plan for as long as it is replayed. */
 ra_status ra_attn_plan_run(ra_attn_plan* plan, const ra_attn_shape* shape, const void* d_q, const void* d_k,
                            const void* d_v, const float* d_lam, const float* d_bias, void* d_out, float* d_stats,
                            ra_stream_t stream);

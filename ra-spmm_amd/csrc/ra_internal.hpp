@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <cstdio>
 #include <functional>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
@@ -74,16 +75,11 @@ public:
     ~DeviceBuffer() { reset(); }
     DeviceBuffer(const DeviceBuffer&) = delete;
     DeviceBuffer& operator=(const DeviceBuffer&) = delete;
-    DeviceBuffer(DeviceBuffer&& o) noexcept : ptr_(o.ptr_), bytes_(o.bytes_), device_(o.device_) {
-        o.ptr_ = nullptr;
-        o.bytes_ = 0;
-    }
+    DeviceBuffer(DeviceBuffer&& o) noexcept { swap(o); }
     DeviceBuffer& operator=(DeviceBuffer&& o) noexcept {
         if (this != &o) {
             reset();
-            std::swap(ptr_, o.ptr_);
-            std::swap(bytes_, o.bytes_);
-            std::swap(device_, o.device_);
+            swap(o);
         }
         return *this;
     }
@@ -103,12 +99,30 @@ public:
     }
     // Grow-only reuse (plan scratch) for work on `stream`.  While that is being
     // captured the driver decides: it refuses, and the run that sizes the scratch
-    // has to come before the capture whatever the pool holds.
+    // has to come before the capture whatever the pool holds.  A block that was
+    // handed to a capture is named by its graph: growth leaves it where it is, for
+    // replays, until the owner goes.
     ra_status ensure(size_t bytes, hipStream_t stream) {
-        if (bytes <= bytes_) return RA_OK;
+        if (bytes == 0) return RA_OK;
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(stream, &capture) != hipSuccess) (void)hipGetLastError();
-        return allocate(bytes, capture == hipStreamCaptureStatusNone);
+        const bool capturing = capture != hipStreamCaptureStatusNone;
+        if (bytes > bytes_) {
+            DeviceBuffer* named = nullptr;
+            if (captured_) {
+                named = new (std::nothrow) DeviceBuffer(std::move(*this));
+                if (!named) return fail(RA_ERR_OUT_OF_MEMORY, "scratch of a captured plan");
+            }
+            const ra_status s = allocate(bytes, !capturing);
+            if (s != RA_OK) {
+                if (named) swap(*named);
+                delete named;
+                return s;
+            }
+            older_ = named;
+        }
+        captured_ = captured_ || capturing;
+        return RA_OK;
     }
     template <typename T>
     ra_status upload(const std::vector<T>& v) {
@@ -129,12 +143,25 @@ public:
 private:
     void release(bool idle) {
         if (ptr_) pool_release(ptr_, bytes_, device_, idle);
+        if (older_) older_->release(idle);
+        delete older_;
+        older_ = nullptr;
         ptr_ = nullptr;
         bytes_ = 0;
+        captured_ = false;
+    }
+    void swap(DeviceBuffer& o) noexcept {
+        std::swap(ptr_, o.ptr_);
+        std::swap(bytes_, o.bytes_);
+        std::swap(device_, o.device_);
+        std::swap(captured_, o.captured_);
+        std::swap(older_, o.older_);
     }
     void* ptr_ = nullptr;
     size_t bytes_ = 0;
     int device_ = 0;
+    bool captured_ = false;           // a graph names the block
+    DeviceBuffer* older_ = nullptr;   // smaller ones that graphs name
 };
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
