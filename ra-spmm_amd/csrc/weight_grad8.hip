@@ -46,10 +46,13 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // 
     return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
-// The upper 8 significant bits of x, and what is left of x (exact).
+// The upper 8 significant bits of x, and what is left of x (exact; nothing is left of
+// an inf, which the first piece holds).
+template <bool FIRST>
 __device__ __forceinline__ uint32_t take_piece(float& x) {
     const uint32_t top = __float_as_uint(x) & 0xFFFF0000u;
-    x -= __uint_as_float(top);
+    const float rest = x - __uint_as_float(top);
+    x = FIRST && fabsf(x) == INFINITY ? 0.f : rest;
     return top;
 }
 
@@ -61,7 +64,8 @@ __device__ __forceinline__ void cut(const float* x, uint4* piece) {
     for (int i = 0; i < 8; ++i) {
         float rest = x[i];
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) word[p][i] = p + 1 < PIECES ? take_piece(rest) : __float_as_uint(rest);
+        for (int p = 0; p < PIECES; ++p)
+            word[p][i] = p + 1 == PIECES ? __float_as_uint(rest) : p == 0 ? take_piece<true>(rest) : take_piece<false>(rest);
     }
 #pragma unroll
     for (int p = 0; p < PIECES; ++p)
