@@ -388,7 +388,8 @@ void ra_tile_plan_destroy(ra_tile_plan* plan);
  *
  * An edge whose bias is -inf takes no part: its key and value are not used, even
  * where they are inf or NaN.  A row without edges, or with no edge left, gives
- * zeros.  Finite biases of any size are scores like others. */
+ * zeros.  Finite biases of any size are scores like others (past 1e38, two that are
+ * neighbours in fp32 may count as equal); one of +inf or NaN makes its row NaN. */
 typedef struct ra_attn_shape {
     int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads     */
     int32_t head_dim;          /* 1 .. 128                           */

@@ -115,7 +115,8 @@ ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStr
 // ------------------------------------------------------------- device side
 constexpr int kAttnThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBiasMost = 2e38f;
+// A bias past kBiasLarge would leave float32's range in powers of two: from there on it goes half as fast.
+constexpr float kBiasLarge = 1e38f;
 
 // Lane moves.  Within a row of 16 lanes by data-parallel moves, between rows and
 // halves by the swaps of two registers' rows and halves.
@@ -371,8 +372,9 @@ __device__ __forceinline__ void load_edges(const AttnArgs& a, Edges<DEEP>& x, in
     }
 }
 // Live edges of a step: in the list (a LAST step only may pass its end), and not
-// left out by their bias, which becomes powers of two here.  A finite bias is kept
-// finite: beyond +-2e38 all are equal.
+// left out by their bias, which becomes powers of two here.  A finite bias stays
+// finite, and the order of two is kept: past +-1e38 their difference is halved, which
+// is beyond any other score's size either way.
 template <int DEEP, bool LAST, int N>
 __device__ __forceinline__ void close_edges(const AttnArgs& a, Edges<N>& x, bool* live, int left, int es, int slots) {
 #pragma unroll
@@ -385,7 +387,8 @@ __device__ __forceinline__ void close_edges(const AttnArgs& a, Edges<N>& x, bool
         for (int d = 0; d < DEEP; ++d) {
             const float b = x.add[d];
             live[d] = live[d] && b != -INFINITY;
-            x.add[d] = (b < -kBiasMost ? -kBiasMost : b > kBiasMost ? kBiasMost : b) * kLog2e;
+            const float half = fmaf(b, 0.5f * kLog2e, copysignf(0.5f * kLog2e * kBiasLarge, b));
+            x.add[d] = fabsf(b) > kBiasLarge ? half : b * kLog2e;
         }
     }
 }
