@@ -467,7 +467,7 @@ typedef struct ra_norm_shape {
     int32_t rows, q_heads, k_heads;
     int32_t head_dim;  /* 1 .. 256                  */
     int32_t rot_dim;   /* even, at most head_dim    */
-    int32_t positions; /* rows of the table         */
+    int32_t positions; /* rows of the table, 1 at least where rot_dim > 0 and there are rows */
     int32_t layout;    /* ra_rotation               */
     int32_t dtype;     /* ra_dtype                  */
     float eps;

@@ -355,6 +355,13 @@ ra_status check(const ra_norm_shape* s) {
     return RA_OK;
 }
 
+// A position outside of the table takes row 0 and gives NaN: there has to be a row.
+ra_status check_table(const ra_norm_shape& s, const float* table) {
+    if (s.rot_dim && !table) return fail(RA_ERR_INVALID_ARGUMENT, "head norm: NULL table");
+    if (s.rot_dim && s.positions < 1) return fail(RA_ERR_INVALID_ARGUMENT, "head norm: the table is empty");
+    return RA_OK;
+}
+
 }  // namespace
 }  // namespace ra
 
@@ -367,7 +374,8 @@ ra_status ra_head_norm(const ra_norm_shape* s, const void* d_q, const void* d_k,
                        ra_stream_t stream) {
     RA_TRY(ra::check(s));
     if (s->rows == 0) return RA_OK;
-    if ((s->q_heads && (!d_q || !d_wq || !d_out_q)) || (s->k_heads && (!d_k || !d_wk || !d_out_k)) || (s->rot_dim && !d_table))
+    RA_TRY(ra::check_table(*s, d_table));
+    if ((s->q_heads && (!d_q || !d_wq || !d_out_q)) || (s->k_heads && (!d_k || !d_wk || !d_out_k)))
         return fail(RA_ERR_INVALID_ARGUMENT, "head norm: NULL tensor");
     const void* x[2] = {d_q, d_k};
     void* y[2] = {d_out_q, d_out_k};
@@ -392,8 +400,9 @@ ra_status ra_head_norm_backward(const ra_norm_shape* s, const void* d_q, const v
     RA_TRY(ra_head_norm_workspace(s, &need));
     if ((s->q_heads && !d_dwq) || (s->k_heads && !d_dwk))
         return fail(RA_ERR_INVALID_ARGUMENT, "head norm: NULL weight gradient");
+    if (s->rows > 0) RA_TRY(ra::check_table(*s, d_table));
     if (s->rows > 0 && ((s->q_heads && (!d_q || !d_wq || !d_grad_q || !d_dq)) ||
-                        (s->k_heads && (!d_k || !d_wk || !d_grad_k || !d_dk)) || (s->rot_dim && !d_table)))
+                        (s->k_heads && (!d_k || !d_wk || !d_grad_k || !d_dk))))
         return fail(RA_ERR_INVALID_ARGUMENT, "head norm: NULL tensor");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "head norm: the workspace is too small");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
