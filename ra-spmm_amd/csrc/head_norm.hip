@@ -102,10 +102,13 @@ __device__ __forceinline__ void angles(const NormArgs& n, const Runs<P>& r, cons
     }
 }
 
-// (f, s) -> (f c - s si, f si + s c) for the pairs of two runs.
+// (f, s) -> (f c - s si, f si + s c) for the pairs of two runs.  Coordinates that are
+// not rotated are not mixed, by factors of 1 and 0 either: what is inf or NaN at one
+// of them stays there.
 template <int P>
-__device__ __forceinline__ void rotate(float* a, float* b, const float* c, const float* s, bool apart, float sign) {
-    if (apart) {
+__device__ __forceinline__ void rotate(const NormArgs& n, const Runs<P>& r, float* a, float* b, const float* c,
+                                       const float* s, float sign) {
+    if (r.apart) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const float x = a[i], y = b[i], si = sign * s[i];
@@ -118,8 +121,9 @@ __device__ __forceinline__ void rotate(float* a, float* b, const float* c, const
             float& fx = 2 * i < P ? a[2 * i] : b[2 * i - P];
             float& fy = 2 * i + 1 < P ? a[2 * i + 1] : b[2 * i + 1 - P];
             const float x = fx, y = fy, si = sign * s[i];
-            fx = x * c[i] - y * si;
-            fy = x * si + y * c[i];
+            const bool rotated = r.pair + i < n.rot / 2;
+            fx = rotated ? x * c[i] - y * si : x;
+            fy = rotated ? x * si + y * c[i] : y;
         }
     }
 }
@@ -176,12 +180,12 @@ __global__ __launch_bounds__(kThreads) void head_norm(const NormArgs n) {
                 a[i] *= rms * wa[i];
                 b[i] *= rms * wb[i];
             }
-            rotate<P>(a, b, c, s, r.apart, 1.f);
+            rotate<P>(n, r, a, b, c, s, 1.f);
         } else {
             float fa[P], fb[P], inner = 0.f;
             ga.to_float(fa);
             gb.to_float(fb);
-            rotate<P>(fa, fb, c, s, r.apart, -1.f);
+            rotate<P>(n, r, fa, fb, c, s, -1.f);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 a[i] *= rms;  // n
