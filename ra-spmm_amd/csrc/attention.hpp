@@ -43,7 +43,8 @@ struct AttnArgs {
     const int32_t* ptr;
     const int32_t* idx;
     const int32_t* edge;
-    int64_t num_units;    // pieces * head blocks
+    uint32_t num_units;   // pieces * head blocks (attn_check_units)
+    uint32_t first_unit;  // of the launch
     int32_t pieces;       // per row, without a list
     int32_t head_blocks;  // waves that share a piece
     int32_t head_items;   // 0: a piece's waves are neighbours; else pieces, all of one head block's first
@@ -92,13 +93,36 @@ inline int64_t attn_forward_slot(const ra_attn_shape& s) { return (int64_t)s.q_h
 inline int64_t attn_row_slot(const ra_attn_shape& s) { return (int64_t)s.q_heads * (4 * s.head_dim + 2); }
 inline int64_t attn_col_slot(const ra_attn_shape& s) { return (int64_t)s.kv_heads * (2 * s.head_dim + s.value_dim); }
 
-// Threads of a launch: the runtime takes fewer than 2^32.
+// Threads of a launch: the runtime takes fewer than 2^32.  Larger ones are cut.
 constexpr int64_t kMostThreads = (int64_t{1} << 32) - 1024;
+constexpr int64_t kMostBlocks = kMostThreads / 256;
+constexpr int64_t kMostUnits = kMostBlocks * 4;  // a wave each, four in a workgroup
 
-// Workgroups of a launch, 0 where there is nothing to do.
-inline ra_status attn_grid(const AttnArgs& a, unsigned& blocks) {
-    if (a.num_units > kMostThreads / 64) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads");
-    blocks = static_cast<unsigned>((a.num_units + 3) / 4);
+// Units are numbered in 32 bits.  Checked before the first launch of a call.
+inline ra_status attn_check_units(int64_t pieces, const AttnLayout& l) {
+    if (pieces * l.head_blocks >= int64_t{1} << 32) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads");
+    return RA_OK;
+}
+
+// launch(part of a, workgroups) for every part of the units.
+template <typename F>
+ra_status attn_launches(const AttnArgs& a, F launch) {
+    AttnArgs part = a;
+    for (int64_t first = 0; first < a.num_units; first += kMostUnits) {
+        const int64_t units = a.num_units - first;
+        part.first_unit = static_cast<uint32_t>(first);
+        RA_TRY(launch(part, static_cast<unsigned>(((units < kMostUnits ? units : kMostUnits) + 3) / 4)));
+    }
+    return RA_OK;
+}
+// launch(first row, workgroups) for `n` rows of `each` workgroups.
+template <typename F>
+ra_status join_launches(int64_t n, int64_t each, F launch) {
+    const int64_t most = kMostBlocks / each;
+    for (int64_t first = 0; first < n; first += most) {
+        const int64_t rows = n - first < most ? n - first : most;
+        RA_TRY(launch(static_cast<int>(first), dim3(static_cast<unsigned>(rows * each))));
+    }
     return RA_OK;
 }
 ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st);
@@ -284,10 +308,10 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
     const int64_t full = gridDim.x - (per - 1) * 8;  // XCDs with `per` workgroups
     const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
     const int64_t block = x < full ? x * per + y : full * per + (x - full) * (per - 1) + y;
-    // Fewer than 2^32 units (attn_grid): 32-bit divisions.
-    const uint64_t at = block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Fewer than 2^32 units (attn_check_units): 32-bit divisions.
+    const uint64_t at = (int64_t)a.first_unit + block * (kAttnThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Unit u{};
-    u.live = at < static_cast<uint64_t>(a.num_units);
+    u.live = at < a.num_units;
     if (!u.live) return u;
     const uint32_t unit = static_cast<uint32_t>(at), blocks = a.head_blocks;
     uint32_t item = unit;

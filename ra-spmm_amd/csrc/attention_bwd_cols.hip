@@ -143,28 +143,25 @@ __global__ __launch_bounds__(256) void attn_cols_join(const AttnArgs a, const in
 }  // namespace
 
 ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    unsigned blocks = 0;
-    RA_TRY(attn_grid(a, blocks));
-    if (blocks == 0) return RA_OK;
     // Without the loop over a head's query heads: power-law graph of 1e6 rows 1.88 against 2.04 ms, social graph of
     // 50,000 rows of 80 472 against 504 us.
-    if (a.group == 1) RA_ATTN_DISPATCH(attn_cols_one, dtype, l, dim3(blocks), st, a);
-    else RA_ATTN_DISPATCH(attn_cols_many, dtype, l, dim3(blocks), st, a);
-    RA_LAUNCH_CHECK("attn_cols");
-    return RA_OK;
+    return attn_launches(a, [&](const AttnArgs& part, unsigned blocks) {
+        if (a.group == 1) RA_ATTN_DISPATCH(attn_cols_one, dtype, l, dim3(blocks), st, part);
+        else RA_ATTN_DISPATCH(attn_cols_many, dtype, l, dim3(blocks), st, part);
+        RA_LAUNCH_CHECK("attn_cols");
+        return RA_OK;
+    });
 }
 
 ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
-    if (n == 0) return RA_OK;
     const int per = (a.kv_heads * (2 * a.head_dim + a.value_dim) + 63) / 64;
-    const int64_t blocks = n * per;
-    if (blocks > kMostThreads / 256) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    const dim3 grid((unsigned)blocks);
-    if (dtype == RA_DTYPE_F32) attn_cols_join<float><<<grid, 256, 0, st>>>(a, splits, per);
-    else if (dtype == RA_DTYPE_F16) attn_cols_join<f16_t><<<grid, 256, 0, st>>>(a, splits, per);
-    else attn_cols_join<bf16_t><<<grid, 256, 0, st>>>(a, splits, per);
-    RA_LAUNCH_CHECK("attn_cols_join");
-    return RA_OK;
+    return join_launches(n, per, [&](int first, dim3 grid) {
+        if (dtype == RA_DTYPE_F32) attn_cols_join<float><<<grid, 256, 0, st>>>(a, splits + first, per);
+        else if (dtype == RA_DTYPE_F16) attn_cols_join<f16_t><<<grid, 256, 0, st>>>(a, splits + first, per);
+        else attn_cols_join<bf16_t><<<grid, 256, 0, st>>>(a, splits + first, per);
+        RA_LAUNCH_CHECK("attn_cols_join");
+        return RA_OK;
+    });
 }
 
 }  // namespace ra

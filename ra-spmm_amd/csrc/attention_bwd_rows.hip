@@ -193,24 +193,21 @@ __global__ __launch_bounds__(64) void attn_lam_final(const float* __restrict__ p
 }  // namespace
 
 ra_status attn_rows_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    unsigned blocks = 0;
-    RA_TRY(attn_grid(a, blocks));
-    if (blocks == 0) return RA_OK;
-    RA_ATTN_DISPATCH(attn_rows, dtype, l, dim3(blocks), st, a);
-    RA_LAUNCH_CHECK("attn_rows");
-    return RA_OK;
+    return attn_launches(a, [&](const AttnArgs& part, unsigned blocks) {
+        RA_ATTN_DISPATCH(attn_rows, dtype, l, dim3(blocks), st, part);
+        RA_LAUNCH_CHECK("attn_rows");
+        return RA_OK;
+    });
 }
 
 ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
-    if (n == 0) return RA_OK;
-    const int64_t blocks = n * a.q_heads;
-    if (blocks > kMostThreads / kJoinThreads) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    const dim3 grid((unsigned)blocks);
-    if (dtype == RA_DTYPE_F32) attn_rows_join<float><<<grid, kJoinThreads, 0, st>>>(a, splits);
-    else if (dtype == RA_DTYPE_F16) attn_rows_join<f16_t><<<grid, kJoinThreads, 0, st>>>(a, splits);
-    else attn_rows_join<bf16_t><<<grid, kJoinThreads, 0, st>>>(a, splits);
-    RA_LAUNCH_CHECK("attn_rows_join");
-    return RA_OK;
+    return join_launches(n, a.q_heads, [&](int first, dim3 grid) {
+        if (dtype == RA_DTYPE_F32) attn_rows_join<float><<<grid, kJoinThreads, 0, st>>>(a, splits + first);
+        else if (dtype == RA_DTYPE_F16) attn_rows_join<f16_t><<<grid, kJoinThreads, 0, st>>>(a, splits + first);
+        else attn_rows_join<bf16_t><<<grid, kJoinThreads, 0, st>>>(a, splits + first);
+        RA_LAUNCH_CHECK("attn_rows_join");
+        return RA_OK;
+    });
 }
 
 ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStream_t st) {

@@ -204,8 +204,8 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
     __shared__ float weight[2][kJoinPieces], sums[2][kJoinThreads];
     __shared__ float2 tops[kJoinThreads / 64], totals[kJoinThreads / 64];
     const int head = blockIdx.x % a.q_heads, which = blockIdx.x / a.q_heads;
-    const int4 sp = splits ? splits[which] : make_int4(which, 0, a.pieces, 0);
-    const int64_t slot0 = splits ? sp.y : (int64_t)which * a.pieces;
+    const int4 sp = splits ? splits[which] : make_int4(a.first_unit + which, 0, a.pieces, 0);
+    const int64_t slot0 = splits ? sp.y : (int64_t)sp.x * a.pieces;
     const int64_t stride = (int64_t)a.q_heads * (2 * a.value_dim + 4);
     const float* const first = a.partial + slot0 * stride;
     int width = 16;
@@ -291,33 +291,33 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
 }  // namespace
 
 ra_status attn_forward_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a, hipStream_t st) {
-    unsigned blocks = 0;
-    RA_TRY(attn_grid(a, blocks));
-    if (blocks == 0) return RA_OK;
-    RA_ATTN_DISPATCH(attn_forward, dtype, l, dim3(blocks), st, a);
-    RA_LAUNCH_CHECK("attn_forward");
-    return RA_OK;
+    return attn_launches(a, [&](const AttnArgs& part, unsigned blocks) {
+        RA_ATTN_DISPATCH(attn_forward, dtype, l, dim3(blocks), st, part);
+        RA_LAUNCH_CHECK("attn_forward");
+        return RA_OK;
+    });
 }
 
 ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st) {
-    if (n == 0) return RA_OK;
-    const int64_t blocks = n * a.q_heads;
-    if (blocks > kMostThreads / kJoinThreads) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows");
-    const dim3 grid((unsigned)blocks);
     // Workgroups that are all resident wait for their loads: 8 of them ahead (4 rows of 6,000 edges, 8 heads: 6.8
     // against 9.5 us).  More are bound by the loads, and most of them have 2 or 3 pieces (power-law graph: 76 against
     // 103 us with 8 ahead).
     constexpr int64_t kResident = 2048;
-    const auto go = [&](auto tag) {
-        using T = decltype(tag);
-        if (blocks <= kResident) attn_forward_join<T, 8><<<grid, kJoinThreads, 0, st>>>(a, splits);
-        else attn_forward_join<T, 0><<<grid, kJoinThreads, 0, st>>>(a, splits);
-    };
-    if (dtype == RA_DTYPE_F32) go(float{});
-    else if (dtype == RA_DTYPE_F16) go(f16_t{});
-    else go(bf16_t{});
-    RA_LAUNCH_CHECK("attn_forward_join");
-    return RA_OK;
+    return join_launches(n, a.q_heads, [&](int first, dim3 grid) {
+        AttnArgs part = a;
+        part.first_unit = first;  // the row, where there is no list
+        const int4* const rows = splits ? splits + first : nullptr;
+        const auto go = [&](auto tag) {
+            using T = decltype(tag);
+            if (n * a.q_heads <= kResident) attn_forward_join<T, 8><<<grid, kJoinThreads, 0, st>>>(part, rows);
+            else attn_forward_join<T, 0><<<grid, kJoinThreads, 0, st>>>(part, rows);
+        };
+        if (dtype == RA_DTYPE_F32) go(float{});
+        else if (dtype == RA_DTYPE_F16) go(f16_t{});
+        else go(bf16_t{});
+        RA_LAUNCH_CHECK("attn_forward_join");
+        return RA_OK;
+    });
 }
 
 }  // namespace ra

@@ -140,6 +140,7 @@ ra_status cut(AttnSide& s, int64_t nnz, Totals* tot, hipStream_t st) {
         return fail(RA_ERR_INVALID_ARGUMENT,
                     "attention plan: rowptr must run from 0 to nnz without decreasing, and colind lie in [0, K)");
     const int64_t items = static_cast<int64_t>(t.items_slots >> 32);
+    if (items > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "attention plan: more than 2^31 - 1 pieces of rows");
     s.num_items = static_cast<int32_t>(items);
     s.num_slots = static_cast<int64_t>(t.items_slots & 0xFFFFFFFFu);
     s.num_splits = t.splits;
@@ -284,7 +285,7 @@ void side_of(AttnArgs& a, const AttnSide& s, bool by_head) {
     a.idx = s.idx;
     a.edge = s.edge;
     a.rows = s.rows;
-    a.num_units = (int64_t)s.num_items * a.head_blocks;
+    a.num_units = static_cast<uint32_t>((int64_t)s.num_items * a.head_blocks);
     a.head_items = by_head ? s.num_items : 0;
 }
 
@@ -463,6 +464,7 @@ ra_status ra_attn_plan_run(ra_attn_plan* p, const ra_attn_shape* shape, const vo
     const ra::AttnLayout l = ra::attn_layout(
         s, s.q_heads, {d_q, d_k, d_v, d_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim},
         p->side[0].num_items, by_head);
+    RA_TRY(ra::attn_check_units(p->side[0].num_items, l));
     ra::AttnArgs a = ra::args_of(s, l);
     ra::side_of(a, p->side[0], by_head);
     a.wide = !ra::narrow(p->info.K, {a.k_pitch, a.v_pitch});
@@ -503,10 +505,13 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
     RA_TRY(check_output(d_dk, "dk"));
     RA_TRY(check_output(d_dv, "dv"));
     RA_TRY(check_output(d_stats, "stats"));
+    const bool rows_by_head = ra::attn_by_head(s, M, K, p->info.nnz), cols_by_head = ra::attn_by_head(s, K, M, p->info.nnz);
+    const ra::AttnLayout l = ra::attn_layout(s, s.q_heads, ptrs, rows.num_items, rows_by_head);
+    const ra::AttnLayout lt = ra::attn_layout(s, s.kv_heads, ptrs, cols.num_items, cols_by_head);
+    RA_TRY(ra::attn_check_units(rows.num_items, l));
+    RA_TRY(ra::attn_check_units(cols.num_items, lt));
     RA_TRY(guarded([&] { return p->partial.ensure(partial * sizeof(float), st); }));
     RA_TRY(guarded([&] { return p->record.ensure((int64_t)M * s.q_heads * 2 * sizeof(float4), st); }));
-    const bool rows_by_head = ra::attn_by_head(s, M, K, p->info.nnz), cols_by_head = ra::attn_by_head(s, K, M, p->info.nnz);
-    ra::AttnLayout l = ra::attn_layout(s, s.q_heads, ptrs, rows.num_items, rows_by_head);
     ra::AttnArgs a = ra::args_of(s, l);
     a.q = d_q;
     a.k = d_k;
@@ -529,15 +534,14 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
     }
     RA_TRY(ra::attn_lam_launch(a, a.partial, d_dlam, st));
     if (K > 0) {
-        l = ra::attn_layout(s, s.kv_heads, ptrs, cols.num_items, cols_by_head);
-        a.head_blocks = l.head_blocks;
-        a.hb_shift = l.hb_shift;
-        a.ragged = l.ragged;
+        a.head_blocks = lt.head_blocks;
+        a.hb_shift = lt.hb_shift;
+        a.ragged = lt.ragged;
         ra::side_of(a, cols, cols_by_head);
         a.wide = !ra::narrow(M, {a.q_pitch, a.g_pitch, static_cast<uint32_t>(s.q_heads * 2 * sizeof(float4))});
         a.out = d_dk;
         a.out2 = d_dv;
-        RA_TRY(ra::attn_cols_launch(s.dtype, l, a, st));
+        RA_TRY(ra::attn_cols_launch(s.dtype, lt, a, st));
         RA_TRY(ra::attn_cols_join_launch(s.dtype, a, cols.splits, cols.num_splits, st));
     }
     return RA_OK;
@@ -576,7 +580,9 @@ ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t 
     a.idx = d_colind;
     a.rows = M;
     a.pieces = pieces;
-    a.num_units = (int64_t)M * a.pieces * a.head_blocks;
+    const int64_t units = (int64_t)M * a.pieces * a.head_blocks;
+    if (units > ra::kMostUnits) return fail(RA_ERR_UNSUPPORTED, "attention: too many rows and heads without a plan");
+    a.num_units = static_cast<uint32_t>(units);
     a.wide = !ra::narrow(K, {a.k_pitch, a.v_pitch});
     a.q = d_q;
     a.k = d_k;
