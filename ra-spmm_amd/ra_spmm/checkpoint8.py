@@ -100,7 +100,8 @@ class _Linear8(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         weight, codes, scales = ctx.saved_tensors
-        gx = grad @ weight if ctx.needs_input_grad[0] else None
+        # Under autocast the output, and so grad, has fewer bits than the weight.
+        gx = grad @ weight.to(grad.dtype) if ctx.needs_input_grad[0] else None
         gw = None
         if ctx.needs_input_grad[1]:
             gw = _C.weight_grad8(_rows(grad), codes, scales, ctx.cols, ctx.signed).to(weight.dtype)
