@@ -72,11 +72,14 @@ class _Relu8(torch.autograd.Function):
         ctx.save_for_backward(codes, scales)
         ctx.cols = x.size(1)
         ctx.mark_non_differentiable(codes, scales)
+        ctx.set_materialize_grads(False)  # no zeros of the codes' size
         return y, codes, scales
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _codes, _scales):
+        if grad is None:
+            return None
         codes, scales = ctx.saved_tensors
         return _C.relu_grad8(_rows(grad), codes, scales, ctx.cols)
 

@@ -64,3 +64,27 @@ def test_model_under_autocast():
     assert F.cosine_similarity(X.grad.flatten(), want.flatten(), 0) > 0.99
     for p, b in zip(model.parameters(), model_grads):
         assert p.grad.dtype == torch.float32 and F.cosine_similarity(p.grad.flatten(), b.flatten(), 0) > 0.98
+
+
+def test_relu_backward_takes_no_memory_of_its_own():
+    """The gradient of the input and nothing else; relu8's codes have no gradient, not one of zeros either."""
+    rows, cols = 200_000, 128
+    x, g = torch.randn(rows, cols, device="cuda", requires_grad=True), torch.randn(rows, cols, device="cuda")
+    y, kept = ra_spmm.relu8(x)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    dx, = torch.autograd.grad(y, x, g)
+    assert torch.cuda.max_memory_allocated() - before <= rows * cols * 4 + (1 << 20)
+    assert torch.equal(dx, g * (x.detach() > 0))
+
+
+def test_relu_whose_output_takes_no_part():
+    x = torch.randn(50, 40, device="cuda", requires_grad=True)
+    y, kept = ra_spmm.relu8(x)
+    (x * 2 + 0 * y.detach()).sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2))
+    w = torch.randn(7, 40, device="cuda", requires_grad=True)
+    h, kept = ra_spmm.relu8(x.detach())  # an input without a gradient
+    ra_spmm.linear8(h, w, kept).sum().backward()
+    assert w.grad.shape == (7, 40)
