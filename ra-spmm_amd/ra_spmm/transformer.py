@@ -71,6 +71,15 @@ class DiffTransformer(nn.Module):
         d = dim // (2 * heads)
         self.register_buffer("table", rotation_table(positions, d // 2 * 2) if positions else None, persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        """Moves and conversions, after which the table is the float32 one: angles rounded to 16 bits would be off by
+        2^-9."""
+        table = self.table
+        super()._apply(fn, recurse)
+        if table is not None and self.table.dtype != table.dtype:
+            self.table = table.to(self.table.device)
+        return self
+
     def forward(self, X, plan, positions=None, bias=None):
         if positions is not None and self.table is None:
             raise ValueError("the model was made without positions")
