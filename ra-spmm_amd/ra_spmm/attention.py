@@ -51,7 +51,7 @@ def diff_attention(plan, q, k, v, lam, scale=None, bias=None) -> torch.Tensor:
     q [M, heads, 2, head_dim], k [K, kv_heads, 2, head_dim], v [K, kv_heads, value_dim] of one dtype (float32, float16 or
     bfloat16), rows possibly strided; lam float32, one weight or one per head; scale defaults to head_dim ** -0.5; bias
     float32 [nnz] in the plan's edge order, without a gradient.  Returns [M, heads, value_dim]."""
-    if bias is not None and bias.requires_grad:
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("diff_attention: bias takes no gradient (detach it)")
     q, k, v = _rows(q), _rows(k), _rows(v)
     if q.dim() == 4 and lam.numel() == 1:
