@@ -204,8 +204,8 @@ __global__ __launch_bounds__(kJoinThreads) void attn_forward_join(const AttnArgs
     __shared__ float weight[2][kJoinPieces], sums[2][kJoinThreads];
     __shared__ float2 tops[kJoinThreads / 64], totals[kJoinThreads / 64];
     const int head = blockIdx.x % a.q_heads, which = blockIdx.x / a.q_heads;
-    const int4 sp = splits ? splits[which] : make_int4(a.first_unit + which, 0, a.pieces, 0);
-    const int64_t slot0 = splits ? sp.y : (int64_t)sp.x * a.pieces;
+    const int4 sp = splits ? splits[which] : make_int4(which, 0, a.pieces, 0);
+    const int64_t slot0 = splits ? sp.y : (int64_t)which * a.pieces;
     const int64_t stride = (int64_t)a.q_heads * (2 * a.value_dim + 4);
     const float* const first = a.partial + slot0 * stride;
     int width = 16;
@@ -305,8 +305,11 @@ ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4*
     constexpr int64_t kResident = 2048;
     return join_launches(n, a.q_heads, [&](int first, dim3 grid) {
         AttnArgs part = a;
-        part.first_unit = first;  // the row, where there is no list
         const int4* const rows = splits ? splits + first : nullptr;
+        if (!splits) {  // row 0 of the launch
+            part.partial += (int64_t)first * a.pieces * a.q_heads * (2 * a.value_dim + 4);
+            part.out = static_cast<char*>(a.out) + (int64_t)first * a.q_heads * a.value_dim * (dtype == RA_DTYPE_F32 ? 4 : 2);
+        }
         const auto go = [&](auto tag) {
             using T = decltype(tag);
             if (n * a.q_heads <= kResident) attn_forward_join<T, 8><<<grid, kJoinThreads, 0, st>>>(part, rows);

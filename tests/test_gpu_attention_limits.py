@@ -84,3 +84,21 @@ def test_more_waves_than_a_launch_holds():
     assert ((dv.flatten().double() - want).abs() <= 80_000 * EPS * mag).all()
     terms = (g * v[j]).double()
     assert (dlam.double() + terms.sum()).abs() <= 80_000 * EPS * terms.abs().sum()
+
+
+def test_rows_without_a_plan():
+    """140,000 rows of 300 edges, 128 heads, in two pieces each: more joining workgroups than a launch holds."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free memory")
+    M, K, H, n = 140_000, 300, 128, 300
+    gen = torch.Generator("cuda").manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    q, k, v, lam = r(M, H, 2, 1), r(K, H, 2, 1), r(K, H, 2), torch.rand(H, generator=gen, device="cuda")
+    rowptr = torch.arange(M + 1, device="cuda", dtype=torch.int32) * n
+    colind = torch.arange(n, device="cuda", dtype=torch.int32).repeat(M)
+    free = ra_spmm.diff_attention_csr(rowptr, colind, q, k, v, lam)
+    for h in (0, 77, 127):
+        p = [(q[:, h, a].double() @ k[:, h, a].double().t().contiguous()).softmax(1) for a in range(2)]
+        A = max(float((q[:, h, a].abs().max() * k[:, h, a].abs().max())) for a in range(2))
+        l, vh = lam[h].double(), v[:, h].double()
+        close(free[:, h], (p[0] - l * p[1]) @ vh, (p[0] + l * p[1]) @ vh.abs(), (32 + 9 * A + 2 + n) * EPS, "out")
