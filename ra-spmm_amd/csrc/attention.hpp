@@ -132,9 +132,9 @@ ra_status attn_cols_launch(int32_t dtype, const AttnLayout& l, const AttnArgs& a
 ra_status attn_forward_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
 ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
 ra_status attn_cols_join_launch(int32_t dtype, const AttnArgs& a, const int4* splits, int64_t n, hipStream_t st);
-// d lam from the records; `partial` holds kLamBlocks * q_heads floats.
+// d lam from the records; `partial` holds kLamBlocks * q_heads doubles.
 constexpr int kLamBlocks = 128;
-ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStream_t st);
+ra_status attn_lam_launch(const AttnArgs& a, double* partial, float* dlam, hipStream_t st);
 
 // ------------------------------------------------------------- device side
 constexpr int kAttnThreads = 256;
@@ -449,6 +449,25 @@ __device__ __forceinline__ float dot(const Run<T, N>& a, const Run<T, N>& b) {
         for (int i = 0; i < N / 2; ++i) t = dot2(a.w[i], b.w[i], t, T());
     }
     return t;
+}
+
+// The same by correctly rounded fused multiply-adds.  The two-term instruction of fp16 rounds downwards a little more often
+// than upwards, which a sum over all rows keeps (dlam: 310,108 rows, 2e-9 of the terms' magnitudes, 2e-6 of the result).
+template <int N>
+__device__ __forceinline__ float dot_rounded(const Run<f16_t, N>& a, const Run<f16_t, N>& b) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    float even = 0.f, odd = 0.f;  // one chain would be made that instruction again
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const h2 x = __builtin_bit_cast(h2, a.w[i]), y = __builtin_bit_cast(h2, b.w[i]);
+        even = fmaf((float)x[0], (float)y[0], even);
+        odd = fmaf((float)x[1], (float)y[1], odd);
+    }
+    return even + odd;
+}
+template <typename T, int N>
+__device__ __forceinline__ float dot_rounded(const Run<T, N>& a, const Run<T, N>& b) {
+    return dot(a, b);
 }
 
 // A lane's run in the rows of a gathered matrix, in packets of PB bytes.  Packets

@@ -35,6 +35,13 @@ __global__ __launch_bounds__(kAttnThreads, PB == 16 ? (sizeof(T) == 2 ? 6 : 4) :
     Run<T, NV> g;
     load_run<T, NV, PB == 16>(
         g, static_cast<const T*>(a.grad) + ((int64_t)u.row * a.q_heads + p.head) * a.value_dim + NV * p.l, p.vcount);
+    // The two-term instruction of bf16 too rounds downwards a little more often: every second lane's part of dp is formed
+    // with its sign turned, so that over the lanes it does not add up (300,000 rows: dlam off by 1e-9 a row without).
+    const uint32_t turned = std::is_same<T, bf16_t>::value && (threadIdx.x & 1) ? 0x80000000u : 0u;
+    if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i) g.w[i] ^= turned | turned >> 16;
+    }
     const int64_t at = ((int64_t)u.row * a.q_heads + p.head) * 2 + p.map;
     const float2 st = reinterpret_cast<const float2*>(a.stats)[at];
     const bool whole = u.slot < 0;
@@ -67,7 +74,7 @@ __global__ __launch_bounds__(kAttnThreads, PB == 16 ? (sizeof(T) == 2 ? 6 : 4) :
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             w[d] = exp2_of(fmaf(lanes_sum<LM>(dot(q, kr[d])), a.scale2, now.add[d]) - st.x) * st.y;
-            dp[d] = lanes_sum<2 * LM>(dot(g, vr[d]));
+            dp[d] = lanes_sum<2 * LM>(__uint_as_float(__float_as_uint(dot_rounded(g, vr[d])) ^ turned));
             if (!live[d]) w[d] = dp[d] = 0.f;
             delta = fmaf(w[d], dp[d], delta);
         }
@@ -167,27 +174,32 @@ __global__ __launch_bounds__(kJoinThreads) void attn_rows_join(const AttnArgs a,
 }
 
 // d lam[h] = -sum_i delta of map 1: a workgroup sums a run of rows for one head, then
-// one workgroup the workgroups' sums, both in a fixed order.
-__global__ __launch_bounds__(256) void attn_lam_partial(const AttnArgs a, float* __restrict__ partial) {
-    __shared__ float part[4];
+// one workgroup the workgroups' sums, both in a fixed order.  In 64 bits: the terms
+// cancel down to about their number's root, and fp32 sums would round at that size.
+__device__ __forceinline__ double wave_sum(double x) {
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    return x;
+}
+__global__ __launch_bounds__(256) void attn_lam_partial(const AttnArgs a, double* __restrict__ partial) {
+    __shared__ double part[4];
     const int64_t per = ((int64_t)a.rows + gridDim.x - 1) / gridDim.x;
     const int64_t first = blockIdx.x * per, end = min(first + per, (int64_t)a.rows);
     const int h = blockIdx.y;
-    float x = 0.f;
+    double x = 0.;
 #pragma unroll 4
     for (int64_t i = first + threadIdx.x; i < end; i += 256) x += record_at(a, i, h)[1].z;
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    x = wave_sum(x);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
     __syncthreads();
     if (threadIdx.x == 0) partial[(int64_t)blockIdx.x * a.q_heads + h] = part[0] + part[1] + part[2] + part[3];
 }
-__global__ __launch_bounds__(64) void attn_lam_final(const float* __restrict__ partial, int blocks, int heads,
+__global__ __launch_bounds__(64) void attn_lam_final(const double* __restrict__ partial, int blocks, int heads,
                                                      float* __restrict__ dlam) {
     const int h = blockIdx.x;
-    float x = 0.f;
+    double x = 0.;
     for (int b = threadIdx.x; b < blocks; b += 64) x += partial[(int64_t)b * heads + h];
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-    if (threadIdx.x == 0) dlam[h] = -x;
+    x = wave_sum(x);
+    if (threadIdx.x == 0) dlam[h] = static_cast<float>(-x);
 }
 
 }  // namespace
@@ -210,7 +222,7 @@ ra_status attn_rows_join_launch(int32_t dtype, const AttnArgs& a, const int4* sp
     });
 }
 
-ra_status attn_lam_launch(const AttnArgs& a, float* partial, float* dlam, hipStream_t st) {
+ra_status attn_lam_launch(const AttnArgs& a, double* partial, float* dlam, hipStream_t st) {
     attn_lam_partial<<<dim3(kLamBlocks, a.q_heads), 256, 0, st>>>(a, partial);
     RA_LAUNCH_CHECK("attn_lam_partial");
     attn_lam_final<<<a.q_heads, 64, 0, st>>>(partial, kLamBlocks, a.q_heads, dlam);

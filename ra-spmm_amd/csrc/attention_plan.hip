@@ -500,7 +500,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
     const ra::AttnPtrs ptrs{d_q, d_k, d_v, d_grad_out, s.ldq, s.ldk, s.ldv, (int64_t)s.q_heads * s.value_dim};
     const ra::AttnSide &rows = p->side[0], &cols = p->side[1];
     const int64_t partial = std::max({rows.num_slots * ra::attn_row_slot(s), cols.num_slots * ra::attn_col_slot(s),
-                                      (int64_t)ra::kLamBlocks * s.q_heads});
+                                      (int64_t)2 * ra::kLamBlocks * s.q_heads});  // doubles
     RA_TRY(check_output(d_dq, "dq"));
     RA_TRY(check_output(d_dk, "dk"));
     RA_TRY(check_output(d_dv, "dv"));
@@ -532,7 +532,7 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* p, const ra_attn_shape* shape,
         RA_TRY(ra::attn_rows_launch(s.dtype, l, a, st));
         RA_TRY(ra::attn_rows_join_launch(s.dtype, a, rows.splits, rows.num_splits, st));
     }
-    RA_TRY(ra::attn_lam_launch(a, a.partial, d_dlam, st));
+    RA_TRY(ra::attn_lam_launch(a, p->partial.get<double>(), d_dlam, st));
     if (K > 0) {
         a.head_blocks = lt.head_blocks;
         a.hb_shift = lt.hb_shift;
