@@ -441,7 +441,8 @@ ra_status ra_attn_plan_run_backward(ra_attn_plan* plan, const ra_attn_shape* sha
                                     ra_stream_t stream);
 /* The forward pass without a plan, for lists that arrive with the call (a few new
  * rows of a served graph).  Every row is cut into the same number of pieces, chosen
- * from M and nnz.  As with ra_spmm_csr_direct, rowptr and colind are not checked.
+ * from M and nnz (a row many times longer than the mean has pieces as many times
+ * longer).  As with ra_spmm_csr_direct, rowptr and colind are not checked.
  * d_workspace: ra_attn_csr_workspace() bytes, 16-byte aligned. */
 ra_status ra_attn_csr_workspace(const ra_attn_shape* shape, int32_t M, int64_t nnz, int64_t* bytes);
 ra_status ra_attn_csr(const int32_t* d_rowptr, const int32_t* d_colind, int32_t M, int32_t K, int64_t nnz,
@@ -511,7 +512,8 @@ ra_status ra_relu_grad8(const void* d_grad, const uint8_t* d_codes, int64_t rows
 /* The weight gradient of y = x W^T from the kept x: d_out [out, cols] fp32 =
  * grad^T (code * scale), grad [rows, out].  On the matrix cores in bf16 with fp32
  * sums; a grad of more bits is cut into bf16 pieces that add up to it exactly (three
- * for fp32, two for fp16), so no product is rounded.  The sums have a fixed order.
+ * for fp32, two for fp16; an inf is one piece), so no product is rounded.  The sums have
+ * a fixed order.
  * d_workspace: ra_weight_grad8_workspace() bytes, 16-byte aligned. */
 ra_status ra_weight_grad8_workspace(int64_t rows, int32_t out, int32_t cols, int64_t* bytes);
 ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint8_t* d_scales, int64_t rows,

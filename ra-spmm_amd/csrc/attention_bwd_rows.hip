@@ -5,8 +5,8 @@
 //     ds_j = c p_j (dp_j - delta)   (c = 1 for map 0, -lam for map 1)
 //     dq   = scale * sum_j ds_j k_j = scale * c * (sum_j p_j dp_j k_j - delta sum_j p_j k_j)
 // The second form needs one pass over the edges: delta is known at its end.  In a
-// row's last step (most rows' only one) it is known before k is added, and the first
-// form is used.  The weights come from the forward pass' maxima and sums.  Lanes as
+// row's last step it is known before k is added, and the first form is used (for all
+// of a row only where it has no more edges than a step).  The weights come from the forward pass' maxima and sums.  Lanes as
 // in the forward pass; the pieces of a long row are plain sums.  It gathers what the
 // forward pass does: power-law graph of 1e6 rows, 23e6 edges of 512 bytes: 1.72 ms, 6.9 TB/s.
 #include <type_traits>

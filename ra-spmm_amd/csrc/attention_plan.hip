@@ -290,7 +290,9 @@ void side_of(AttnArgs& a, const AttnSide& s, bool by_head) {
 }
 
 // Pieces of every row of a plan-free call: about kAttnPiece edges, fewer where that
-// leaves most of the GPU's wave slots empty, but at least 32.
+// leaves most of the GPU's wave slots empty, but at least 32.  The number goes by the
+// mean: the rows' own lengths are not known on the host, and a row many times longer
+// than the others has pieces as many times longer.
 int plan_free_pieces(const ra_attn_shape& s, int32_t M, int64_t nnz) {
     if (M <= 0 || nnz <= 0) return 1;
     const int64_t mean = (nnz + M - 1) / M;

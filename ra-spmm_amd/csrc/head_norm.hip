@@ -12,7 +12,7 @@
 // stride over its heads, with the weights (and the sums of dw) in registers.
 // Measured: 1e6 rows of 8 + 8 heads of 16 in bf16, cut out of one projection: forward 216 us
 // (1.02 GB, 4.7 TB/s), backward 335 (1.54 GB, 4.6); a large copy reaches 5.1.  150,000 rows of 12 + 4
-// heads of 20 in fp32, 12 of each head rotated, a table row per position: 102 and 136 us (3.8 and
+// heads of 20 in fp32, 12 of each head rotated, a table row per position: 85 and 137 us (4.6 and
 // 4.2 TB/s).  One row: 3 us on the GPU.
 #include <algorithm>
 #include <type_traits>

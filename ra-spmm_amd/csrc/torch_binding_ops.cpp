@@ -434,7 +434,7 @@ void bind_operators(pybind11::module_& m) {
     m.def("make_attention_plan", &make_attention_plan,
           "Plan of differential attention over a graph's neighbour lists (built on the GPU; refers to rowptr and colind)",
           py::arg("rowptr"), py::arg("colind"), py::arg("M"), py::arg("K"), py::arg("backward") = true);
-    m.def("run_attention_plan", &run_attention_plan, "Differential attention, inference", py::arg("plan"), py::arg("q"),
+    m.def("run_attention_plan", &run_attention_plan, "Differential attention, inference (the result records no gradient)", py::arg("plan"), py::arg("q"),
           py::arg("k"), py::arg("v"), py::arg("lam"), py::arg("scale") = py::none(), py::arg("bias") = py::none());
     m.def("run_attention_plan_train", &run_attention_plan_train,
           "Differential attention: (out, stats), stats for run_attention_plan_backward", py::arg("plan"), py::arg("q"),
@@ -443,7 +443,8 @@ void bind_operators(pybind11::module_& m) {
           py::arg("plan"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lam"), py::arg("stats"),
           py::arg("grad_out"), py::arg("scale") = py::none(), py::arg("bias") = py::none());
     m.def("diff_attention_csr", &diff_attention_csr,
-          "Differential attention over lists that arrive with the call (no plan; rowptr and colind are not checked)",
+          "Differential attention over lists that arrive with the call (no plan; rowptr and colind are not checked; the "
+          "result records no gradient, unlike diff_attention's)",
           py::arg("rowptr"), py::arg("colind"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lam"),
           py::arg("scale") = py::none(), py::arg("bias") = py::none());
     m.def("export_attention_plan",

@@ -13,8 +13,8 @@
 // writes one 16-byte vector per piece to LDS, where they are read as they lie.  Each
 // element is converted once per workgroup.  Workgroups hold up to 128 x 256 of the
 // output and split the rows; a second launch adds their sums in order.
-// Measured: 1e6 rows, 256 columns, fp32 grad of 47: 129 us and 8 for the joining launch (0.45 GB,
-// 3.3 TB/s); 512,000 rows, 128 columns, bf16 grad of 256: 97 and 7 (0.33 GB, 3.2 TB/s, 0.32
+// Measured: 1e6 rows, 256 columns, fp32 grad of 47: 128 us and 8 for the joining launch (0.45 GB,
+// 3.3 TB/s); 512,000 rows, 128 columns, bf16 grad of 256: 96 and 7 (0.33 GB, 3.2 TB/s, 0.32
 // PFLOP/s).  Bound by the turn of a stage: loads, cut, LDS and barrier, with two stages in flight.
 #include <type_traits>
 

@@ -10,7 +10,7 @@ codes of a ReLU's output are unsigned and at least 1 where the input was positiv
     relu_grad8(g, p)    gradient through the ReLU
     weight_grad8(g, p)  g^T (code * scale), float32
 
-relu8 and linear8 are the differentiable forms: a linear layer after a ReLU keeps 1 byte per input element for both of
+None of these records a gradient.  relu8 and linear8 are the differentiable forms: a linear layer after a ReLU keeps 1 byte per input element for both of
 them, where float32 autograd keeps 4.
 """
 from __future__ import annotations

@@ -8,7 +8,8 @@ A layer, on node features x [M, dim]:
     x       += (1 - lam_0) rms_norm(o) W_o                 per head, head_norm_rotate without a table
     x       += relu(x W_1) W_2                             relu8 and linear8: one byte kept per hidden unit
 
-with lam = exp(a_1 . b_1) - exp(a_2 . b_2) + lam_0 per head, learned.
+with lam = exp(a_1 . b_1) - exp(a_2 . b_2) + lam_0 per head, learned.  The gradients of W_qkv, W_o and W_2 are those of the
+kept 8-bit inputs, in float32 models too (each value within 1/64 of its group's largest); all others are of the inputs themselves.
 """
 from __future__ import annotations
 
