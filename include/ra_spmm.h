@@ -520,6 +520,106 @@ ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint
                           int32_t out, int32_t cols, int64_t ldg, int32_t is_signed, int32_t dtype, float* d_out,
                           void* d_workspace, int64_t bytes, ra_stream_t stream);
 
+/* ------------------------------------------------------------ embedding lookup
+ * out[i] = scale * table[ids[i]] (no reference counterpart).  Positions whose id is
+ * `padding` give zeros, and their table row is not read; an id outside of
+ * [0, rows) gives NaN.  The gradient of the table is
+ *     d_table[v] = scale * sum over the positions i with ids[i] = v of grad[i]
+ * without those positions; it is written whole.  Its sums are fp32 and in a fixed
+ * order: the positions are sorted by id first, equal inputs give equal bits.  Rows
+ * of the table and of grad may lie ld_table, ld_grad elements apart; out [count,
+ * dim] and d_table [rows, dim] are contiguous. */
+typedef struct ra_embed_shape {
+    int64_t count;     /* positions, below 2^31 - 2^24       */
+    int64_t rows;      /* of the table, below 2^31 - 2       */
+    int32_t dim;       /* 1 .. 2^20                          */
+    int32_t dtype;     /* ra_dtype of table, out and grads   */
+    int32_t ids64;     /* ids are int64, else int32          */
+    int32_t has_padding;
+    int64_t padding;
+    int64_t ld_table, ld_grad;
+    float scale;
+} ra_embed_shape;
+ra_status ra_embed(const ra_embed_shape* shape, const void* d_ids, const void* d_table, void* d_out,
+                   ra_stream_t stream);
+/* d_workspace: ra_embed_workspace() bytes, 16-byte aligned. */
+ra_status ra_embed_workspace(const ra_embed_shape* shape, int64_t* bytes);
+ra_status ra_embed_backward(const ra_embed_shape* shape, const void* d_ids, const void* d_grad, void* d_dtable,
+                            void* d_workspace, int64_t bytes, ra_stream_t stream);
+
+/* ------------------------------------------------------------------- layer norm
+ * Of every row of h = x, or of h = x + residual rounded to the type, which is then
+ * written to d_sum (no reference counterpart):
+ *     n = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps),  y = n * weight + bias
+ * weight and bias are fp32 [dim]; NULL: 1 and 0.  Rows of x and residual may lie
+ * ldx, ldr elements apart; y and d_sum are contiguous.  Statistics are fp32, those
+ * of the variance taken around the mean.
+ * d_stats [rows, 2] fp32 (mean, 1 / deviation), for the backward pass, or NULL. */
+typedef struct ra_layer_norm_shape {
+    int64_t rows;     /* below 2^31             */
+    int32_t dim;      /* 1 .. 16384             */
+    int32_t dtype;    /* ra_dtype               */
+    float eps;
+    int64_t ldx, ldr; /* elements between rows  */
+} ra_layer_norm_shape;
+ra_status ra_layer_norm(const ra_layer_norm_shape* shape, const void* d_x, const void* d_residual,
+                        const float* d_weight, const float* d_bias, void* d_y, void* d_sum, float* d_stats,
+                        ra_stream_t stream);
+/* From h (rows ldx apart), its stats and the gradient of y (contiguous):
+ *     dx = (w g - mean(w g) - n mean(w g n)) / deviation + grad_sum
+ *     dweight = sum over the rows of g n,  dbias = sum over the rows of g
+ * grad_sum (contiguous): the gradient of d_sum, or NULL.  dx (of x and of the
+ * residual) is contiguous; d_dweight and d_dbias may be NULL.  Sums have a fixed
+ * order.  d_workspace: ra_layer_norm_workspace() bytes, 16-byte aligned (none
+ * without d_dweight and d_dbias). */
+ra_status ra_layer_norm_workspace(const ra_layer_norm_shape* shape, int64_t* bytes);
+ra_status ra_layer_norm_backward(const ra_layer_norm_shape* shape, const void* d_h, const float* d_weight,
+                                 const float* d_stats, const void* d_grad_y, const void* d_grad_sum, void* d_dx,
+                                 float* d_dweight, float* d_dbias, void* d_workspace, int64_t bytes,
+                                 ra_stream_t stream);
+
+/* ---------------------------------------- distillation from a teacher's top logits
+ * For every row of the student's logits s [rows, classes], with the teacher's kept
+ * entries (ids [rows, kept], logits t [rows, kept]) and, with d_labels, a label (no
+ * reference counterpart):
+ *     p    = softmax(t / temperature) over the row's entries
+ *     kl   = sum_e p_e (log p_e - log softmax(s / temperature)[id_e])
+ *     ce   = -log softmax(s)[label]
+ *     loss = (1 - hard) temperature^2 kl + hard ce
+ * Entries with a negative id or t = -inf take no part; a row without entries has no
+ * kl, one with a negative label (or without d_labels) no ce, and a row with neither
+ * has loss and gradient 0 whatever its logits are.  An id may stand in several
+ * entries of a row: their probabilities add up.  An id or label >= classes, a t of
+ * +inf or NaN, and a logit of +inf or NaN in a row that counts make the row's loss
+ * and gradient NaN; logits of -inf are classes of probability 0.
+ * t may have another type than s.  Sums and losses are fp32 or more, in a fixed
+ * order. */
+typedef enum ra_reduction { RA_REDUCE_NONE = 0, RA_REDUCE_MEAN = 1, RA_REDUCE_SUM = 2 } ra_reduction;
+typedef struct ra_distill_shape {
+    int64_t rows;            /* below 2^31                                  */
+    int32_t classes;         /* 1 .. 2^30                                   */
+    int32_t kept;            /* 0 .. 1024                                   */
+    int32_t dtype;           /* ra_dtype of logits and their gradient       */
+    int32_t teacher_dtype;
+    int32_t ids64, labels64; /* int64, else int32                           */
+    int32_t reduction;       /* ra_reduction; the mean is over all rows     */
+    float temperature;       /* 1e-3 .. 1e3                                 */
+    float hard;              /* 0 .. 1, 0 without labels                    */
+    int64_t ld_logits, ld_teacher, ld_ids;
+} ra_distill_shape;
+/* d_loss: [rows] without a reduction, else [1].  d_stats [rows, 4] fp32, for the
+ * backward pass, or NULL.  d_grad [rows, classes] (contiguous): the gradient of the
+ * reduced loss (of every row's without a reduction) times *d_factor (NULL: 1) in the
+ * same call, or NULL.  d_workspace: ra_distill_workspace() bytes, 16-byte aligned. */
+ra_status ra_distill_workspace(const ra_distill_shape* shape, int64_t* bytes);
+ra_status ra_distill_loss(const ra_distill_shape* shape, const void* d_logits, const void* d_teacher,
+                          const void* d_ids, const void* d_labels, const float* d_factor, float* d_loss,
+                          float* d_stats, void* d_grad, void* d_workspace, int64_t bytes, ra_stream_t stream);
+/* The gradient from d_stats and d_grad_loss ([rows] without a reduction, else [1]). */
+ra_status ra_distill_backward(const ra_distill_shape* shape, const void* d_logits, const void* d_teacher,
+                              const void* d_ids, const void* d_labels, const float* d_stats,
+                              const float* d_grad_loss, void* d_grad, ra_stream_t stream);
+
 /* ------------------------------------------------------------ utilities */
 /* fp32 -> fp16/bf16 round-to-nearest-even conversion of a [rows, cols] matrix
  * into a buffer with leading dimension ldo (columns cols..ldo-1 zero-filled).

@@ -49,6 +49,9 @@ SOURCES = {
     "head_norm.hip": [],
     "pack8.hip": [],
     "weight_grad8.hip": [],
+    "embed.hip": [],
+    "layer_norm.hip": [],
+    "distill.hip": [],
 }
 LIB_NAME = "libra_spmm_hip.so"
 
@@ -116,7 +119,7 @@ def build_binding() -> Path:
             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
             "-DTORCH_API_INCLUDE_EXTENSION_H"]
            + incs + ["-I", py_inc, "-I", "/opt/rocm/include", str(CSRC / "torch_binding.cpp"),
-                     str(CSRC / "torch_binding_ops.cpp"), "-o", str(out), "-L", str(OUT_DIR), "-lra_spmm_hip", "-L", str(torch_lib),
+                     str(CSRC / "torch_binding_ops.cpp"), str(CSRC / "torch_binding_model.cpp"), "-o", str(out), "-L", str(OUT_DIR), "-lra_spmm_hip", "-L", str(torch_lib),
                      "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-L/opt/rocm/lib", "-lamdhip64",
                      "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     _run(cmd)

@@ -1,0 +1,56 @@
+// torch_checks.hpp — what the torch surfaces of the operators share: status and argument
+// checks, the current stream.
+#pragma once
+
+#include <torch/extension.h>
+#include <c10/hip/HIPStream.h>
+
+#include "../../include/ra_spmm.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+inline ra_stream_t current_stream() {
+    return reinterpret_cast<ra_stream_t>(c10::hip::getCurrentHIPStream().stream());
+}
+
+inline void check(ra_status s, const char* what) {
+    TORCH_CHECK(s == RA_OK, what, " failed: ", ra_status_string(s), ": ", ra_last_error());
+}
+
+inline int dtype_of(const Tensor& t, const char* name) {
+    if (t.scalar_type() == torch::kFloat32) return RA_DTYPE_F32;
+    if (t.scalar_type() == torch::kFloat16) return RA_DTYPE_F16;
+    if (t.scalar_type() == torch::kBFloat16) return RA_DTYPE_BF16;
+    TORCH_CHECK(false, name, " must be float32, float16 or bfloat16");
+    return -1;
+}
+
+inline void check_on(const Tensor& t, const char* name, const torch::Device& dev) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", is on ", t.device());
+}
+
+inline const float* f32_vector(const Tensor& t, const char* name, int64_t n, const torch::Device& dev) {
+    check_on(t, name, dev);
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be float32");
+    TORCH_CHECK(t.dim() == 1 && t.numel() == n, name, " must have shape [", n, "], has ", t.sizes());
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    return t.data_ptr<float>();
+}
+
+// Distance between the rows of t, whose other dimensions have to be contiguous.
+inline int64_t row_stride(const Tensor& t, const char* name) {
+    int64_t run = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        TORCH_CHECK(t.size(d) <= 1 || t.stride(d) == run, name, " must be contiguous within its rows");
+        run *= t.size(d);
+    }
+    if (t.size(0) <= 1) return run;
+    TORCH_CHECK(t.stride(0) >= run, name, " must not have rows that overlap");
+    return t.stride(0);
+}
+
+}  // namespace

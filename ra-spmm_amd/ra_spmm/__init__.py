@@ -32,6 +32,9 @@ from .attention import diff_attention, head_norm_rotate, rotation_table  # noqa:
 from .checkpoint8 import (  # noqa: F401
     Packed8, linear8, pack8, relu8, relu_grad8, relu_pack8, unpack8, weight_grad8,
 )
+from .distill import distill_loss, distill_loss_grad  # noqa: F401
+from .embedding import embed  # noqa: F401
+from .norms import layer_norm  # noqa: F401
 from .dispatch import (  # noqa: F401
     BASE_ATOL, COLD_ITERS, COLD_ZO_MIN_CV, DEPLOYED_KERNELS, HARD_FAIL_THRESHOLD, TC_EXTRA_FACTOR, TILE_KERNELS, TIMED_ITERS,
     WARMUP, benchmark_cusparse, benchmark_cusparse_cold, benchmark_cusparse_fp16, benchmark_cusparse_fp16_cold,

@@ -32,6 +32,9 @@ EXPORTED = [
     "ra_attn_plan_run_backward", "ra_attn_csr_workspace", "ra_attn_csr",
     "ra_head_norm", "ra_head_norm_workspace", "ra_head_norm_backward",
     "ra_pack8", "ra_relu_pack8", "ra_unpack8", "ra_relu_grad8", "ra_weight_grad8_workspace", "ra_weight_grad8",
+    "ra_embed", "ra_embed_workspace", "ra_embed_backward",
+    "ra_layer_norm", "ra_layer_norm_workspace", "ra_layer_norm_backward",
+    "ra_distill_workspace", "ra_distill_loss", "ra_distill_backward",
 ]
 
 
@@ -130,6 +133,25 @@ class NormShape(ctypes.Structure):
                 [("eps", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("ldq", "ldk")])
 
 
+class EmbedShape(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int64) for n in ("count", "rows")] +
+                [(n, ctypes.c_int32) for n in ("dim", "dtype", "ids64", "has_padding")] +
+                [(n, ctypes.c_int64) for n in ("padding", "ld_table", "ld_grad")] + [("scale", ctypes.c_float)])
+
+
+class LayerNormShape(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("ldx", ctypes.c_int64), ("ldr", ctypes.c_int64)]
+
+
+class DistillShape(ctypes.Structure):
+    _fields_ = ([("rows", ctypes.c_int64)] +
+                [(n, ctypes.c_int32) for n in ("classes", "kept", "dtype", "teacher_dtype", "ids64", "labels64",
+                                               "reduction")] +
+                [(n, ctypes.c_float) for n in ("temperature", "hard")] +
+                [(n, ctypes.c_int64) for n in ("ld_logits", "ld_teacher", "ld_ids")])
+
+
 _lib = None
 
 
@@ -199,6 +221,15 @@ def load():
         "ra_relu_grad8": (ctypes.c_int, [P, P, I64, I32, I64, I32, P, P]),
         "ra_weight_grad8_workspace": (ctypes.c_int, [I64, I32, I32, ctypes.POINTER(I64)]),
         "ra_weight_grad8": (ctypes.c_int, [P, P, P, I64, I32, I32, I64, I32, I32, P, P, I64, P]),
+        "ra_embed": (ctypes.c_int, [ctypes.POINTER(EmbedShape)] + [P] * 4),
+        "ra_embed_workspace": (ctypes.c_int, [ctypes.POINTER(EmbedShape), ctypes.POINTER(I64)]),
+        "ra_embed_backward": (ctypes.c_int, [ctypes.POINTER(EmbedShape)] + [P] * 4 + [I64, P]),
+        "ra_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormShape)] + [P] * 8),
+        "ra_layer_norm_workspace": (ctypes.c_int, [ctypes.POINTER(LayerNormShape), ctypes.POINTER(I64)]),
+        "ra_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormShape)] + [P] * 9 + [I64, P]),
+        "ra_distill_workspace": (ctypes.c_int, [ctypes.POINTER(DistillShape), ctypes.POINTER(I64)]),
+        "ra_distill_loss": (ctypes.c_int, [ctypes.POINTER(DistillShape)] + [P] * 9 + [I64, P]),
+        "ra_distill_backward": (ctypes.c_int, [ctypes.POINTER(DistillShape)] + [P] * 8),
         "ra_convert_f32": (ctypes.c_int, [P, P, I64, I32, I32, I32, P]),
     }
     for name, (res, args) in sig.items():

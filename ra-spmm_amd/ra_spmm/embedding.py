@@ -1,0 +1,41 @@
+"""Embedding lookup: rows of a table by id, and the table's gradient by sorted ids.
+
+    out[i] = scale * table[ids[i]],    d table[v] = scale * sum over i with ids[i] = v of d out[i]
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _C
+from .attention import _rows
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.padding = table.size(0), scale, padding
+        return _C.run_embed(ids, table, scale, padding)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        grad = _rows(grad.reshape(ids.numel(), grad.size(-1)))
+        return None, _C.run_embed_backward(ids, grad, ctx.rows, ctx.scale, ctx.padding), None, None
+
+
+def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding: Optional[int] = None) -> torch.Tensor:
+    """scale * table[ids], of shape [*ids.shape, dim], differentiable in table.
+
+    ids int32 or int64 of any shape; table [rows, dim] float32, float16 or bfloat16, rows possibly strided.  Positions whose
+    id is `padding` (any value, inside of the table or not) give zeros and take no gradient; an id outside of the table
+    gives NaN and takes none.  The gradient is dense and of the table's type; its sums are float32, and equal inputs give
+    equal bits."""
+    ids, table = ids.contiguous(), _rows(table)
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _Embed.apply(ids, table, scale, padding)
+    return _C.run_embed(ids, table, scale, padding)
