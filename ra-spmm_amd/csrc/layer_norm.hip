@@ -5,9 +5,15 @@
 //     y = n w + b
 //     dx = r (w g - mean(w g) - n mean(w g n)) + grad_sum;  dw = sum g n,  db = sum g
 //
-// A workgroup takes a row; the variance is summed around the mean.  The sums of dw and
-// db run over pieces of the rows, which a second launch adds in order.
+// Bound by memory: every element is read once and written once (x and residual to y and
+// the sum forward, h and the gradients to dx backward).  A row lies in the registers of a
+// group of lanes, at most 16 elements a lane: of a part of a wave for short rows, of a
+// wave up to 1,024 elements, of a workgroup up to 16,384.  So the variance is summed
+// around the mean without reading again.  A lane's elements are K packets of P, the packets
+// of a row side by side over the lanes.  Backward, groups go on to further rows with the sums
+// of dw and db in registers; a second launch adds the workgroups' sums in order.
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "lanes.hpp"
@@ -17,103 +23,274 @@
 namespace ra {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;       // of a workgroup that holds several rows
 constexpr int kMaxDim = 16384;
-constexpr int kPieces = 256;       // pieces of the rows in the sums of dw and db
-constexpr int64_t kMaxBlocks = 1 << 16;
+constexpr int kMaxLane = 16;        // elements of a row in a lane
+constexpr int kForwardBlocks = 8192;
+constexpr int kBackwardBlocks = 2048;
+constexpr int kColumns = 16;        // columns of a workgroup that adds the parts of dw and db
 
 struct LayerNormArgs {
     const void *x, *res, *gy, *gs;
     void *y, *sum;
     const float *w, *b;
     float* stats;
-    float* part;  // [pieces][2][dim]
+    float* part;  // [workgroups][2][dim], or NULL
     int64_t rows, ldx, ldr;
-    int32_t dim;
+    int32_t dim, lanes_shift;
     float eps, count;  // dim as a float
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_forward(const LayerNormArgs a) {
-    __shared__ float part[2][kThreads / 64];
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// P elements as they lie in memory, zeros where there are none.
+template <typename T, int P>
+struct Packet {
+    typedef T vec __attribute__((ext_vector_type(P)));
+    vec v;
+    __device__ __forceinline__ void load(const T* p, bool there) {
+        v = *reinterpret_cast<const vec*>(there ? p : reinterpret_cast<const T*>(kZeroRun));
+    }
+    __device__ __forceinline__ float at(int e) const { return (float)v[e]; }
+};
+template <typename T, int P>
+__device__ __forceinline__ void store_packet(T* p, const float* f) {
+    typename Packet<T, P>::vec v;
+#pragma unroll
+    for (int e = 0; e < P; ++e) v[e] = (T)f[e];
+    *reinterpret_cast<typename Packet<T, P>::vec*>(p) = v;
+}
+
+// The group of lanes that a row lies in.  WAVE: a part of a wave; else the workgroup,
+// whose waves exchange sums through LDS (two sets in turn, so that one barrier a sum is enough).
+template <bool WAVE>
+struct Group {
+    int lane, lanes;
+    float* lds;  // [2][2][16]
+    int turn = 0;
+    __device__ __forceinline__ void sum2(float& a, float& b) {
+        if constexpr (WAVE) {
+            a = over_lanes<Add>(a, lanes);
+            b = over_lanes<Add>(b, lanes);
+        } else {
+            a = over_lanes<Add>(a, 64);
+            b = over_lanes<Add>(b, 64);
+            float* const to = lds + turn * 32;
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) {
+                to[threadIdx.x >> 6] = a;
+                to[16 + (threadIdx.x >> 6)] = b;
+            }
+            __syncthreads();
+            a = to[0];
+            b = to[16];
+            for (int w = 1; w < (int)(blockDim.x >> 6); ++w) {
+                a += to[w];
+                b += to[16 + w];
+            }
+        }
+    }
+    __device__ __forceinline__ float sum(float a) {
+        if constexpr (WAVE) return over_lanes<Add>(a, lanes);
+        float none = 0.f;
+        sum2(a, none);
+        return a;
+    }
+};
+
+template <typename T, int P, int K, bool WAVE>
+__global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(const LayerNormArgs a) {
+    __shared__ float lds[64];
+    Group<WAVE> group{};
+    group.lds = lds;
+    group.lanes = WAVE ? 1 << a.lanes_shift : blockDim.x;
+    group.lane = WAVE ? threadIdx.x & (group.lanes - 1) : threadIdx.x;
+    const int64_t units = WAVE ? (int64_t)gridDim.x * (kThreads >> a.lanes_shift) : gridDim.x;
+    int64_t row = WAVE ? (int64_t)blockIdx.x * (kThreads >> a.lanes_shift) + (threadIdx.x >> a.lanes_shift) : blockIdx.x;
+    float w[K][P], b[K][P];
+    bool there[K];
+    int at[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        at[k] = (k * group.lanes + group.lane) * P;
+        there[k] = at[k] < a.dim;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
+            b[k][e] = a.b && there[k] ? a.b[at[k] + e] : 0.f;
+        }
+    }
+    for (; row < a.rows; row += units) {
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
-        const T* const r = a.res ? static_cast<const T*>(a.res) + row * a.ldr : nullptr;
-        auto value = [&](int d) { return r ? (float)(T)((float)x[d] + (float)r[d]) : (float)x[d]; };
-        float s = 0.f;
-        for (int d = threadIdx.x; d < a.dim; d += kThreads) s += value(d);
-        const float mean = over_workgroup<Add>(s, part[0]) / a.count;
+        const int64_t out = row * a.dim;
+        Packet<T, P> px[K], pr[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) px[k].load(x + at[k], there[k]);
+        float h[K][P], s = 0.f;
+        if (a.res) {
+            const T* const r = static_cast<const T*>(a.res) + row * a.ldr;
+#pragma unroll
+            for (int k = 0; k < K; ++k) pr[k].load(r + at[k], there[k]);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < P; ++e) h[k][e] = px[k].at(e) + pr[k].at(e);
+                if (there[k]) store_packet<T, P>(static_cast<T*>(a.sum) + out + at[k], h[k]);
+#pragma unroll
+                for (int e = 0; e < P; ++e) h[k][e] = (float)(T)h[k][e];  // the norm is that of the sum as it is kept
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < P; ++e) h[k][e] = px[k].at(e);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < P; ++e) s += h[k][e];
+        const float mean = group.sum(s) / a.count;
         s = 0.f;
-        for (int d = threadIdx.x; d < a.dim; d += kThreads) {
-            const float c = value(d) - mean;
-            s = fmaf(c, c, s);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                h[k][e] = there[k] ? h[k][e] - mean : 0.f;
+                s = fmaf(h[k][e], h[k][e], s);
+            }
+        const float inv = rsqrtf(group.sum(s) / a.count + a.eps);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) h[k][e] = fmaf(h[k][e] * inv, w[k][e], b[k][e]);
+            if (there[k]) store_packet<T, P>(static_cast<T*>(a.y) + out + at[k], h[k]);
         }
-        const float inv = rsqrtf(over_workgroup<Add>(s, part[1]) / a.count + a.eps);
-        for (int d = threadIdx.x; d < a.dim; d += kThreads) {
-            const float h = value(d);
-            const float n = (h - mean) * inv;
-            static_cast<T*>(a.y)[row * a.dim + d] = (T)fmaf(n, a.w ? a.w[d] : 1.f, a.b ? a.b[d] : 0.f);
-            if (r) static_cast<T*>(a.sum)[row * a.dim + d] = (T)h;
-        }
-        if (a.stats && threadIdx.x == 0) {
-            a.stats[2 * row] = mean;
-            a.stats[2 * row + 1] = inv;
-        }
-        __syncthreads();
+        if (a.stats && group.lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, inv);
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_backward(const LayerNormArgs a) {
-    __shared__ float part[2][kThreads / 64];
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+template <typename T, int P, int K, bool WAVE>
+__global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(const LayerNormArgs a) {
+    __shared__ float lds[64];
+    extern __shared__ float sums[];  // WAVE: [waves][2][dim]
+    Group<WAVE> group{};
+    group.lds = lds;
+    group.lanes = WAVE ? 1 << a.lanes_shift : blockDim.x;
+    group.lane = WAVE ? threadIdx.x & (group.lanes - 1) : threadIdx.x;
+    const int64_t units = WAVE ? (int64_t)gridDim.x * (kThreads >> a.lanes_shift) : gridDim.x;
+    int64_t row = WAVE ? (int64_t)blockIdx.x * (kThreads >> a.lanes_shift) + (threadIdx.x >> a.lanes_shift) : blockIdx.x;
+    float w[K][P], dw[K][P], db[K][P];
+    bool there[K];
+    int at[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        at[k] = (k * group.lanes + group.lane) * P;
+        there[k] = at[k] < a.dim;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
+            dw[k][e] = db[k][e] = 0.f;
+        }
+    }
+    for (; row < a.rows; row += units) {
+        const int64_t out = row * a.dim;
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
-        const T* const g = static_cast<const T*>(a.gy) + row * a.dim;
-        const float mean = a.stats[2 * row], inv = a.stats[2 * row + 1];
-        float s = 0.f, t = 0.f;
-        for (int d = threadIdx.x; d < a.dim; d += kThreads) {
-            const float wg = (a.w ? a.w[d] : 1.f) * (float)g[d], n = ((float)x[d] - mean) * inv;
-            s += wg;
-            t = fmaf(wg, n, t);
+        const T* const gy = static_cast<const T*>(a.gy) + out;
+        Packet<T, P> px[K], pg[K], ps[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) px[k].load(x + at[k], there[k]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) pg[k].load(gy + at[k], there[k]);
+        if (a.gs) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) ps[k].load(static_cast<const T*>(a.gs) + out + at[k], there[k]);
         }
-        s = over_workgroup<Add>(s, part[0]) / a.count;
-        t = over_workgroup<Add>(t, part[1]) / a.count;
-        for (int d = threadIdx.x; d < a.dim; d += kThreads) {
-            const float wg = (a.w ? a.w[d] : 1.f) * (float)g[d], n = ((float)x[d] - mean) * inv;
-            float dx = inv * (wg - s - n * t);
-            if (a.gs) dx += (float)static_cast<const T*>(a.gs)[row * a.dim + d];
-            static_cast<T*>(a.y)[row * a.dim + d] = (T)dx;
+        const float2 stats = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+        const float mean = stats.x, inv = stats.y;
+        float n[K][P], g[K][P], s = 0.f, t = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                n[k][e] = (px[k].at(e) - mean) * inv;
+                const float from = pg[k].at(e);  // 0 where there is no element
+                dw[k][e] = there[k] ? fmaf(from, n[k][e], dw[k][e]) : 0.f;
+                db[k][e] += from;
+                g[k][e] = from * w[k][e];
+                s += g[k][e];
+                t = there[k] ? fmaf(g[k][e], n[k][e], t) : t;
+            }
+        group.sum2(s, t);
+        s /= a.count;
+        t /= a.count;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                g[k][e] = inv * (g[k][e] - s - n[k][e] * t);
+                if (a.gs) g[k][e] += ps[k].at(e);
+            }
+            if (there[k]) store_packet<T, P>(static_cast<T*>(a.y) + out + at[k], g[k]);
+        }
+    }
+    if (!a.part) return;
+    float* const part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    if constexpr (!WAVE) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < P; ++e)
+                if (there[k]) {
+                    part[at[k] + e] = dw[k][e];
+                    part[a.dim + at[k] + e] = db[k][e];
+                }
+    } else {
+        for (int o = group.lanes; o < 64; o <<= 1) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    dw[k][e] += __shfl_xor(dw[k][e], o, 64);
+                    db[k][e] += __shfl_xor(db[k][e], o, 64);
+                }
+        }
+        if ((int)(threadIdx.x & 63) < group.lanes) {
+            float* const to = sums + (threadIdx.x >> 6) * 2 * a.dim;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < P; ++e)
+                    if (there[k]) {
+                        to[at[k] + e] = dw[k][e];
+                        to[a.dim + at[k] + e] = db[k][e];
+                    }
         }
         __syncthreads();
+        for (int d = threadIdx.x; d < 2 * a.dim; d += kThreads) {
+            float x = 0.f;
+            for (int v = 0; v < kThreads / 64; ++v) x += sums[v * 2 * a.dim + d];
+            part[d] = x;
+        }
     }
 }
 
-// dw and db over a piece of the rows: a thread per column.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_columns(const LayerNormArgs a) {
-    const int d = blockIdx.y * kThreads + threadIdx.x;
-    const int64_t per = (a.rows + kPieces - 1) / kPieces, first = blockIdx.x * per, end = min(a.rows, first + per);
-    if (d >= a.dim) return;
-    float dw = 0.f, db = 0.f;
-    for (int64_t row = first; row < end; ++row) {
-        const float g = (float)static_cast<const T*>(a.gy)[row * a.dim + d];
-        const float n = ((float)static_cast<const T*>(a.x)[row * a.ldx + d] - a.stats[2 * row]) * a.stats[2 * row + 1];
-        dw = fmaf(g, n, dw);
-        db += g;
-    }
-    float* const to = a.part + (int64_t)blockIdx.x * 2 * a.dim;
-    to[d] = dw;
-    to[a.dim + d] = db;
-}
-
-__global__ __launch_bounds__(kThreads) void layer_norm_weights(const float* __restrict__ part, int pieces, int dim,
+// Sums of the workgroups' parts: kColumns columns a workgroup, its threads' slices of the
+// parts in order.
+__global__ __launch_bounds__(kThreads) void layer_norm_weights(const float* __restrict__ part, int parts, int dim,
                                                                float* dw, float* db) {
-    const int d = blockIdx.x * kThreads + threadIdx.x;
-    if (d >= 2 * dim) return;
+    constexpr int kSlices = kThreads / kColumns;
+    __shared__ float sums[kSlices][kColumns];
+    const int d = blockIdx.x * kColumns + threadIdx.x % kColumns, slice = threadIdx.x / kColumns;
     float s = 0.f;
-    for (int p = 0; p < pieces; ++p) s += part[(int64_t)p * 2 * dim + d];
-    float* const to = d < dim ? dw : db;
-    if (to) to[d < dim ? d : d - dim] = s;
+    if (d < 2 * dim) {
+#pragma unroll 8
+        for (int p = slice; p < parts; p += kSlices) s += part[(int64_t)p * 2 * dim + d];
+    }
+    sums[slice][threadIdx.x % kColumns] = s;
+    __syncthreads();
+    if (slice == 0 && d < 2 * dim) {
+        for (int i = 1; i < kSlices; ++i) s += sums[i][threadIdx.x];
+        float* const to = d < dim ? dw : db;
+        if (to) to[d < dim ? d : d - dim] = s;
+    }
 }
 
 ra_status check(const ra_layer_norm_shape* s) {
@@ -127,11 +304,65 @@ ra_status check(const ra_layer_norm_shape* s) {
     return RA_OK;
 }
 
+// How a row lies in lanes: packets of P elements, K of them in a lane, groups of
+// 1 << shift lanes (wave) or of `threads`.
+struct Layout {
+    int p, k, shift, threads, blocks;
+    bool wave;
+};
+
+// Packets as wide as the sizes and addresses allow (16 bytes; 8 for 16-bit types; else
+// single elements, neighbouring lanes the neighbouring ones), as few in a lane as a wave needs.
+Layout layout_of(const ra_layer_norm_shape& s, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides,
+                 int most_blocks) {
+    const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
+    auto fits = [&](int p) {
+        bool ok = s.dim % p == 0;
+        for (const void* ptr : pointers) ok = ok && reinterpret_cast<uintptr_t>(ptr) % (p * size) == 0;
+        for (int64_t ld : strides) ok = ok && (s.rows <= 1 || ld % p == 0);
+        return ok;
+    };
+    Layout l{};
+    l.p = 16 / size;
+    while (l.p > 1 && !(fits(l.p) && l.p >= 4)) l.p /= 2;
+    const int packets = s.dim / l.p, most = kMaxLane / l.p;
+    l.wave = packets <= 64 * most;
+    l.k = 1;
+    while (l.k < most && packets > 64 * l.k) l.k *= l.p == 1 ? 4 : 2;
+    if (l.wave) {
+        while (((int64_t)l.k << l.shift) < packets) ++l.shift;
+        l.threads = kThreads;
+    } else {
+        l.threads = 128;
+        while (l.threads * l.k < packets) l.threads *= 2;
+    }
+    const int64_t per = l.wave ? kThreads >> l.shift : 1;
+    // Never more than min(rows, most_blocks): the workspace holds a part for each.
+    l.blocks = static_cast<int>(std::min<int64_t>((s.rows + per - 1) / per, std::min(most_blocks, most_blocks * kThreads / l.threads)));
+    return l;
+}
+
 template <typename F>
-void by_type(int32_t dtype, F f) {
-    if (dtype == RA_DTYPE_F32) f(float());
-    else if (dtype == RA_DTYPE_F16) f(f16_t());
-    else f(bf16_t());
+void by_layout(int32_t dtype, const Layout& l, F f) {
+    auto packets = [&](auto t, auto p, auto k) {
+        if (l.wave) f(t, p, k, std::true_type());
+        else if constexpr (decltype(p)::value * decltype(k)::value == kMaxLane) f(t, p, k, std::false_type());
+    };
+    auto of_type = [&](auto t) {
+        using I1 = std::integral_constant<int, 1>;
+        using I2 = std::integral_constant<int, 2>;
+        using I4 = std::integral_constant<int, 4>;
+        using I8 = std::integral_constant<int, 8>;
+        using I16 = std::integral_constant<int, 16>;
+        if constexpr (sizeof(t) == 2) {
+            if (l.p == 8) return l.k == 1 ? packets(t, I8(), I1()) : packets(t, I8(), I2());
+        }
+        if (l.p == 4) return l.k == 1 ? packets(t, I4(), I1()) : l.k == 2 ? packets(t, I4(), I2()) : packets(t, I4(), I4());
+        return l.k == 1 ? packets(t, I1(), I1()) : l.k == 4 ? packets(t, I1(), I4()) : packets(t, I1(), I16());
+    };
+    if (dtype == RA_DTYPE_F32) of_type(float());
+    else if (dtype == RA_DTYPE_F16) of_type(f16_t());
+    else of_type(bf16_t());
 }
 
 }  // namespace
@@ -164,9 +395,11 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
     a.dim = s->dim;
     a.eps = s->eps;
     a.count = static_cast<float>(s->dim);
-    const int blocks = static_cast<int>(std::min(s->rows, ra::kMaxBlocks));
-    ra::by_type(s->dtype, [&](auto t) {
-        ra::layer_norm_forward<decltype(t)><<<blocks, ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+    const ra::Layout l = ra::layout_of(*s, {d_x, d_residual, d_y, d_sum}, {s->ldx, d_residual ? s->ldr : 0}, ra::kForwardBlocks);
+    a.lanes_shift = l.shift;
+    ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave) {
+        ra::layer_norm_forward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value>
+            <<<l.blocks, l.threads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
     });
     RA_LAUNCH_CHECK("layer_norm");
     return RA_OK;
@@ -175,7 +408,7 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
 ra_status ra_layer_norm_workspace(const ra_layer_norm_shape* s, int64_t* bytes) {
     if (!bytes) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: bytes is NULL");
     RA_TRY(ra::check(s));
-    *bytes = s->rows == 0 ? 0 : (int64_t)ra::kPieces * 2 * s->dim * (int64_t)sizeof(float);
+    *bytes = s->rows == 0 ? 0 : std::min<int64_t>(s->rows, ra::kBackwardBlocks) * 2 * s->dim * (int64_t)sizeof(float);
     return RA_OK;
 }
 
@@ -198,24 +431,25 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
     a.w = d_weight;
     a.y = d_dx;
     a.stats = const_cast<float*>(d_stats);
-    a.part = static_cast<float*>(d_workspace);
+    a.part = d_dweight || d_dbias ? static_cast<float*>(d_workspace) : nullptr;
     a.rows = s->rows;
     a.ldx = s->ldx;
     a.dim = s->dim;
     a.count = static_cast<float>(s->dim);
-    const int pieces = s->rows ? ra::kPieces : 0;  // without rows the sums are empty
+    ra::Layout l{};
     if (s->rows) {
-        const int blocks = static_cast<int>(std::min(s->rows, ra::kMaxBlocks));
-        const dim3 columns(pieces, (s->dim + ra::kThreads - 1) / ra::kThreads);
-        ra::by_type(s->dtype, [&](auto t) {
-            ra::layer_norm_backward<decltype(t)><<<blocks, ra::kThreads, 0, st>>>(a);
-            if (d_dweight || d_dbias) ra::layer_norm_columns<decltype(t)><<<columns, ra::kThreads, 0, st>>>(a);
+        l = ra::layout_of(*s, {d_h, d_grad_y, d_grad_sum, d_dx}, {s->ldx}, ra::kBackwardBlocks);
+        a.lanes_shift = l.shift;
+        const size_t lds = l.wave && a.part ? (size_t)ra::kThreads / 64 * 2 * s->dim * sizeof(float) : 0;
+        ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave) {
+            ra::layer_norm_backward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value>
+                <<<l.blocks, l.threads, lds, st>>>(a);
         });
         RA_LAUNCH_CHECK("layer_norm backward");
     }
-    if (d_dweight || d_dbias) {
-        ra::layer_norm_weights<<<(2 * s->dim + ra::kThreads - 1) / ra::kThreads, ra::kThreads, 0, st>>>(
-            a.part, pieces, s->dim, d_dweight, d_dbias);
+    if (d_dweight || d_dbias) {  // without rows the sums are empty
+        ra::layer_norm_weights<<<(2 * s->dim + ra::kColumns - 1) / ra::kColumns, ra::kThreads, 0, st>>>(
+            a.part, l.blocks, s->dim, d_dweight, d_dbias);
         RA_LAUNCH_CHECK("layer_norm_weights");
     }
     return RA_OK;
