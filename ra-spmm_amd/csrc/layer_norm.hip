@@ -29,6 +29,7 @@ constexpr int kMaxLane = 16;        // elements of a row in a lane
 constexpr int kForwardBlocks = 8192;
 constexpr int kBackwardBlocks = 2048;
 constexpr int kColumns = 16;        // columns of a workgroup that adds the parts of dw and db
+constexpr int kAddThreads = 1024;   // and its threads
 
 struct LayerNormArgs {
     const void *x, *res, *gy, *gs;
@@ -274,9 +275,9 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(co
 
 // Sums of the workgroups' parts: kColumns columns a workgroup, its threads' slices of the
 // parts in order.
-__global__ __launch_bounds__(kThreads) void layer_norm_weights(const float* __restrict__ part, int parts, int dim,
+__global__ __launch_bounds__(kAddThreads) void layer_norm_weights(const float* __restrict__ part, int parts, int dim,
                                                                float* dw, float* db) {
-    constexpr int kSlices = kThreads / kColumns;
+    constexpr int kSlices = kAddThreads / kColumns;
     __shared__ float sums[kSlices][kColumns];
     const int d = blockIdx.x * kColumns + threadIdx.x % kColumns, slice = threadIdx.x / kColumns;
     float s = 0.f;
@@ -338,8 +339,16 @@ Layout layout_of(const ra_layer_norm_shape& s, std::initializer_list<const void*
     }
     const int64_t per = l.wave ? kThreads >> l.shift : 1;
     // Never more than min(rows, most_blocks): the workspace holds a part for each.
-    l.blocks = static_cast<int>(std::min<int64_t>((s.rows + per - 1) / per, std::min(most_blocks, most_blocks * kThreads / l.threads)));
+    l.blocks = static_cast<int>(std::min<int64_t>((s.rows + per - 1) / per, most_blocks));
     return l;
+}
+
+// Workgroups of the backward pass that a CU holds at once, by their registers: with a
+// few more, those would run alone at the end.
+int resident(const Layout& l) {
+    if (!l.wave) return 1024 / l.threads;
+    const int elements = l.p * l.k;
+    return elements <= 4 ? 8 : elements == 8 ? 5 : l.p > 1 ? 3 : 1;
 }
 
 template <typename F>
@@ -439,6 +448,7 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
     ra::Layout l{};
     if (s->rows) {
         l = ra::layout_of(*s, {d_h, d_grad_y, d_grad_sum, d_dx}, {s->ldx}, ra::kBackwardBlocks);
+        l.blocks = std::min(l.blocks, 256 * ra::resident(l));
         a.lanes_shift = l.shift;
         const size_t lds = l.wave && a.part ? (size_t)ra::kThreads / 64 * 2 * s->dim * sizeof(float) : 0;
         ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave) {
@@ -448,7 +458,7 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
         RA_LAUNCH_CHECK("layer_norm backward");
     }
     if (d_dweight || d_dbias) {  // without rows the sums are empty
-        ra::layer_norm_weights<<<(2 * s->dim + ra::kColumns - 1) / ra::kColumns, ra::kThreads, 0, st>>>(
+        ra::layer_norm_weights<<<(2 * s->dim + ra::kColumns - 1) / ra::kColumns, ra::kAddThreads, 0, st>>>(
             a.part, l.blocks, s->dim, d_dweight, d_dbias);
         RA_LAUNCH_CHECK("layer_norm_weights");
     }
