@@ -554,7 +554,8 @@ ra_status ra_embed_backward(const ra_embed_shape* shape, const void* d_ids, cons
  * weight and bias are fp32 [dim]; NULL: 1 and 0.  Rows of x and residual may lie
  * ldx, ldr elements apart; y and d_sum are contiguous.  Statistics are fp32, those
  * of the variance taken around the mean.
- * d_stats [rows, 2] fp32 (mean, 1 / deviation), for the backward pass, or NULL. */
+ * d_stats [rows, 2] fp32 (mean, 1 / deviation) on 8-byte addresses, for the backward
+ * pass, or NULL. */
 typedef struct ra_layer_norm_shape {
     int64_t rows;     /* below 2^31             */
     int32_t dim;      /* 1 .. 16384             */
@@ -607,8 +608,8 @@ typedef struct ra_distill_shape {
     float hard;              /* 0 .. 1, 0 without labels                    */
     int64_t ld_logits, ld_teacher, ld_ids;
 } ra_distill_shape;
-/* d_loss: [rows] without a reduction, else [1].  d_stats [rows, 4] fp32, for the
- * backward pass, or NULL.  d_grad [rows, classes] (contiguous): the gradient of the
+/* d_loss: [rows] without a reduction, else [1].  d_stats [rows, 4] fp32 on 16-byte
+ * addresses, for the backward pass of the same shape, or NULL.  d_grad [rows, classes] (contiguous): the gradient of the
  * reduced loss (of every row's without a reduction) times *d_factor (NULL: 1) in the
  * same call, or NULL.  d_workspace: ra_distill_workspace() bytes, 16-byte aligned. */
 ra_status ra_distill_workspace(const ra_distill_shape* shape, int64_t* bytes);

@@ -22,7 +22,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxKept = 1024;
-constexpr int kParts = 1024;  // workgroups' parts of a reduced loss
+constexpr int kMaxBlocks = 4096;       // workgroups, and so parts of a reduced loss
+constexpr int kMaxShort = 1024;        // classes of a row that a wave holds
+constexpr int kStageBytes = 16384;     // rows of a workgroup at once, about
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DistillArgs {
@@ -34,14 +36,17 @@ struct DistillArgs {
     double* part;        // [workgroups] sums of the rows' losses, or NULL
     float* stats;        // [rows][4]: maximum, sum of exponentials at T and at 1
     const float* kept_stats;
+    float* piece_stats;  // [rows][pieces][4], where a row is cut
     void* grad;
     int64_t rows, ld, ldt, ldi;
     int32_t classes, kept, teacher_dtype;
     bool ids64, labels64;
     float inv_t;                // 1 / T
-    double inv_t64;
     float soft, hard;           // (1 - hard) T^2 and hard
     float soft_grad;            // (1 - hard) T
+    int32_t stage_rows, lanes_shift;   // short rows: rows of a workgroup at once, lanes of a row
+    bool whole;                 // rows lie one after the other on 16-byte addresses, the gradient's too
+    int32_t pieces, piece;      // long rows: pieces of a row, classes of one
 };
 
 __device__ __forceinline__ float teacher_at(const DistillArgs& a, int64_t at) {
@@ -55,115 +60,393 @@ __device__ __forceinline__ int64_t id_at(const DistillArgs& a, int64_t at) {
 // exp(x / T) for x <= 0 (or -inf), c = log2(e) / T
 __device__ __forceinline__ float exp_of(float x, float c) { return __builtin_amdgcn_exp2f(x * c); }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_rows(const DistillArgs a) {
-    extern __shared__ char lds[];
-    float* const amount = reinterpret_cast<float*>(lds);                      // [kept + 1]: taken off the gradient
-    int32_t* const place = reinterpret_cast<int32_t*>(amount + a.kept + 1);   // its class, -1: none
-    __shared__ float part[6][kThreads / 64];
+// The lanes that share a row: a part of a wave, or the workgroup, whose waves exchange
+// through LDS.
+struct WaveTeam {
+    int lane, lanes;
+    template <typename Op>
+    __device__ __forceinline__ float all(float x) { return over_lanes<Op>(x, lanes); }
+    __device__ __forceinline__ float sum(float x) { return all<Add>(x); }
+    __device__ __forceinline__ void sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+};
+struct WorkgroupTeam {
+    int lane, lanes;
+    float* lds;  // [2][16], in turn
+    int turn = 0;
+    template <typename Op>
+    __device__ __forceinline__ float all(float x) {
+        turn ^= 1;
+        return over_workgroup<Op>(x, lds + 16 * turn);
+    }
+    __device__ __forceinline__ float sum(float x) { return all<Add>(x); }
+    __device__ __forceinline__ void sync() { __syncthreads(); }
+};
+
+// A row's teacher entries and label: place[e] is the entry's class (-1: takes no part),
+// amount[e] its logit; entry `kept` is the label.
+struct Targets {
+    float* amount;
+    int32_t* place;
+    float top, sum;
+    int64_t label;
+    bool soft, hard;
+};
+
+template <typename Team>
+__device__ __forceinline__ void read_targets(const DistillArgs& a, int64_t row, Team& team, Targets& t) {
+    float top = -INFINITY;
+    bool outside = false;
+    for (int e = team.lane; e < a.kept; e += team.lanes) {
+        const int64_t id = id_at(a, row * a.ldi + e);
+        const float x = teacher_at(a, row * a.ldt + e);
+        const bool used = id >= 0 && x != -INFINITY;
+        outside |= used && id >= a.classes;
+        t.place[e] = used && id < a.classes ? (int32_t)id : -1;
+        t.amount[e] = x;
+        if (used) top = x != x ? INFINITY : fmaxf(top, x);
+    }
+    t.top = team.template all<Max>(top);
+    t.soft = a.soft > 0.f && t.top != -INFINITY;
+    float sum = 0.f;
+    for (int e = team.lane; e < a.kept; e += team.lanes)
+        if (t.place[e] >= 0) sum += exp_of(t.amount[e] - t.top, kLog2e * a.inv_t);
+    t.sum = team.sum(outside ? NAN : sum);
+    t.label = -1;
+    if (a.labels) t.label = a.labels64 ? static_cast<const int64_t*>(a.labels)[row] : (int64_t)static_cast<const int32_t*>(a.labels)[row];
+    t.hard = a.hard > 0.f && t.label >= 0;
+}
+
+// The row's loss from its maximum and sums of exponentials; x(j): the logit of class j.
+template <typename Team, typename X>
+__device__ __forceinline__ float row_loss(const DistillArgs& a, Team& team, const Targets& t, float most, float at_t, float at_1, X x) {
+    const float shift = logf(at_t) - logf(t.sum);
+    float loss = 0.f;
+    for (int e = team.lane; e < a.kept; e += team.lanes) {
+        if (!t.soft || t.place[e] < 0) continue;
+        const float p = exp_of(t.amount[e] - t.top, kLog2e * a.inv_t) / t.sum;
+        if (p != 0.f) loss = fmaf(p, fmaf((t.amount[e] - t.top) - (x(t.place[e]) - most), a.inv_t, shift), loss);
+    }
+    loss = team.sum(loss) * a.soft;
+    if (!t.soft) loss = 0.f;
+    else if (t.sum != t.sum) loss = NAN;
+    if (t.hard) loss += t.label < a.classes ? a.hard * (logf(at_1) - (x((int)t.label) - most)) : NAN;
+    return loss;
+}
+
+// Factors of the row's gradient: it is soft exp((s - most) / T) + hard exp(s - most) without
+// the entries, and amount[e] becomes what each entry takes off.
+struct Factors {
+    float soft, hard, most;
+    // of s - most
+    __device__ __forceinline__ float operator()(const DistillArgs& a, float d) const {
+        float g = 0.f;
+        if (soft != 0.f) g = soft * exp_of(d, kLog2e * a.inv_t);
+        if (hard != 0.f) g = fmaf(hard, exp_of(d, kLog2e), g);
+        return g;
+    }
+};
+template <typename Team>
+__device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t row, Team& team, const Targets& t, float most,
+                                                 float at_t, float at_1) {
+    const float up = (a.up ? a.up[row * a.up_step] : 1.f) * a.up_scale;
+    const float soft_up = !t.soft ? 0.f : t.sum != t.sum ? NAN : a.soft_grad * up;
+    const float hard_up = !t.hard ? 0.f : t.label < a.classes ? a.hard * up : NAN;
+    for (int e = team.lane; e <= a.kept; e += team.lanes) {
+        if (e < a.kept) {
+            t.amount[e] = t.soft && t.place[e] >= 0 ? soft_up * (exp_of(t.amount[e] - t.top, kLog2e * a.inv_t) / t.sum) : 0.f;
+            if (!t.soft) t.place[e] = -1;
+        } else {
+            t.amount[e] = hard_up;
+            t.place[e] = t.hard && t.label < a.classes ? (int32_t)t.label : -1;
+        }
+    }
+    return {t.soft ? soft_up / at_t : 0.f, t.hard ? hard_up / at_1 : 0.f, most};
+}
+// What all entries of e's class take off; `first`: no earlier entry has it.
+__device__ __forceinline__ float class_amount(const Targets& t, int kept, int e, bool& first) {
+    float off = 0.f;
+    first = true;
+    for (int f = 0; f <= kept; ++f) {
+        if (t.place[f] != t.place[e]) continue;
+        first &= f >= e;
+        off += t.amount[f];
+    }
+    return off;
+}
+
+// ------------------------------------------------------------------ short rows
+// Rows of up to 1,024 classes.  A workgroup takes stage_rows of them, one run of memory,
+// through LDS: whole 16-byte packets whatever the number of classes is, where rows of 47
+// elements would be read by single ones.  A row is held by 2^lanes_shift lanes, K elements
+// each; its gradient takes its place in LDS and goes out the same way.
+template <typename T, int K>
+__global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
+    extern __shared__ __align__(16) char lds[];
     __shared__ double part64[kThreads / 64];
+    constexpr int kPer = 16 / sizeof(T);
+    const int lanes = 1 << a.lanes_shift, group = threadIdx.x >> a.lanes_shift, groups = kThreads >> a.lanes_shift;
+    const int C = a.classes, entries = a.kept + 1;
+    T* const stage = reinterpret_cast<T*>(lds);
+    float* const arrays = reinterpret_cast<float*>(lds + (a.stage_rows * C * (int)sizeof(T) + 15) / 16 * 16);
+    WaveTeam team{(int)threadIdx.x & (lanes - 1), lanes};
+    Targets t{};
+    t.amount = arrays + group * entries;
+    t.place = reinterpret_cast<int32_t*>(arrays) + (groups + group) * entries;
+    float* const value = arrays + (2 * groups + group) * entries;  // what an entry writes, and where (-1: another does)
+    int32_t* const to = reinterpret_cast<int32_t*>(arrays) + (3 * groups + group) * entries;
+    uint16_t* const owner = reinterpret_cast<uint16_t*>(arrays + 4 * groups * entries) + group * C;
     const float c = kLog2e * a.inv_t;
     double total = 0.0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* const x = static_cast<const T*>(a.logits) + row * a.ld;
-        // The teacher's entries.
-        float top = -INFINITY;
-        bool outside = false;
-        for (int e = threadIdx.x; e < a.kept; e += kThreads) {
-            const int64_t id = id_at(a, row * a.ldi + e);
-            const float t = teacher_at(a, row * a.ldt + e);
-            const bool used = id >= 0 && t != -INFINITY;
-            outside |= used && id >= a.classes;
-            place[e] = used && id < a.classes ? (int32_t)id : -1;
-            amount[e] = t;
-            if (used) top = t != t ? INFINITY : fmaxf(top, t);
+    for (int64_t first = (int64_t)blockIdx.x * a.stage_rows; first < a.rows; first += (int64_t)gridDim.x * a.stage_rows) {
+        const int rows = (int)min((int64_t)a.stage_rows, a.rows - first), n = rows * C;
+        const T* const from = static_cast<const T*>(a.logits) + first * a.ld;
+        if (a.whole) {
+            for (int i = threadIdx.x * kPer; i + kPer <= n; i += kThreads * kPer)
+                *reinterpret_cast<uint4*>(stage + i) = *reinterpret_cast<const uint4*>(from + i);
+            const int i = n / kPer * kPer + (int)threadIdx.x;
+            if (i < n) stage[i] = from[i];
+        } else {
+            for (int r = threadIdx.x >> 6; r < rows; r += kThreads / 64)
+                for (int j = threadIdx.x & 63; j < C; j += 64) stage[r * C + j] = from[r * a.ld + j];
         }
-        top = over_workgroup<Max>(top, part[0]);
-        const bool soft = a.soft > 0.f && top != -INFINITY;
-        float sum = 0.f;
-        for (int e = threadIdx.x; e < a.kept; e += kThreads)
-            if (place[e] >= 0) sum += exp_of(amount[e] - top, c);
-        sum = over_workgroup<Add>(outside ? NAN : sum, part[1]);
-        // The label.
-        int64_t label = -1;
-        if (a.labels) label = a.labels64 ? static_cast<const int64_t*>(a.labels)[row] : (int64_t)static_cast<const int32_t*>(a.labels)[row];
-        const bool hard = a.hard > 0.f && label >= 0;
-        // The logits' sums of exponentials.
+        __syncthreads();
+        for (int r0 = 0; r0 < rows; r0 += groups) {
+            const bool there = r0 + group < rows;
+            const int r = there ? r0 + group : 0;  // lanes without a row go along with the first and keep nothing
+            const int64_t row = first + r;
+            T* const x = stage + r * C;
+            auto logit = [&](int j) { return (float)x[j]; };
+            read_targets(a, row, team, t);
+            float v[K], most = -FLT_MAX, at_t = 0.f, at_1 = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int j = k * lanes + team.lane;
+                v[k] = j < C ? (float)x[j] : -INFINITY;
+                most = fmaxf(most, v[k]);
+            }
+            most = team.template all<Max>(most);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                v[k] -= most;
+                at_t += exp_of(v[k], c);
+            }
+            at_t = team.sum(at_t);
+            if (a.hard > 0.f) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) at_1 += exp_of(v[k], kLog2e);
+                at_1 = team.sum(at_1);
+            }
+            if (a.loss || a.part) {
+                const float loss = row_loss(a, team, t, most, at_t, at_1, logit);
+                if (there && team.lane == 0) {
+                    if (a.loss) a.loss[row] = loss;
+                    total += loss;
+                }
+            }
+            if (!a.grad) continue;
+            const Factors f = entry_amounts(a, row, team, t, most, at_t, at_1);
+            team.sync();
+            // Whether a class has several entries: one of them is not its owner then.
+            for (int e = team.lane; e < entries; e += lanes)
+                if (t.place[e] >= 0) owner[t.place[e]] = (uint16_t)e;
+            team.sync();
+            bool twice = false;
+            for (int e = team.lane; e < entries; e += lanes) twice |= t.place[e] >= 0 && owner[t.place[e]] != e;
+            const bool any_twice = __any(twice);
+            for (int e = team.lane; e < entries; e += lanes) {
+                const int32_t j = t.place[e];
+                bool first_of = true;
+                float off = t.amount[e];
+                if (any_twice && j >= 0) off = class_amount(t, a.kept, e, first_of);
+                value[e] = j >= 0 ? f(a, logit(j) - most) - off : 0.f;
+                to[e] = first_of && there ? j : -1;
+            }
+            team.sync();
+            if (there) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int j = k * lanes + team.lane;
+                    if (j < C) x[j] = (T)f(a, v[k]);
+                }
+            }
+            team.sync();
+            for (int e = team.lane; e < entries; e += lanes)
+                if (to[e] >= 0) x[to[e]] = (T)value[e];
+        }
+        __syncthreads();
+        if (a.grad) {
+            T* const out = static_cast<T*>(a.grad) + first * C;
+            if (a.whole) {
+                for (int i = threadIdx.x * kPer; i + kPer <= n; i += kThreads * kPer)
+                    *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(stage + i);
+                const int i = n / kPer * kPer + (int)threadIdx.x;
+                if (i < n) out[i] = stage[i];
+            } else {
+                for (int i = threadIdx.x; i < n; i += kThreads) out[i] = stage[i];
+            }
+            __syncthreads();
+        }
+    }
+    if (a.part) {
+        total = sum_workgroup(total, part64);
+        if (threadIdx.x == 0) a.part[blockIdx.x] = total;
+    }
+}
+
+// ------------------------------------------------------------------- long rows
+// 16 bytes of a row; elements past the packets, at both ends, are taken one by one.
+template <typename T>
+struct Span {
+    static constexpr int kPer = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(kPer)));
+    int first, packets, end;  // [first, first + kPer * packets) lies on whole packets
+    __device__ __forceinline__ Span(const T* x, int begin, int end_) : end(end_) {
+        const int off = (int)((reinterpret_cast<uintptr_t>(x + begin) % 16) / sizeof(T));
+        first = min(end, begin + (off ? kPer - off : 0));
+        packets = (end - first) / kPer;
+    }
+};
+
+// A team's maximum of a part of a row and the sums of its exponentials at T and at 1, in one
+// pass: every lane scales its sums down when its maximum grows.
+template <typename T, typename Team>
+__device__ __forceinline__ void scan_part(const DistillArgs& a, Team& team, const T* x, int begin, int end, float& most, float& at_t,
+                                          float& at_1) {
+    using S = Span<T>;
+    constexpr int kAhead = 4;  // packets of a lane at once
+    const float c = kLog2e * a.inv_t;
+    const bool hard = a.hard > 0.f;
+    most = -FLT_MAX;
+    at_t = at_1 = 0.f;
+    const S s(x, begin, end);
+    auto add = [&](const float* v, int n) {
+        float top = most;
+        for (int i = 0; i < n; ++i) top = fmaxf(top, v[i]);
+        const float down = most - top;
+        at_t *= exp_of(down, c);
+        for (int i = 0; i < n; ++i) at_t += exp_of(v[i] - top, c);
+        if (hard) {
+            at_1 *= exp_of(down, kLog2e);
+            for (int i = 0; i < n; ++i) at_1 += exp_of(v[i] - top, kLog2e);
+        }
+        most = top;
+    };
+    for (int p = team.lane; p < s.packets; p += kAhead * team.lanes) {
+        typename S::vec v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            v[u] = *reinterpret_cast<const typename S::vec*>(x + s.first + min(p + u * team.lanes, s.packets - 1) * S::kPer);
+        float f[kAhead * S::kPer];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int e = 0; e < S::kPer; ++e) f[u * S::kPer + e] = p + u * team.lanes < s.packets ? (float)v[u][e] : -INFINITY;
+        add(f, kAhead * S::kPer);
+    }
+    const int tail = s.first + s.packets * S::kPer;
+    for (int j = begin + team.lane; j < s.first; j += team.lanes) {
+        const float f = (float)x[j];
+        add(&f, 1);
+    }
+    for (int j = tail + team.lane; j < end; j += team.lanes) {
+        const float f = (float)x[j];
+        add(&f, 1);
+    }
+    const float top = team.template all<Max>(most);
+    at_t = team.sum(at_t * exp_of(most - top, c));
+    if (hard) at_1 = team.sum(at_1 * exp_of(most - top, kLog2e));
+    most = top;
+}
+
+// Rows cut into pieces: each piece's maximum and sums.
+template <typename T>
+__global__ __launch_bounds__(1024) void distill_pieces(const DistillArgs a) {
+    __shared__ float lds[32];
+    WorkgroupTeam team{(int)threadIdx.x, (int)blockDim.x, lds};
+    for (int64_t work = blockIdx.x; work < a.rows * a.pieces; work += gridDim.x) {
+        const int64_t row = work / a.pieces;
+        const int begin = (int)(work - row * a.pieces) * a.piece, end = min(a.classes, begin + a.piece);
+        float most, at_t, at_1;
+        scan_part(a, team, static_cast<const T*>(a.logits) + row * a.ld, begin, end, most, at_t, at_1);
+        if (threadIdx.x == 0) *reinterpret_cast<float4*>(a.piece_stats + 4 * work) = make_float4(most, at_t, at_1, 0.f);
+        __syncthreads();
+    }
+}
+
+// A workgroup per row, or per piece of one where the gradient is wanted; the loss is formed
+// by the first piece.
+template <typename T>
+__global__ __launch_bounds__(1024) void distill_long(const DistillArgs a) {
+    extern __shared__ float entries[];
+    __shared__ float lds[32];
+    using S = Span<T>;
+    WorkgroupTeam team{(int)threadIdx.x, (int)blockDim.x, lds};
+    Targets t{};
+    t.amount = entries;
+    t.place = reinterpret_cast<int32_t*>(entries) + a.kept + 1;
+    const int pieces = a.grad ? a.pieces : 1;
+    double total = 0.0;
+    for (int64_t work = blockIdx.x; work < a.rows * pieces; work += gridDim.x) {
+        const int64_t row = work / pieces;
+        const int piece = (int)(work - row * pieces);
+        const int begin = a.grad ? piece * a.piece : 0, end = a.grad ? min(a.classes, begin + a.piece) : a.classes;
+        const T* const x = static_cast<const T*>(a.logits) + row * a.ld;
+        auto logit = [&](int j) { return (float)x[j]; };
+        read_targets(a, row, team, t);
         float most = -FLT_MAX, at_t = 0.f, at_1 = 0.f;
         if (a.kept_stats) {
-            most = a.kept_stats[4 * row];
-            at_t = a.kept_stats[4 * row + 1];
-            at_1 = a.kept_stats[4 * row + 2];
-        } else if (soft || hard) {
-            for (int j = threadIdx.x; j < a.classes; j += kThreads) most = fmaxf(most, (float)x[j]);
-            most = over_workgroup<Max>(most, part[2]);
-            for (int j = threadIdx.x; j < a.classes; j += kThreads) {
-                at_t += exp_of((float)x[j] - most, c);
-                at_1 += exp_of((float)x[j] - most, kLog2e);
+            const float4 k = *reinterpret_cast<const float4*>(a.kept_stats + 4 * row);
+            most = k.x;
+            at_t = k.y;
+            at_1 = k.z;
+        } else if (a.piece_stats) {
+            const float4* const from = reinterpret_cast<const float4*>(a.piece_stats) + row * a.pieces;
+            for (int p = team.lane; p < a.pieces; p += team.lanes) most = fmaxf(most, from[p].x);
+            most = team.template all<Max>(most);
+            for (int p = team.lane; p < a.pieces; p += team.lanes) {
+                at_t = fmaf(from[p].y, exp_of(from[p].x - most, kLog2e * a.inv_t), at_t);
+                at_1 = fmaf(from[p].z, exp_of(from[p].x - most, kLog2e), at_1);
             }
-            at_t = over_workgroup<Add>(at_t, part[3]);
-            at_1 = over_workgroup<Add>(at_1, part[4]);
+            at_t = team.sum(at_t);
+            at_1 = team.sum(at_1);
+        } else if (t.soft || t.hard) {
+            scan_part(a, team, x, 0, a.classes, most, at_t, at_1);
         }
-        if (a.stats && threadIdx.x == 0) {
-            a.stats[4 * row] = most;
-            a.stats[4 * row + 1] = at_t;
-            a.stats[4 * row + 2] = at_1;
-            a.stats[4 * row + 3] = 0.f;
-        }
-        if (a.loss || a.part) {
-            double loss = 0.0;
-            if (soft) {
-                const double shift = log((double)at_t) - log((double)sum);
-                for (int e = threadIdx.x; e < a.kept; e += kThreads) {
-                    if (place[e] < 0) continue;
-                    const float p = exp_of(amount[e] - top, c) / sum;
-                    if (p != 0.f)
-                        loss += (double)p * ((((double)amount[e] - top) - ((double)(float)x[place[e]] - most)) * a.inv_t64 + shift);
-                }
-                loss = sum_workgroup(loss, part64) * a.soft;
-                if (sum != sum) loss = NAN;
-                __syncthreads();
+        if (piece == 0) {
+            if (a.stats && threadIdx.x == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(most, at_t, at_1, 0.f);
+            if (a.loss || a.part) {
+                const float loss = row_loss(a, team, t, most, at_t, at_1, logit);
+                if (a.loss && threadIdx.x == 0) a.loss[row] = loss;
+                total += loss;
             }
-            if (hard) loss += label < a.classes ? a.hard * (log((double)at_1) - ((double)(float)x[label] - most)) : NAN;
-            if (a.loss && threadIdx.x == 0) a.loss[row] = (float)loss;
-            total += loss;
         }
         if (a.grad) {
-            const float up = (a.up ? a.up[row * a.up_step] : 1.f) * a.up_scale;
-            const float soft_up = !soft ? 0.f : sum != sum ? NAN : a.soft_grad * up;
-            const float hard_up = !hard ? 0.f : label < a.classes ? a.hard * up : NAN;
-            const float ft = soft ? soft_up / at_t : 0.f, f1 = hard ? hard_up / at_1 : 0.f;
-            auto without = [&](float s) {
-                float g = 0.f;
-                if (soft) g = ft * exp_of(s - most, c);
-                if (hard) g += f1 * exp_of(s - most, kLog2e);
-                return g;
-            };
-            __syncthreads();  // the loss has been read
-            for (int e = threadIdx.x; e <= a.kept; e += kThreads) {
-                if (e < a.kept) {
-                    amount[e] = soft && place[e] >= 0 ? soft_up * (exp_of(amount[e] - top, c) / sum) : 0.f;
-                    if (!soft) place[e] = -1;
-                } else {
-                    amount[e] = hard_up;
-                    place[e] = hard && label < a.classes ? (int32_t)label : -1;
-                }
-            }
+            __syncthreads();  // all have read the amounts
+            const Factors f = entry_amounts(a, row, team, t, most, at_t, at_1);
             T* const g = static_cast<T*>(a.grad) + row * a.classes;
-            for (int j = threadIdx.x; j < a.classes; j += kThreads) g[j] = (T)without((float)x[j]);
+            const S s(x, begin, end);
+            auto one = [&](int j) { g[j] = (T)f(a, (float)x[j] - most); };
+            if ((reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(x)) % 16 == 0) {
+                for (int p = team.lane; p < s.packets; p += team.lanes) {
+                    const auto v = *reinterpret_cast<const typename S::vec*>(x + s.first + p * S::kPer);
+                    typename S::vec out;
+#pragma unroll
+                    for (int e = 0; e < S::kPer; ++e) out[e] = (T)f(a, (float)v[e] - most);
+                    *reinterpret_cast<typename S::vec*>(g + s.first + p * S::kPer) = out;
+                }
+                for (int j = begin + team.lane; j < s.first; j += team.lanes) one(j);
+                for (int j = s.first + s.packets * S::kPer + team.lane; j < end; j += team.lanes) one(j);
+            } else {
+                for (int j = begin + team.lane; j < end; j += team.lanes) one(j);
+            }
             __threadfence_block();
             __syncthreads();
-            for (int e = threadIdx.x; e <= a.kept; e += kThreads) {
-                const int32_t j = place[e];
-                if (j < 0) continue;
-                float off = 0.f;
-                bool first = true;
-                for (int f = 0; f <= a.kept; ++f) {
-                    if (place[f] != j) continue;
-                    first &= f >= e;
-                    off += amount[f];
-                }
-                if (first) g[j] = (T)(without((float)x[j]) - off);
+            for (int e = team.lane; e <= a.kept; e += team.lanes) {
+                const int32_t j = t.place[e];
+                if (j < begin || j >= end) continue;
+                bool first;
+                const float off = class_amount(t, a.kept, e, first);
+                if (first) g[j] = (T)(f(a, logit(j) - most) - off);
             }
         }
         __syncthreads();
@@ -222,22 +505,87 @@ DistillArgs args_of(const ra_distill_shape& s, const void* logits, const void* t
     a.teacher_dtype = s.teacher_dtype;
     a.ids64 = s.ids64 != 0;
     a.labels64 = s.labels64 != 0;
-    a.inv_t64 = 1.0 / s.temperature;
-    a.inv_t = static_cast<float>(a.inv_t64);
+    a.inv_t = static_cast<float>(1.0 / s.temperature);
     a.soft = static_cast<float>((1.0 - s.hard) * s.temperature * s.temperature);
     a.hard = s.hard;
     a.soft_grad = static_cast<float>((1.0 - s.hard) * s.temperature);
     return a;
 }
 
-int blocks_of(const ra_distill_shape& s) { return static_cast<int>(std::min<int64_t>(s.rows, kParts)); }
+bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.kept <= 256; }
 
-void run(const ra_distill_shape& s, const DistillArgs& a, hipStream_t st) {
+// Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements
+// (16 past 256 classes), more lanes where the entries of all groups would pass 16 kB.
+struct ShortPlan {
+    int shift, rows, blocks;
+    size_t lds;
+};
+ShortPlan short_plan(const ra_distill_shape& s) {
+    const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2, k = s.classes <= 256 ? 4 : 16, entries = s.kept + 1;
+    ShortPlan p{};
+    while ((k << p.shift) < s.classes || (kThreads >> p.shift) * entries * 16 > 4 * 257 * 16) ++p.shift;
+    const int groups = kThreads >> p.shift;
+    p.rows = std::max(groups, 8);  // 8 rows are whole packets
+    while (2 * p.rows * s.classes * size <= kStageBytes) p.rows *= 2;
+    p.blocks = static_cast<int>(std::min<int64_t>((s.rows + p.rows - 1) / p.rows, kMaxBlocks));
+    p.lds = (size_t)(p.rows * s.classes * size + 15) / 16 * 16 + (size_t)groups * entries * 16 + (size_t)groups * s.classes * 2;
+    return p;
+}
+
+// Long rows: a row a workgroup where there are two for every CU, else pieces of at least
+// 4,096 classes.
+struct LongPlan {
+    int pieces, piece, threads;
+};
+LongPlan long_plan(const ra_distill_shape& s) {
+    LongPlan p{};
+    const int64_t want = s.rows ? (512 + s.rows - 1) / s.rows : 1;
+    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, s.classes / 4096)));
+    p.piece = (s.classes + p.pieces - 1) / p.pieces;
+    p.threads = p.piece >= 16384 ? 1024 : 256;
+    return p;
+}
+int long_blocks(const ra_distill_shape& s, int pieces) {
+    return static_cast<int>(std::min<int64_t>(s.rows * pieces, kMaxBlocks));
+}
+
+// Workgroups that leave a part of the loss.
+int loss_parts(const ra_distill_shape& s, bool grad) {
+    if (s.rows == 0) return 0;
+    return is_short(s) ? short_plan(s).blocks : long_blocks(s, grad ? long_plan(s).pieces : 1);
+}
+
+template <typename F>
+void by_type(int32_t dtype, F f) {
+    if (dtype == RA_DTYPE_F32) f(float());
+    else if (dtype == RA_DTYPE_F16) f(f16_t());
+    else f(bf16_t());
+}
+
+void run(const ra_distill_shape& s, DistillArgs& a, hipStream_t st) {
+    if (is_short(s)) {
+        const ShortPlan p = short_plan(s);
+        a.stage_rows = p.rows;
+        a.lanes_shift = p.shift;
+        a.whole = (s.rows <= 1 || s.ld_logits == s.classes) && aligned16(a.logits) && aligned16(a.grad);
+        by_type(s.dtype, [&](auto t) {
+            using T = decltype(t);
+            if (s.classes <= 256) distill_short<T, 4><<<p.blocks, kThreads, p.lds, st>>>(a);
+            else distill_short<T, 16><<<p.blocks, kThreads, p.lds, st>>>(a);
+        });
+        return;
+    }
+    const LongPlan p = long_plan(s);
+    a.pieces = p.pieces;
+    a.piece = p.piece;
     const size_t lds = (size_t)(s.kept + 1) * 8;
-    auto go = [&](auto t) { distill_rows<decltype(t)><<<blocks_of(s), kThreads, lds, st>>>(a); };
-    if (s.dtype == RA_DTYPE_F32) go(float());
-    else if (s.dtype == RA_DTYPE_F16) go(f16_t());
-    else go(bf16_t());
+    by_type(s.dtype, [&](auto t) {
+        using T = decltype(t);
+        if (a.kept_stats || p.pieces == 1) a.piece_stats = nullptr;
+        else distill_pieces<T><<<long_blocks(s, p.pieces), p.threads, 0, st>>>(a);
+        const int threads = a.grad || p.pieces == 1 ? p.threads : 256;
+        distill_long<T><<<long_blocks(s, a.grad ? p.pieces : 1), threads, lds, st>>>(a);
+    });
 }
 
 }  // namespace
@@ -250,7 +598,10 @@ extern "C" {
 ra_status ra_distill_workspace(const ra_distill_shape* s, int64_t* bytes) {
     if (!bytes) return fail(RA_ERR_INVALID_ARGUMENT, "distill: bytes is NULL");
     RA_TRY(ra::check(s));
-    *bytes = s->reduction == RA_REDUCE_NONE || s->rows == 0 ? 0 : (int64_t)ra::blocks_of(*s) * (int64_t)sizeof(double);
+    *bytes = 0;
+    if (s->rows == 0) return RA_OK;
+    if (s->reduction != RA_REDUCE_NONE) *bytes = (int64_t)ra::kMaxBlocks * (int64_t)sizeof(double);
+    if (!ra::is_short(*s)) *bytes += s->rows * (ra::long_plan(*s).pieces > 1 ? ra::long_plan(*s).pieces : 0) * 16;
     return RA_OK;
 }
 
@@ -263,20 +614,27 @@ ra_status ra_distill_loss(const ra_distill_shape* s, const void* d_logits, const
     if (!d_loss && (s->rows || s->reduction != RA_REDUCE_NONE)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: NULL loss");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: the workspace is too small");
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: the workspace must be 16-byte aligned");
+    if (!ra::aligned16(d_stats)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::DistillArgs a = ra::args_of(*s, d_logits, d_teacher, d_ids, d_labels);
     a.up = d_factor;
     a.stats = d_stats;
     a.grad = d_grad;
-    if (s->reduction == RA_REDUCE_NONE) a.loss = d_loss;
-    else a.part = static_cast<double*>(d_workspace);
+    char* work = static_cast<char*>(d_workspace);
+    if (s->reduction == RA_REDUCE_NONE) {
+        a.loss = d_loss;
+    } else {
+        a.part = reinterpret_cast<double*>(work);
+        work += (int64_t)ra::kMaxBlocks * (int64_t)sizeof(double);
+    }
+    a.piece_stats = reinterpret_cast<float*>(work);
     if (s->rows) {
         ra::run(*s, a, st);
         RA_LAUNCH_CHECK("distill");
     }
     if (s->reduction != RA_REDUCE_NONE) {  // the mean of no rows is NaN
         const double scale = s->reduction == RA_REDUCE_SUM ? 1.0 : s->rows ? 1.0 / static_cast<double>(s->rows) : NAN;
-        ra::distill_reduce<<<1, ra::kThreads, 0, st>>>(a.part, s->rows ? ra::blocks_of(*s) : 0, scale, d_loss);
+        ra::distill_reduce<<<1, ra::kThreads, 0, st>>>(a.part, ra::loss_parts(*s, d_grad != nullptr), scale, d_loss);
         RA_LAUNCH_CHECK("distill_reduce");
     }
     return RA_OK;
@@ -289,6 +647,7 @@ ra_status ra_distill_backward(const ra_distill_shape* s, const void* d_logits, c
     RA_TRY(ra::check_tensors(*s, d_logits, d_teacher, d_ids, d_labels));
     if (s->rows == 0) return RA_OK;
     if (!d_stats || !d_grad_loss || !d_grad) return fail(RA_ERR_INVALID_ARGUMENT, "distill: NULL tensor");
+    if (!ra::aligned16(d_stats)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
     ra::DistillArgs a = ra::args_of(*s, d_logits, d_teacher, d_ids, d_labels);
     a.kept_stats = d_stats;
     a.up = d_grad_loss;

@@ -390,6 +390,7 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
         return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: a residual and the sum go together");
     if (d_residual && s->rows > 1 && s->ldr < s->dim)
         return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: rows overlap (ldr is too small)");
+    if (reinterpret_cast<uintptr_t>(d_stats) % 8) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: stats must be 8-byte aligned");
     ra::LayerNormArgs a{};
     a.x = d_x;
     a.res = d_residual;
@@ -430,6 +431,7 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
     if (!d_dweight && !d_dbias) need = 0;
     if (s->rows > 0 && (!d_h || !d_stats || !d_grad_y || !d_dx))
         return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: NULL tensor");
+    if (reinterpret_cast<uintptr_t>(d_stats) % 8) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: stats must be 8-byte aligned");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: the workspace is too small");
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: the workspace must be 16-byte aligned");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);

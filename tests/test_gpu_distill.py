@@ -2,8 +2,8 @@
 
 Tolerances, u = 2^-24.  An exponential exp((x - max) / T) is off by 6 |x - max| / T u + 2 u of itself (the difference, the factor, its
 product, the function).  A sum over C classes is of at least min(C, 64) chains: (C / 64 + 80) u and the mean of its terms'
-errors; one over k entries (k + 16) u.  Probabilities follow, losses sum products of them with logarithms that are formed in 64
-bits from those sums, and a rounding to float32.  Exponentials below 2^-126 may count as 0: 1e-34 with the
+errors; one over k entries (k + 16) u.  Probabilities follow.  A loss sums p ((t - top) - (x - max)) / T + log's difference), in float32:
+4 u of the two differences' magnitudes, 3 u of the logarithms', u of the term, and its rounding.  Exponentials below 2^-126 may count as 0: 1e-34 with the
 largest factor, 1000.  16-bit gradients add half a unit of their last place (2^-11, 2^-8), or half
 the smallest fp16 step."""
 import math
@@ -34,14 +34,14 @@ def close(got, want, err, what):
 
 
 def softmax(x, T, chain):
-    """(softmax, its relative error, log of the sum) of a row, as relative errors of the kernel's order."""
+    """(softmax, its relative error, log of the sum, that sum's relative error, |x - max| / T, |log of the sum of exp((x - max) / T)|)."""
     m = x.max()
     d = ((x - m) / T).clamp(min=-1e4)
     e = torch.exp(d)
     term = 6 * d.abs() * U + 2 * U
     total = e.sum()
     rel_total = (chain + 2) * U + (e * term).sum() / total
-    return e / total, term + rel_total + 2 * U, torch.log(total) + m / T, rel_total
+    return e / total, term + rel_total + 2 * U, torch.log(total) + m / T, rel_total, ((x - m) / T).abs(), torch.log(total).abs()
 
 
 def exact(x, t, ids, T, labels, hard, up):
@@ -58,13 +58,14 @@ def exact(x, t, ids, T, labels, hard, up):
             if (at >= C).any() or not (tt < math.inf).all() or not (x[i] < math.inf).all() or x[i].max() == -math.inf:
                 loss[i], grad[i] = math.nan, math.nan
                 continue
-            p, prel, tl, trel = softmax(tt, T, len(tt) + 16)
-            q, qrel, xl, xrel = softmax(x[i], T, C / 64 + 80)
+            p, prel, tl, trel, td, tlog = softmax(tt, T, len(tt) + 16)
+            q, qrel, xl, xrel, xd, xlog = softmax(x[i], T, C / 64 + 80)
             # Entries of probability 0 (in float32) add nothing.
             p = torch.where(p < 1e-37, 0.0, p)
             term = torch.where(p > 0, (tt / T - tl) - (x[i][at] / T - xl), 0.0)
             loss[i] += a * T * torch.where(p > 0, p * term, 0.0).sum()
-            lerr[i] += a * T * (torch.where(p > 0, p * prel * term.abs(), 0.0).sum() + xrel + trel + 4 * U)
+            steps = 4 * U * (td + xd[at]) + 3 * U * (tlog + xlog) + U * term.abs()
+            lerr[i] += a * T * (torch.where(p > 0, p * (prel * term.abs() + steps), 0.0).sum() + xrel + trel + 4 * U)
             P = torch.zeros(C, dtype=torch.float64).index_add_(0, at, p)
             Perr = torch.zeros(C, dtype=torch.float64).index_add_(0, at, p * (prel + (len(tt) + 3) * U))
             grad[i] += a * up[i] * (q - P)
@@ -74,9 +75,9 @@ def exact(x, t, ids, T, labels, hard, up):
             if y >= C or not (x[i] < math.inf).all() or x[i].max() == -math.inf:
                 loss[i], grad[i] = math.nan, math.nan
                 continue
-            q, qrel, xl, xrel = softmax(x[i], 1.0, C / 64 + 80)
+            q, qrel, xl, xrel, xd, xlog = softmax(x[i], 1.0, C / 64 + 80)
             loss[i] += hard * (xl - x[i, y])
-            lerr[i] += hard * (xrel + U)
+            lerr[i] += hard * (xrel + U + 3 * U * (xlog + xd[y]))
             h = hard * up[i] * q
             h[y] -= hard * up[i]
             grad[i] += h
