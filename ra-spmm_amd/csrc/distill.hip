@@ -524,9 +524,11 @@ ShortPlan short_plan(const ra_distill_shape& s) {
     const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2, k = s.classes <= 256 ? 4 : 16, entries = s.kept + 1;
     ShortPlan p{};
     while ((k << p.shift) < s.classes || (kThreads >> p.shift) * entries * 16 > 4 * 257 * 16) ++p.shift;
+    // Few rows: more lanes for each, and fewer rows a workgroup, so that all CUs have some.
+    while (p.shift < 6 && (s.rows << p.shift) < 256 * kThreads && (1 << p.shift) < s.classes) ++p.shift;
     const int groups = kThreads >> p.shift;
     p.rows = std::max(groups, 8);  // 8 rows are whole packets
-    while (2 * p.rows * s.classes * size <= kStageBytes) p.rows *= 2;
+    while (2 * p.rows * s.classes * size <= kStageBytes && s.rows / (2 * p.rows) >= 1024) p.rows *= 2;
     p.blocks = static_cast<int>(std::min<int64_t>((s.rows + p.rows - 1) / p.rows, kMaxBlocks));
     p.lds = (size_t)(p.rows * s.classes * size + 15) / 16 * 16 + (size_t)groups * entries * 16 + (size_t)groups * s.classes * 2;
     return p;

@@ -9,7 +9,14 @@
 //
 // The sort goes by digits of up to 11 bits, lowest first, three launches a digit: counts
 // of every workgroup's piece, their running sums for every digit, and the move, in which
-// lanes of a wave with one digit find their order by ballots.
+// lanes of a wave with one digit find their order by ballots.  Up to 8,192 positions, one
+// launch counts for each how many come before it.
+//
+// The sum takes equal runs of sorted positions, not of table rows, so that a row with most
+// of the positions costs no more than others: a group of lanes adds its run's gradients and
+// writes each table row that begins and ends there; what reaches over an edge is joined in
+// LDS, and between workgroups by a second launch.  Table rows without positions are
+// written by further workgroups of the first.
 #include <algorithm>
 #include <type_traits>
 
@@ -27,6 +34,9 @@ constexpr int64_t kMaxBlocks = 1 << 16;
 constexpr int kDigitBits = 11;
 constexpr int kPiece = 4096;      // pairs of a workgroup in the sort, more where there would be over
 constexpr int kMaxPieces = 512;   // this many of them
+constexpr int kRankMost = 8192;   // positions that are sorted by counting
+constexpr int kTiles = 2048;      // workgroups of the sum, about
+constexpr int kJoinThreads = 1024;
 
 struct EmbedArgs {
     const void* ids;
@@ -48,15 +58,43 @@ __device__ __forceinline__ uint32_t key_at(const EmbedArgs& a, int64_t i) {
     return (uint64_t)id < (uint64_t)a.rows && !is_padding(a, id) ? (uint32_t)id : (uint32_t)a.rows;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a) {
-    for (int64_t i = blockIdx.x * kWaves + (threadIdx.x >> 6); i < a.count; i += (int64_t)gridDim.x * kWaves) {
-        const int64_t id = id_at(a, i);
-        const bool padding = is_padding(a, id), inside = (uint64_t)id < (uint64_t)a.rows;
-        const T* const from = static_cast<const T*>(a.from) + (inside && !padding ? id : 0) * a.ld;
-        T* const to = static_cast<T*>(a.to) + i * a.dim;
-        for (int d = threadIdx.x & 63; d < a.dim; d += 64)
-            to[d] = (T)(padding ? 0.f : inside ? a.scale * (float)from[d] : __builtin_nanf(""));
+// P elements as they lie in memory.
+template <typename T, int P>
+struct Packet {
+    typedef T vec __attribute__((ext_vector_type(P)));
+};
+
+// A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane.
+template <typename T, int P>
+__global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const int shift) {
+    using vec = typename Packet<T, P>::vec;
+    constexpr int kAhead = 4;
+    const int lane = threadIdx.x & ((1 << shift) - 1), groups = kThreads >> shift;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    for (int64_t i0 = (int64_t)blockIdx.x * groups + (threadIdx.x >> shift); i0 < a.count; i0 += kAhead * step) {
+        const T* from[kAhead];
+        bool padding[kAhead], inside[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t id = id_at(a, min(i0 + u * step, a.count - 1));
+            padding[u] = is_padding(a, id);
+            inside[u] = !padding[u] && (uint64_t)id < (uint64_t)a.rows;
+            from[u] = static_cast<const T*>(a.from) + (inside[u] ? id * a.ld : 0);
+        }
+        for (int d = lane * P; d < a.dim; d += P << shift) {
+            vec v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                v[u] = *reinterpret_cast<const vec*>(inside[u] ? from[u] + d : reinterpret_cast<const T*>(kZeroRun));
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+                for (int e = 0; e < P; ++e)
+                    v[u][e] = (T)(inside[u] ? a.scale * (float)v[u][e] : padding[u] ? 0.f : __builtin_nanf(""));
+                if (i0 + u * step < a.count)
+                    *reinterpret_cast<vec*>(static_cast<T*>(a.to) + (i0 + u * step) * a.dim + d) = v[u];
+            }
+        }
     }
 }
 
@@ -164,26 +202,225 @@ __global__ __launch_bounds__(kThreads) void sort_move(const SortArgs a) {
     }
 }
 
-// The first sorted pair whose key is not below `key`.
-__device__ __forceinline__ int lower_bound(const uint2* pairs, int count, uint32_t key) {
-    int lo = 0, hi = count;
+// Few positions: how many come before each, 64 of them a workgroup, whose waves share the
+// others.  Keys of 64 positions before these count where they are not above, later ones
+// where they are below.
+__global__ __launch_bounds__(1024) void sort_rank(const EmbedArgs a, uint2* __restrict__ to) {
+    __shared__ __align__(16) uint32_t keys[kRankMost];
+    __shared__ int counts[16][64];
+    const int n = (int)a.count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int all = (n + 63) / 64;
+    for (int j = threadIdx.x; j < all * 64; j += blockDim.x) keys[j] = j < n ? key_at(a, j) : 0xFFFFFFFFu;
+    __syncthreads();
+    const int mine = blockIdx.x * 64 + lane;
+    const uint32_t key = keys[mine];
+    int before = 0;
+    for (int c = wave; c < all; c += waves) {
+        if (c == (int)blockIdx.x) {
+            for (int j = 0; j < 64; ++j) {
+                const uint32_t k = keys[c * 64 + j];
+                before += k < key || (k == key && j < lane);
+            }
+        } else {
+            const uint32_t below = key + (c < (int)blockIdx.x);  // keys are below 2^31
+#pragma unroll 4
+            for (int j = 0; j < 64; j += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(keys + c * 64 + j);
+                before += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+            }
+        }
+    }
+    counts[wave][lane] = before;
+    __syncthreads();
+    if (wave == 0 && mine < n) {
+        for (int w = 1; w < waves; ++w) before += counts[w][lane];
+        to[before] = make_uint2(key, (uint32_t)mine);
+    }
+}
+
+// ------------------------------------------------------------ the sums
+// The first sorted pair of [lo, hi) whose key is not below `key`.
+__device__ __forceinline__ int lower_bound(const uint2* pairs, int lo, int hi, uint32_t key) {
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
+        const int mid = lo + (hi - lo) / 2;
         if (pairs[mid].x < key) lo = mid + 1;
         else hi = mid;
     }
     return lo;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void embed_grad(const EmbedArgs a, const uint2* __restrict__ pairs) {
-    for (int64_t v = blockIdx.x * kWaves + (threadIdx.x >> 6); v < a.rows; v += (int64_t)gridDim.x * kWaves) {
-        const int first = lower_bound(pairs, (int)a.count, (uint32_t)v), end = lower_bound(pairs, (int)a.count, (uint32_t)v + 1);
-        for (int d = threadIdx.x & 63; d < a.dim; d += 64) {
-            float s = 0.f;
-            for (int e = first; e < end; ++e) s += (float)static_cast<const T*>(a.from)[pairs[e].y * a.ld + d];
-            static_cast<T*>(a.to)[v * a.dim + d] = (T)(a.scale * s);
+struct SumArgs {
+    EmbedArgs e;
+    const uint2* pairs;
+    float *heads, *tails;  // [tiles][dim]: what a tile adds to a row of an earlier one, and leaves for later ones
+    int32_t count, shift, per, tile, tiles;
+};
+
+// kThreads table rows from first_row on: zeros where no position names them.
+template <typename T, int P>
+__device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t first_row, int* lds) {
+    using vec = typename Packet<T, P>::vec;
+    const int rows = (int)min((int64_t)kThreads, a.e.rows - first_row);
+    if (threadIdx.x < 2) lds[threadIdx.x] = lower_bound(a.pairs, 0, a.count, (uint32_t)(first_row + (threadIdx.x ? rows : 0)));
+    __syncthreads();
+    const int lo = lds[0], hi = lds[1];
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        const uint32_t v = (uint32_t)first_row + threadIdx.x;
+        const int at = lower_bound(a.pairs, lo, hi, v);
+        lds[threadIdx.x] = at < hi && a.pairs[at].x == v;
+    }
+    __syncthreads();
+    vec zero;
+#pragma unroll
+    for (int e = 0; e < P; ++e) zero[e] = (T)0.f;
+    const int lane = threadIdx.x & ((1 << a.shift) - 1), groups = kThreads >> a.shift;
+    for (int r = threadIdx.x >> a.shift; r < rows; r += groups) {
+        if (lds[r]) continue;
+        T* const to = static_cast<T*>(a.e.to) + (first_row + r) * a.e.dim;
+        for (int d = lane * P; d < a.e.dim; d += P << a.shift) *reinterpret_cast<vec*>(to + d) = zero;
+    }
+    __syncthreads();
+}
+
+// blockIdx.x: a tile of sorted positions, or past those workgroups that clear table rows
+// (of the first column block); blockIdx.y: a block of P << shift columns.  A group of
+// 2^shift lanes takes `per` positions of the tile, a packet of columns per lane.
+template <typename T, int P>
+__global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
+    using vec = typename Packet<T, P>::vec;
+    constexpr int kAhead = 4;
+    __shared__ float edge[2][kThreads * P];  // heads and tails of the groups
+    __shared__ int flags[kThreads];          // 1: has a head, 2: has a tail, 4: the head reaches past the group
+    if ((int)blockIdx.x >= a.tiles) {
+        if (blockIdx.y != 0) return;
+        const int64_t step = (int64_t)(gridDim.x - a.tiles) * kThreads;
+        for (int64_t row = (int64_t)(blockIdx.x - a.tiles) * kThreads; row < a.e.rows; row += step) zero_rows<T, P>(a, row, flags);
+        return;
+    }
+    const int group = threadIdx.x >> a.shift, groups = kThreads >> a.shift, lane = threadIdx.x & ((1 << a.shift) - 1);
+    const int d = (((int)blockIdx.y << a.shift) + lane) * P;  // this lane's columns
+    const bool there = d < a.e.dim;
+    const T* const from = static_cast<const T*>(a.e.from) + (there ? d : 0);
+    const uint32_t rows = (uint32_t)a.e.rows;
+    const int first = (int)blockIdx.x * a.tile + group * a.per, end = min(a.count, first + a.per);
+    float acc[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) acc[e] = 0.f;
+    auto write = [&](uint32_t row, const float* f) {
+        if (!there) return;
+        vec v;
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[e] = (T)(a.e.scale * f[e]);
+        *reinterpret_cast<vec*>(static_cast<T*>(a.e.to) + (int64_t)row * a.e.dim + d) = v;
+    };
+    float* const head = edge[0] + threadIdx.x * P;
+    float* const tail = edge[1] + threadIdx.x * P;
+    int flag = 0;
+    if (first < end) {
+        uint32_t row = a.pairs[first].x;
+        bool begun = first == 0 || a.pairs[first - 1].x != row;  // the run of `row` begins in this group
+        for (int e0 = first; e0 < end && row < rows; e0 += kAhead) {
+            uint2 pair[kAhead];
+            vec v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) pair[u] = a.pairs[min(e0 + u, end - 1)];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const vec*>(from + pair[u].y * a.e.ld);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (e0 + u >= end) continue;
+                if (pair[u].x != row) {
+                    if (begun) {
+                        write(row, acc);
+                    } else {
+                        flag |= 1;
+#pragma unroll
+                        for (int e = 0; e < P; ++e) head[e] = acc[e];
+                    }
+                    row = pair[u].x;
+                    begun = true;
+#pragma unroll
+                    for (int e = 0; e < P; ++e) acc[e] = 0.f;
+                    if (row >= rows) break;  // positions that take no part are the last
+                }
+#pragma unroll
+                for (int e = 0; e < P; ++e) acc[e] += (float)v[u][e];
+            }
         }
+        if (row < rows) {  // the last run
+            const bool on = end < a.count && a.pairs[end].x == row;
+            if (begun && !on) {
+                write(row, acc);
+            } else {
+                flag |= begun ? 2 : on ? 5 : 1;
+                float* const to = begun ? tail : head;
+#pragma unroll
+                for (int e = 0; e < P; ++e) to[e] = acc[e];
+            }
+        }
+    }
+    if (lane == 0) flags[group] = flag;
+    __syncthreads();
+    // What reaches over an edge: from the group where the run begins, and from the tile's edge.
+    auto follow = [&](int g) {  // adds the heads from group g on; whether the run reaches past the tile
+        for (; g < groups; ++g) {
+            const float* const from_head = edge[0] + ((g << a.shift) + lane) * P;
+#pragma unroll
+            for (int e = 0; e < P; ++e) acc[e] += from_head[e];
+            if (!(flags[g] & 4)) return false;
+        }
+        return true;
+    };
+    const int64_t part = (int64_t)blockIdx.x * a.e.dim + d;
+    if (group == 0 && (flags[0] & 1)) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) acc[e] = 0.f;
+        follow(0);
+        if (there) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) a.heads[part + e] = acc[e];
+        }
+    }
+    if (flag & 2) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) acc[e] = tail[e];
+        if (!follow(group + 1)) {
+            write(a.pairs[end - 1].x, acc);
+        } else if (there) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) a.tails[part + e] = acc[e];
+        }
+    }
+}
+
+// Rows that reach over tiles: a workgroup per tile in which one begins, whose threads' slices
+// take the later tiles' heads in turn.
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void embed_join(const SumArgs a, const int shift) {
+    __shared__ float sums[kJoinThreads];
+    const int tile = blockIdx.x, first = tile * a.tile, end = first + a.tile;
+    if (end >= a.count) return;
+    const uint32_t row = a.pairs[end - 1].x;
+    if (row >= (uint32_t)a.e.rows || a.pairs[end].x != row) return;               // nothing reaches past this tile
+    if (first > 0 && a.pairs[first - 1].x == row) return;                         // it begins in an earlier one
+    const int last = (lower_bound(a.pairs, end, a.count, row + 1) - 1) / a.tile;  // its last tile
+    const int lane = threadIdx.x & ((1 << shift) - 1), slice = threadIdx.x >> shift, slices = kJoinThreads >> shift;
+    for (int d0 = (int)blockIdx.y << shift; d0 < a.e.dim; d0 += (int)gridDim.y << shift) {
+        const int d = d0 + lane;
+        float x = 0.f;
+        if (d < a.e.dim) {
+#pragma unroll 4
+            for (int t = tile + 1 + slice; t <= last; t += slices) x += a.heads[(int64_t)t * a.e.dim + d];
+        }
+        sums[threadIdx.x] = x;
+        __syncthreads();
+        if (slice == 0 && d < a.e.dim) {
+            x = a.tails[(int64_t)tile * a.e.dim + d];
+            for (int i = 0; i < slices; ++i) x += sums[(i << shift) + lane];
+            static_cast<T*>(a.e.to)[(int64_t)row * a.e.dim + d] = (T)(a.e.scale * x);
+        }
+        __syncthreads();
     }
 }
 
@@ -215,13 +452,17 @@ EmbedArgs args_of(const ra_embed_shape& s, const void* ids, const void* from, vo
     return a;
 }
 
-// Digits, pieces and the workspace of the sort: pairs twice, counts, totals.
+// Digits, pieces and the workspace of the sort: pairs twice (once where it is by counting),
+// counts, totals.
 struct SortPlan {
     int bits, passes, digit_bits, piece, pieces;
-    int64_t pairs_bytes, counts_bytes;
+    int64_t pairs_bytes, bytes;
 };
 SortPlan sort_plan(const ra_embed_shape& s) {
     SortPlan p{};
+    p.pairs_bytes = (s.count * 8 + 255) / 256 * 256;
+    p.bytes = p.pairs_bytes;
+    if (s.count <= kRankMost) return p;
     for (int64_t x = s.rows; x; x >>= 1) ++p.bits;  // keys are 0 .. rows
     p.bits = std::max(p.bits, 1);
     p.passes = (p.bits + kDigitBits - 1) / kDigitBits;
@@ -229,14 +470,17 @@ SortPlan sort_plan(const ra_embed_shape& s) {
     p.piece = kPiece;
     while ((s.count + p.piece - 1) / p.piece > kMaxPieces) p.piece *= 2;
     p.pieces = static_cast<int>((s.count + p.piece - 1) / p.piece);
-    p.pairs_bytes = (s.count * 8 + 255) / 256 * 256;
-    p.counts_bytes = ((int64_t(1) << p.digit_bits) * (p.pieces + 1) * 4 + 255) / 256 * 256;
+    p.bytes = 2 * p.pairs_bytes + ((int64_t(1) << p.digit_bits) * (p.pieces + 1) * 4 + 255) / 256 * 256;
     return p;
 }
 
-// The sorted pairs, in one of the workspace's two halves.
+// The sorted pairs, in the workspace.
 const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t st) {
     uint2* const half[2] = {reinterpret_cast<uint2*>(work), reinterpret_cast<uint2*>(work + p.pairs_bytes)};
+    if (p.passes == 0) {
+        sort_rank<<<static_cast<int>((e.count + 63) / 64), e.count > 1024 ? 1024 : 256, 0, st>>>(e, half[0]);
+        return half[0];
+    }
     SortArgs a{};
     a.e = e;
     a.count = static_cast<int32_t>(e.count);
@@ -256,15 +500,60 @@ const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t
     return a.from;
 }
 
-template <typename F>
-void by_type(int32_t dtype, F f) {
-    if (dtype == RA_DTYPE_F32) f(float());
-    else if (dtype == RA_DTYPE_F16) f(f16_t());
-    else f(bf16_t());
+// Packets of P elements: 16 bytes, 8 for 16-bit types, or single elements.
+int packet_of(const ra_embed_shape& s, const void* a, const void* b, int64_t rows, int64_t ld) {
+    const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
+    auto fits = [&](int p) {
+        return s.dim % p == 0 && (rows <= 1 || ld % p == 0) && reinterpret_cast<uintptr_t>(a) % (p * size) == 0 &&
+               reinterpret_cast<uintptr_t>(b) % (p * size) == 0;
+    };
+    if (size == 2 && fits(8)) return 8;
+    return fits(4) ? 4 : 1;
+}
+// Lanes of a row: a power of two, a wave at most.
+int shift_of(int dim, int p) {
+    int shift = 0;
+    while (shift < 6 && (p << shift) < dim) ++shift;
+    return shift;
 }
 
-int blocks_of(int64_t rows) {
-    return static_cast<int>(std::min((rows + kWaves - 1) / kWaves, kMaxBlocks));
+// How the sum is cut: groups of lanes with `per` positions, tiles of a workgroup, blocks of
+// columns.
+struct SumPlan {
+    int shift, per, tile, tiles, blocks;
+};
+SumPlan sum_plan(const ra_embed_shape& s, int p) {
+    SumPlan x{};
+    x.shift = shift_of(s.dim, p);
+    x.blocks = (s.dim + (p << x.shift) - 1) / (p << x.shift);
+    const int64_t groups = kThreads >> x.shift, most = std::max(kTiles / x.blocks, 256);
+    x.per = static_cast<int>(std::max<int64_t>(4, (s.count + groups * most - 1) / (groups * most)));
+    x.per = (x.per + 3) / 4 * 4;
+    x.tile = static_cast<int>(groups * x.per);
+    x.tiles = static_cast<int>((s.count + x.tile - 1) / x.tile);
+    return x;
+}
+// The workspace holds the tiles of any width of packets: the addresses that choose it are
+// not known when its size is asked for.
+int64_t most_tiles(const ra_embed_shape& s) {
+    int64_t tiles = 0;
+    for (int p : {1, 4, 8}) tiles = std::max<int64_t>(tiles, sum_plan(s, p).tiles);
+    return tiles;
+}
+
+template <typename F>
+void by_packet(int32_t dtype, int p, F f) {
+    using I1 = std::integral_constant<int, 1>;
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    auto of_type = [&](auto t) {
+        if constexpr (sizeof(t) == 2)
+            if (p == 8) return f(t, I8());
+        return p == 4 ? f(t, I4()) : f(t, I1());
+    };
+    if (dtype == RA_DTYPE_F32) of_type(float());
+    else if (dtype == RA_DTYPE_F16) of_type(f16_t());
+    else of_type(bf16_t());
 }
 
 }  // namespace
@@ -280,8 +569,13 @@ ra_status ra_embed(const ra_embed_shape* s, const void* d_ids, const void* d_tab
     if (!d_ids || !d_out || (s->rows && !d_table)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: NULL tensor");
     if (s->rows > 1 && s->ld_table < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_table is too small)");
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
-    ra::by_type(s->dtype, [&](auto t) {
-        ra::embed_rows<decltype(t)><<<ra::blocks_of(s->count), ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+    const int p = ra::packet_of(*s, d_table, d_out, s->rows, s->ld_table), shift = ra::shift_of(s->dim, p);
+    const int64_t groups = ra::kThreads >> shift, full = (s->count + groups - 1) / groups;
+    // Rows one by one where there are few, else several in flight.
+    const int blocks = static_cast<int>(std::min(std::max(std::min<int64_t>(full, 2048), (full + 3) / 4), ra::kMaxBlocks));
+    ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
+        ra::embed_rows<decltype(t), decltype(packet)::value>
+            <<<blocks, ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a, shift);
     });
     RA_LAUNCH_CHECK("embed");
     return RA_OK;
@@ -292,8 +586,7 @@ ra_status ra_embed_workspace(const ra_embed_shape* s, int64_t* bytes) {
     RA_TRY(ra::check(s));
     *bytes = 0;
     if (s->count == 0) return RA_OK;
-    const ra::SortPlan p = ra::sort_plan(*s);
-    *bytes = 2 * p.pairs_bytes + p.counts_bytes;
+    *bytes = ra::sort_plan(*s).bytes + 2 * ra::most_tiles(*s) * s->dim * (int64_t)sizeof(float);
     return RA_OK;
 }
 
@@ -308,15 +601,31 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: the workspace must be 16-byte aligned");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_grad, d_dtable, s->ld_grad);
-    const uint2* pairs = nullptr;
+    const int p = ra::packet_of(*s, d_grad, d_dtable, s->count, s->ld_grad);
+    const ra::SumPlan plan = ra::sum_plan(*s, p);
+    ra::SumArgs sum{};
+    sum.e = a;
+    sum.count = static_cast<int32_t>(s->count);
+    sum.shift = plan.shift;
+    sum.per = plan.per;
+    sum.tile = plan.tile;
+    sum.tiles = plan.tiles;
     if (s->count) {
-        pairs = ra::sort(a, ra::sort_plan(*s), static_cast<char*>(d_workspace), st);
+        const ra::SortPlan sorted = ra::sort_plan(*s);
+        sum.pairs = ra::sort(a, sorted, static_cast<char*>(d_workspace), st);
         RA_LAUNCH_CHECK("embed sort");
+        sum.heads = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + sorted.bytes);
+        sum.tails = sum.heads + (int64_t)plan.tiles * s->dim;
     }
-    ra::by_type(s->dtype, [&](auto t) {
-        ra::embed_grad<decltype(t)><<<ra::blocks_of(s->rows), ra::kThreads, 0, st>>>(a, pairs);
+    const int64_t clear = std::min<int64_t>((s->rows + ra::kThreads - 1) / ra::kThreads, std::max(256, 65536 / plan.blocks));
+    const dim3 grid(static_cast<uint32_t>(plan.tiles + clear), plan.blocks);
+    ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
+        ra::embed_sum<decltype(t), decltype(packet)::value><<<grid, ra::kThreads, 0, st>>>(sum);
+        if (plan.tiles > 1)
+            ra::embed_join<decltype(t)><<<dim3(plan.tiles, std::min((s->dim + 63) / 64, 16)), ra::kJoinThreads, 0, st>>>(
+                sum, ra::shift_of(s->dim, 1));
     });
-    RA_LAUNCH_CHECK("embed_grad");
+    RA_LAUNCH_CHECK("embed_sum");
     return RA_OK;
 }
 
