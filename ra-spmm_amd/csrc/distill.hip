@@ -22,7 +22,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxKept = 1024;
-constexpr int kMaxBlocks = 4096;       // workgroups, and so parts of a reduced loss
+constexpr int kMaxBlocks = 16384;      // workgroups, and so parts of a reduced loss
+constexpr int kLaneClasses = 64;       // classes of a row that a lane takes,
+constexpr int kLaneKept = 16;          // its entries,
+constexpr int64_t kLaneRows = 16384;   // where there are as many rows
 constexpr int kMaxShort = 1024;        // classes of a row that a wave holds
 constexpr int kStageBytes = 16384;     // rows of a workgroup at once, about
 constexpr float kLog2e = 1.4426950408889634f;
@@ -136,8 +139,8 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, Team& team, cons
 // Factors of the row's gradient: it is soft exp((s - most) / T) + hard exp(s - most) without
 // the entries, and amount[e] becomes what each entry takes off.
 struct Factors {
-    float soft, hard, most;
-    // of s - most
+    float soft, hard;
+    // Of s - most.  A row without a part of the loss has its gradient 0 whatever its logits are.
     __device__ __forceinline__ float operator()(const DistillArgs& a, float d) const {
         float g = 0.f;
         if (soft != 0.f) g = soft * exp_of(d, kLog2e * a.inv_t);
@@ -146,8 +149,8 @@ struct Factors {
     }
 };
 template <typename Team>
-__device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t row, Team& team, const Targets& t, float most,
-                                                 float at_t, float at_1) {
+__device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t row, Team& team, const Targets& t, float at_t,
+                                                 float at_1) {
     const float up = (a.up ? a.up[row * a.up_step] : 1.f) * a.up_scale;
     const float soft_up = !t.soft ? 0.f : t.sum != t.sum ? NAN : a.soft_grad * up;
     const float hard_up = !t.hard ? 0.f : t.label < a.classes ? a.hard * up : NAN;
@@ -160,7 +163,7 @@ __device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t r
             t.place[e] = t.hard && t.label < a.classes ? (int32_t)t.label : -1;
         }
     }
-    return {t.soft ? soft_up / at_t : 0.f, t.hard ? hard_up / at_1 : 0.f, most};
+    return {t.soft ? soft_up / at_t : 0.f, t.hard ? hard_up / at_1 : 0.f};
 }
 // What all entries of e's class take off; `first`: no earlier entry has it.
 __device__ __forceinline__ float class_amount(const Targets& t, int kept, int e, bool& first) {
@@ -244,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
                 }
             }
             if (!a.grad) continue;
-            const Factors f = entry_amounts(a, row, team, t, most, at_t, at_1);
+            const Factors f = entry_amounts(a, row, team, t, at_t, at_1);
             team.sync();
             // Whether a class has several entries: one of them is not its owner then.
             for (int e = team.lane; e < entries; e += lanes)
@@ -293,7 +296,184 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
     }
 }
 
+// ------------------------------------------------------- many rows of few classes
+// A lane per row, 64 rows of up to 64 classes in LDS as floats, rows at an odd pitch: no
+// sums between lanes, and the logarithms, divisions and entries of 64 rows at once.  The
+// rows come and go as one run of memory, like those of distill_short, and so do the
+// entries: read by their lanes, each load would touch 64 lines.
+template <typename T>
+__global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
+    extern __shared__ __align__(16) float stage[];
+    constexpr int kPer = 16 / sizeof(T), kPackets = kLaneClasses / kPer;
+    typedef T vec __attribute__((ext_vector_type(kPer)));
+    const int C = a.classes, pitch = C | 1, lane = threadIdx.x;
+    const uint32_t magic = ((1u << 20) + C - 1) / C;  // i / C = i * magic >> 20 for i < 64 C <= 4096
+    const int k = a.kept, entry_pitch = k | 1;
+    const uint32_t entry_magic = k ? ((1u << 20) + k - 1) / k : 0;
+    const float c = kLog2e * a.inv_t;
+    float* const x = stage + lane * pitch;
+    int32_t* const places = reinterpret_cast<int32_t*>(stage + 64 * pitch);  // class, -1: takes no part, -2: no class
+    float* const amounts = stage + 64 * (pitch + entry_pitch);
+    const int32_t* const place = places + lane * entry_pitch;
+    float* const amount = amounts + lane * entry_pitch;  // logit, then exp((logit - top) / T)
+    double total = 0.0;
+    for (int64_t first = (int64_t)blockIdx.x * 64; first < a.rows; first += (int64_t)gridDim.x * 64) {
+        const int rows = (int)min((int64_t)64, a.rows - first), n = rows * C;
+        const T* const from = static_cast<const T*>(a.logits) + first * a.ld;
+        const int packets = a.whole ? n / kPer : 0;
+        // All loads of the 64 rows before the first use: few waves fit a CU, so each keeps much in flight.
+        vec v[kPackets];
+#pragma unroll
+        for (int u = 0; u < kPackets; ++u)
+            if (u * 64 < packets) v[u] = *reinterpret_cast<const vec*>(from + min(u * 64 + lane, packets - 1) * kPer);
+        const int64_t row = first + min(lane, rows - 1);
+        int64_t label = -1;
+        if (a.labels) label = a.labels64 ? static_cast<const int64_t*>(a.labels)[row] : (int64_t)static_cast<const int32_t*>(a.labels)[row];
+        for (int u0 = 0; u0 < k; u0 += 8) {
+            int64_t ids[8];
+            float logits[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = min((u0 + u) * 64 + lane, rows * k - 1), r = (int)((uint32_t)i * entry_magic >> 20), e = i - r * k;
+                ids[u] = id_at(a, (first + r) * a.ldi + e);
+                logits[u] = teacher_at(a, (first + r) * a.ldt + e);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = min((u0 + u) * 64 + lane, rows * k - 1), r = (int)((uint32_t)i * entry_magic >> 20), e = i - r * k;
+                places[r * entry_pitch + e] = ids[u] < 0 || logits[u] == -INFINITY ? -1 : ids[u] < C ? (int)ids[u] : -2;
+                amounts[r * entry_pitch + e] = logits[u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kPackets; ++u) {
+            const int p = u * 64 + lane;
+            if (u * 64 < packets && p < packets) {
+                if (pitch == C) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) stage[p * kPer + e] = (float)v[u][e];
+                } else {
+                    int r = (int)((uint32_t)(p * kPer) * magic >> 20), j = p * kPer - r * C;
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        stage[r * pitch + j] = (float)v[u][e];
+                        const bool next = ++j == C;
+                        r += next;
+                        j = next ? 0 : j;
+                    }
+                }
+            }
+        }
+        for (int i = packets * kPer + lane; i < n; i += 64) {
+            const int r = (int)((uint32_t)i * magic >> 20), j = i - r * C;
+            stage[r * pitch + j] = (float)from[r * a.ld + j];
+        }
+        __syncthreads();
+        const bool there = lane < rows;  // the other lanes go along and keep nothing
+        float most = -FLT_MAX;
+#pragma unroll 8
+        for (int j = 0; j < C; ++j) most = fmaxf(most, x[j]);
+        float top = -INFINITY;
+        bool outside = false;
+        for (int e = 0; e < k; ++e) {
+            outside |= place[e] == -2;
+            if (place[e] != -1) top = amount[e] != amount[e] ? INFINITY : fmaxf(top, amount[e]);
+        }
+        const bool soft = a.soft > 0.f && top != -INFINITY;
+        float sum = outside ? NAN : 0.f, inner = 0.f;
+        for (int e = 0; e < k; ++e) {
+            const float t = amount[e];
+            const float w = place[e] >= 0 ? exp_of(t - top, c) : 0.f;
+            sum += w;
+            if (w != 0.f) inner = fmaf(w, (t - top) - (x[place[e]] - most), inner);
+            amount[e] = w;
+        }
+        const bool hard = a.hard > 0.f && label >= 0, inside = label >= 0 && label < C;
+        const float at_label = x[inside ? (int)label : 0] - most;
+        float at_t = 0.f, at_1 = 0.f;
+        if (a.hard > 0.f) {
+#pragma unroll 8
+            for (int j = 0; j < C; ++j) {
+                const float v = x[j] - most;
+                at_t += exp_of(v, c);
+                at_1 += exp_of(v, kLog2e);
+            }
+        } else {  // one exponential an element: it stays for the gradient
+#pragma unroll 8
+            for (int j = 0; j < C; ++j) {
+                const float e = exp_of(x[j] - most, c);
+                at_t += e;
+                x[j] = e;
+            }
+        }
+        const float per_sum = 1.f / sum;
+        if (a.loss || a.part) {
+            float loss = 0.f;
+            if (soft) loss = a.soft * fmaf(inner * per_sum, a.inv_t, logf(at_t) - logf(sum));
+            if (hard) loss += inside ? a.hard * (logf(at_1) - at_label) : NAN;
+            if (there) {
+                if (a.loss) a.loss[row] = loss;
+                total += loss;
+            }
+        }
+        if (a.grad) {
+            const float up = (a.up ? a.up[row * a.up_step] : 1.f) * a.up_scale;
+            const float soft_up = !soft ? 0.f : sum != sum ? NAN : a.soft_grad * up;
+            const float hard_up = !hard ? 0.f : inside ? a.hard * up : NAN;
+            const float fs = soft ? soft_up / at_t : 0.f, fh = hard ? hard_up / at_1 : 0.f;
+            if (a.hard > 0.f) {
+#pragma unroll 8
+                for (int j = 0; j < C; ++j) {
+                    const float v = x[j] - most;
+                    x[j] = fmaf(fh, exp_of(v, kLog2e), fs * exp_of(v, c));
+                }
+            } else {
+#pragma unroll 8
+                for (int j = 0; j < C; ++j) x[j] *= fs;
+            }
+            if (!soft && !hard)  // whatever the logits are
+                for (int j = 0; j < C; ++j) x[j] = 0.f;
+            if (soft)
+                for (int e = 0; e < k; ++e)
+                    if (place[e] >= 0) x[place[e]] -= soft_up * (amount[e] * per_sum);
+            if (hard && inside) x[label] -= hard_up;
+            __syncthreads();
+            T* const to = static_cast<T*>(a.grad) + first * C;
+#pragma unroll 2
+            for (int p = lane; p < packets; p += 64) {
+                vec out;
+                if (pitch == C) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) out[e] = (T)stage[p * kPer + e];
+                } else {
+                    int r = (int)((uint32_t)(p * kPer) * magic >> 20), j = p * kPer - r * C;
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        out[e] = (T)stage[r * pitch + j];
+                        if (++j == C) {
+                            j = 0;
+                            ++r;
+                        }
+                    }
+                }
+                *reinterpret_cast<vec*>(to + p * kPer) = out;
+            }
+            for (int i = packets * kPer + lane; i < n; i += 64) {
+                const int r = (int)((uint32_t)i * magic >> 20), j = i - r * C;
+                to[i] = (T)stage[r * pitch + j];
+            }
+        }
+        __syncthreads();
+    }
+    if (a.part) {
+        total = sum_lanes(total, 64);
+        if (lane == 0) a.part[blockIdx.x] = total;
+    }
+}
+
 // ------------------------------------------------------------------- long rows
+constexpr int kAhead = 4;  // packets of a lane at once
+
 // 16 bytes of a row; elements past the packets, at both ends, are taken one by one.
 template <typename T>
 struct Span {
@@ -313,7 +493,6 @@ template <typename T, typename Team>
 __device__ __forceinline__ void scan_part(const DistillArgs& a, Team& team, const T* x, int begin, int end, float& most, float& at_t,
                                           float& at_1) {
     using S = Span<T>;
-    constexpr int kAhead = 4;  // packets of a lane at once
     const float c = kLog2e * a.inv_t;
     const bool hard = a.hard > 0.f;
     most = -FLT_MAX;
@@ -358,9 +537,35 @@ __device__ __forceinline__ void scan_part(const DistillArgs& a, Team& team, cons
     most = top;
 }
 
+// to[j] = f(x[j]) over a part of a row, in whole packets where both lie alike.
+template <typename T, typename Team, typename F>
+__device__ __forceinline__ void write_part(const Team& team, const T* x, T* to, int begin, int end, F f) {
+    using S = Span<T>;
+    if ((reinterpret_cast<uintptr_t>(to) - reinterpret_cast<uintptr_t>(x)) % 16 != 0) {
+        for (int j = begin + team.lane; j < end; j += team.lanes) to[j] = (T)f((float)x[j]);
+        return;
+    }
+    const S s(x, begin, end);
+    for (int p = team.lane; p < s.packets; p += kAhead * team.lanes) {
+        typename S::vec v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            v[u] = *reinterpret_cast<const typename S::vec*>(x + s.first + min(p + u * team.lanes, s.packets - 1) * S::kPer);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (p + u * team.lanes >= s.packets) break;
+#pragma unroll
+            for (int e = 0; e < S::kPer; ++e) v[u][e] = (T)f((float)v[u][e]);
+            *reinterpret_cast<typename S::vec*>(to + s.first + (p + u * team.lanes) * S::kPer) = v[u];
+        }
+    }
+    for (int j = begin + team.lane; j < s.first; j += team.lanes) to[j] = (T)f((float)x[j]);
+    for (int j = s.first + s.packets * S::kPer + team.lane; j < end; j += team.lanes) to[j] = (T)f((float)x[j]);
+}
+
 // Rows cut into pieces: each piece's maximum and sums.
 template <typename T>
-__global__ __launch_bounds__(1024) void distill_pieces(const DistillArgs a) {
+__global__ __launch_bounds__(512) void distill_pieces(const DistillArgs a) {
     __shared__ float lds[32];
     WorkgroupTeam team{(int)threadIdx.x, (int)blockDim.x, lds};
     for (int64_t work = blockIdx.x; work < a.rows * a.pieces; work += gridDim.x) {
@@ -376,10 +581,9 @@ __global__ __launch_bounds__(1024) void distill_pieces(const DistillArgs a) {
 // A workgroup per row, or per piece of one where the gradient is wanted; the loss is formed
 // by the first piece.
 template <typename T>
-__global__ __launch_bounds__(1024) void distill_long(const DistillArgs a) {
+__global__ __launch_bounds__(512) void distill_long(const DistillArgs a) {
     extern __shared__ float entries[];
     __shared__ float lds[32];
-    using S = Span<T>;
     WorkgroupTeam team{(int)threadIdx.x, (int)blockDim.x, lds};
     Targets t{};
     t.amount = entries;
@@ -422,23 +626,17 @@ __global__ __launch_bounds__(1024) void distill_long(const DistillArgs a) {
         }
         if (a.grad) {
             __syncthreads();  // all have read the amounts
-            const Factors f = entry_amounts(a, row, team, t, most, at_t, at_1);
+            const Factors f = entry_amounts(a, row, team, t, at_t, at_1);
             T* const g = static_cast<T*>(a.grad) + row * a.classes;
-            const S s(x, begin, end);
-            auto one = [&](int j) { g[j] = (T)f(a, (float)x[j] - most); };
-            if ((reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(x)) % 16 == 0) {
-                for (int p = team.lane; p < s.packets; p += team.lanes) {
-                    const auto v = *reinterpret_cast<const typename S::vec*>(x + s.first + p * S::kPer);
-                    typename S::vec out;
-#pragma unroll
-                    for (int e = 0; e < S::kPer; ++e) out[e] = (T)f(a, (float)v[e] - most);
-                    *reinterpret_cast<typename S::vec*>(g + s.first + p * S::kPer) = out;
-                }
-                for (int j = begin + team.lane; j < s.first; j += team.lanes) one(j);
-                for (int j = s.first + s.packets * S::kPer + team.lane; j < end; j += team.lanes) one(j);
-            } else {
-                for (int j = begin + team.lane; j < end; j += team.lanes) one(j);
-            }
+            // The same in every lane: the loops over the row have no choice left in them.
+            const float soft = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(f.soft)));
+            const float hard = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(f.hard)));
+            const float c = kLog2e * a.inv_t;
+            if (soft == 0.f && hard == 0.f) write_part<T>(team, x, g, begin, end, [&](float) { return 0.f; });
+            else if (hard == 0.f) write_part<T>(team, x, g, begin, end, [&](float v) { return soft * exp_of(v - most, c); });
+            else write_part<T>(team, x, g, begin, end, [&](float v) {
+                return fmaf(hard, exp_of(v - most, kLog2e), soft * exp_of(v - most, c));
+            });
             __threadfence_block();
             __syncthreads();
             for (int e = team.lane; e <= a.kept; e += team.lanes) {
@@ -455,10 +653,11 @@ __global__ __launch_bounds__(1024) void distill_long(const DistillArgs a) {
 }
 
 // The workgroups' parts in order.
-__global__ __launch_bounds__(kThreads) void distill_reduce(const double* __restrict__ part, int parts, double scale, float* loss) {
-    __shared__ double sums[kThreads / 64];
+__global__ __launch_bounds__(1024) void distill_reduce(const double* __restrict__ part, int parts, double scale, float* loss) {
+    __shared__ double sums[16];
     double s = 0.0;
-    for (int p = threadIdx.x; p < parts; p += kThreads) s += part[p];
+#pragma unroll 4
+    for (int p = threadIdx.x; p < parts; p += 1024) s += part[p];
     s = sum_workgroup(s, sums);
     if (threadIdx.x == 0) *loss = (float)(s * scale);
 }
@@ -512,6 +711,10 @@ DistillArgs args_of(const ra_distill_shape& s, const void* logits, const void* t
     return a;
 }
 
+bool by_lanes(const ra_distill_shape& s) { return s.classes <= kLaneClasses && s.kept <= kLaneKept && s.rows >= kLaneRows; }
+size_t lane_lds(const ra_distill_shape& s) { return (size_t)64 * ((s.classes | 1) + 2 * (s.kept | 1)) * 4; }
+int lane_blocks(const ra_distill_shape& s) { return static_cast<int>(std::min<int64_t>((s.rows + 63) / 64, kMaxBlocks)); }
+
 bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.kept <= 256; }
 
 // Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements
@@ -544,7 +747,7 @@ LongPlan long_plan(const ra_distill_shape& s) {
     const int64_t want = s.rows ? (512 + s.rows - 1) / s.rows : 1;
     p.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, s.classes / 4096)));
     p.piece = (s.classes + p.pieces - 1) / p.pieces;
-    p.threads = p.piece >= 16384 ? 1024 : 256;
+    p.threads = p.piece >= 16384 ? 512 : 256;
     return p;
 }
 int long_blocks(const ra_distill_shape& s, int pieces) {
@@ -554,6 +757,7 @@ int long_blocks(const ra_distill_shape& s, int pieces) {
 // Workgroups that leave a part of the loss.
 int loss_parts(const ra_distill_shape& s, bool grad) {
     if (s.rows == 0) return 0;
+    if (by_lanes(s)) return lane_blocks(s);
     return is_short(s) ? short_plan(s).blocks : long_blocks(s, grad ? long_plan(s).pieces : 1);
 }
 
@@ -565,11 +769,17 @@ void by_type(int32_t dtype, F f) {
 }
 
 void run(const ra_distill_shape& s, DistillArgs& a, hipStream_t st) {
+    a.whole = (s.rows <= 1 || s.ld_logits == s.classes) && aligned16(a.logits) && aligned16(a.grad);
+    if (by_lanes(s)) {
+        by_type(s.dtype, [&](auto t) {
+            distill_lanes<decltype(t)><<<lane_blocks(s), 64, lane_lds(s), st>>>(a);
+        });
+        return;
+    }
     if (is_short(s)) {
         const ShortPlan p = short_plan(s);
         a.stage_rows = p.rows;
         a.lanes_shift = p.shift;
-        a.whole = (s.rows <= 1 || s.ld_logits == s.classes) && aligned16(a.logits) && aligned16(a.grad);
         by_type(s.dtype, [&](auto t) {
             using T = decltype(t);
             if (s.classes <= 256) distill_short<T, 4><<<p.blocks, kThreads, p.lds, st>>>(a);
@@ -603,7 +813,7 @@ ra_status ra_distill_workspace(const ra_distill_shape* s, int64_t* bytes) {
     *bytes = 0;
     if (s->rows == 0) return RA_OK;
     if (s->reduction != RA_REDUCE_NONE) *bytes = (int64_t)ra::kMaxBlocks * (int64_t)sizeof(double);
-    if (!ra::is_short(*s)) *bytes += s->rows * (ra::long_plan(*s).pieces > 1 ? ra::long_plan(*s).pieces : 0) * 16;
+    if (!ra::by_lanes(*s) && !ra::is_short(*s)) *bytes += s->rows * (ra::long_plan(*s).pieces > 1 ? ra::long_plan(*s).pieces : 0) * 16;
     return RA_OK;
 }
 
@@ -636,7 +846,7 @@ ra_status ra_distill_loss(const ra_distill_shape* s, const void* d_logits, const
     }
     if (s->reduction != RA_REDUCE_NONE) {  // the mean of no rows is NaN
         const double scale = s->reduction == RA_REDUCE_SUM ? 1.0 : s->rows ? 1.0 / static_cast<double>(s->rows) : NAN;
-        ra::distill_reduce<<<1, ra::kThreads, 0, st>>>(a.part, ra::loss_parts(*s, d_grad != nullptr), scale, d_loss);
+        ra::distill_reduce<<<1, 1024, 0, st>>>(a.part, ra::loss_parts(*s, d_grad != nullptr), scale, d_loss);
         RA_LAUNCH_CHECK("distill_reduce");
     }
     return RA_OK;

@@ -30,13 +30,14 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxDim = 1 << 20;
 constexpr int64_t kMaxCount = (int64_t(1) << 31) - (1 << 24);
-constexpr int64_t kMaxBlocks = 1 << 16;
+constexpr int kRowBlocks = 1536;  // of the lookup: 6 workgroups for every CU, as many as are resident
 constexpr int kDigitBits = 11;
-constexpr int kPiece = 4096;      // pairs of a workgroup in the sort, more where there would be over
-constexpr int kMaxPieces = 512;   // this many of them
+constexpr int kPiece = 4096;      // pairs of a workgroup in the sort,
+constexpr int kMaxPieces = 512;   // more where there would be over this many of them,
+constexpr int kMostPiece = 32768; // up to as many: more pieces then
+constexpr int kMoveThreads = 512;
 constexpr int kRankMost = 8192;   // positions that are sorted by counting
 constexpr int kTiles = 2048;      // workgroups of the sum, about
-constexpr int kJoinThreads = 1024;
 
 struct EmbedArgs {
     const void* ids;
@@ -64,28 +65,35 @@ struct Packet {
     typedef T vec __attribute__((ext_vector_type(P)));
 };
 
-// A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane.
+// A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane, and loads the
+// next rows' ids with them.
 template <typename T, int P>
 __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const int shift) {
     using vec = typename Packet<T, P>::vec;
     constexpr int kAhead = 4;
     const int lane = threadIdx.x & ((1 << shift) - 1), groups = kThreads >> shift;
     const int64_t step = (int64_t)gridDim.x * groups;
-    for (int64_t i0 = (int64_t)blockIdx.x * groups + (threadIdx.x >> shift); i0 < a.count; i0 += kAhead * step) {
+    int64_t i0 = (int64_t)blockIdx.x * groups + (threadIdx.x >> shift), id[kAhead];
+    auto load_ids = [&](int64_t i) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) id[u] = id_at(a, min(i + u * step, a.count - 1));
+    };
+    load_ids(i0);
+    for (; i0 < a.count; i0 += kAhead * step) {
         const T* from[kAhead];
         bool padding[kAhead], inside[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int64_t id = id_at(a, min(i0 + u * step, a.count - 1));
-            padding[u] = is_padding(a, id);
-            inside[u] = !padding[u] && (uint64_t)id < (uint64_t)a.rows;
-            from[u] = static_cast<const T*>(a.from) + (inside[u] ? id * a.ld : 0);
+            padding[u] = is_padding(a, id[u]);
+            inside[u] = !padding[u] && (uint64_t)id[u] < (uint64_t)a.rows;
+            from[u] = static_cast<const T*>(a.from) + (inside[u] ? id[u] * a.ld : 0);
         }
         for (int d = lane * P; d < a.dim; d += P << shift) {
             vec v[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
                 v[u] = *reinterpret_cast<const vec*>(inside[u] ? from[u] + d : reinterpret_cast<const T*>(kZeroRun));
+            if (d == lane * P) load_ids(i0 + kAhead * step);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
@@ -144,15 +152,16 @@ __global__ __launch_bounds__(kThreads) void sort_offsets(const SortArgs a) {
     if (lane == 0) a.totals[digit] = before;
 }
 
-__global__ __launch_bounds__(kThreads) void sort_move(const SortArgs a) {
-    extern __shared__ uint32_t lds[];  // [waves][digits] places, then [digits] totals' sums, [waves]
-    uint32_t* const start = lds + kWaves * a.digits;
-    uint32_t* const wave_sums = start + a.digits;
+__global__ __launch_bounds__(kMoveThreads) void sort_move(const SortArgs a) {
+    constexpr int kMoveWaves = kMoveThreads / 64;
+    extern __shared__ uint32_t lds[];  // [digits] first places, [waves] sums, then [waves][digits] places past them, 16 bits each
+    uint32_t* const start = lds;
+    uint32_t* const wave_sums = lds + a.digits;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    volatile uint32_t* const place = lds + wave * a.digits;
-    for (int d = threadIdx.x; d < kWaves * a.digits; d += kThreads) lds[d] = 0;
+    uint32_t* const counts = lds + a.digits + kMoveWaves + wave * (a.digits / 2);  // two digits a word
+    for (int d = threadIdx.x; d < kMoveWaves * a.digits / 2; d += kMoveThreads) lds[a.digits + kMoveWaves + d] = 0;
     // Sums of the totals before each digit: a run of digits per thread.
-    const int run = (a.digits + kThreads - 1) / kThreads, d0 = threadIdx.x * run;
+    const int run = (a.digits + kMoveThreads - 1) / kMoveThreads, d0 = threadIdx.x * run;
     uint32_t mine = 0;
     for (int k = 0; k < run; ++k) mine += d0 + k < a.digits ? a.totals[d0 + k] : 0;
     uint32_t sum = mine;
@@ -165,22 +174,28 @@ __global__ __launch_bounds__(kThreads) void sort_move(const SortArgs a) {
     uint32_t before = sum - mine;
     for (int w = 0; w < wave; ++w) before += wave_sums[w];
     for (int k = 0; k < run && d0 + k < a.digits; ++k) {
-        start[d0 + k] = before;
+        start[d0 + k] = before + a.counts[(int64_t)(d0 + k) * a.pieces + blockIdx.x];
         before += a.totals[d0 + k];
     }
-    // Every wave takes a quarter of the piece, in order.
-    const int quarter = a.piece / kWaves, first = blockIdx.x * a.piece + wave * quarter, end = min(a.count, first + quarter);
-    for (int i = first + lane; i < end; i += 64) atomicAdd(&lds[wave * a.digits + ((pair_at(a, i).x >> a.shift) & (a.digits - 1))], 1u);
+    // Every wave takes its part of the piece, in order.
+    const int part = a.piece / kMoveWaves, first = blockIdx.x * a.piece + wave * part, end = min(a.count, first + part);
+    for (int i = first + lane; i < end; i += 64) {
+        const uint32_t digit = (pair_at(a, i).x >> a.shift) & (a.digits - 1);
+        atomicAdd(&counts[digit / 2], digit & 1 ? 0x10000u : 1u);
+    }
     __syncthreads();
-    for (int d = threadIdx.x; d < a.digits; d += kThreads) {
-        uint32_t at = start[d] + a.counts[(int64_t)d * a.pieces + blockIdx.x];
-        for (int w = 0; w < kWaves; ++w) {
-            const uint32_t n = lds[w * a.digits + d];
-            lds[w * a.digits + d] = at;
+    // Counts to places: those of the waves before.  A piece holds fewer than 2^16 pairs.
+    for (int d = threadIdx.x; d < a.digits / 2; d += kMoveThreads) {
+        uint32_t at = 0;
+        for (int w = 0; w < kMoveWaves; ++w) {
+            uint32_t& x = lds[a.digits + kMoveWaves + w * (a.digits / 2) + d];
+            const uint32_t n = x;
+            x = at;
             at += n;
         }
     }
     __syncthreads();
+    volatile uint16_t* const place = reinterpret_cast<volatile uint16_t*>(counts);
     for (int i0 = first; i0 < end; i0 += 64) {
         const int i = i0 + lane;
         const bool there = i < end;
@@ -195,45 +210,45 @@ __global__ __launch_bounds__(kThreads) void sort_move(const SortArgs a) {
         if (there) {
             const uint32_t at = place[digit];
             __builtin_amdgcn_wave_barrier();
-            if (before_me == 0) place[digit] = at + __popcll(same);
+            if (before_me == 0) place[digit] = (uint16_t)(at + __popcll(same));
             __builtin_amdgcn_wave_barrier();
-            a.to[at + before_me] = pair;
+            a.to[start[digit] + at + before_me] = pair;
         }
     }
 }
 
-// Few positions: how many come before each, 64 of them a workgroup, whose waves share the
-// others.  Keys of 64 positions before these count where they are not above, later ones
-// where they are below.
+// Few positions: how many come before each, 32 of them a workgroup.  Its waves' halves share
+// the others, 32 at a time: keys of positions before these count where they are not above,
+// later ones where they are below.
 __global__ __launch_bounds__(1024) void sort_rank(const EmbedArgs a, uint2* __restrict__ to) {
     __shared__ __align__(16) uint32_t keys[kRankMost];
-    __shared__ int counts[16][64];
-    const int n = (int)a.count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int all = (n + 63) / 64;
-    for (int j = threadIdx.x; j < all * 64; j += blockDim.x) keys[j] = j < n ? key_at(a, j) : 0xFFFFFFFFu;
+    __shared__ int counts[32][32];
+    const int n = (int)a.count, lane = threadIdx.x & 31, half = threadIdx.x >> 5, halves = blockDim.x >> 5;
+    const int all = (n + 31) / 32;
+    for (int j = threadIdx.x; j < all * 32; j += blockDim.x) keys[j] = j < n ? key_at(a, j) : 0xFFFFFFFFu;
     __syncthreads();
-    const int mine = blockIdx.x * 64 + lane;
+    const int mine = blockIdx.x * 32 + lane;
     const uint32_t key = keys[mine];
     int before = 0;
-    for (int c = wave; c < all; c += waves) {
+    for (int c = half; c < all; c += halves) {
         if (c == (int)blockIdx.x) {
-            for (int j = 0; j < 64; ++j) {
-                const uint32_t k = keys[c * 64 + j];
+            for (int j = 0; j < 32; ++j) {
+                const uint32_t k = keys[c * 32 + j];
                 before += k < key || (k == key && j < lane);
             }
         } else {
             const uint32_t below = key + (c < (int)blockIdx.x);  // keys are below 2^31
-#pragma unroll 4
-            for (int j = 0; j < 64; j += 4) {
-                const uint4 k = *reinterpret_cast<const uint4*>(keys + c * 64 + j);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(keys + c * 32 + j);
                 before += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
             }
         }
     }
-    counts[wave][lane] = before;
+    counts[half][lane] = before;
     __syncthreads();
-    if (wave == 0 && mine < n) {
-        for (int w = 1; w < waves; ++w) before += counts[w][lane];
+    if (half == 0 && mine < n) {
+        for (int h = 1; h < halves; ++h) before += counts[h][lane];
         to[before] = make_uint2(key, (uint32_t)mine);
     }
 }
@@ -289,7 +304,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t first_row, i
 template <typename T, int P>
 __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
     using vec = typename Packet<T, P>::vec;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = P == 8 || sizeof(T) == 4 ? 4 : 8;  // rows in flight
     __shared__ float edge[2][kThreads * P];  // heads and tails of the groups
     __shared__ int flags[kThreads];          // 1: has a head, 2: has a tail, 4: the head reaches past the group
     if ((int)blockIdx.x >= a.tiles) {
@@ -320,13 +335,18 @@ __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
     if (first < end) {
         uint32_t row = a.pairs[first].x;
         bool begun = first == 0 || a.pairs[first - 1].x != row;  // the run of `row` begins in this group
+        uint2 next[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) next[u] = a.pairs[min(first + u, end - 1)];
         for (int e0 = first; e0 < end && row < rows; e0 += kAhead) {
             uint2 pair[kAhead];
             vec v[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) pair[u] = a.pairs[min(e0 + u, end - 1)];
+            for (int u = 0; u < kAhead; ++u) pair[u] = next[u];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const vec*>(from + pair[u].y * a.e.ld);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) next[u] = a.pairs[min(e0 + kAhead + u, end - 1)];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 if (e0 + u >= end) continue;
@@ -397,21 +417,33 @@ __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
 // Rows that reach over tiles: a workgroup per tile in which one begins, whose threads' slices
 // take the later tiles' heads in turn.
 template <typename T>
-__global__ __launch_bounds__(kJoinThreads) void embed_join(const SumArgs a, const int shift) {
-    __shared__ float sums[kJoinThreads];
+__global__ __launch_bounds__(kThreads) void embed_join(const SumArgs a, const int shift) {
+    __shared__ float sums[kThreads];
     const int tile = blockIdx.x, first = tile * a.tile, end = first + a.tile;
     if (end >= a.count) return;
-    const uint32_t row = a.pairs[end - 1].x;
-    if (row >= (uint32_t)a.e.rows || a.pairs[end].x != row) return;               // nothing reaches past this tile
-    if (first > 0 && a.pairs[first - 1].x == row) return;                         // it begins in an earlier one
-    const int last = (lower_bound(a.pairs, end, a.count, row + 1) - 1) / a.tile;  // its last tile
-    const int lane = threadIdx.x & ((1 << shift) - 1), slice = threadIdx.x >> shift, slices = kJoinThreads >> shift;
+    const uint32_t row = a.pairs[end - 1].x, next = a.pairs[end].x, before = first > 0 ? a.pairs[first - 1].x : row + 1;
+    if (row >= (uint32_t)a.e.rows || next != row || before == row) return;  // nothing begins here and reaches past
+    // Its last tile: most rows end in the next one; else steps of 1, 2, 4 .. tiles, then halves.
+    int lo = tile + 1, hi = a.tiles;  // the last tile is in [lo, hi)
+    for (int step = 1; lo + step < hi; step *= 2) {
+        if (a.pairs[(lo + step) * a.tile].x != row) {
+            hi = lo + step;
+            break;
+        }
+        lo += step;
+    }
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.pairs[mid * a.tile].x == row) lo = mid;
+        else hi = mid;
+    }
+    const int lane = threadIdx.x & ((1 << shift) - 1), slice = threadIdx.x >> shift, slices = kThreads >> shift;
     for (int d0 = (int)blockIdx.y << shift; d0 < a.e.dim; d0 += (int)gridDim.y << shift) {
         const int d = d0 + lane;
         float x = 0.f;
         if (d < a.e.dim) {
-#pragma unroll 4
-            for (int t = tile + 1 + slice; t <= last; t += slices) x += a.heads[(int64_t)t * a.e.dim + d];
+#pragma unroll 8
+            for (int t = tile + 1 + slice; t <= lo; t += slices) x += a.heads[(int64_t)t * a.e.dim + d];
         }
         sums[threadIdx.x] = x;
         __syncthreads();
@@ -464,11 +496,11 @@ SortPlan sort_plan(const ra_embed_shape& s) {
     p.bytes = p.pairs_bytes;
     if (s.count <= kRankMost) return p;
     for (int64_t x = s.rows; x; x >>= 1) ++p.bits;  // keys are 0 .. rows
-    p.bits = std::max(p.bits, 1);
+    p.bits = std::max(p.bits, 2);
     p.passes = (p.bits + kDigitBits - 1) / kDigitBits;
     p.digit_bits = (p.bits + p.passes - 1) / p.passes;
     p.piece = kPiece;
-    while ((s.count + p.piece - 1) / p.piece > kMaxPieces) p.piece *= 2;
+    while ((s.count + p.piece - 1) / p.piece > kMaxPieces && p.piece < kMostPiece) p.piece *= 2;
     p.pieces = static_cast<int>((s.count + p.piece - 1) / p.piece);
     p.bytes = 2 * p.pairs_bytes + ((int64_t(1) << p.digit_bits) * (p.pieces + 1) * 4 + 255) / 256 * 256;
     return p;
@@ -478,7 +510,7 @@ SortPlan sort_plan(const ra_embed_shape& s) {
 const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t st) {
     uint2* const half[2] = {reinterpret_cast<uint2*>(work), reinterpret_cast<uint2*>(work + p.pairs_bytes)};
     if (p.passes == 0) {
-        sort_rank<<<static_cast<int>((e.count + 63) / 64), e.count > 1024 ? 1024 : 256, 0, st>>>(e, half[0]);
+        sort_rank<<<static_cast<int>((e.count + 31) / 32), e.count > 1024 ? 1024 : 256, 0, st>>>(e, half[0]);
         return half[0];
     }
     SortArgs a{};
@@ -494,7 +526,7 @@ const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t
         a.shift = pass * p.digit_bits;
         sort_count<<<p.pieces, kThreads, a.digits * 4, st>>>(a);
         sort_offsets<<<(a.digits + kWaves - 1) / kWaves, kThreads, 0, st>>>(a);
-        sort_move<<<p.pieces, kThreads, (kWaves * a.digits + a.digits + kWaves) * 4, st>>>(a);
+        sort_move<<<p.pieces, kMoveThreads, a.digits * 4 + kMoveThreads / 64 * (4 + a.digits * 2), st>>>(a);
         a.from = a.to;
     }
     return a.from;
@@ -571,8 +603,7 @@ ra_status ra_embed(const ra_embed_shape* s, const void* d_ids, const void* d_tab
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
     const int p = ra::packet_of(*s, d_table, d_out, s->rows, s->ld_table), shift = ra::shift_of(s->dim, p);
     const int64_t groups = ra::kThreads >> shift, full = (s->count + groups - 1) / groups;
-    // Rows one by one where there are few, else several in flight.
-    const int blocks = static_cast<int>(std::min(std::max(std::min<int64_t>(full, 2048), (full + 3) / 4), ra::kMaxBlocks));
+    const int blocks = static_cast<int>(std::min<int64_t>(full, ra::kRowBlocks));
     ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
         ra::embed_rows<decltype(t), decltype(packet)::value>
             <<<blocks, ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a, shift);
@@ -622,8 +653,8 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
         ra::embed_sum<decltype(t), decltype(packet)::value><<<grid, ra::kThreads, 0, st>>>(sum);
         if (plan.tiles > 1)
-            ra::embed_join<decltype(t)><<<dim3(plan.tiles, std::min((s->dim + 63) / 64, 16)), ra::kJoinThreads, 0, st>>>(
-                sum, ra::shift_of(s->dim, 1));
+            ra::embed_join<decltype(t)><<<dim3(plan.tiles, std::min((s->dim + 31) / 32, 16)), ra::kThreads, 0, st>>>(
+                sum, std::min(ra::shift_of(s->dim, 1), 5));
     });
     RA_LAUNCH_CHECK("embed_sum");
     return RA_OK;

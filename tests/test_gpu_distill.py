@@ -152,6 +152,43 @@ def test_rows(M, C):
     check(*make(M, C, 4, torch.float32), T=3.0, hard=0.5)
 
 
+@pytest.mark.parametrize("C", [1, 2, 3, 8, 31, 32, 47, 48, 63, 64, 65])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_many_rows_of_few_classes(C, dtype):
+    """Row by row the same as a few rows at a time, to the tolerances of both: the first 150 and the last 83 rows against the
+    definition, with every kind of row among them."""
+    M = 20_003
+    x, t, ids, labels = make(M, C, min(C, 5), dtype, seed=2)
+    some = torch.cat([torch.arange(150), torch.arange(M - 83, M)])
+    x[7, 0], x[9], ids[11, 0], labels[13], labels[15] = math.nan, -math.inf, C, C, -1
+    if C > 2:
+        ids[17, 1], ids[18, :], labels[18], x[19, 1] = ids[17, 0], -1, -1, -math.inf
+        x[18, 2] = math.nan
+    t[21, 0], t[22, 0], t[23, :] = -math.inf, math.inf, -math.inf
+    for hard, T in ((0.0, 2.0), (0.4, 2.0), (1.0, 1.0)):
+        kw = {"temperature": T, "labels": labels.cuda(), "hard": hard}
+        up = torch.randn(M, generator=torch.Generator().manual_seed(5))
+        want, werr, grad, gerr = exact(x[some], t[some], ids[some], T, labels[some], hard, up[some].double())
+        leaf = x.cuda().requires_grad_(True)
+        loss = ra_spmm.distill_loss(leaf, t.cuda(), ids.cuda(), reduction="none", **kw)
+        g, = torch.autograd.grad(loss, leaf, up.cuda())
+        close(loss[some.cuda()], want, werr, "loss of the rows")
+        close(g[some.cuda()], grad, gerr, "gradient of the rows")
+        clean = x.clone()
+        clean[:150] = 0.5
+        good = ids.clone()
+        good[:150] = 0
+        y = labels.clamp(max=C - 1)
+        kw["labels"] = y.cuda()
+        rows = ra_spmm.distill_loss(clean.cuda(), t.clamp(-9, 9).cuda(), good.cuda(), reduction="none", **kw)
+        both, fused = ra_spmm.distill_loss_grad(clean.cuda(), t.clamp(-9, 9).cuda(), good.cuda(), reduction="sum", factor=-2.0, **kw)
+        assert abs(float(both) - float(rows.double().sum())) <= U * float(rows.double().abs().sum())
+        minus = torch.full((M,), -2.0, device="cuda")
+        leaf = clean.cuda().requires_grad_(True)
+        again, = torch.autograd.grad(ra_spmm.distill_loss(leaf, t.clamp(-9, 9).cuda(), good.cuda(), reduction="none", **kw), leaf, minus)
+        assert torch.equal(fused, again)
+
+
 @pytest.mark.parametrize("k", [0, 1, 2, 15, 16, 17, 63, 64, 65, 200, 256, 257, 1000, 1024])
 @pytest.mark.parametrize("C", [1024, 20_000])
 def test_kept_entries(k, C):
