@@ -537,7 +537,7 @@ typedef struct ra_embed_shape {
     int32_t ids64;     /* ids are int64, else int32          */
     int32_t has_padding;
     int64_t padding;
-    int64_t ld_table, ld_grad;
+    int64_t ld_table, ld_grad; /* below 2^31                  */
     float scale;
 } ra_embed_shape;
 ra_status ra_embed(const ra_embed_shape* shape, const void* d_ids, const void* d_table, void* d_out,

@@ -30,22 +30,25 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxDim = 1 << 20;
 constexpr int64_t kMaxCount = (int64_t(1) << 31) - (1 << 24);
-constexpr int kRowBlocks = 1536;  // of the lookup: 6 workgroups for every CU, as many as are resident
+constexpr int64_t kMaxBlocks = 1 << 20;
+constexpr int kRowsAhead = 4;     // rows that a group of the lookup takes at once
 constexpr int kDigitBits = 11;
 constexpr int kPiece = 4096;      // pairs of a workgroup in the sort,
 constexpr int kMaxPieces = 512;   // more where there would be over this many of them,
 constexpr int kMostPiece = 32768; // up to as many: more pieces then
 constexpr int kMoveThreads = 512;
 constexpr int kRankMost = 8192;   // positions that are sorted by counting
-constexpr int kTiles = 2048;      // workgroups of the sum, about
+constexpr int kTiles = 1536;      // workgroups of the sum, about
 
 struct EmbedArgs {
     const void* ids;
     const void* from;  // the table, or the gradient of out
     void* to;          // out, or the gradient of the table
-    int64_t count, rows, padding, ld;
+    int64_t count, rows, padding;
+    int64_t ld;  // below 2^31 where there is a second row
     int32_t dim;
     bool ids64, has_padding;
+    bool around;  // out is written around the caches
     float scale;
 };
 
@@ -65,42 +68,38 @@ struct Packet {
     typedef T vec __attribute__((ext_vector_type(P)));
 };
 
-// A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane, and loads the
-// next rows' ids with them.
+// A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane.  The rows of a
+// workgroup lie side by side: lines that two workgroups share go to memory in two parts.
 template <typename T, int P>
 __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const int shift) {
     using vec = typename Packet<T, P>::vec;
-    constexpr int kAhead = 4;
-    const int lane = threadIdx.x & ((1 << shift) - 1), groups = kThreads >> shift;
-    const int64_t step = (int64_t)gridDim.x * groups;
-    int64_t i0 = (int64_t)blockIdx.x * groups + (threadIdx.x >> shift), id[kAhead];
-    auto load_ids = [&](int64_t i) {
+    constexpr int kAhead = kRowsAhead;
+    const uint32_t lane = threadIdx.x & ((1 << shift) - 1), groups = kThreads >> shift, count = (uint32_t)a.count;
+    for (uint64_t first = (uint64_t)blockIdx.x * groups * kAhead; first < count; first += (uint64_t)gridDim.x * groups * kAhead) {
+        const uint32_t i0 = (uint32_t)first + (threadIdx.x >> shift);
+        int64_t id[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) id[u] = id_at(a, min(i + u * step, a.count - 1));
-    };
-    load_ids(i0);
-    for (; i0 < a.count; i0 += kAhead * step) {
+        for (int u = 0; u < kAhead; ++u) id[u] = id_at(a, min(i0 + u * groups, count - 1));
         const T* from[kAhead];
-        bool padding[kAhead], inside[kAhead];
+        float add[kAhead];  // scale * v + add: -0 leaves the product, NaN is for ids outside; v is 0 without a row
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            padding[u] = is_padding(a, id[u]);
-            inside[u] = !padding[u] && (uint64_t)id[u] < (uint64_t)a.rows;
-            from[u] = static_cast<const T*>(a.from) + (inside[u] ? id[u] * a.ld : 0);
+            const bool padding = is_padding(a, id[u]), inside = !padding && (uint64_t)id[u] < (uint64_t)a.rows;
+            from[u] = inside ? static_cast<const T*>(a.from) + (uint64_t)(uint32_t)id[u] * (uint32_t)a.ld : nullptr;
+            add[u] = inside || padding ? -0.f : __builtin_nanf("");
         }
-        for (int d = lane * P; d < a.dim; d += P << shift) {
+        T* const to = static_cast<T*>(a.to) + (uint64_t)i0 * (uint32_t)a.dim;
+        for (uint32_t d = lane * P; d < (uint32_t)a.dim; d += P << shift) {
             vec v[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                v[u] = *reinterpret_cast<const vec*>(inside[u] ? from[u] + d : reinterpret_cast<const T*>(kZeroRun));
-            if (d == lane * P) load_ids(i0 + kAhead * step);
+                v[u] = *reinterpret_cast<const vec*>(from[u] ? from[u] + d : reinterpret_cast<const T*>(kZeroRun));
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
-                for (int e = 0; e < P; ++e)
-                    v[u][e] = (T)(inside[u] ? a.scale * (float)v[u][e] : padding[u] ? 0.f : __builtin_nanf(""));
-                if (i0 + u * step < a.count)
-                    *reinterpret_cast<vec*>(static_cast<T*>(a.to) + (i0 + u * step) * a.dim + d) = v[u];
+                for (int e = 0; e < P; ++e) v[u][e] = (T)fmaf(a.scale, (float)v[u][e], add[u]);
+                if (i0 + u * groups < count) 
+                    store_vec(reinterpret_cast<vec*>(to + (uint64_t)(u * groups) * (uint32_t)a.dim + d), v[u], a.around);
             }
         }
     }
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) pair[u] = next[u];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const vec*>(from + pair[u].y * a.e.ld);
+            for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const vec*>(from + (uint64_t)pair[u].y * (uint32_t)a.e.ld);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) next[u] = a.pairs[min(e0 + kAhead + u, end - 1)];
 #pragma unroll
@@ -465,6 +464,11 @@ ra_status check(const ra_embed_shape* s) {
     if (s->dim > kMaxDim) return fail(RA_ERR_UNSUPPORTED, "embed: dim is at most 2^20");
     if (s->count >= kMaxCount) return fail(RA_ERR_UNSUPPORTED, "embed: too many positions (below 2^31 - 2^24)");
     if (s->rows >= INT32_MAX - 1) return fail(RA_ERR_UNSUPPORTED, "embed: too many table rows (below 2^31 - 2)");
+    return RA_OK;
+}
+
+ra_status check_stride(int64_t rows, int64_t ld) {
+    if (rows > 1 && ld > INT32_MAX) return fail(RA_ERR_UNSUPPORTED, "embed: rows are at most 2^31 - 1 elements apart");
     return RA_OK;
 }
 
@@ -598,12 +602,14 @@ extern "C" {
 ra_status ra_embed(const ra_embed_shape* s, const void* d_ids, const void* d_table, void* d_out, ra_stream_t stream) {
     RA_TRY(ra::check(s));
     if (s->count == 0) return RA_OK;
+    RA_TRY(ra::check_stride(s->rows, s->ld_table));
     if (!d_ids || !d_out || (s->rows && !d_table)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: NULL tensor");
     if (s->rows > 1 && s->ld_table < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_table is too small)");
-    const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
+    ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
+    a.around = s->count * s->dim * (s->dtype == RA_DTYPE_F32 ? 4 : 2) > ra::kStreamBytes;
     const int p = ra::packet_of(*s, d_table, d_out, s->rows, s->ld_table), shift = ra::shift_of(s->dim, p);
-    const int64_t groups = ra::kThreads >> shift, full = (s->count + groups - 1) / groups;
-    const int blocks = static_cast<int>(std::min<int64_t>(full, ra::kRowBlocks));
+    const int64_t rows = (int64_t)(ra::kThreads >> shift) * ra::kRowsAhead;
+    const int blocks = static_cast<int>(std::min((s->count + rows - 1) / rows, ra::kMaxBlocks));
     ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
         ra::embed_rows<decltype(t), decltype(packet)::value>
             <<<blocks, ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a, shift);
@@ -626,6 +632,7 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     int64_t need = 0;
     RA_TRY(ra_embed_workspace(s, &need));
     if (s->rows == 0) return RA_OK;
+    RA_TRY(ra::check_stride(s->count, s->ld_grad));
     if (!d_dtable || (s->count && (!d_ids || !d_grad))) return fail(RA_ERR_INVALID_ARGUMENT, "embed: NULL tensor");
     if (s->count > 1 && s->ld_grad < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_grad is too small)");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: the workspace is too small");
