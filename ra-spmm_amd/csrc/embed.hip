@@ -31,6 +31,10 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxDim = 1 << 20;
 constexpr int64_t kMaxCount = (int64_t(1) << 31) - (1 << 24);
 constexpr int64_t kMaxBlocks = 1 << 20;
+// An output past the last-level cache (256 MB) is written around the caches: lines that wait
+// there to be written slow down what is read (rows of a small table to 384 MB: 102 us, around
+// the caches 67); a smaller one, which the next kernel finds there, is not (192 MB: 30 us, 34).
+constexpr int64_t kAroundBytes = int64_t(256) << 20;
 constexpr int kRowsAhead = 4;     // rows that a group of the lookup takes at once
 constexpr int kDigitBits = 11;
 constexpr int kPiece = 4096;      // pairs of a workgroup in the sort,
@@ -48,7 +52,6 @@ struct EmbedArgs {
     int64_t ld;  // below 2^31 where there is a second row
     int32_t dim;
     bool ids64, has_padding;
-    bool around;  // out is written around the caches
     float scale;
 };
 
@@ -62,15 +65,17 @@ __device__ __forceinline__ uint32_t key_at(const EmbedArgs& a, int64_t i) {
     return (uint64_t)id < (uint64_t)a.rows && !is_padding(a, id) ? (uint32_t)id : (uint32_t)a.rows;
 }
 
-// P elements as they lie in memory.
+// P elements as they lie in memory: 16 bytes, at any address.  The last packet of a row that is
+// not made of whole ones ends with the row: what it shares with the one before is computed and
+// written by both, the same bits.
 template <typename T, int P>
 struct Packet {
-    typedef T vec __attribute__((ext_vector_type(P)));
+    typedef T vec __attribute__((ext_vector_type(P), aligned(sizeof(T))));
 };
 
 // A group of 2^shift lanes takes kAhead rows at once, a packet of each per lane.  The rows of a
 // workgroup lie side by side: lines that two workgroups share go to memory in two parts.
-template <typename T, int P>
+template <typename T, int P, bool AROUND>
 __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const int shift) {
     using vec = typename Packet<T, P>::vec;
     constexpr int kAhead = kRowsAhead;
@@ -89,7 +94,8 @@ __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const 
             add[u] = inside || padding ? -0.f : __builtin_nanf("");
         }
         T* const to = static_cast<T*>(a.to) + (uint64_t)i0 * (uint32_t)a.dim;
-        for (uint32_t d = lane * P; d < (uint32_t)a.dim; d += P << shift) {
+        for (uint32_t d0 = lane * P; d0 < (uint32_t)a.dim; d0 += P << shift) {
+            const uint32_t d = min(d0, (uint32_t)a.dim - P);
             vec v[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
@@ -98,8 +104,10 @@ __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const 
             for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
                 for (int e = 0; e < P; ++e) v[u][e] = (T)fmaf(a.scale, (float)v[u][e], add[u]);
-                if (i0 + u * groups < count) 
-                    store_vec(reinterpret_cast<vec*>(to + (uint64_t)(u * groups) * (uint32_t)a.dim + d), v[u], a.around);
+                if (i0 + u * groups >= count) continue;
+                vec* const at = reinterpret_cast<vec*>(to + (uint64_t)(u * groups) * (uint32_t)a.dim + d);
+                if constexpr (AROUND) __builtin_nontemporal_store(v[u], at);
+                else *at = v[u];
             }
         }
     }
@@ -292,7 +300,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t first_row, i
     for (int r = threadIdx.x >> a.shift; r < rows; r += groups) {
         if (lds[r]) continue;
         T* const to = static_cast<T*>(a.e.to) + (first_row + r) * a.e.dim;
-        for (int d = lane * P; d < a.e.dim; d += P << a.shift) *reinterpret_cast<vec*>(to + d) = zero;
+        for (int d = lane * P; d < a.e.dim; d += P << a.shift) *reinterpret_cast<vec*>(to + min(d, a.e.dim - P)) = zero;
     }
     __syncthreads();
 }
@@ -303,7 +311,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t first_row, i
 template <typename T, int P>
 __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
     using vec = typename Packet<T, P>::vec;
-    constexpr int kAhead = P == 8 || sizeof(T) == 4 ? 4 : 8;  // rows in flight
+    constexpr int kAhead = 4;  // rows in flight
     __shared__ float edge[2][kThreads * P];  // heads and tails of the groups
     __shared__ int flags[kThreads];          // 1: has a head, 2: has a tail, 4: the head reaches past the group
     if ((int)blockIdx.x >= a.tiles) {
@@ -313,9 +321,9 @@ __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
         return;
     }
     const int group = threadIdx.x >> a.shift, groups = kThreads >> a.shift, lane = threadIdx.x & ((1 << a.shift) - 1);
-    const int d = (((int)blockIdx.y << a.shift) + lane) * P;  // this lane's columns
-    const bool there = d < a.e.dim;
-    const T* const from = static_cast<const T*>(a.e.from) + (there ? d : 0);
+    const int d0 = (((int)blockIdx.y << a.shift) + lane) * P, d = min(d0, a.e.dim - P);  // this lane's columns
+    const bool there = d0 < a.e.dim;
+    const T* const from = static_cast<const T*>(a.e.from) + d;
     const uint32_t rows = (uint32_t)a.e.rows;
     const int first = (int)blockIdx.x * a.tile + group * a.per, end = min(a.count, first + a.per);
     float acc[P];
@@ -536,15 +544,10 @@ const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t
     return a.from;
 }
 
-// Packets of P elements: 16 bytes, 8 for 16-bit types, or single elements.
-int packet_of(const ra_embed_shape& s, const void* a, const void* b, int64_t rows, int64_t ld) {
-    const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
-    auto fits = [&](int p) {
-        return s.dim % p == 0 && (rows <= 1 || ld % p == 0) && reinterpret_cast<uintptr_t>(a) % (p * size) == 0 &&
-               reinterpret_cast<uintptr_t>(b) % (p * size) == 0;
-    };
-    if (size == 2 && fits(8)) return 8;
-    return fits(4) ? 4 : 1;
+// Elements of a packet: 16 bytes, or one where a row has not as many.
+int packet_of(const ra_embed_shape& s) {
+    const int p = s.dtype == RA_DTYPE_F32 ? 4 : 8;
+    return s.dim < p ? 1 : p;
 }
 // Lanes of a row: a power of two, a wave at most.
 int shift_of(int dim, int p) {
@@ -558,7 +561,8 @@ int shift_of(int dim, int p) {
 struct SumPlan {
     int shift, per, tile, tiles, blocks;
 };
-SumPlan sum_plan(const ra_embed_shape& s, int p) {
+SumPlan sum_plan(const ra_embed_shape& s) {
+    const int p = packet_of(s);
     SumPlan x{};
     x.shift = shift_of(s.dim, p);
     x.blocks = (s.dim + (p << x.shift) - 1) / (p << x.shift);
@@ -569,23 +573,11 @@ SumPlan sum_plan(const ra_embed_shape& s, int p) {
     x.tiles = static_cast<int>((s.count + x.tile - 1) / x.tile);
     return x;
 }
-// The workspace holds the tiles of any width of packets: the addresses that choose it are
-// not known when its size is asked for.
-int64_t most_tiles(const ra_embed_shape& s) {
-    int64_t tiles = 0;
-    for (int p : {1, 4, 8}) tiles = std::max<int64_t>(tiles, sum_plan(s, p).tiles);
-    return tiles;
-}
-
 template <typename F>
 void by_packet(int32_t dtype, int p, F f) {
-    using I1 = std::integral_constant<int, 1>;
-    using I4 = std::integral_constant<int, 4>;
-    using I8 = std::integral_constant<int, 8>;
     auto of_type = [&](auto t) {
-        if constexpr (sizeof(t) == 2)
-            if (p == 8) return f(t, I8());
-        return p == 4 ? f(t, I4()) : f(t, I1());
+        if (p == 1) f(t, std::integral_constant<int, 1>());
+        else f(t, std::integral_constant<int, 16 / sizeof(t)>());
     };
     if (dtype == RA_DTYPE_F32) of_type(float());
     else if (dtype == RA_DTYPE_F16) of_type(f16_t());
@@ -605,14 +597,16 @@ ra_status ra_embed(const ra_embed_shape* s, const void* d_ids, const void* d_tab
     RA_TRY(ra::check_stride(s->rows, s->ld_table));
     if (!d_ids || !d_out || (s->rows && !d_table)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: NULL tensor");
     if (s->rows > 1 && s->ld_table < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_table is too small)");
-    ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
-    a.around = s->count * s->dim * (s->dtype == RA_DTYPE_F32 ? 4 : 2) > ra::kStreamBytes;
-    const int p = ra::packet_of(*s, d_table, d_out, s->rows, s->ld_table), shift = ra::shift_of(s->dim, p);
+    const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
+    const bool around = s->count * s->dim * (s->dtype == RA_DTYPE_F32 ? 4 : 2) > ra::kAroundBytes;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int p = ra::packet_of(*s), shift = ra::shift_of(s->dim, p);
     const int64_t rows = (int64_t)(ra::kThreads >> shift) * ra::kRowsAhead;
     const int blocks = static_cast<int>(std::min((s->count + rows - 1) / rows, ra::kMaxBlocks));
     ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
-        ra::embed_rows<decltype(t), decltype(packet)::value>
-            <<<blocks, ra::kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a, shift);
+        using T = decltype(t);
+        if (around) ra::embed_rows<T, decltype(packet)::value, true><<<blocks, ra::kThreads, 0, st>>>(a, shift);
+        else ra::embed_rows<T, decltype(packet)::value, false><<<blocks, ra::kThreads, 0, st>>>(a, shift);
     });
     RA_LAUNCH_CHECK("embed");
     return RA_OK;
@@ -623,7 +617,7 @@ ra_status ra_embed_workspace(const ra_embed_shape* s, int64_t* bytes) {
     RA_TRY(ra::check(s));
     *bytes = 0;
     if (s->count == 0) return RA_OK;
-    *bytes = ra::sort_plan(*s).bytes + 2 * ra::most_tiles(*s) * s->dim * (int64_t)sizeof(float);
+    *bytes = ra::sort_plan(*s).bytes + (int64_t)2 * ra::sum_plan(*s).tiles * s->dim * (int64_t)sizeof(float);
     return RA_OK;
 }
 
@@ -639,8 +633,7 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: the workspace must be 16-byte aligned");
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_grad, d_dtable, s->ld_grad);
-    const int p = ra::packet_of(*s, d_grad, d_dtable, s->count, s->ld_grad);
-    const ra::SumPlan plan = ra::sum_plan(*s, p);
+    const ra::SumPlan plan = ra::sum_plan(*s);
     ra::SumArgs sum{};
     sum.e = a;
     sum.count = static_cast<int32_t>(s->count);
@@ -657,7 +650,7 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     }
     const int64_t clear = std::min<int64_t>((s->rows + ra::kThreads - 1) / ra::kThreads, std::max(256, 65536 / plan.blocks));
     const dim3 grid(static_cast<uint32_t>(plan.tiles + clear), plan.blocks);
-    ra::by_packet(s->dtype, p, [&](auto t, auto packet) {
+    ra::by_packet(s->dtype, ra::packet_of(*s), [&](auto t, auto packet) {
         ra::embed_sum<decltype(t), decltype(packet)::value><<<grid, ra::kThreads, 0, st>>>(sum);
         if (plan.tiles > 1)
             ra::embed_join<decltype(t)><<<dim3(plan.tiles, std::min((s->dim + 31) / 32, 16)), ra::kThreads, 0, st>>>(

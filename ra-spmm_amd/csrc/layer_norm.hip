@@ -9,11 +9,12 @@
 // the sum forward, h and the gradients to dx backward).  A row lies in the registers of a
 // group of lanes, at most 16 elements a lane: of a part of a wave for short rows, of a
 // wave up to 1,024 elements, of a workgroup up to 16,384.  So the variance is summed
-// around the mean without reading again.  A lane's elements are K packets of P, the packets
-// of a row side by side over the lanes.  Backward, groups go on to further rows with the sums
+// around the mean without reading again.  A lane's elements are K packets of 16 bytes, the
+// packets of a row side by side over the lanes, at whatever address the row begins; the last
+// packet of a row that is not made of whole ones ends with the row, and what it shares with
+// the one before is left out of the sums (TAIL) and written by both, the same bits.  Backward, groups go on to further rows with the sums
 // of dw and db in registers; a second launch adds the workgroups' sums in order.
 #include <algorithm>
-#include <initializer_list>
 #include <type_traits>
 
 #include "lanes.hpp"
@@ -45,7 +46,7 @@ struct LayerNormArgs {
 // P elements as they lie in memory, zeros where there are none.
 template <typename T, int P>
 struct Packet {
-    typedef T vec __attribute__((ext_vector_type(P)));
+    typedef T vec __attribute__((ext_vector_type(P), aligned(sizeof(T))));
     vec v;
     __device__ __forceinline__ void load(const T* p, bool there) {
         v = *reinterpret_cast<const vec*>(there ? p : reinterpret_cast<const T*>(kZeroRun));
@@ -59,6 +60,24 @@ __device__ __forceinline__ void store_packet(T* p, const float* f) {
     for (int e = 0; e < P; ++e) v[e] = (T)f[e];
     *reinterpret_cast<typename Packet<T, P>::vec*>(p) = v;
 }
+
+// Where a lane's packets begin, which exist, and how many elements of one belong to the
+// packet before.
+template <int P, int K, bool TAIL>
+struct Places {
+    int at[K], skip[K];
+    bool there[K];
+    __device__ __forceinline__ Places(int lane, int lanes, int dim) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int first = (k * lanes + lane) * P;
+            there[k] = first < dim;
+            at[k] = TAIL ? min(first, dim - P) : first;
+            skip[k] = first - at[k];
+        }
+    }
+    __device__ __forceinline__ bool counts(int k, int e) const { return there[k] && (!TAIL || e >= skip[k]); }
+};
 
 // The group of lanes that a row lies in.  WAVE: a part of a wave; else the workgroup,
 // whose waves exchange sums through LDS (two sets in turn, so that one barrier a sum is enough).
@@ -97,7 +116,7 @@ struct Group {
     }
 };
 
-template <typename T, int P, int K, bool WAVE>
+template <typename T, int P, int K, bool WAVE, bool TAIL>
 __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(const LayerNormArgs a) {
     __shared__ float lds[64];
     Group<WAVE> group{};
@@ -106,19 +125,17 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
     group.lane = WAVE ? threadIdx.x & (group.lanes - 1) : threadIdx.x;
     const int64_t units = WAVE ? (int64_t)gridDim.x * (kThreads >> a.lanes_shift) : gridDim.x;
     int64_t row = WAVE ? (int64_t)blockIdx.x * (kThreads >> a.lanes_shift) + (threadIdx.x >> a.lanes_shift) : blockIdx.x;
+    const Places<P, K, TAIL> place(group.lane, group.lanes, a.dim);
+    const auto& at = place.at;
+    const auto& there = place.there;
     float w[K][P], b[K][P];
-    bool there[K];
-    int at[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        at[k] = (k * group.lanes + group.lane) * P;
-        there[k] = at[k] < a.dim;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
             b[k][e] = a.b && there[k] ? a.b[at[k] + e] : 0.f;
         }
-    }
     for (; row < a.rows; row += units) {
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
         const int64_t out = row * a.dim;
@@ -147,15 +164,15 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < P; ++e) s += h[k][e];
+            for (int e = 0; e < P; ++e) s += !TAIL || place.counts(k, e) ? h[k][e] : 0.f;
         const float mean = group.sum(s) / a.count;
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < P; ++e) {
-                h[k][e] = there[k] ? h[k][e] - mean : 0.f;
-                s = fmaf(h[k][e], h[k][e], s);
+                h[k][e] -= mean;
+                s = place.counts(k, e) ? fmaf(h[k][e], h[k][e], s) : s;
             }
         const float inv = rsqrtf(group.sum(s) / a.count + a.eps);
 #pragma unroll
@@ -168,8 +185,8 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
     }
 }
 
-template <typename T, int P, int K, bool WAVE>
-__global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(const LayerNormArgs a) {
+template <typename T, int P, int K, bool WAVE, bool TAIL>
+__global__ __launch_bounds__(WAVE ? kThreads : 1024, WAVE ? 3 : 4) void layer_norm_backward(const LayerNormArgs a) {
     __shared__ float lds[64];
     extern __shared__ float sums[];  // WAVE: [waves][2][dim]
     Group<WAVE> group{};
@@ -178,19 +195,17 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(co
     group.lane = WAVE ? threadIdx.x & (group.lanes - 1) : threadIdx.x;
     const int64_t units = WAVE ? (int64_t)gridDim.x * (kThreads >> a.lanes_shift) : gridDim.x;
     int64_t row = WAVE ? (int64_t)blockIdx.x * (kThreads >> a.lanes_shift) + (threadIdx.x >> a.lanes_shift) : blockIdx.x;
+    const Places<P, K, TAIL> place(group.lane, group.lanes, a.dim);
+    const auto& at = place.at;
+    const auto& there = place.there;
     float w[K][P], dw[K][P], db[K][P];
-    bool there[K];
-    int at[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        at[k] = (k * group.lanes + group.lane) * P;
-        there[k] = at[k] < a.dim;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
             dw[k][e] = db[k][e] = 0.f;
         }
-    }
     for (; row < a.rows; row += units) {
         const int64_t out = row * a.dim;
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -213,11 +228,12 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(co
             for (int e = 0; e < P; ++e) {
                 n[k][e] = (px[k].at(e) - mean) * inv;
                 const float from = pg[k].at(e);  // 0 where there is no element
-                dw[k][e] = there[k] ? fmaf(from, n[k][e], dw[k][e]) : 0.f;
-                db[k][e] += from;
+                const bool counts = place.counts(k, e);
+                dw[k][e] = counts ? fmaf(from, n[k][e], dw[k][e]) : dw[k][e];
+                db[k][e] += from;  // not read where the element is the packet's before
                 g[k][e] = from * w[k][e];
-                s += g[k][e];
-                t = there[k] ? fmaf(g[k][e], n[k][e], t) : t;
+                s += !TAIL || counts ? g[k][e] : 0.f;
+                t = counts ? fmaf(g[k][e], n[k][e], t) : t;
             }
         group.sum2(s, t);
         s /= a.count;
@@ -239,7 +255,7 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(co
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < P; ++e)
-                if (there[k]) {
+                if (place.counts(k, e)) {
                     part[at[k] + e] = dw[k][e];
                     part[a.dim + at[k] + e] = db[k][e];
                 }
@@ -259,7 +275,7 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_backward(co
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int e = 0; e < P; ++e)
-                    if (there[k]) {
+                    if (place.counts(k, e)) {
                         to[at[k] + e] = dw[k][e];
                         to[a.dim + at[k] + e] = db[k][e];
                     }
@@ -309,29 +325,22 @@ ra_status check(const ra_layer_norm_shape* s) {
 // 1 << shift lanes (wave) or of `threads`.
 struct Layout {
     int p, k, shift, threads, blocks;
-    bool wave;
+    bool wave, tail;
 };
 
-// Packets as wide as the sizes and addresses allow (16 bytes; 8 for 16-bit types; else
-// single elements, neighbouring lanes the neighbouring ones), as few in a lane as a wave needs.
-Layout layout_of(const ra_layer_norm_shape& s, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides,
-                 int most_blocks) {
-    const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2;
-    auto fits = [&](int p) {
-        bool ok = s.dim % p == 0;
-        for (const void* ptr : pointers) ok = ok && reinterpret_cast<uintptr_t>(ptr) % (p * size) == 0;
-        for (int64_t ld : strides) ok = ok && (s.rows <= 1 || ld % p == 0);
-        return ok;
-    };
+// Packets of 16 bytes (single elements where a row has not one), as few in a lane as a wave
+// needs.
+Layout layout_of(const ra_layer_norm_shape& s, int most_blocks) {
     Layout l{};
-    l.p = 16 / size;
-    while (l.p > 1 && !(fits(l.p) && l.p >= 4)) l.p /= 2;
-    const int packets = s.dim / l.p, most = kMaxLane / l.p;
+    l.p = s.dtype == RA_DTYPE_F32 ? 4 : 8;
+    if (s.dim < l.p) l.p = 1;
+    l.tail = s.dim % l.p != 0;
+    const int packets = (s.dim + l.p - 1) / l.p, most = kMaxLane / l.p;
     l.wave = packets <= 64 * most;
     l.k = 1;
-    while (l.k < most && packets > 64 * l.k) l.k *= l.p == 1 ? 4 : 2;
+    while (l.k < most && packets > 64 * l.k) l.k *= 2;
     if (l.wave) {
-        while (((int64_t)l.k << l.shift) < packets) ++l.shift;
+        while ((l.k << l.shift) < packets) ++l.shift;
         l.threads = kThreads;
     } else {
         l.threads = 128;
@@ -348,26 +357,30 @@ Layout layout_of(const ra_layer_norm_shape& s, std::initializer_list<const void*
 int resident(const Layout& l) {
     if (!l.wave) return 1024 / l.threads;
     const int elements = l.p * l.k;
-    return elements <= 4 ? 8 : elements == 8 ? 5 : l.p > 1 ? 3 : 1;
+    return elements <= 4 ? 8 : elements == 8 ? 5 : 3;
 }
 
 template <typename F>
 void by_layout(int32_t dtype, const Layout& l, F f) {
     auto packets = [&](auto t, auto p, auto k) {
-        if (l.wave) f(t, p, k, std::true_type());
-        else if constexpr (decltype(p)::value * decltype(k)::value == kMaxLane) f(t, p, k, std::false_type());
+        auto tail = [&](auto wave) {
+            if constexpr (decltype(p)::value > 1)
+                if (l.tail) return f(t, p, k, wave, std::true_type());
+            f(t, p, k, wave, std::false_type());
+        };
+        if (l.wave) tail(std::true_type());
+        else if constexpr (decltype(p)::value * decltype(k)::value == kMaxLane) tail(std::false_type());
     };
     auto of_type = [&](auto t) {
+        constexpr int kPer = 16 / sizeof(t);
+        using P = std::integral_constant<int, kPer>;
         using I1 = std::integral_constant<int, 1>;
         using I2 = std::integral_constant<int, 2>;
         using I4 = std::integral_constant<int, 4>;
-        using I8 = std::integral_constant<int, 8>;
-        using I16 = std::integral_constant<int, 16>;
-        if constexpr (sizeof(t) == 2) {
-            if (l.p == 8) return l.k == 1 ? packets(t, I8(), I1()) : packets(t, I8(), I2());
-        }
-        if (l.p == 4) return l.k == 1 ? packets(t, I4(), I1()) : l.k == 2 ? packets(t, I4(), I2()) : packets(t, I4(), I4());
-        return l.k == 1 ? packets(t, I1(), I1()) : l.k == 4 ? packets(t, I1(), I4()) : packets(t, I1(), I16());
+        if (l.p == 1) return packets(t, I1(), I1());
+        if constexpr (kPer == 4)
+            if (l.k == 4) return packets(t, P(), I4());
+        l.k == 1 ? packets(t, P(), I1()) : packets(t, P(), I2());
     };
     if (dtype == RA_DTYPE_F32) of_type(float());
     else if (dtype == RA_DTYPE_F16) of_type(f16_t());
@@ -405,10 +418,10 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
     a.dim = s->dim;
     a.eps = s->eps;
     a.count = static_cast<float>(s->dim);
-    const ra::Layout l = ra::layout_of(*s, {d_x, d_residual, d_y, d_sum}, {s->ldx, d_residual ? s->ldr : 0}, ra::kForwardBlocks);
+    const ra::Layout l = ra::layout_of(*s, ra::kForwardBlocks);
     a.lanes_shift = l.shift;
-    ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave) {
-        ra::layer_norm_forward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value>
+    ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave, auto tail) {
+        ra::layer_norm_forward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value, decltype(tail)::value>
             <<<l.blocks, l.threads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
     });
     RA_LAUNCH_CHECK("layer_norm");
@@ -449,12 +462,12 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
     a.count = static_cast<float>(s->dim);
     ra::Layout l{};
     if (s->rows) {
-        l = ra::layout_of(*s, {d_h, d_grad_y, d_grad_sum, d_dx}, {s->ldx}, ra::kBackwardBlocks);
+        l = ra::layout_of(*s, ra::kBackwardBlocks);
         l.blocks = std::min(l.blocks, 256 * ra::resident(l));
         a.lanes_shift = l.shift;
         const size_t lds = l.wave && a.part ? (size_t)ra::kThreads / 64 * 2 * s->dim * sizeof(float) : 0;
-        ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave) {
-            ra::layer_norm_backward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value>
+        ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave, auto tail) {
+            ra::layer_norm_backward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value, decltype(tail)::value>
                 <<<l.blocks, l.threads, lds, st>>>(a);
         });
         RA_LAUNCH_CHECK("layer_norm backward");

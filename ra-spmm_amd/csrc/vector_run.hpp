@@ -100,16 +100,4 @@ __device__ __forceinline__ void store_run(T* p, const float* f, int count) {
     }
 }
 
-// Outputs past the last-level cache (256 MB) are written around the caches: lines that wait
-// there to be written slow down what is read (rows of a small table to 384 MB: 102 us,
-// around the caches 67); smaller ones, which the next kernel finds there, are not (192 MB:
-// 30 us, 34).
-constexpr int64_t kStreamBytes = int64_t(256) << 20;
-
-template <typename V>
-__device__ __forceinline__ void store_vec(V* p, V v, bool around) {
-    if (around) __builtin_nontemporal_store(v, p);
-    else *p = v;
-}
-
 }  // namespace ra
