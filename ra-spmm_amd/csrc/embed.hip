@@ -34,6 +34,8 @@ constexpr int64_t kMaxBlocks = 1 << 20;
 // An output past the last-level cache (256 MB) is written around the caches: lines that wait
 // there to be written slow down what is read (rows of a small table to 384 MB: 102 us, around
 // the caches 67); a smaller one, which the next kernel finds there, is not (192 MB: 30 us, 34).
+// So is a gradient's: lookup and gradient of 1e6 positions on 1e6 rows of 256 in bf16 one after
+// the other, 399 us, 382.
 constexpr int64_t kAroundBytes = int64_t(256) << 20;
 constexpr int kRowsAhead = 4;     // rows that a group of the lookup takes at once
 constexpr int kDigitBits = 11;
@@ -308,7 +310,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t first_row, i
 // blockIdx.x: a tile of sorted positions, or past those workgroups that clear table rows
 // (of the first column block); blockIdx.y: a block of P << shift columns.  A group of
 // 2^shift lanes takes `per` positions of the tile, a packet of columns per lane.
-template <typename T, int P>
+template <typename T, int P, bool AROUND>
 __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
     using vec = typename Packet<T, P>::vec;
     constexpr int kAhead = 4;  // rows in flight
@@ -334,7 +336,9 @@ __global__ __launch_bounds__(kThreads) void embed_sum(const SumArgs a) {
         vec v;
 #pragma unroll
         for (int e = 0; e < P; ++e) v[e] = (T)(a.e.scale * f[e]);
-        *reinterpret_cast<vec*>(static_cast<T*>(a.e.to) + (int64_t)row * a.e.dim + d) = v;
+        vec* const at = reinterpret_cast<vec*>(static_cast<T*>(a.e.to) + (int64_t)row * a.e.dim + d);
+        if constexpr (AROUND) __builtin_nontemporal_store(v, at);
+        else *at = v;
     };
     float* const head = edge[0] + threadIdx.x * P;
     float* const tail = edge[1] + threadIdx.x * P;
@@ -650,8 +654,11 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     }
     const int64_t clear = std::min<int64_t>((s->rows + ra::kThreads - 1) / ra::kThreads, std::max(256, 65536 / plan.blocks));
     const dim3 grid(static_cast<uint32_t>(plan.tiles + clear), plan.blocks);
+    const bool around = s->rows * s->dim * (s->dtype == RA_DTYPE_F32 ? 4 : 2) > ra::kAroundBytes;
     ra::by_packet(s->dtype, ra::packet_of(*s), [&](auto t, auto packet) {
-        ra::embed_sum<decltype(t), decltype(packet)::value><<<grid, ra::kThreads, 0, st>>>(sum);
+        using T = decltype(t);
+        if (around) ra::embed_sum<T, decltype(packet)::value, true><<<grid, ra::kThreads, 0, st>>>(sum);
+        else ra::embed_sum<T, decltype(packet)::value, false><<<grid, ra::kThreads, 0, st>>>(sum);
         if (plan.tiles > 1)
             ra::embed_join<decltype(t)><<<dim3(plan.tiles, std::min((s->dim + 31) / 32, 16)), ra::kThreads, 0, st>>>(
                 sum, std::min(ra::shift_of(s->dim, 1), 5));

@@ -27,7 +27,11 @@ namespace {
 constexpr int kThreads = 256;       // of a workgroup that holds several rows
 constexpr int kMaxDim = 16384;
 constexpr int kMaxLane = 16;        // elements of a row in a lane
-constexpr int kForwardBlocks = 8192;
+constexpr int kForwardBlocks = 2048;
+// Outputs past the last-level cache (256 MB) are written around the caches, where lines that wait
+// to be written slow down what is read next: forward and backward pass of 1e6 x 256 in bf16,
+// one after the other, 402 + 429 us, around the caches 398 + 407.
+constexpr int64_t kAroundBytes = int64_t(256) << 20;
 constexpr int kBackwardBlocks = 2048;
 constexpr int kColumns = 16;        // columns of a workgroup that adds the parts of dw and db
 constexpr int kAddThreads = 1024;   // and its threads
@@ -53,12 +57,23 @@ struct Packet {
     }
     __device__ __forceinline__ float at(int e) const { return (float)v[e]; }
 };
-template <typename T, int P>
+template <bool AROUND, typename T, int P>
 __device__ __forceinline__ void store_packet(T* p, const float* f) {
     typename Packet<T, P>::vec v;
 #pragma unroll
     for (int e = 0; e < P; ++e) v[e] = (T)f[e];
-    *reinterpret_cast<typename Packet<T, P>::vec*>(p) = v;
+    auto* const to = reinterpret_cast<typename Packet<T, P>::vec*>(p);
+    if constexpr (AROUND) __builtin_nontemporal_store(v, to);
+    else *to = v;
+}
+
+// A packet's weights, `none` without any.
+template <int P>
+__device__ __forceinline__ void load_weights(float* to, const float* from, int at, bool there, float none) {
+    Packet<float, P> p;
+    p.load(from + at, from && there);
+#pragma unroll
+    for (int e = 0; e < P; ++e) to[e] = from ? p.at(e) : none;
 }
 
 // Where a lane's packets begin, which exist, and how many elements of one belong to the
@@ -116,7 +131,7 @@ struct Group {
     }
 };
 
-template <typename T, int P, int K, bool WAVE, bool TAIL>
+template <typename T, int P, int K, bool WAVE, bool TAIL, bool AROUND>
 __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(const LayerNormArgs a) {
     __shared__ float lds[64];
     Group<WAVE> group{};
@@ -130,12 +145,10 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
     const auto& there = place.there;
     float w[K][P], b[K][P];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int e = 0; e < P; ++e) {
-            w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
-            b[k][e] = a.b && there[k] ? a.b[at[k] + e] : 0.f;
-        }
+    for (int k = 0; k < K; ++k) {
+        load_weights<P>(w[k], a.w, at[k], there[k], 1.f);
+        load_weights<P>(b[k], a.b, at[k], there[k], 0.f);
+    }
     for (; row < a.rows; row += units) {
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
         const int64_t out = row * a.dim;
@@ -151,7 +164,7 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
             for (int k = 0; k < K; ++k) {
 #pragma unroll
                 for (int e = 0; e < P; ++e) h[k][e] = px[k].at(e) + pr[k].at(e);
-                if (there[k]) store_packet<T, P>(static_cast<T*>(a.sum) + out + at[k], h[k]);
+                if (there[k]) store_packet<AROUND, T, P>(static_cast<T*>(a.sum) + out + at[k], h[k]);
 #pragma unroll
                 for (int e = 0; e < P; ++e) h[k][e] = (float)(T)h[k][e];  // the norm is that of the sum as it is kept
             }
@@ -179,13 +192,13 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int e = 0; e < P; ++e) h[k][e] = fmaf(h[k][e] * inv, w[k][e], b[k][e]);
-            if (there[k]) store_packet<T, P>(static_cast<T*>(a.y) + out + at[k], h[k]);
+            if (there[k]) store_packet<AROUND, T, P>(static_cast<T*>(a.y) + out + at[k], h[k]);
         }
         if (a.stats && group.lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, inv);
     }
 }
 
-template <typename T, int P, int K, bool WAVE, bool TAIL>
+template <typename T, int P, int K, bool WAVE, bool TAIL, bool AROUND>
 __global__ __launch_bounds__(WAVE ? kThreads : 1024, WAVE ? 3 : 4) void layer_norm_backward(const LayerNormArgs a) {
     __shared__ float lds[64];
     extern __shared__ float sums[];  // WAVE: [waves][2][dim]
@@ -200,12 +213,11 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024, WAVE ? 3 : 4) void layer_no
     const auto& there = place.there;
     float w[K][P], dw[K][P], db[K][P];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        load_weights<P>(w[k], a.w, at[k], there[k], 1.f);
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-            w[k][e] = a.w && there[k] ? a.w[at[k] + e] : 1.f;
-            dw[k][e] = db[k][e] = 0.f;
-        }
+        for (int e = 0; e < P; ++e) dw[k][e] = db[k][e] = 0.f;
+    }
     for (; row < a.rows; row += units) {
         const int64_t out = row * a.dim;
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -245,7 +257,7 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024, WAVE ? 3 : 4) void layer_no
                 g[k][e] = inv * (g[k][e] - s - n[k][e] * t);
                 if (a.gs) g[k][e] += ps[k].at(e);
             }
-            if (there[k]) store_packet<T, P>(static_cast<T*>(a.y) + out + at[k], g[k]);
+            if (there[k]) store_packet<AROUND, T, P>(static_cast<T*>(a.y) + out + at[k], g[k]);
         }
     }
     if (!a.part) return;
@@ -343,6 +355,8 @@ Layout layout_of(const ra_layer_norm_shape& s, int most_blocks) {
         while ((l.k << l.shift) < packets) ++l.shift;
         l.threads = kThreads;
     } else {
+        l.k = 8 / l.p;  // 8 elements a lane up to 1,024 lanes: more rows in flight, no registers short
+        if (packets > 1024 * l.k) l.k *= 2;
         l.threads = 128;
         while (l.threads * l.k < packets) l.threads *= 2;
     }
@@ -350,6 +364,10 @@ Layout layout_of(const ra_layer_norm_shape& s, int most_blocks) {
     // Never more than min(rows, most_blocks): the workspace holds a part for each.
     l.blocks = static_cast<int>(std::min<int64_t>((s.rows + per - 1) / per, most_blocks));
     return l;
+}
+
+bool passes_caches(const ra_layer_norm_shape& s) {
+    return s.rows * s.dim * (s.dtype == RA_DTYPE_F32 ? 4 : 2) > kAroundBytes;
 }
 
 // Workgroups of the backward pass that a CU holds at once, by their registers: with a
@@ -369,7 +387,7 @@ void by_layout(int32_t dtype, const Layout& l, F f) {
             f(t, p, k, wave, std::false_type());
         };
         if (l.wave) tail(std::true_type());
-        else if constexpr (decltype(p)::value * decltype(k)::value == kMaxLane) tail(std::false_type());
+        else if constexpr (decltype(p)::value * decltype(k)::value >= 8) tail(std::false_type());
     };
     auto of_type = [&](auto t) {
         constexpr int kPer = 16 / sizeof(t);
@@ -418,11 +436,15 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
     a.dim = s->dim;
     a.eps = s->eps;
     a.count = static_cast<float>(s->dim);
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const ra::Layout l = ra::layout_of(*s, ra::kForwardBlocks);
     a.lanes_shift = l.shift;
     ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave, auto tail) {
-        ra::layer_norm_forward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value, decltype(tail)::value>
-            <<<l.blocks, l.threads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+        using T = decltype(t);
+        constexpr int kPer = decltype(p)::value, kEach = decltype(k)::value;
+        constexpr bool kWave = decltype(wave)::value, kTail = decltype(tail)::value;
+        if (ra::passes_caches(*s)) ra::layer_norm_forward<T, kPer, kEach, kWave, kTail, true><<<l.blocks, l.threads, 0, st>>>(a);
+        else ra::layer_norm_forward<T, kPer, kEach, kWave, kTail, false><<<l.blocks, l.threads, 0, st>>>(a);
     });
     RA_LAUNCH_CHECK("layer_norm");
     return RA_OK;
@@ -467,8 +489,11 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
         a.lanes_shift = l.shift;
         const size_t lds = l.wave && a.part ? (size_t)ra::kThreads / 64 * 2 * s->dim * sizeof(float) : 0;
         ra::by_layout(s->dtype, l, [&](auto t, auto p, auto k, auto wave, auto tail) {
-            ra::layer_norm_backward<decltype(t), decltype(p)::value, decltype(k)::value, decltype(wave)::value, decltype(tail)::value>
-                <<<l.blocks, l.threads, lds, st>>>(a);
+            using T = decltype(t);
+            constexpr int kPer = decltype(p)::value, kEach = decltype(k)::value;
+            constexpr bool kWave = decltype(wave)::value, kTail = decltype(tail)::value;
+            if (ra::passes_caches(*s)) ra::layer_norm_backward<T, kPer, kEach, kWave, kTail, true><<<l.blocks, l.threads, lds, st>>>(a);
+            else ra::layer_norm_backward<T, kPer, kEach, kWave, kTail, false><<<l.blocks, l.threads, lds, st>>>(a);
         });
         RA_LAUNCH_CHECK("layer_norm backward");
     }
