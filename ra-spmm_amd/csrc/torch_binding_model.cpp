@@ -5,6 +5,8 @@
 #include <string>
 #include <tuple>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "torch_checks.hpp"
 
 namespace {
@@ -232,10 +234,169 @@ Tensor run_distill_backward(Tensor logits, Tensor teacher, Tensor ids, double te
     return grad;
 }
 
+// --------------------------------------------------------------------- autograd
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// t itself where only its rows are strided, else a contiguous copy.
+Tensor with_rows(const Tensor& t) {
+    int64_t run = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        if (t.size(d) > 1 && t.stride(d) != run) return t.contiguous();
+        run *= t.size(d);
+    }
+    return t.dim() == 0 || t.size(0) <= 1 || t.stride(0) >= run ? t : t.contiguous();
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+    if (!torch::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// Gradients that a second differentiation must not pass silently: as Python's
+// once_differentiable, they raise where they are differentiated.
+variable_list once(variable_list grads, const variable_list& inputs) {
+    if (!torch::GradMode::is_enabled()) return grads;
+    bool any = false;
+    for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
+    if (!any) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", static_cast<int64_t>(grads.size()));
+    for (Tensor& t : grads)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
+    return (*error)(std::move(grads));
+}
+
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor raw(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+struct EmbedNode : torch::autograd::Function<EmbedNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& table, double scale,
+                          c10::optional<int64_t> padding) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["rows"] = table.size(0);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        return run_embed(ids, table, scale, padding);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor ids = ctx->get_saved_variables()[0];
+        Tensor out;
+        {
+            const torch::NoGradGuard guard;
+            const Tensor grad = with_rows(grads[0].reshape({ids.numel(), grads[0].size(-1)}));
+            out = run_embed_backward(ids, grad, ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                     ctx->saved_data["padding"].toOptional<int64_t>());
+        }
+        return once({Tensor(), out, Tensor(), Tensor()}, {grads[0]});
+    }
+};
+
+Tensor embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
+    ids = ids.contiguous();
+    table = with_rows(table);
+    return wants_grad({&table}) ? EmbedNode::apply(ids, table, scale, padding) : run_embed(ids, table, scale, padding);
+}
+
+// With a residual two outputs: y and the sum.
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& weight,
+                                 const OptTensor& bias, double eps) {
+        auto [y, sum, stats] = run_layer_norm(x, residual, weight, bias, eps, true);
+        // Without a residual the input itself is kept, else the sum, which the caller has anyway.
+        ctx->save_for_backward({sum.has_value() ? *sum : x, raw(weight), *stats});
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->set_materialize_grads(false);
+        if (sum.has_value()) return {y, *sum};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &h = saved[0], &weight = saved[1];
+        size_t given = 0;  // inputs that are not given are not counted
+        const bool x_grad = ctx->needs_input_grad(given++), residual_grad = grads.size() > 1 && ctx->needs_input_grad(given++);
+        const bool weight_grad = weight.defined() && ctx->needs_input_grad(given++);
+        const bool bias_grad = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(given++);
+        Tensor dx, dw, db, of_sum = grads.size() > 1 ? grads[1] : Tensor();
+        {
+            const torch::NoGradGuard guard;
+            if (grads[0].defined()) {
+                if (of_sum.defined()) of_sum = of_sum.contiguous();
+                auto [x, w, b] = run_layer_norm_backward(h, opt(weight), saved[2], grads[0].contiguous(), opt(of_sum), weight_grad,
+                                                         bias_grad);
+                dx = x;
+                dw = raw(w);
+                db = raw(b);
+            } else if (of_sum.defined()) {  // only the sum was used
+                dx = of_sum;
+                if (weight_grad) dw = torch::zeros_like(weight);
+                if (bias_grad) db = torch::zeros({h.size(1)}, h.options().dtype(torch::kFloat32));
+            }
+        }
+        return once({x_grad ? dx : Tensor(), residual_grad ? dx : Tensor(), dw, db, Tensor()},
+                    {grads[0], grads.size() > 1 ? grads[1] : Tensor(), h, weight});
+    }
+};
+
+// (y, x + residual or nothing) of matrices.
+std::tuple<Tensor, OptTensor> layer_norm(Tensor x, OptTensor residual, OptTensor weight, OptTensor bias, double eps) {
+    x = with_rows(x);
+    if (residual.has_value()) residual = with_rows(*residual);
+    const Tensor r = raw(residual), w = raw(weight), b = raw(bias);
+    if (wants_grad({&x, &r, &w, &b})) {
+        const variable_list out = LayerNormNode::apply(x, residual, weight, bias, eps);
+        return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+    }
+    auto [y, sum, stats] = run_layer_norm(x, residual, weight, bias, eps, false);
+    return {y, sum};
+}
+
+struct DistillNode : torch::autograd::Function<DistillNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& ids,
+                          const OptTensor& labels, double temperature, double hard, std::string reduction) {
+        auto [loss, stats, grad] = run_distill(logits, teacher, ids, temperature, labels, hard, reduction, true, false,
+                                               OptTensor());
+        ctx->save_for_backward({logits, teacher, ids, raw(labels), *stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["hard"] = hard;
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        Tensor out;
+        {
+            const torch::NoGradGuard guard;
+            out = run_distill_backward(saved[0], saved[1], saved[2], ctx->saved_data["temperature"].toDouble(), opt(saved[3]),
+                                       ctx->saved_data["hard"].toDouble(), ctx->saved_data["reduction"].toStringRef(), saved[4],
+                                       grads[0].contiguous());
+        }
+        return once({out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, {grads[0], saved[0]});
+    }
+};
+
+Tensor distill_loss(Tensor logits, Tensor teacher, Tensor ids, double temperature, OptTensor labels, double hard,
+                    std::string reduction) {
+    logits = with_rows(logits);
+    teacher = with_rows(teacher);
+    ids = with_rows(ids);
+    if (labels.has_value()) labels = labels->contiguous();
+    if (wants_grad({&logits})) return DistillNode::apply(logits, teacher, ids, labels, temperature, hard, reduction);
+    return std::get<0>(run_distill(logits, teacher, ids, temperature, labels, hard, reduction, false, false, OptTensor()));
+}
+
 }  // namespace
 
 void bind_model_operators(pybind11::module_& m) {
     namespace py = pybind11;
+    m.def("embed", &embed, "scale * table[ids], differentiable in table", py::arg("ids"), py::arg("table"), py::arg("scale"),
+          py::arg("padding"));
+    m.def("layer_norm", &layer_norm, "Layer norm of a matrix's rows: (y, x + residual), differentiable", py::arg("x"),
+          py::arg("residual"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
+    m.def("distill_loss", &distill_loss, "Distillation loss, differentiable in logits", py::arg("logits"), py::arg("teacher"),
+          py::arg("ids"), py::arg("temperature"), py::arg("labels"), py::arg("hard"), py::arg("reduction"));
     m.def("run_embed", &run_embed, "scale * table[ids]", py::arg("ids"), py::arg("table"), py::arg("scale"),
           py::arg("padding"));
     m.def("run_embed_backward", &run_embed_backward, "Gradient of run_embed's table, [rows, dim]", py::arg("ids"),

@@ -15,33 +15,14 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C
 from .attention import _rows
 
 
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher, ids, temperature, labels, hard, reduction):
-        loss, stats, _ = _C.run_distill(logits, teacher, ids, temperature, labels, hard, reduction, True, False, None)
-        ctx.save_for_backward(logits, teacher, ids, labels, stats)
-        ctx.args = temperature, hard, reduction
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, teacher, ids, labels, stats = ctx.saved_tensors
-        temperature, hard, reduction = ctx.args
-        grad = _C.run_distill_backward(logits, teacher, ids, temperature, labels, hard, reduction, stats, grad.contiguous())
-        return grad, None, None, None, None, None, None
-
-
-def _inputs(name, logits, teacher, ids, labels):
+def _check_teacher(name, teacher):
     if torch.is_grad_enabled() and teacher.requires_grad:
         raise RuntimeError(f"{name}: teacher takes no gradient (detach it)")
-    return _rows(logits), _rows(teacher), _rows(ids), None if labels is None else labels.contiguous()
 
 
 def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0,
@@ -51,10 +32,8 @@ def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, ids: torch.Tensor,
     logits [rows, classes] and teacher [rows, kept] (the values of a top-k, kept at most 1024) float32, float16 or bfloat16;
     ids [rows, kept] int32 or int64; labels [rows] int32 or int64; rows possibly strided; 1e-3 <= temperature <= 1e3 and
     0 <= hard <= 1.  Differentiable in logits."""
-    logits, teacher, ids, labels = _inputs("distill_loss", logits, teacher, ids, labels)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Distill.apply(logits, teacher, ids, temperature, labels, hard, reduction)
-    return _C.run_distill(logits, teacher, ids, temperature, labels, hard, reduction, False, False, None)[0]
+    _check_teacher("distill_loss", teacher)
+    return _C.distill_loss(logits, teacher, ids, temperature, labels, hard, reduction)
 
 
 def distill_loss_grad(logits: torch.Tensor, teacher: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0,
@@ -64,7 +43,8 @@ def distill_loss_grad(logits: torch.Tensor, teacher: torch.Tensor, ids: torch.Te
 
     The gradient is that of factor * loss (factor: a number, or one float32 value on the logits' device, such as a loss
     scale; None: 1), for logits.backward(gradient); the loss is without the factor."""
-    logits, teacher, ids, labels = _inputs("distill_loss_grad", logits, teacher, ids, labels)
+    _check_teacher("distill_loss_grad", teacher)
+    logits, teacher, ids, labels = _rows(logits), _rows(teacher), _rows(ids), None if labels is None else labels.contiguous()
     if factor is not None and not isinstance(factor, torch.Tensor):
         factor = torch.full((1,), float(factor), dtype=torch.float32, device=logits.device)
     with torch.no_grad():

@@ -7,25 +7,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C
-from .attention import _rows
-
-
-class _Embed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, table, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.padding = table.size(0), scale, padding
-        return _C.run_embed(ids, table, scale, padding)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        ids, = ctx.saved_tensors
-        grad = _rows(grad.reshape(ids.numel(), grad.size(-1)))
-        return None, _C.run_embed_backward(ids, grad, ctx.rows, ctx.scale, ctx.padding), None, None
 
 
 def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding: Optional[int] = None) -> torch.Tensor:
@@ -35,7 +18,4 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding: O
     id is `padding` (any value, inside of the table or not) give zeros and take no gradient; an id outside of the table
     gives NaN and takes none.  The gradient is dense and of the table's type; its sums are float32, and equal inputs give
     equal bits."""
-    ids, table = ids.contiguous(), _rows(table)
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _Embed.apply(ids, table, scale, padding)
-    return _C.run_embed(ids, table, scale, padding)
+    return _C.embed(ids, table, scale, padding)

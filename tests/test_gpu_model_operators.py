@@ -166,3 +166,44 @@ def test_a_captured_step():
         torch.cuda.synchronize()
         for a, b in zip(outs[i % 2], want):
             assert torch.equal(a, b), i
+
+
+def test_second_derivatives_are_refused():
+    """They raise where they are differentiated; a first derivative with create_graph is the same as without."""
+    table, x = torch.randn(9, 16, device="cuda", requires_grad=True), torch.randn(5, 16, device="cuda", requires_grad=True)
+    w = torch.rand(16, device="cuda", requires_grad=True)
+    ids = torch.tensor([1, 2, 3, 1, 8], device="cuda")
+    teacher, top = torch.randn(5, 16, device="cuda").topk(3, dim=1)
+    for f, leaf in ((lambda: (ra_spmm.embed(ids, table) * x).sum(), table), (lambda: (ra_spmm.layer_norm(x, w) * table[:5]).sum(), w),
+                    (lambda: ra_spmm.layer_norm(x, w, residual=x)[0].square().sum(), x),
+                    (lambda: ra_spmm.distill_loss(x * 2.0, teacher, top), x)):
+        plain, = torch.autograd.grad(f(), leaf)
+        first, = torch.autograd.grad(f(), leaf, create_graph=True)
+        assert torch.equal(first.detach(), plain)
+        with pytest.raises(RuntimeError, match="twice"):
+            first.square().sum().backward()
+
+
+def test_gradients_that_are_switched_off():
+    """No graph under no_grad, nor of inputs without gradients; a frozen table below a trained norm."""
+    table, w = torch.randn(9, 16, device="cuda"), torch.ones(16, device="cuda", requires_grad=True)
+    ids = torch.tensor([1, 2, 3], device="cuda")
+    x = ra_spmm.embed(ids, table)
+    assert not x.requires_grad
+    y = ra_spmm.layer_norm(x, w)
+    assert y.requires_grad and torch.autograd.grad(y.sum(), w)[0].shape == (16,)
+    with torch.no_grad():
+        assert not ra_spmm.layer_norm(x, w).requires_grad
+        assert not ra_spmm.embed(ids, table.requires_grad_(True)).requires_grad
+        assert not ra_spmm.distill_loss(w[None], x[:1, :2], ids[None, :2]).requires_grad
+    with torch.inference_mode():
+        assert not ra_spmm.layer_norm(x, w, residual=x)[1].requires_grad
+
+
+def test_inputs_changed_after_the_forward_pass():
+    """What a backward pass has kept must not have changed."""
+    x, w = torch.randn(5, 16, device="cuda"), torch.ones(16, device="cuda", requires_grad=True)
+    y = ra_spmm.layer_norm(x, w)
+    x.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
