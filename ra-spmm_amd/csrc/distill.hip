@@ -23,9 +23,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxKept = 1024;
 constexpr int kMaxBlocks = 16384;      // workgroups, and so parts of a reduced loss
-constexpr int kLaneClasses = 64;       // classes of a row that a lane takes,
-constexpr int kLaneKept = 16;          // its entries,
-constexpr int64_t kLaneRows = 16384;   // where there are as many rows
+// Rows of up to 64 classes and 16 entries go by lanes from 32,768 rows on: of 47 classes in fp32,
+// loss and gradient in one call, 16,384 rows take 14.3 us (by parts of waves 11.1), 32,768 15.1
+// (14.9), 65,536 17.4 (23.4), 262,144 39 (60).
+constexpr int kLaneClasses = 64;
+constexpr int kLaneKept = 16;
+constexpr int64_t kLaneRows = 32768;
 constexpr int kMaxShort = 1024;        // classes of a row that a wave holds
 constexpr int kStageBytes = 16384;     // rows of a workgroup at once, about
 // A gradient past the last-level cache (256 MB) is written around the caches, which hold the row
@@ -303,27 +306,29 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
 // A lane per row, 64 rows of up to 64 classes in LDS as floats, rows at an odd pitch: no
 // sums between lanes, and the logarithms, divisions and entries of 64 rows at once.  The
 // rows come and go as one run of memory, like those of distill_short, and so do the
-// entries: read by their lanes, each load would touch 64 lines.
-template <typename T>
-__global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
+// entries: read by their lanes, each load would touch 64 lines.  FLAT: the number of classes is
+// odd, and so the pitch itself.
+template <typename T, bool FLAT>
+__global__ __launch_bounds__(64, FLAT ? 3 : 2) void distill_lanes(const DistillArgs a) {
     extern __shared__ __align__(16) float stage[];
     constexpr int kPer = 16 / sizeof(T), kPackets = kLaneClasses / kPer;
     typedef T vec __attribute__((ext_vector_type(kPer)));
-    const int C = a.classes, pitch = C | 1, lane = threadIdx.x;
+    constexpr uint8_t kOutside = 254, kNone = 255;
+    const int C = a.classes, pitch = FLAT ? C : C | 1, lane = threadIdx.x;
     const uint32_t magic = ((1u << 20) + C - 1) / C;  // i / C = i * magic >> 20 for i < 64 C <= 4096
     const int k = a.kept, entry_pitch = k | 1;
     const uint32_t entry_magic = k ? ((1u << 20) + k - 1) / k : 0;
     const float c = kLog2e * a.inv_t;
     float* const x = stage + lane * pitch;
-    int32_t* const places = reinterpret_cast<int32_t*>(stage + 64 * pitch);  // class, -1: takes no part, -2: no class
-    float* const amounts = stage + 64 * (pitch + entry_pitch);
-    const int32_t* const place = places + lane * entry_pitch;
+    float* const amounts = stage + 64 * pitch;
+    uint8_t* const places = reinterpret_cast<uint8_t*>(amounts + 64 * entry_pitch);  // class, kNone or kOutside
+    const uint8_t* const place = places + lane * entry_pitch;
     float* const amount = amounts + lane * entry_pitch;  // logit, then exp((logit - top) / T)
     double total = 0.0;
     for (int64_t first = (int64_t)blockIdx.x * 64; first < a.rows; first += (int64_t)gridDim.x * 64) {
         const int rows = (int)min((int64_t)64, a.rows - first), n = rows * C;
         const T* const from = static_cast<const T*>(a.logits) + first * a.ld;
-        const int packets = a.whole ? n / kPer : 0;
+        const int packets = FLAT || a.whole ? n / kPer : 0;
         // All loads of the 64 rows before the first use: few waves fit a CU, so each keeps much in flight.
         vec v[kPackets];
 #pragma unroll
@@ -344,7 +349,7 @@ __global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int i = min((u0 + u) * 64 + lane, rows * k - 1), r = (int)((uint32_t)i * entry_magic >> 20), e = i - r * k;
-                places[r * entry_pitch + e] = ids[u] < 0 || logits[u] == -INFINITY ? -1 : ids[u] < C ? (int)ids[u] : -2;
+                places[r * entry_pitch + e] = ids[u] < 0 || logits[u] == -INFINITY ? kNone : ids[u] < C ? (uint8_t)ids[u] : kOutside;
                 amounts[r * entry_pitch + e] = logits[u];
             }
         }
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
         for (int u = 0; u < kPackets; ++u) {
             const int p = u * 64 + lane;
             if (u * 64 < packets && p < packets) {
-                if (pitch == C) {
+                if constexpr (FLAT) {
 #pragma unroll
                     for (int e = 0; e < kPer; ++e) stage[p * kPer + e] = (float)v[u][e];
                 } else {
@@ -379,14 +384,14 @@ __global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
         float top = -INFINITY;
         bool outside = false;
         for (int e = 0; e < k; ++e) {
-            outside |= place[e] == -2;
-            if (place[e] != -1) top = amount[e] != amount[e] ? INFINITY : fmaxf(top, amount[e]);
+            outside |= place[e] == kOutside;
+            if (place[e] != kNone) top = amount[e] != amount[e] ? INFINITY : fmaxf(top, amount[e]);
         }
         const bool soft = a.soft > 0.f && top != -INFINITY;
         float sum = outside ? NAN : 0.f, inner = 0.f;
         for (int e = 0; e < k; ++e) {
             const float t = amount[e];
-            const float w = place[e] >= 0 ? exp_of(t - top, c) : 0.f;
+            const float w = place[e] < C ? exp_of(t - top, c) : 0.f;
             sum += w;
             if (w != 0.f) inner = fmaf(w, (t - top) - (x[place[e]] - most), inner);
             amount[e] = w;
@@ -438,14 +443,14 @@ __global__ __launch_bounds__(64) void distill_lanes(const DistillArgs a) {
                 for (int j = 0; j < C; ++j) x[j] = 0.f;
             if (soft)
                 for (int e = 0; e < k; ++e)
-                    if (place[e] >= 0) x[place[e]] -= soft_up * (amount[e] * per_sum);
+                    if (place[e] < C) x[place[e]] -= soft_up * (amount[e] * per_sum);
             if (hard && inside) x[label] -= hard_up;
             __syncthreads();
             T* const to = static_cast<T*>(a.grad) + first * C;
 #pragma unroll 2
             for (int p = lane; p < packets; p += 64) {
                 vec out;
-                if (pitch == C) {
+                if constexpr (FLAT) {
 #pragma unroll
                     for (int e = 0; e < kPer; ++e) out[e] = (T)stage[p * kPer + e];
                 } else {
@@ -717,7 +722,7 @@ DistillArgs args_of(const ra_distill_shape& s, const void* logits, const void* t
 }
 
 bool by_lanes(const ra_distill_shape& s) { return s.classes <= kLaneClasses && s.kept <= kLaneKept && s.rows >= kLaneRows; }
-size_t lane_lds(const ra_distill_shape& s) { return (size_t)64 * ((s.classes | 1) + 2 * (s.kept | 1)) * 4; }
+size_t lane_lds(const ra_distill_shape& s) { return (size_t)64 * ((s.classes | 1) * 4 + (s.kept | 1) * 5); }
 int lane_blocks(const ra_distill_shape& s) { return static_cast<int>(std::min<int64_t>((s.rows + 63) / 64, kMaxBlocks)); }
 
 bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.kept <= 256; }
@@ -777,7 +782,9 @@ void run(const ra_distill_shape& s, DistillArgs& a, hipStream_t st) {
     a.whole = (s.rows <= 1 || s.ld_logits == s.classes) && aligned16(a.logits) && aligned16(a.grad);
     if (by_lanes(s)) {
         by_type(s.dtype, [&](auto t) {
-            distill_lanes<decltype(t)><<<lane_blocks(s), 64, lane_lds(s), st>>>(a);
+            using T = decltype(t);
+            if (a.whole && s.classes % 2) distill_lanes<T, true><<<lane_blocks(s), 64, lane_lds(s), st>>>(a);
+            else distill_lanes<T, false><<<lane_blocks(s), 64, lane_lds(s), st>>>(a);
         });
         return;
     }

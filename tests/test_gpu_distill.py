@@ -157,7 +157,7 @@ def test_rows(M, C):
 def test_many_rows_of_few_classes(C, dtype):
     """Row by row the same as a few rows at a time, to the tolerances of both: the first 150 and the last 83 rows against the
     definition, with every kind of row among them."""
-    M = 20_003
+    M = 40_003
     x, t, ids, labels = make(M, C, min(C, 5), dtype, seed=2)
     some = torch.cat([torch.arange(150), torch.arange(M - 83, M)])
     x[7, 0], x[9], ids[11, 0], labels[13], labels[15] = math.nan, -math.inf, C, C, -1
