@@ -5,15 +5,20 @@
 //     y = n w + b
 //     dx = r (w g - mean(w g) - n mean(w g n)) + grad_sum;  dw = sum g n,  db = sum g
 //
-// Bound by memory: every element is read once and written once (x and residual to y and
-// the sum forward, h and the gradients to dx backward).  A row lies in the registers of a
-// group of lanes, at most 16 elements a lane: of a part of a wave for short rows, of a
-// wave up to 1,024 elements, of a workgroup up to 16,384.  So the variance is summed
-// around the mean without reading again.  A lane's elements are K packets of 16 bytes, the
-// packets of a row side by side over the lanes, at whatever address the row begins; the last
-// packet of a row that is not made of whole ones ends with the row, and what it shares with
-// the one before is left out of the sums (TAIL) and written by both, the same bits.  Backward, groups go on to further rows with the sums
-// of dw and db in registers; a second launch adds the workgroups' sums in order.
+// Bound by memory: every element is read once and written once (x and residual to y and the sum
+// forward, h and the gradients to dx backward).  A row lies in the registers of a group of lanes,
+// so the variance is summed around the mean without reading again: of a part of a wave for short
+// rows, of a wave up to 1,024 elements (at most 16 a lane), of a workgroup up to 16,384 (8 a
+// lane, past 8,192 elements 16).  A lane's elements are K packets of 16 bytes, the packets of a
+// row side by side over the lanes, at whatever address the row begins; the last packet of a row
+// that is not made of whole ones ends with the row, and what it shares with the one before is
+// left out of the sums (TAIL) and written by both, the same bits.  Backward, groups go on to
+// further rows with the sums of dw and db in registers; a second launch adds the workgroups' sums
+// in order.
+//
+// Measured, forward, backward and the last sum: 1e6 x 256 in bf16 with a residual 398 us (5.2 TB/s), 406
+// (5.0) and 6; 4,096 x 8,192 in fp32 with a residual 91 (5.9: the inputs of a repeated pass are partly
+// cached), 117 (4.6) and 8; 150,000 x 147 in fp16 26 (3.4), 37 (3.6) and 5.  A large copy: 4.75 TB/s.
 #include <algorithm>
 #include <type_traits>
 

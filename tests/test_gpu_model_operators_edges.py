@@ -1,0 +1,129 @@
+"""Calls of embedding lookup, layer norm and distillation that a program may make beside the ordinary ones: tensors at odd
+addresses, two streams at once, long lists of entries with the same classes, one wide row."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import ra_spmm  # noqa: E402
+from test_gpu_distill import check as check_distill  # noqa: E402
+from test_gpu_distill import make as make_distill  # noqa: E402
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def odd(t, by):
+    """t's values `by` elements past the beginning of an allocation."""
+    wide = torch.zeros(t.numel() + by + 3, dtype=t.dtype, device=t.device)
+    out = wide[by:by + t.numel()].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("by", [1, 2, 4])
+@pytest.mark.parametrize("D", [5, 16, 47, 256, 1100])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_addresses_do_not_change_the_bits(D, dtype, by):
+    gen = torch.Generator("cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dtype)  # noqa: E731
+    x, res, gy, gh = r(37, D), r(37, D), r(37, D), r(37, D)
+    w, b = r(D).float(), r(D).float()
+    ids = torch.randint(-1, 37, (300,), generator=gen, device="cuda")
+    g = r(300, D)
+    results = []
+    for put in (lambda t: t.clone(), lambda t: odd(t, by)):
+        leaves = [put(t).detach().requires_grad_(True) for t in (x, res, w, b)]
+        out = ra_spmm.layer_norm(leaves[0], leaves[2], leaves[3], residual=leaves[1])
+        grads = torch.autograd.grad(out, leaves, (put(gy), put(gh)))
+        table = put(x).detach().requires_grad_(True)
+        rows = ra_spmm.embed(put(ids), table, 1.5, padding=-1)
+        results.append([t.detach() for t in (*out, *grads, rows, *torch.autograd.grad(rows, table, put(g)))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("by", [1, 2, 4])
+@pytest.mark.parametrize("C", [7, 47, 300, 1500, 20_000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_logits_at_odd_addresses(C, dtype, by):
+    x, t, ids, labels = make_distill(9, C, 5, dtype)
+    check_distill(x, t, ids, labels, T=2.0, hard=0.3, put=lambda v: odd(v.cuda(), by))
+
+
+@pytest.mark.parametrize("k", [17, 256, 300, 1024])
+@pytest.mark.parametrize("C", [1, 5, 700, 3000])
+def test_many_entries_of_few_classes(C, k):
+    """Every class several times, some entries missing."""
+    gen = torch.Generator().manual_seed(k)
+    x, t = torch.randn(5, C, generator=gen), torch.randn(5, k, generator=gen)
+    ids = torch.randint(-2, C, (5, k), generator=gen)
+    check_distill(x, t, ids, torch.randint(-1, C, (5,), generator=gen), T=2.0, hard=0.4)
+
+
+def test_two_streams_at_once():
+    gen = torch.Generator("cuda").manual_seed(3)
+    data = []
+    for i in range(2):
+        x = torch.randn(4000, 300, generator=gen, device="cuda")
+        t, top = torch.randn(4000, 300, generator=gen, device="cuda").topk(6, dim=1)
+        data.append((x, torch.randint(0, 4000, (20_000,), generator=gen, device="cuda"),
+                     torch.randn(20_000, 300, generator=gen, device="cuda"), t, top))
+
+    def work(x, ids, g, t, top):
+        table = x.detach().requires_grad_(True)
+        rows = ra_spmm.embed(ids, table)
+        y, h = ra_spmm.layer_norm(table, residual=x)
+        loss, dx = ra_spmm.distill_loss_grad(y.detach(), t, top, 2.0)
+        return [loss, dx, rows.detach(), *torch.autograd.grad((rows, y, h), table, (g, dx, x))]
+
+    want = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = []
+    for _ in range(5):
+        got = []
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(work(*d))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_one_wide_row(dtype):
+    """n of a row of +-1 is the row, its gradient g - mean(g) - n mean(g n)."""
+    D = 16_384
+    x = torch.ones(1, D, device="cuda", dtype=dtype)
+    x[0, ::2] = -1
+    x.requires_grad_(True)
+    y = ra_spmm.layer_norm(x, eps=0.0)
+    assert torch.equal(y, x)
+    g = torch.zeros(1, D, device="cuda", dtype=dtype)
+    g[0, 3] = 1
+    dx, = torch.autograd.grad(y, x, g)
+    assert float(dx[0, 3]) == pytest.approx(1 - 2 / D, rel=2.0 ** -8) and abs(float(dx[0, 2])) < 2.0 ** -20
+    assert float(dx[0, 5]) == pytest.approx(-2 / D, rel=2.0 ** -7)
+
+
+def test_a_table_of_one_row_and_one_position():
+    table = torch.randn(1, 1, device="cuda", requires_grad=True)
+    out = ra_spmm.embed(torch.zeros(1, dtype=torch.int32, device="cuda"), table, -2.0)
+    assert float(out) == -2.0 * float(table)
+    assert float(torch.autograd.grad(out, table, torch.full((1, 1), 3.0, device="cuda"))[0]) == -6.0
+
+
+def test_a_gradient_that_is_scaled_before_it_is_rounded():
+    """A mean over many rows in fp16: with a loss scale all bits are there; without one 1 / (70,000 * 40) = 5.99 * 2^-24 is 6 of the
+    smallest steps, of which fp16 has no part."""
+    M, C = 70_000, 40
+    x = torch.zeros(M, C, device="cuda", dtype=torch.float16)
+    t, ids = torch.ones(M, 1, device="cuda"), torch.zeros(M, 1, dtype=torch.int64, device="cuda")
+    for factor in (65536.0, torch.tensor(65536.0, device="cuda")):
+        _, g = ra_spmm.distill_loss_grad(x, t, ids, factor=factor)
+        assert math.isclose(float(g[5, 3]), 65536 / (M * C), rel_tol=2.0 ** -9)
+    leaf = x.requires_grad_(True)
+    (65536.0 * ra_spmm.distill_loss(leaf, t, ids)).backward()
+    assert torch.equal(leaf.grad, g)
+    assert (ra_spmm.distill_loss_grad(x.detach(), t, ids)[1][:, 1:] == 6 * 2.0 ** -24).all()
