@@ -47,6 +47,7 @@ constexpr int kStageBytes = 16384;     // rows of a workgroup at once, about
 // A gradient past the last-level cache (256 MB) is written around the caches, which hold the row
 // that is read again: 224 us, 211 (2,048 x 100,003 bf16).
 constexpr int64_t kAroundBytes = int64_t(256) << 20;
+constexpr int kAhead = 4;  // packets of a lane at once
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DistillArgs {
@@ -204,8 +205,13 @@ __device__ __forceinline__ float class_amount(const Targets& t, int kept, int e,
 // through LDS: whole 16-byte packets whatever the number of classes is, where rows of 47
 // elements would be read by single ones.  A row is held by 2^lanes_shift lanes, K elements
 // each; its gradient takes its place in LDS and goes out the same way.
-template <typename T, int K>
-__global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
+// SHIFT: lanes_shift, or -1 where it is only known at run time; HARD: labels count.  Both are
+// constants because the choices they leave would stand at every element and every sum.
+template <typename T, int K, int SHIFT, bool HARD>
+__global__ __launch_bounds__(kThreads, 4) void distill_short(const DistillArgs args) {
+    DistillArgs a = args;
+    if constexpr (SHIFT >= 0) a.lanes_shift = SHIFT;
+    if constexpr (!HARD) a.hard = 0.f;
     extern __shared__ __align__(16) char lds[];
     __shared__ double part64[kThreads / 64];
     constexpr int kPer = 16 / sizeof(T);
@@ -222,15 +228,31 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
     uint16_t* const owner = reinterpret_cast<uint16_t*>(arrays + 4 * groups * entries) + group * C;
     const float c = kLog2e * a.inv_t;
     // A lane's classes; groups begin at different ones, which keeps rows of 64 classes apart in LDS.
-    auto place_of = [&](int k) { return ((k + group) & (K - 1)) * lanes + (int)team.lane; };
+    // What is past the row is read at class 0 and written past the stage.
+    int at[K];
+    bool inside[K];
+    T* const past = reinterpret_cast<T*>(owner - group * C + groups * C);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        at[k] = ((k + group) & (K - 1)) * lanes + (int)team.lane;
+        inside[k] = at[k] < C;
+        at[k] = inside[k] ? at[k] : 0;
+    }
     double total = 0.0;
     for (int64_t first = (int64_t)blockIdx.x * a.stage_rows; first < a.rows; first += (int64_t)gridDim.x * a.stage_rows) {
         const int rows = (int)min((int64_t)a.stage_rows, a.rows - first), n = rows * C;
         const T* const from = static_cast<const T*>(a.logits) + first * a.ld;
+        const int packets = a.whole ? n / kPer : 0;
+        for (int p0 = threadIdx.x; p0 < packets; p0 += kAhead * kThreads) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) v[u] = reinterpret_cast<const uint4*>(from)[min(p0 + u * kThreads, packets - 1)];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (p0 + u * kThreads < packets) reinterpret_cast<uint4*>(stage)[p0 + u * kThreads] = v[u];
+        }
         if (a.whole) {
-            for (int i = threadIdx.x * kPer; i + kPer <= n; i += kThreads * kPer)
-                *reinterpret_cast<uint4*>(stage + i) = *reinterpret_cast<const uint4*>(from + i);
-            const int i = n / kPer * kPer + (int)threadIdx.x;
+            const int i = packets * kPer + (int)threadIdx.x;
             if (i < n) stage[i] = from[i];
         } else {
             for (int r = threadIdx.x >> 6; r < rows; r += kThreads / 64)
@@ -247,22 +269,21 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
             float v[K], most = -FLT_MAX, at_t = 0.f, at_1 = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int j = place_of(k);
-                v[k] = j < C ? (float)x[j] : -INFINITY;
+                const float value_at = (float)x[at[k]];
+                v[k] = inside[k] ? value_at : -INFINITY;
                 most = fmaxf(most, v[k]);
             }
             most = team.template all<Max>(most);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 v[k] -= most;
-                at_t += exp_of(v[k], c);
+                const float e = exp_of(v[k], c);
+                at_t += e;
+                if constexpr (HARD) at_1 += exp_of(v[k], kLog2e);
+                else v[k] = e;  // stays for the gradient
             }
             at_t = team.sum(at_t);
-            if (a.hard > 0.f) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) at_1 += exp_of(v[k], kLog2e);
-                at_1 = team.sum(at_1);
-            }
+            if constexpr (HARD) at_1 = team.sum(at_1);
             if (a.loss || a.part) {
                 const float loss = row_loss(a, team, t, most, at_t, at_1, logit);
                 if (there && team.lane == 0) {
@@ -290,10 +311,11 @@ __global__ __launch_bounds__(kThreads) void distill_short(const DistillArgs a) {
             }
             team.sync();
             if (there) {
+                const bool live = t.soft || t.hard;  // else 0 whatever the logits are
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    const int j = place_of(k);
-                    if (j < C) x[j] = (T)f(a, v[k]);
+                    const float g = HARD ? fmaf(f.hard, exp_of(v[k], kLog2e), f.soft * exp_of(v[k], c)) : f.soft * v[k];
+                    *(inside[k] ? x + at[k] : past) = (T)(live ? g : 0.f);
                 }
             }
             team.sync();
@@ -497,8 +519,6 @@ __global__ __launch_bounds__(64, FLAT ? 3 : 2) void distill_lanes(const DistillA
 }
 
 // ------------------------------------------------------------------- long rows
-constexpr int kAhead = 4;  // packets of a lane at once
-
 // 16 bytes of a row; elements past the packets, at both ends, are taken one by one.
 template <typename T>
 struct Span {
@@ -767,6 +787,7 @@ ShortPlan short_plan(const ra_distill_shape& s) {
     const int size = s.dtype == RA_DTYPE_F32 ? 4 : 2, entries = s.kept + 1;
     ShortPlan p{};
     p.k = s.classes <= 256 && (s.classes <= 32 || s.rows * s.classes < 16 * 256 * kThreads) ? 4 : 16;
+    if (p.k == 16) p.shift = 3;  // 8 lanes at least: kernels of their own for each number
     while ((p.k << p.shift) < s.classes || (kThreads >> p.shift) * entries * 16 > 4 * 257 * 16) ++p.shift;
     // Few rows: more lanes for each, and fewer rows a workgroup, so that all CUs have some.
     while (p.shift < 6 && (s.rows << p.shift) < 256 * kThreads && (1 << p.shift) < s.classes) ++p.shift;
@@ -774,7 +795,8 @@ ShortPlan short_plan(const ra_distill_shape& s) {
     p.rows = std::max(groups, 8);  // 8 rows are whole packets
     while (2 * p.rows * s.classes * size <= kStageBytes && s.rows / (2 * p.rows) >= 1024) p.rows *= 2;
     p.blocks = static_cast<int>(std::min<int64_t>((s.rows + p.rows - 1) / p.rows, kMaxBlocks));
-    p.lds = (size_t)(p.rows * s.classes * size + 15) / 16 * 16 + (size_t)groups * entries * 16 + (size_t)groups * s.classes * 2;
+    p.lds = (size_t)(p.rows * s.classes * size + 15) / 16 * 16 + (size_t)groups * entries * 16 +
+            ((size_t)groups * s.classes * 2 + 3) / 4 * 4 + 4;
     return p;
 }
 
@@ -807,6 +829,9 @@ int loss_parts(const ra_distill_shape& s, bool grad) {
     return is_short(s) ? short_plan(s).blocks : long_blocks(s, grad ? long_plan(s).pieces : 1);
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 template <typename F>
 void by_type(int32_t dtype, F f) {
     if (dtype == RA_DTYPE_F32) f(float());
@@ -830,8 +855,15 @@ void run(const ra_distill_shape& s, DistillArgs& a, hipStream_t st) {
         a.lanes_shift = p.shift;
         by_type(s.dtype, [&](auto t) {
             using T = decltype(t);
-            if (p.k == 4) distill_short<T, 4><<<p.blocks, kThreads, p.lds, st>>>(a);
-            else distill_short<T, 16><<<p.blocks, kThreads, p.lds, st>>>(a);
+            auto go = [&](auto k, auto shift) {
+                if (s.hard > 0.f) distill_short<T, k.value, shift.value, true><<<p.blocks, kThreads, p.lds, st>>>(a);
+                else distill_short<T, k.value, shift.value, false><<<p.blocks, kThreads, p.lds, st>>>(a);
+            };
+            if (p.k == 4) go(Int<4>(), Int<-1>());
+            else if (p.shift == 3) go(Int<16>(), Int<3>());
+            else if (p.shift == 4) go(Int<16>(), Int<4>());
+            else if (p.shift == 5) go(Int<16>(), Int<5>());
+            else go(Int<16>(), Int<6>());
         });
         return;
     }
