@@ -49,6 +49,7 @@ constexpr int kPiece = 4096;      // pairs of a workgroup in the sort,
 constexpr int kMaxPieces = 512;   // more where there would be over this many of them,
 constexpr int kMostPiece = 32768; // up to as many: more pieces then
 constexpr int kMoveThreads = 512;
+constexpr int kCountThreads = 1024;
 // Positions that are sorted by counting, which is one launch but takes n^2 comparisons.  The
 // gradient of 1,025 positions on 200,000 rows 12.6 us (by digits 39), of 8,192 20 (50); on 2,000
 // rows, one digit, 12.4 (26) and 21 (34).
@@ -140,17 +141,24 @@ __device__ __forceinline__ uint2 pair_at(const SortArgs& a, int i) {
     return a.from ? a.from[i] : make_uint2(key_at(a.e, i), (uint32_t)i);
 }
 
-__global__ __launch_bounds__(kThreads) void sort_count(const SortArgs a) {
+__global__ __launch_bounds__(kCountThreads) void sort_count(const SortArgs a) {
     extern __shared__ uint32_t counts[];
-    for (int d = threadIdx.x; d < a.digits; d += kThreads) counts[d] = 0;
+    for (int d = threadIdx.x; d < a.digits; d += kCountThreads) counts[d] = 0;
     __syncthreads();
     const int first = blockIdx.x * a.piece, end = min(a.count, first + a.piece);
-    for (int i = first + threadIdx.x; i < end; i += kThreads) {
-        const uint32_t key = a.from ? a.from[i].x : key_at(a.e, i);
-        atomicAdd(&counts[(key >> a.shift) & (a.digits - 1)], 1u);
+    for (int i0 = first + threadIdx.x; i0 < end; i0 += 4 * kCountThreads) {
+        uint32_t key[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + u * kCountThreads, end - 1);
+            key[u] = a.from ? a.from[i].x : key_at(a.e, i);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * kCountThreads < end) atomicAdd(&counts[(key[u] >> a.shift) & (a.digits - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < a.digits; d += kThreads) a.counts[(int64_t)d * a.pieces + blockIdx.x] = counts[d];
+    for (int d = threadIdx.x; d < a.digits; d += kCountThreads) a.counts[(int64_t)d * a.pieces + blockIdx.x] = counts[d];
 }
 
 // A wave per digit: the pieces' counts to their sums before each piece.
@@ -173,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void sort_offsets(const SortArgs a) {
 }
 
 __global__ __launch_bounds__(kMoveThreads) void sort_move(const SortArgs a) {
-    constexpr int kMoveWaves = kMoveThreads / 64;
+    constexpr int kMoveWaves = kMoveThreads / 64, kRounds = kPiece / kMoveThreads;
     extern __shared__ uint32_t lds[];  // [digits] first places, [waves] sums, then [waves][digits] places past them, 16 bits each
     uint32_t* const start = lds;
     uint32_t* const wave_sums = lds + a.digits;
@@ -199,9 +207,18 @@ __global__ __launch_bounds__(kMoveThreads) void sort_move(const SortArgs a) {
     }
     // Every wave takes its part of the piece, in order.
     const int part = a.piece / kMoveWaves, first = blockIdx.x * a.piece + wave * part, end = min(a.count, first + part);
-    for (int i = first + lane; i < end; i += 64) {
-        const uint32_t digit = (pair_at(a, i).x >> a.shift) & (a.digits - 1);
-        atomicAdd(&counts[digit / 2], digit & 1 ? 0x10000u : 1u);
+    uint2 pair[kRounds];  // of kRounds rounds of the wave, loaded at once; most pieces have no more
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) pair[r] = pair_at(a, min(i0 + r * 64 + lane, a.count - 1));
+    };
+    for (int i0 = first; i0 < end; i0 += 64 * kRounds) {
+        load(i0);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const uint32_t digit = (pair[r].x >> a.shift) & (a.digits - 1);
+            if (i0 + r * 64 + lane < end) atomicAdd(&counts[digit / 2], digit & 1 ? 0x10000u : 1u);
+        }
     }
     __syncthreads();
     // Counts to places: those of the waves before.  A piece holds fewer than 2^16 pairs.
@@ -216,23 +233,25 @@ __global__ __launch_bounds__(kMoveThreads) void sort_move(const SortArgs a) {
     }
     __syncthreads();
     volatile uint16_t* const place = reinterpret_cast<volatile uint16_t*>(counts);
-    for (int i0 = first; i0 < end; i0 += 64) {
-        const int i = i0 + lane;
-        const bool there = i < end;
-        const uint2 pair = there ? pair_at(a, i) : make_uint2(0, 0);
-        const uint32_t digit = (pair.x >> a.shift) & (a.digits - 1);
-        uint64_t same = __ballot(there);  // the lanes with this lane's digit
-        for (uint32_t bit = 1; bit < (uint32_t)a.digits; bit <<= 1) {
-            const uint64_t set = __ballot(there && (digit & bit));
-            same &= digit & bit ? set : ~set;
-        }
-        const int before_me = __popcll(same & ((uint64_t(1) << lane) - 1));
-        if (there) {
-            const uint32_t at = place[digit];
-            __builtin_amdgcn_wave_barrier();
-            if (before_me == 0) place[digit] = (uint16_t)(at + __popcll(same));
-            __builtin_amdgcn_wave_barrier();
-            a.to[start[digit] + at + before_me] = pair;
+    for (int i0 = first; i0 < end; i0 += 64 * kRounds) {
+        if (part > 64 * kRounds) load(i0);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const bool there = i0 + r * 64 + lane < end;
+            const uint32_t digit = (pair[r].x >> a.shift) & (a.digits - 1);
+            uint64_t same = __ballot(there);  // the lanes with this lane's digit
+            for (uint32_t bit = 1; bit < (uint32_t)a.digits; bit <<= 1) {
+                const uint64_t set = __ballot(there && (digit & bit));
+                same &= digit & bit ? set : ~set;
+            }
+            const int before_me = __popcll(same & ((uint64_t(1) << lane) - 1));
+            if (there) {
+                const uint32_t at = place[digit];
+                __builtin_amdgcn_wave_barrier();
+                if (before_me == 0) place[digit] = (uint16_t)(at + __popcll(same));
+                __builtin_amdgcn_wave_barrier();
+                a.to[start[digit] + at + before_me] = pair[r];
+            }
         }
     }
 }
@@ -551,7 +570,7 @@ const uint2* sort(const EmbedArgs& e, const SortPlan& p, char* work, hipStream_t
     for (int pass = 0; pass < p.passes; ++pass) {
         a.to = half[pass & 1];
         a.shift = pass * p.digit_bits;
-        sort_count<<<p.pieces, kThreads, a.digits * 4, st>>>(a);
+        sort_count<<<p.pieces, kCountThreads, a.digits * 4, st>>>(a);
         sort_offsets<<<(a.digits + kWaves - 1) / kWaves, kThreads, 0, st>>>(a);
         sort_move<<<p.pieces, kMoveThreads, a.digits * 4 + kMoveThreads / 64 * (4 + a.digits * 2), st>>>(a);
         a.from = a.to;
