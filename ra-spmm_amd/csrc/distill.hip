@@ -19,9 +19,10 @@
 // exponentials together (scaled down where the maximum grows), once for the gradient, out of the
 // caches.
 //
-// Measured: 2,048 x 100,003 in bf16, loss and gradient in one call, 209 us (0.82 GB, 3.9 TB/s; 126 us of it
-// is the vector unit's time); 1e6 x 47 in fp32, loss and gradient 107 us each (44 us of it the vector
-// unit's); 16 x 50,000 in fp16 5 us for the pieces, 9 for the loss and 9 for the gradient.
+// Measured: 2,048 x 100,003 in bf16, loss and gradient in one call, 208 us (0.82 GB, 3.9 TB/s; 126 us of it
+// is the vector unit's time); 50,000 x 2,000 122 us (3.3 TB/s), 1e6 x 100 205 (2.0); 1e6 x 47 in fp32, loss
+// and gradient 93 us each (44 us of it the vector unit's); 16 x 50,000 in fp16 5 us for the pieces, 9 for
+// the loss and 9 for the gradient.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -777,8 +778,10 @@ int lane_blocks(const ra_distill_shape& s) { return static_cast<int>(std::min<in
 
 bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.kept <= 256; }
 
-// Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements
-// (16 past 256 classes), more lanes where the entries of all groups would pass 16 kB.
+// Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements, and 16
+// past 256 classes, or past 32 where rows are enough to fill the machine with a quarter of the
+// lanes: what is done once a row is done by fewer (1e6 x 100 bf16 436 us with 4, 257 with 16).
+// More lanes where the entries of all groups would pass 16 kB.
 struct ShortPlan {
     int k, shift, rows, blocks;
     size_t lds;

@@ -11,7 +11,7 @@
 // The sort goes by digits of up to 11 bits, lowest first, three launches a digit: counts of every
 // workgroup's piece, their running sums for every digit, and the move, in which lanes of a wave
 // with one digit find their order by ballots.  Up to 8,192 positions, one launch counts for each
-// how many come before it (8,192: 11.6 us; the digits' six launches take 73 at 1e6).
+// how many come before it (8,192: 11.6 us; the digits' six launches take 55 at 1e6).
 //
 // The sum takes equal runs of sorted positions, not of table rows, so that a row with most of the
 // positions costs no more than others: a group of lanes adds its run's gradients and writes each
@@ -19,9 +19,9 @@
 // workgroups by a second launch.  Table rows without positions are written by further workgroups
 // of the first.
 //
-// Measured, lookup and gradient on the GPU: 1e6 positions on 1e6 rows of 256 in bf16 173 us (5.9 TB/s)
-// and 222 (4.6 TB/s), the sort 73 and the join 9; 1e6 positions on 61 rows of 100 in fp16 43 and 57 (the
-// gathers of 200 bytes take lines of 128: 5 TB/s of lines), 25 and 9; 8,192 positions on 200,000
+// Measured, lookup and gradient on the GPU: 1e6 positions on 1e6 rows of 256 in bf16 171 us (6.0 TB/s)
+// and 221 (4.6 TB/s), the sort 55 and the join 9; 1e6 positions on 61 rows of 100 in fp16 44 and 58 (the
+// gathers of 200 bytes take lines of 128: 5 TB/s of lines), 20 and 9; 8,192 positions on 200,000
 // rows of 128 in fp32 4 and 20 (5.3 TB/s), 12 and 5.
 #include <algorithm>
 #include <type_traits>
