@@ -20,7 +20,7 @@
 // caches.
 //
 // Measured: 2,048 x 100,003 in bf16, loss and gradient in one call, 208 us (0.82 GB, 3.9 TB/s; 126 us of it
-// is the vector unit's time); 50,000 x 2,000 122 us (3.3 TB/s), 1e6 x 100 205 (2.0); 1e6 x 47 in fp32, loss
+// is the vector unit's time); 50,000 x 2,000 122 us (3.3 TB/s), 1e6 x 100 198 (2.0); 1e6 x 47 in fp32, loss
 // and gradient 93 us each (44 us of it the vector unit's); 16 x 50,000 in fp16 5 us for the pieces, 9 for
 // the loss and 9 for the gradient.
 #include <algorithm>
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads, 4) void distill_short(const DistillArgs a
     T* const past = reinterpret_cast<T*>(owner - group * C + groups * C);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        at[k] = ((k + group) & (K - 1)) * lanes + (int)team.lane;
+        at[k] = (k + group) % K * lanes + (int)team.lane;
         inside[k] = at[k] < C;
         at[k] = inside[k] ? at[k] : 0;
     }
@@ -780,8 +780,10 @@ bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.ke
 
 // Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements, and 16
 // past 256 classes, or past 32 where rows are enough to fill the machine with a quarter of the
-// lanes: what is done once a row is done by fewer (1e6 x 100 bf16 436 us with 4, 257 with 16).
-// More lanes where the entries of all groups would pass 16 kB.
+// lanes: what is done once a row is done by fewer (1e6 x 100 bf16 436 us with 4, 257 with 16);
+// 8, 10 or 13 where the same lanes hold the row so (with 16 alone, 200 MB of logits in bf16:
+// 1.54e6 x 65 212 us, 267, 1.25e6 x 80 182, 229, 333,333 x 300 181, 226, 156,250 x 640 176, 219;
+// fp32 500,000 x 100 123, 144).  More lanes where the entries of all groups would pass 16 kB.
 struct ShortPlan {
     int k, shift, rows, blocks;
     size_t lds;
@@ -794,6 +796,9 @@ ShortPlan short_plan(const ra_distill_shape& s) {
     while ((p.k << p.shift) < s.classes || (kThreads >> p.shift) * entries * 16 > 4 * 257 * 16) ++p.shift;
     // Few rows: more lanes for each, and fewer rows a workgroup, so that all CUs have some.
     while (p.shift < 6 && (s.rows << p.shift) < 256 * kThreads && (1 << p.shift) < s.classes) ++p.shift;
+    if (p.k == 16)
+        for (int k : {13, 10, 8})
+            if ((k << p.shift) >= s.classes) p.k = k;
     const int groups = kThreads >> p.shift;
     p.rows = std::max(groups, 8);  // 8 rows are whole packets
     while (2 * p.rows * s.classes * size <= kStageBytes && s.rows / (2 * p.rows) >= 1024) p.rows *= 2;
@@ -862,11 +867,17 @@ void run(const ra_distill_shape& s, DistillArgs& a, hipStream_t st) {
                 if (s.hard > 0.f) distill_short<T, k.value, shift.value, true><<<p.blocks, kThreads, p.lds, st>>>(a);
                 else distill_short<T, k.value, shift.value, false><<<p.blocks, kThreads, p.lds, st>>>(a);
             };
+            auto by_shift = [&](auto k) {
+                if (p.shift == 3) go(k, Int<3>());
+                else if (p.shift == 4) go(k, Int<4>());
+                else if (p.shift == 5) go(k, Int<5>());
+                else go(k, Int<6>());
+            };
             if (p.k == 4) go(Int<4>(), Int<-1>());
-            else if (p.shift == 3) go(Int<16>(), Int<3>());
-            else if (p.shift == 4) go(Int<16>(), Int<4>());
-            else if (p.shift == 5) go(Int<16>(), Int<5>());
-            else go(Int<16>(), Int<6>());
+            else if (p.k == 8) by_shift(Int<8>());
+            else if (p.k == 10) by_shift(Int<10>());
+            else if (p.k == 13) by_shift(Int<13>());
+            else by_shift(Int<16>());
         });
         return;
     }

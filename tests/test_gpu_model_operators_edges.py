@@ -9,6 +9,8 @@ pytestmark = pytest.mark.gpu
 
 import ra_spmm  # noqa: E402
 from test_gpu_distill import check as check_distill  # noqa: E402
+from test_gpu_distill import close  # noqa: E402
+from test_gpu_distill import exact as exact_distill  # noqa: E402
 from test_gpu_distill import make as make_distill  # noqa: E402
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -49,6 +51,27 @@ def test_addresses_do_not_change_the_bits(D, dtype, by):
 def test_logits_at_odd_addresses(C, dtype, by):
     x, t, ids, labels = make_distill(9, C, 5, dtype)
     check_distill(x, t, ids, labels, T=2.0, hard=0.3, put=lambda v: odd(v.cuda(), by))
+
+
+@pytest.mark.parametrize("C", [33, 64, 65, 80, 81, 104, 105, 128, 129, 160, 208, 209, 256, 257, 320, 321, 416, 417, 512, 513, 640,
+                               641, 832, 833, 1024])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_lengths_of_many_rows(C, dtype):
+    """Row lengths at which the lanes of a row and the classes of a lane change, with rows enough for as few lanes as there
+    can be; the first, middle and last rows against the definition."""
+    M = 2 ** 20 // C + 77
+    x, t, ids, labels = make_distill(M, C, 20, dtype, seed=C)
+    some = torch.cat([torch.arange(20), torch.arange(M // 2, M // 2 + 8), torch.arange(M - 12, M)])
+    x[3, C - 1], x[5] = math.nan, -math.inf
+    ids[7], labels[7], x[7, 0] = -1, -1, math.nan
+    up = torch.randn(M, generator=torch.Generator().manual_seed(5))
+    for hard in (0.0, 0.4):
+        want, werr, grad, gerr = exact_distill(x[some], t[some], ids[some], 2.0, labels[some], hard, up[some].double())
+        leaf = x.cuda().requires_grad_(True)
+        loss = ra_spmm.distill_loss(leaf, t.cuda(), ids.cuda(), 2.0, labels.cuda(), hard, "none")
+        g, = torch.autograd.grad(loss, leaf, up.cuda())
+        close(loss[some.cuda()], want, werr, "loss of the rows")
+        close(g[some.cuda()], grad, gerr, "gradient of the rows")
 
 
 @pytest.mark.parametrize("k", [17, 256, 300, 1024])
