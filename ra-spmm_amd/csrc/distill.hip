@@ -20,7 +20,7 @@
 // caches.
 //
 // Measured: 2,048 x 100,003 in bf16, loss and gradient in one call, 208 us (0.82 GB, 3.9 TB/s; 126 us of it
-// is the vector unit's time); 50,000 x 2,000 122 us (3.3 TB/s), 1e6 x 100 198 (2.0); 1e6 x 47 in fp32, loss
+// is the vector unit's time); 50,000 x 2,000 122 us (3.3 TB/s), 1e6 x 100 188 (2.1); 1e6 x 47 in fp32, loss
 // and gradient 93 us each (44 us of it the vector unit's); 16 x 50,000 in fp16 5 us for the pieces, 9 for
 // the loss and 9 for the gradient.
 #include <algorithm>
@@ -172,13 +172,15 @@ struct Factors {
         return g;
     }
 };
+// The entries that there are: without `hard` labels are none.
+__device__ __forceinline__ int entries_of(const DistillArgs& a) { return a.kept + (a.hard > 0.f); }
 template <typename Team>
 __device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t row, Team& team, const Targets& t, float at_t,
                                                  float at_1) {
     const float up = (a.up ? a.up[row * a.up_step] : 1.f) * a.up_scale;
     const float soft_up = !t.soft ? 0.f : t.sum != t.sum ? NAN : a.soft_grad * up;
     const float hard_up = !t.hard ? 0.f : t.label < a.classes ? a.hard * up : NAN;
-    for (int e = team.lane; e <= a.kept; e += team.lanes) {
+    for (int e = team.lane; e < entries_of(a); e += team.lanes) {
         if (e < a.kept) {
             t.amount[e] = t.soft && t.place[e] >= 0 ? soft_up * (exp_of(t.amount[e] - t.top, kLog2e * a.inv_t) / t.sum) : 0.f;
             if (!t.soft) t.place[e] = -1;
@@ -189,11 +191,11 @@ __device__ __forceinline__ Factors entry_amounts(const DistillArgs& a, int64_t r
     }
     return {t.soft ? soft_up / at_t : 0.f, t.hard ? hard_up / at_1 : 0.f};
 }
-// What all entries of e's class take off; `first`: no earlier entry has it.
-__device__ __forceinline__ float class_amount(const Targets& t, int kept, int e, bool& first) {
+// What all of the first n entries of e's class take off; `first`: no earlier entry has it.
+__device__ __forceinline__ float class_amount(const Targets& t, int n, int e, bool& first) {
     float off = 0.f;
     first = true;
-    for (int f = 0; f <= kept; ++f) {
+    for (int f = 0; f < n; ++f) {
         if (t.place[f] != t.place[e]) continue;
         first &= f >= e;
         off += t.amount[f];
@@ -208,8 +210,10 @@ __device__ __forceinline__ float class_amount(const Targets& t, int kept, int e,
 // each; its gradient takes its place in LDS and goes out the same way.
 // SHIFT: lanes_shift, or -1 where it is only known at run time; HARD: labels count.  Both are
 // constants because the choices they leave would stand at every element and every sum.
+// Up to 10 classes a lane five workgroups fit a CU, in 16 bits with up to ten registers spilled
+// (769,230 x 65 in fp32 with labels 169 us, with four workgroups 195; in bf16 twice as many 279, 298).
 template <typename T, int K, int SHIFT, bool HARD>
-__global__ __launch_bounds__(kThreads, 4) void distill_short(const DistillArgs args) {
+__global__ __launch_bounds__(kThreads, K <= 10 ? 5 : 4) void distill_short(const DistillArgs args) {
     DistillArgs a = args;
     if constexpr (SHIFT >= 0) a.lanes_shift = SHIFT;
     if constexpr (!HARD) a.hard = 0.f;
@@ -295,18 +299,30 @@ __global__ __launch_bounds__(kThreads, 4) void distill_short(const DistillArgs a
             if (!a.grad) continue;
             const Factors f = entry_amounts(a, row, team, t, at_t, at_1);
             team.sync();
-            // Whether a class has several entries: one of them is not its owner then.
-            for (int e = team.lane; e < entries; e += lanes)
+            // Whether a class has several entries: one of them is not its owner then.  The label is
+            // often one of the teacher's classes: an entry of its class takes it along (1e6 x 100 in bf16
+            // 227 us, 267 where that counted as twice); else it is an entry of its own.
+            const int32_t label = HARD ? t.place[a.kept] : -1;
+            if (HARD) {
+                if (label >= 0) owner[label] = (uint16_t)a.kept;
+                team.sync();
+            }
+            for (int e = team.lane; e < a.kept; e += lanes)
                 if (t.place[e] >= 0) owner[t.place[e]] = (uint16_t)e;
             team.sync();
             bool twice = false;
-            for (int e = team.lane; e < entries; e += lanes) twice |= t.place[e] >= 0 && owner[t.place[e]] != e;
+            for (int e = team.lane; e < a.kept; e += lanes) twice |= t.place[e] >= 0 && owner[t.place[e]] != e;
             const bool any_twice = __any(twice);
-            for (int e = team.lane; e < entries; e += lanes) {
+            for (int e = team.lane; e < a.kept + HARD; e += lanes) {
                 const int32_t j = t.place[e];
                 bool first_of = true;
                 float off = t.amount[e];
-                if (any_twice && j >= 0) off = class_amount(t, a.kept, e, first_of);
+                if (HARD && e == a.kept) {
+                    first_of = j >= 0 && owner[j] == e;
+                } else {
+                    if (any_twice && j >= 0) off = class_amount(t, a.kept, e, first_of);
+                    if (HARD && j == label) off += t.amount[a.kept];
+                }
                 value[e] = j >= 0 ? f(a, logit(j) - most) - off : 0.f;
                 to[e] = first_of && there ? j : -1;
             }
@@ -320,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 4) void distill_short(const DistillArgs a
                 }
             }
             team.sync();
-            for (int e = team.lane; e < entries; e += lanes)
+            for (int e = team.lane; e < a.kept + HARD; e += lanes)
                 if (to[e] >= 0) x[to[e]] = (T)value[e];
         }
         __syncthreads();
@@ -694,11 +710,12 @@ __global__ __launch_bounds__(512) void distill_long(const DistillArgs a) {
             });
             __threadfence_block();
             team.sync();
-            for (int e = team.lane; e <= a.kept; e += team.lanes) {
+            const int n = entries_of(a);
+            for (int e = team.lane; e < n; e += team.lanes) {
                 const int32_t j = t.place[e];
                 if (j < begin || j >= end) continue;
                 bool first;
-                const float off = class_amount(t, a.kept, e, first);
+                const float off = class_amount(t, n, e, first);
                 if (first) g[j] = (T)(f(a, logit(j) - most) - off);
             }
         }
