@@ -75,7 +75,7 @@ Tensor run_embed_backward(Tensor ids, Tensor grad, int64_t rows, double scale, c
 
 // ------------------------------------------------------------------- layer norm
 ra_layer_norm_shape layer_norm_shape(const Tensor& x, double eps) {
-    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    check_cuda(x, "x");
     ra_layer_norm_shape s{};
     s.ldx = matrix_stride(x, "x");
     TORCH_CHECK(x.size(1) > 0 && x.size(1) < INT32_MAX, "x has no columns");
@@ -159,7 +159,7 @@ struct DistillCall {
 
 DistillCall distill_call(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature,
                          const OptTensor& labels, double hard, const std::string& reduction) {
-    TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+    check_cuda(logits, "logits");
     const auto dev = logits.device();
     check_on(teacher, "teacher", dev);
     check_on(ids, "ids", dev);
@@ -295,6 +295,7 @@ struct EmbedNode : torch::autograd::Function<EmbedNode> {
 };
 
 Tensor embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
+    check_no_tangent(table, "table");
     ids = ids.contiguous();
     table = with_rows(table);
     return wants_grad({&table}) ? EmbedNode::apply(ids, table, scale, padding) : run_embed(ids, table, scale, padding);
@@ -345,6 +346,10 @@ std::tuple<Tensor, OptTensor> layer_norm(Tensor x, OptTensor residual, OptTensor
     x = with_rows(x);
     if (residual.has_value()) residual = with_rows(*residual);
     const Tensor r = raw(residual), w = raw(weight), b = raw(bias);
+    check_no_tangent(x, "x");
+    check_no_tangent(r, "residual");
+    check_no_tangent(w, "weight");
+    check_no_tangent(b, "bias");
     if (wants_grad({&x, &r, &w, &b})) {
         const variable_list out = LayerNormNode::apply(x, residual, weight, bias, eps);
         return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
@@ -379,6 +384,8 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
 
 Tensor distill_loss(Tensor logits, Tensor teacher, Tensor ids, double temperature, OptTensor labels, double hard,
                     std::string reduction) {
+    check_no_tangent(logits, "logits");
+    check_no_tangent(teacher, "teacher");
     logits = with_rows(logits);
     teacher = with_rows(teacher);
     ids = with_rows(ids);

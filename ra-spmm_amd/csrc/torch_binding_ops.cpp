@@ -190,7 +190,7 @@ int64_t heads_of(const Tensor& t, const char* name) {
 
 NormCall norm_call(const Tensor& q, const OptTensor& k, const Tensor& wq, const OptTensor& wk, const OptTensor& table,
                    const OptTensor& positions, double eps, const std::string& layout) {
-    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    check_cuda(q, "q");
     const auto dev = q.device();
     NormCall c;
     ra_norm_shape& s = c.shape;
@@ -288,7 +288,7 @@ Tensor empty_scales(const Tensor& x) {
 }
 
 int64_t check_matrix(const Tensor& x, const char* name) {
-    TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+    check_cuda(x, name);
     TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) < INT32_MAX - 64, name, " must be [rows, cols], has ", x.sizes());
     dtype_of(x, name);
     return row_stride(x, name);

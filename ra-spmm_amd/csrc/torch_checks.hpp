@@ -3,6 +3,7 @@
 #pragma once
 
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/ra_spmm.h"
@@ -28,8 +29,20 @@ inline int dtype_of(const Tensor& t, const char* name) {
     return -1;
 }
 
-inline void check_on(const Tensor& t, const char* name, const torch::Device& dev) {
+// A tensor with a tangent need not require a gradient: without this check the result would be
+// one whose tangent is missing.
+inline void check_no_tangent(const Tensor& t, const char* name) {
+    TORCH_CHECK(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
+                " carries a forward-mode tangent, this operator has reverse-mode derivatives only");
+}
+
+inline void check_cuda(const Tensor& t, const char* name) {
+    check_no_tangent(t, name);
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+}
+
+inline void check_on(const Tensor& t, const char* name, const torch::Device& dev) {
+    check_cuda(t, name);
     TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", is on ", t.device());
 }
 

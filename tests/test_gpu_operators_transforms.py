@@ -1,0 +1,61 @@
+"""The operators under torch's transformations other than reverse-mode autograd, on tensors of the GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+pytestmark = pytest.mark.gpu
+
+import ra_spmm  # noqa: E402
+
+
+def inputs():
+    gen = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(6, 8, generator=gen, device="cuda")
+    teacher, top = torch.randn(6, 8, generator=gen, device="cuda").topk(3, dim=1)
+    rowptr = torch.arange(7, dtype=torch.int32, device="cuda")
+    plan = ra_spmm.make_attention_plan(rowptr, torch.arange(6, dtype=torch.int32, device="cuda").flip(0).contiguous(), 6, 6)
+    q, v = torch.randn(6, 2, 2, 8, generator=gen, device="cuda"), torch.randn(6, 2, 8, generator=gen, device="cuda")
+    return x, torch.rand(8, generator=gen, device="cuda"), teacher, top, plan, q, v, torch.ones(2, device="cuda")
+
+
+def operators(x, w, teacher, top, plan, q, v, lam):
+    ids = torch.tensor([1, 5, 0], device="cuda")
+    return {
+        "embed": (x, lambda t: ra_spmm.embed(ids, t)),
+        "layer_norm": (x, lambda t: ra_spmm.layer_norm(t, w)),
+        "layer_norm weight": (w, lambda t: ra_spmm.layer_norm(x, t)),
+        "layer_norm residual": (x, lambda t: ra_spmm.layer_norm(x, w, residual=t)[0]),
+        "distill_loss": (x, lambda t: ra_spmm.distill_loss(t, teacher, top)),
+        "head_norm_rotate": (q, lambda t: ra_spmm.head_norm_rotate(t, None, w, None)[0]),
+        "diff_attention": (q, lambda t: ra_spmm.diff_attention(plan, t, q, v, lam)),
+        "diff_attention lam": (lam, lambda t: ra_spmm.diff_attention(plan, q, q, v, t)),
+        "relu8": (x, lambda t: ra_spmm.relu8(t)[0]),
+    }
+
+
+NAMES = ["embed", "layer_norm", "layer_norm weight", "layer_norm residual", "distill_loss", "head_norm_rotate", "diff_attention",
+         "diff_attention lam", "relu8"]
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name, requires_grad):
+    """Whether a gradient is required beside it or not."""
+    at, f = operators(*inputs())[name]
+    with forward_ad.dual_level():
+        leaf = at.clone().requires_grad_(requires_grad)
+        dual = forward_ad.make_dual(leaf, torch.ones_like(at))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward-mode tangent|jvp|forward mode"):
+            f(dual)
+    assert torch.equal(f(at), f(at.clone().requires_grad_(True)).detach())
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_tangent_of_the_incoming_gradient_is_refused(name):
+    at, f = operators(*inputs())[name]
+    leaf = at.clone().requires_grad_(True)
+    y = f(leaf)
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode tangent"):
+            torch.autograd.grad(y, leaf, g)

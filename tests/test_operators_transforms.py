@@ -1,0 +1,45 @@
+"""The operators under torch's transformations other than reverse-mode autograd, on a host without a GPU: what they cannot take
+part in is refused before anything else is looked at, where a result without its tangent would be silently wrong."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import ra_spmm
+from ra_spmm import _C
+
+X, IDS = torch.ones(4, 8), torch.zeros(4, 2, dtype=torch.int64)
+W = torch.ones(8)
+
+
+def calls(dual):
+    """Every operator with one input after the other carrying a tangent."""
+    x, w = dual(X), dual(W)
+    yield lambda: ra_spmm.embed(IDS, x)
+    yield lambda: ra_spmm.layer_norm(x)
+    yield lambda: ra_spmm.layer_norm(X, w)
+    yield lambda: ra_spmm.layer_norm(X, W, w)
+    yield lambda: ra_spmm.layer_norm(X, residual=x)
+    yield lambda: ra_spmm.layer_norm(x.view(2, 2, 8), residual=X.view(2, 2, 8))
+    yield lambda: ra_spmm.distill_loss(x, X[:, :2], IDS)
+    yield lambda: ra_spmm.distill_loss(X, x[:, :2], IDS)
+    yield lambda: ra_spmm.distill_loss_grad(x, X[:, :2], IDS)
+    yield lambda: ra_spmm.head_norm_rotate(x, None, W, None)
+    yield lambda: ra_spmm.pack8(x)
+    yield lambda: ra_spmm.relu_pack8(x)
+
+
+@pytest.mark.parametrize("n", range(12))
+def test_forward_mode_is_refused(n):
+    with forward_ad.dual_level():
+        call = list(calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))))[n]
+        with pytest.raises(RuntimeError, match="forward-mode tangent"):
+            call()
+    with pytest.raises(RuntimeError, match="CUDA"):  # the same call without tangents
+        list(calls(lambda t: t))[n]()
+
+
+def test_tangents_may_be_switched_off():
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(X, X)
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA"):
+            _C.embed(IDS, x, 1.0, None)
