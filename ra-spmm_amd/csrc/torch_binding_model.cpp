@@ -199,6 +199,7 @@ DistillCall distill_call(const Tensor& logits, const Tensor& teacher, const Tens
 std::tuple<Tensor, OptTensor, OptTensor> run_distill(Tensor logits, Tensor teacher, Tensor ids, double temperature,
                                                      OptTensor labels, double hard, std::string reduction, bool with_stats,
                                                      bool with_grad, OptTensor factor) {
+    check_no_tracer("distill_loss");
     const DistillCall c = distill_call(logits, teacher, ids, temperature, labels, hard, reduction);
     const float* const up = factor.has_value() ? f32_vector(factor->reshape({-1}), "factor", 1, logits.device()) : nullptr;
     const c10::DeviceGuard guard(logits.device());
@@ -295,7 +296,9 @@ struct EmbedNode : torch::autograd::Function<EmbedNode> {
 };
 
 Tensor embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
+    check_no_tracer("embed");
     check_no_tangent(table, "table");
+    check_no_proxies("table");
     ids = ids.contiguous();
     table = with_rows(table);
     return wants_grad({&table}) ? EmbedNode::apply(ids, table, scale, padding) : run_embed(ids, table, scale, padding);
@@ -343,6 +346,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 
 // (y, x + residual or nothing) of matrices.
 std::tuple<Tensor, OptTensor> layer_norm(Tensor x, OptTensor residual, OptTensor weight, OptTensor bias, double eps) {
+    check_no_tracer("layer_norm");
     x = with_rows(x);
     if (residual.has_value()) residual = with_rows(*residual);
     const Tensor r = raw(residual), w = raw(weight), b = raw(bias);
@@ -384,6 +388,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
 
 Tensor distill_loss(Tensor logits, Tensor teacher, Tensor ids, double temperature, OptTensor labels, double hard,
                     std::string reduction) {
+    check_no_tracer("distill_loss");
     check_no_tangent(logits, "logits");
     check_no_tangent(teacher, "teacher");
     logits = with_rows(logits);

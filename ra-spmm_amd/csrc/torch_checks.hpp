@@ -4,7 +4,9 @@
 
 #include <torch/extension.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/ra_spmm.h"
 
@@ -36,8 +38,21 @@ inline void check_no_tangent(const Tensor& t, const char* name) {
                 " carries a forward-mode tangent, this operator has reverse-mode derivatives only");
 }
 
+// Tracers record torch's own operations: of a call here they would keep the outputs' allocation
+// and no launch, and a replay would return memory that nobody wrote.
+inline void check_no_tracer(const char* what) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced: torch.jit.trace does not see its launches");
+}
+inline void check_no_proxies(const char* name) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK(!TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE),
+                name, ": this operator cannot be traced (make_fx, torch.export or fake tensors)");
+}
+
 inline void check_cuda(const Tensor& t, const char* name) {
     check_no_tangent(t, name);
+    check_no_proxies(name);
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
 }
 

@@ -59,3 +59,19 @@ def test_a_tangent_of_the_incoming_gradient_is_refused(name):
         g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(RuntimeError, match="forward-mode tangent"):
             torch.autograd.grad(y, leaf, g)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.filterwarnings("ignore")
+def test_traces(name):
+    """Refused, or right on other inputs than those of the trace."""
+    at, f = operators(*inputs())[name]
+    if name.split()[0] in ("embed", "layer_norm", "distill_loss"):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (at,), check_trace=False)
+        return
+    traced = torch.jit.trace(f, (at,), check_trace=False)
+    for factor in (1.0, -0.5, 2.0):
+        other = at * factor
+        torch.empty(1 << 20, device="cuda").fill_(float("nan"))  # what unwritten memory would hold
+        assert torch.equal(traced(other), f(other)), factor

@@ -3,6 +3,7 @@ part in is refused before anything else is looked at, where a result without its
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import ra_spmm
 from ra_spmm import _C
@@ -43,3 +44,22 @@ def test_tangents_may_be_switched_off():
         x = forward_ad.make_dual(X, X)
         with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA"):
             _C.embed(IDS, x, 1.0, None)
+
+
+@pytest.mark.parametrize("n", range(4))
+def test_traces_are_refused(n):
+    """A tracer would keep the output's allocation and no launch: its replay would return memory that nobody wrote."""
+    f = [lambda x: ra_spmm.embed(IDS, x), lambda x: ra_spmm.layer_norm(x, residual=x)[0], lambda x: ra_spmm.distill_loss(x, x[:, :2], IDS),
+         lambda x: ra_spmm.distill_loss_grad(x, x[:, :2], IDS)[1]][n]
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(f, (X,), check_trace=False)
+
+
+@pytest.mark.parametrize("n,mode", [(n, "real") for n in range(12)] + [(n, "fake") for n in (0, 1, 2, 9, 10, 11)])
+def test_proxies_are_refused(n, mode):
+    def f(x):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            list(calls(lambda t: x if t is X else t))[n]()
+        return x + 1
+
+    make_fx(f, tracing_mode=mode)(X.clone())
