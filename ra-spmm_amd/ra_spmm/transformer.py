@@ -20,6 +20,7 @@ themselves.  keep8=False keeps the inputs as they are: plain layers, more memory
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -137,12 +138,30 @@ def train_step(model, plan, X, y, optimizer, positions=None, bias=None) -> torch
 
 
 def distill_step(model, plan, X, teacher, ids, optimizer, temperature: float = 1.0, labels=None, hard: float = 0.0,
-                 positions=None, bias=None) -> torch.Tensor:
+                 positions=None, bias=None, loss_scale: Optional[float] = None) -> torch.Tensor:
     """One forward, backward and optimizer step on a teacher's largest logits (teacher and ids [M, kept], as of a top-k) and
-    the labels of some nodes (-1: none); the loss, distill_loss's."""
+    the labels of some nodes (-1: none); the loss, distill_loss's.
+
+    The backward pass runs on loss_scale times the loss, and every gradient is divided by it before it is added to its
+    parameter's (or X's): a mean over many rows leaves a row's gradient of float16 logits below their smallest steps.  None: 1,
+    but for float16 logits of more than 1024 rows the power of two that divides a row's by 1024 at most (1e6 rows: 1024).
+    A parameter's gradient is rounded to the parameter's own type after that."""
+    if loss_scale is not None and not 0.0 < loss_scale < math.inf:
+        raise ValueError(f"distill_step: loss_scale must be positive and finite, got {loss_scale}")
     optimizer.zero_grad(set_to_none=True)
     logits = model(X, plan, positions, bias)
-    loss, grad = distill_loss_grad(logits.detach(), teacher, ids, temperature, labels, hard)
-    logits.backward(grad)
+    if loss_scale is None:
+        rows = logits.size(0) if logits.dtype == torch.float16 else 1
+        loss_scale = max(1.0, 2.0 ** (rows - 1).bit_length() / 1024)
+    # A factor of 1 is none: no tensor for it.
+    loss, grad = distill_loss_grad(logits.detach(), teacher, ids, temperature, labels, hard,
+                                   factor=None if loss_scale == 1.0 else loss_scale)
+    leaves = [] if loss_scale == 1.0 else [t for t in (*model.parameters(), X) if t.requires_grad]
+    handles = [t.register_hook(lambda g: g * (1.0 / loss_scale)) for t in leaves]
+    try:
+        logits.backward(grad)
+    finally:
+        for handle in handles:
+            handle.remove()
     optimizer.step()
     return loss
