@@ -201,7 +201,8 @@ std::tuple<Tensor, OptTensor, OptTensor> run_distill(Tensor logits, Tensor teach
                                                      bool with_grad, OptTensor factor) {
     check_no_tracer("distill_loss");
     const DistillCall c = distill_call(logits, teacher, ids, temperature, labels, hard, reduction);
-    const float* const up = factor.has_value() ? f32_vector(factor->reshape({-1}), "factor", 1, logits.device()) : nullptr;
+    if (factor.has_value()) factor = factor->reshape({-1});
+    const float* const up = factor.has_value() ? f32_vector(*factor, "factor", 1, logits.device()) : nullptr;
     const c10::DeviceGuard guard(logits.device());
     const auto f32 = logits.options().dtype(torch::kFloat32);
     auto loss = c.shape.reduction == RA_REDUCE_NONE ? torch::empty({logits.size(0)}, f32) : torch::empty({}, f32);
@@ -226,7 +227,8 @@ Tensor run_distill_backward(Tensor logits, Tensor teacher, Tensor ids, double te
                     stats.size(0) == logits.size(0) && stats.size(1) == 4,
                 "stats must be what run_distill returned for these inputs");
     const int64_t n = c.shape.reduction == RA_REDUCE_NONE ? logits.size(0) : 1;
-    const float* const up = f32_vector(grad_loss.reshape({-1}), "grad_loss", n, logits.device());
+    grad_loss = grad_loss.reshape({-1});  // a copy of it has to live until the launch
+    const float* const up = f32_vector(grad_loss, "grad_loss", n, logits.device());
     const c10::DeviceGuard guard(logits.device());
     auto grad = torch::empty(logits.sizes(), logits.options());
     check(ra_distill_backward(&c.shape, logits.data_ptr(), teacher.data_ptr(), ids.data_ptr(), c.labels,

@@ -150,3 +150,17 @@ def test_a_gradient_that_is_scaled_before_it_is_rounded():
     (65536.0 * ra_spmm.distill_loss(leaf, t, ids)).backward()
     assert torch.equal(leaf.grad, g)
     assert (ra_spmm.distill_loss_grad(x.detach(), t, ids)[1][:, 1:] == 6 * 2.0 ** -24).all()
+
+
+def test_an_incoming_gradient_that_has_to_be_copied():
+    """The copy must not be given to the gradient that is written from it."""
+    M, C = 20_000, 12
+    gen = torch.Generator("cuda").manual_seed(2)
+    x, up = torch.randn(M, C, generator=gen, device="cuda"), torch.randn(2, M // 2, generator=gen, device="cuda").t()
+    t, ids = torch.randn(M, C, generator=gen, device="cuda").topk(3, dim=1)
+    _, stats, _ = ra_spmm._C.run_distill(x, t, ids, 2.0, None, 0.0, "none", True, False, None)
+    back = lambda g: ra_spmm._C.run_distill_backward(x, t, ids, 2.0, None, 0.0, "none", stats, g)  # noqa: E731
+    want = back(up.reshape(-1))
+    assert not up.is_contiguous()
+    for _ in range(5):
+        assert torch.equal(back(up), want)
