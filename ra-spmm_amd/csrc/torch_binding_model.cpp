@@ -243,6 +243,7 @@ using torch::autograd::variable_list;
 
 // t itself where only its rows are strided, else a contiguous copy.
 Tensor with_rows(const Tensor& t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();
     int64_t run = 1;
     for (int64_t d = t.dim() - 1; d > 0; --d) {
         if (t.size(d) > 1 && t.stride(d) != run) return t.contiguous();

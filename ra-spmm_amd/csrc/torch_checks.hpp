@@ -54,6 +54,7 @@ inline void check_cuda(const Tensor& t, const char* name) {
     check_no_tangent(t, name);
     check_no_proxies(name);
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(!t.is_neg(), name, " is a view of the negated values (resolve_neg() gives them)");
 }
 
 inline void check_on(const Tensor& t, const char* name, const torch::Device& dev) {

@@ -20,6 +20,8 @@ from . import _C
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where only its rows are strided, else a contiguous copy."""
+    if t.is_neg():  # the imaginary part of a conjugate, say: its memory holds the opposite
+        return t.resolve_neg().contiguous()
     run = 1
     for d in range(t.dim() - 1, 0, -1):
         if t.size(d) > 1 and t.stride(d) != run:

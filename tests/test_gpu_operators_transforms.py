@@ -1,4 +1,6 @@
 """The operators under torch's transformations other than reverse-mode autograd, on tensors of the GPU."""
+import re
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -75,3 +77,28 @@ def test_traces(name):
         other = at * factor
         torch.empty(1 << 20, device="cuda").fill_(float("nan"))  # what unwritten memory would hold
         assert torch.equal(traced(other), f(other)), factor
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_views_of_negated_values(name):
+    """Memory that holds the opposite of the tensor's values, as the imaginary part of a conjugate."""
+    at, f = operators(*inputs())[name]
+    view = torch.complex(torch.zeros_like(at), at).conj().imag
+    for t in (view, torch._neg_view(at)):
+        assert t.is_neg() and torch.equal(t, -at)
+        try:
+            y = f(t)
+        except RuntimeError as e:  # weights are taken as they lie
+            assert at.dim() == 1 and re.search("negated|contiguous", str(e))
+        else:
+            assert torch.equal(y, f(-at))
+    leaf = at.clone().requires_grad_(True)
+    y = f(leaf)
+    g = torch.randn(y.shape, generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    want, = torch.autograd.grad(y, leaf, -g, retain_graph=True)
+    try:
+        got, = torch.autograd.grad(y, leaf, torch._neg_view(g))
+    except RuntimeError as e:
+        assert "negated" in str(e)
+    else:
+        assert torch.equal(got, want)
