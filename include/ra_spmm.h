@@ -528,7 +528,8 @@ ra_status ra_weight_grad8(const void* d_grad, const uint8_t* d_codes, const uint
  * without those positions; it is written whole.  Its sums are fp32 and in a fixed
  * order: the positions are sorted by id first, equal inputs give equal bits.  Rows
  * of the table and of grad may lie ld_table, ld_grad elements apart; out [count,
- * dim] and d_table [rows, dim] are contiguous. */
+ * dim] and d_table [rows, dim] are contiguous.  No output and no workspace may
+ * share memory with an input or with each other: that is refused. */
 typedef struct ra_embed_shape {
     int64_t count;     /* positions, below 2^31 - 2^24       */
     int64_t rows;      /* of the table, below 2^31 - 2       */
@@ -555,7 +556,10 @@ ra_status ra_embed_backward(const ra_embed_shape* shape, const void* d_ids, cons
  * ldx, ldr elements apart; y and d_sum are contiguous.  Statistics are fp32, those
  * of the variance taken around the mean.
  * d_stats [rows, 2] fp32 (mean, 1 / deviation) on 8-byte addresses, for the backward
- * pass, or NULL. */
+ * pass, or NULL.
+ * d_y or d_sum may be d_x or d_residual themselves where those rows are contiguous
+ * (ldx, ldr = dim), in the backward pass dx may be h, grad_y or grad_sum; any other
+ * sharing of memory by an output or a workspace is refused. */
 typedef struct ra_layer_norm_shape {
     int64_t rows;     /* below 2^31             */
     int32_t dim;      /* 1 .. 16384             */
@@ -594,7 +598,8 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* shape, const void* d
  * +inf or NaN, and a logit of +inf or NaN in a row that counts make the row's loss
  * and gradient NaN; logits of -inf are classes of probability 0.
  * t may have another type than s.  Sums and losses are fp32 or more, in a fixed
- * order. */
+ * order.  No output (the gradient in the place of the logits neither) and no
+ * workspace may share memory with an input or with each other: that is refused. */
 typedef enum ra_reduction { RA_REDUCE_NONE = 0, RA_REDUCE_MEAN = 1, RA_REDUCE_SUM = 2 } ra_reduction;
 typedef struct ra_distill_shape {
     int64_t rows;            /* below 2^31                                  */

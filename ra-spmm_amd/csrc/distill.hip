@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "lanes.hpp"
+#include "overlap.hpp"
 #include "ra_internal.hpp"
 #include "vector_run.hpp"
 
@@ -766,6 +767,19 @@ ra_status check_tensors(const ra_distill_shape& s, const void* logits, const voi
     return RA_OK;
 }
 
+int64_t size_of(int32_t dtype) { return dtype == RA_DTYPE_F32 ? 4 : 2; }
+
+// The gradient of long rows is written before what is kept of them has been read for the last time, so no output may
+// take an input's place.
+ra_status refuse_shared(const ra_distill_shape& s, std::initializer_list<Extent> outputs, const void* logits, const void* teacher,
+                        const void* ids, const void* labels, const Extent& factor, const Extent& stats) {
+    return refuse_overlap("distill", outputs,
+                          {rows_of("logits", logits, s.rows, s.classes, s.ld_logits, size_of(s.dtype)),
+                           rows_of("teacher", s.kept ? teacher : nullptr, s.rows, s.kept, s.ld_teacher, size_of(s.teacher_dtype)),
+                           rows_of("ids", s.kept ? ids : nullptr, s.rows, s.kept, s.ld_ids, s.ids64 ? 8 : 4),
+                           rows_of("labels", labels, s.rows, 1, 1, s.labels64 ? 8 : 4), factor, stats});
+}
+
 DistillArgs args_of(const ra_distill_shape& s, const void* logits, const void* teacher, const void* ids, const void* labels) {
     DistillArgs a{};
     a.logits = logits;
@@ -948,6 +962,12 @@ ra_status ra_distill_loss(const ra_distill_shape* s, const void* d_logits, const
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: the workspace is too small");
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: the workspace must be 16-byte aligned");
     if (!ra::aligned16(d_stats)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
+    RA_TRY(ra::refuse_shared(*s,
+                             {ra::rows_of("loss", d_loss, s->reduction == RA_REDUCE_NONE ? s->rows : 1, 1, 1, sizeof(float)),
+                              ra::rows_of("stats", d_stats, s->rows, 4, 4, sizeof(float)),
+                              ra::rows_of("the gradient", d_grad, s->rows, s->classes, s->classes, ra::size_of(s->dtype)),
+                              {"the workspace", d_workspace, static_cast<uint64_t>(need)}},
+                             d_logits, d_teacher, d_ids, d_labels, {"factor", d_factor, sizeof(float)}, {}));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::DistillArgs a = ra::args_of(*s, d_logits, d_teacher, d_ids, d_labels);
     a.up = d_factor;
@@ -981,6 +1001,10 @@ ra_status ra_distill_backward(const ra_distill_shape* s, const void* d_logits, c
     if (s->rows == 0) return RA_OK;
     if (!d_stats || !d_grad_loss || !d_grad) return fail(RA_ERR_INVALID_ARGUMENT, "distill: NULL tensor");
     if (!ra::aligned16(d_stats)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
+    RA_TRY(ra::refuse_shared(*s, {ra::rows_of("the gradient", d_grad, s->rows, s->classes, s->classes, ra::size_of(s->dtype))}, d_logits,
+                             d_teacher, d_ids, d_labels,
+                             ra::rows_of("grad_loss", d_grad_loss, s->reduction == RA_REDUCE_NONE ? s->rows : 1, 1, 1, sizeof(float)),
+                             ra::rows_of("stats", d_stats, s->rows, 4, 4, sizeof(float))));
     ra::DistillArgs a = ra::args_of(*s, d_logits, d_teacher, d_ids, d_labels);
     a.kept_stats = d_stats;
     a.up = d_grad_loss;

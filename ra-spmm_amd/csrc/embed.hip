@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "overlap.hpp"
 #include "ra_internal.hpp"
 #include "vector_run.hpp"
 
@@ -631,6 +632,10 @@ ra_status ra_embed(const ra_embed_shape* s, const void* d_ids, const void* d_tab
     RA_TRY(ra::check_stride(s->rows, s->ld_table));
     if (!d_ids || !d_out || (s->rows && !d_table)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: NULL tensor");
     if (s->rows > 1 && s->ld_table < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_table is too small)");
+    const int64_t size = s->dtype == RA_DTYPE_F32 ? 4 : 2;
+    RA_TRY(ra::refuse_overlap("embed", {ra::rows_of("out", d_out, s->count, s->dim, s->dim, size)},
+                              {ra::rows_of("ids", d_ids, s->count, 1, 1, s->ids64 ? 8 : 4),
+                               ra::rows_of("the table", d_table, s->rows, s->dim, s->ld_table, size)}));
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_table, d_out, s->ld_table);
     const bool around = s->count * s->dim * (s->dtype == RA_DTYPE_F32 ? 4 : 2) > ra::kAroundBytes;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -665,6 +670,12 @@ ra_status ra_embed_backward(const ra_embed_shape* s, const void* d_ids, const vo
     if (s->count > 1 && s->ld_grad < s->dim) return fail(RA_ERR_INVALID_ARGUMENT, "embed: rows overlap (ld_grad is too small)");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: the workspace is too small");
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "embed: the workspace must be 16-byte aligned");
+    const int64_t size = s->dtype == RA_DTYPE_F32 ? 4 : 2;
+    RA_TRY(ra::refuse_overlap("embed",
+                              {ra::rows_of("the table's gradient", d_dtable, s->rows, s->dim, s->dim, size),
+                               {"the workspace", d_workspace, static_cast<uint64_t>(need)}},
+                              {ra::rows_of("ids", d_ids, s->count, 1, 1, s->ids64 ? 8 : 4),
+                               ra::rows_of("grad", d_grad, s->count, s->dim, s->ld_grad, size)}));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const ra::EmbedArgs a = ra::args_of(*s, d_ids, d_grad, d_dtable, s->ld_grad);
     const ra::SumPlan plan = ra::sum_plan(*s);

@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "lanes.hpp"
+#include "overlap.hpp"
 #include "ra_internal.hpp"
 #include "vector_run.hpp"
 
@@ -168,10 +169,7 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
-                for (int e = 0; e < P; ++e) h[k][e] = px[k].at(e) + pr[k].at(e);
-                if (there[k]) store_packet<AROUND, T, P>(static_cast<T*>(a.sum) + out + at[k], h[k]);
-#pragma unroll
-                for (int e = 0; e < P; ++e) h[k][e] = (float)(T)h[k][e];  // the norm is that of the sum as it is kept
+                for (int e = 0; e < P; ++e) h[k][e] = (float)(T)(px[k].at(e) + pr[k].at(e));  // the norm is that of the sum as it is kept
             }
         } else {
 #pragma unroll
@@ -184,6 +182,12 @@ __global__ __launch_bounds__(WAVE ? kThreads : 1024) void layer_norm_forward(con
 #pragma unroll
             for (int e = 0; e < P; ++e) s += !TAIL || place.counts(k, e) ? h[k][e] : 0.f;
         const float mean = group.sum(s) / a.count;
+        // From here on the whole row has been read, by all waves: the sum may take the place of x or of the residual.
+        if (a.res) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (there[k]) store_packet<AROUND, T, P>(static_cast<T*>(a.sum) + out + at[k], h[k]);
+        }
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -338,6 +342,17 @@ ra_status check(const ra_layer_norm_shape* s) {
     return RA_OK;
 }
 
+int64_t size_of(const ra_layer_norm_shape& s) { return s.dtype == RA_DTYPE_F32 ? 4 : 2; }
+
+// An output in the place of an input row by row is fine (a row is read whole before any of it is written), any other
+// overlap is not.
+ra_status refuse_shared_rows(const ra_layer_norm_shape& s, std::initializer_list<Extent> outputs, const Extent& in, int64_t ld) {
+    for (const Extent& o : outputs)
+        if (overlap(o, in) && !(o.at == in.at && (s.rows <= 1 || ld == s.dim)))
+            return fail(RA_ERR_INVALID_ARGUMENT, std::string("layer norm: ") + o.name + " overlaps " + in.name);
+    return RA_OK;
+}
+
 // How a row lies in lanes: packets of P elements, K of them in a lane, groups of
 // 1 << shift lanes (wave) or of `threads`.
 struct Layout {
@@ -427,6 +442,18 @@ ra_status ra_layer_norm(const ra_layer_norm_shape* s, const void* d_x, const voi
     if (d_residual && s->rows > 1 && s->ldr < s->dim)
         return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: rows overlap (ldr is too small)");
     if (reinterpret_cast<uintptr_t>(d_stats) % 8) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: stats must be 8-byte aligned");
+    const int64_t size = ra::size_of(*s);
+    const ra::Extent x = ra::rows_of("x", d_x, s->rows, s->dim, s->ldx, size);
+    const ra::Extent residual = ra::rows_of("the residual", d_residual, s->rows, s->dim, s->ldr, size);
+    const ra::Extent weight = ra::rows_of("weight", d_weight, 1, s->dim, 0, sizeof(float));
+    const ra::Extent bias = ra::rows_of("bias", d_bias, 1, s->dim, 0, sizeof(float));
+    const ra::Extent y = ra::rows_of("y", d_y, s->rows, s->dim, s->dim, size);
+    const ra::Extent sum = ra::rows_of("the sum", d_sum, s->rows, s->dim, s->dim, size);
+    const ra::Extent stats = ra::rows_of("stats", d_stats, s->rows, 2, 2, sizeof(float));
+    RA_TRY(ra::refuse_overlap("layer norm", {y, sum}, {weight, bias}));
+    RA_TRY(ra::refuse_overlap("layer norm", {stats}, {x, residual, weight, bias, y, sum}));
+    RA_TRY(ra::refuse_shared_rows(*s, {y, sum}, x, s->ldx));
+    RA_TRY(ra::refuse_shared_rows(*s, {y, sum}, residual, s->ldr));
     ra::LayerNormArgs a{};
     a.x = d_x;
     a.res = d_residual;
@@ -474,6 +501,21 @@ ra_status ra_layer_norm_backward(const ra_layer_norm_shape* s, const void* d_h, 
     if (reinterpret_cast<uintptr_t>(d_stats) % 8) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: stats must be 8-byte aligned");
     if (bytes < need || (need && !d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: the workspace is too small");
     if (need && !ra::aligned16(d_workspace)) return fail(RA_ERR_INVALID_ARGUMENT, "layer norm: the workspace must be 16-byte aligned");
+    const int64_t size = ra::size_of(*s);
+    const ra::Extent h = ra::rows_of("h", d_h, s->rows, s->dim, s->ldx, size);
+    const ra::Extent weight = ra::rows_of("weight", d_weight, 1, s->dim, 0, sizeof(float));
+    const ra::Extent stats = ra::rows_of("stats", d_stats, s->rows, 2, 2, sizeof(float));
+    const ra::Extent grad_y = ra::rows_of("grad_y", d_grad_y, s->rows, s->dim, s->dim, size);
+    const ra::Extent grad_sum = ra::rows_of("grad_sum", d_grad_sum, s->rows, s->dim, s->dim, size);
+    const ra::Extent dx = ra::rows_of("dx", d_dx, s->rows, s->dim, s->dim, size);
+    const ra::Extent dweight = ra::rows_of("dweight", d_dweight, 1, s->dim, 0, sizeof(float));
+    const ra::Extent dbias = ra::rows_of("dbias", d_dbias, 1, s->dim, 0, sizeof(float));
+    const ra::Extent workspace{"the workspace", d_workspace, static_cast<uint64_t>(need)};
+    RA_TRY(ra::refuse_overlap("layer norm", {dx}, {weight, stats}));
+    RA_TRY(ra::refuse_overlap("layer norm", {dweight, dbias, workspace}, {h, weight, stats, grad_y, grad_sum, dx}));
+    RA_TRY(ra::refuse_shared_rows(*s, {dx}, h, s->ldx));
+    RA_TRY(ra::refuse_shared_rows(*s, {dx}, grad_y, s->dim));
+    RA_TRY(ra::refuse_shared_rows(*s, {dx}, grad_sum, s->dim));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     ra::LayerNormArgs a{};
     a.x = d_h;
