@@ -613,10 +613,12 @@ typedef struct ra_distill_shape {
     float hard;              /* 0 .. 1, 0 without labels                    */
     int64_t ld_logits, ld_teacher, ld_ids;
 } ra_distill_shape;
-/* d_loss: [rows] without a reduction, else [1].  d_stats [rows, 4] fp32 on 16-byte
- * addresses, for the backward pass of the same shape, or NULL.  d_grad [rows, classes] (contiguous): the gradient of the
+/* d_loss: [rows] without a reduction, else [1].  d_stats: ra_distill_stats_bytes() bytes on 16-byte addresses, for the
+ * backward pass of the same shape, or NULL (rows of up to 1,024 classes leave nothing there, 16 bytes are enough: the
+ * backward pass forms their statistics again).  d_grad [rows, classes] (contiguous): the gradient of the
  * reduced loss (of every row's without a reduction) times *d_factor (NULL: 1) in the
  * same call, or NULL.  d_workspace: ra_distill_workspace() bytes, 16-byte aligned. */
+ra_status ra_distill_stats_bytes(const ra_distill_shape* shape, int64_t* bytes);
 ra_status ra_distill_workspace(const ra_distill_shape* shape, int64_t* bytes);
 ra_status ra_distill_loss(const ra_distill_shape* shape, const void* d_logits, const void* d_teacher,
                           const void* d_ids, const void* d_labels, const float* d_factor, float* d_loss,

@@ -59,7 +59,7 @@ struct DistillArgs {
     float up_scale;      // and this
     float* loss;         // [rows], or NULL
     double* part;        // [workgroups] sums of the rows' losses, or NULL
-    float* stats;        // [rows][4]: maximum, sum of exponentials at T and at 1
+    float* stats;        // of long rows, [rows][4]: maximum, sum of exponentials at T and at 1
     const float* kept_stats;
     float* piece_stats;  // [rows][pieces][4], where a row is cut
     void* grad;
@@ -809,6 +809,9 @@ int lane_blocks(const ra_distill_shape& s) { return static_cast<int>(std::min<in
 
 bool is_short(const ra_distill_shape& s) { return s.classes <= kMaxShort && s.kept <= 256; }
 
+// What the forward pass leaves for the backward pass: only long rows' statistics cost another reading.
+int64_t stats_bytes(const ra_distill_shape& s) { return s.rows == 0 ? 0 : by_lanes(s) || is_short(s) ? 16 : s.rows * 16; }
+
 // Short rows: lanes of a row and rows of a workgroup at once.  A lane takes 4 elements, and 16
 // past 256 classes, or past 32 where rows are enough to fill the machine with a quarter of the
 // lanes: what is done once a row is done by fewer (1e6 x 100 bf16 436 us with 4, 257 with 16);
@@ -952,6 +955,13 @@ ra_status ra_distill_workspace(const ra_distill_shape* s, int64_t* bytes) {
     return RA_OK;
 }
 
+ra_status ra_distill_stats_bytes(const ra_distill_shape* s, int64_t* bytes) {
+    if (!bytes) return fail(RA_ERR_INVALID_ARGUMENT, "distill: bytes is NULL");
+    RA_TRY(ra::check(s));
+    *bytes = ra::stats_bytes(*s);
+    return RA_OK;
+}
+
 ra_status ra_distill_loss(const ra_distill_shape* s, const void* d_logits, const void* d_teacher, const void* d_ids,
                           const void* d_labels, const float* d_factor, float* d_loss, float* d_stats, void* d_grad,
                           void* d_workspace, int64_t bytes, ra_stream_t stream) {
@@ -964,7 +974,7 @@ ra_status ra_distill_loss(const ra_distill_shape* s, const void* d_logits, const
     if (!ra::aligned16(d_stats)) return fail(RA_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
     RA_TRY(ra::refuse_shared(*s,
                              {ra::rows_of("loss", d_loss, s->reduction == RA_REDUCE_NONE ? s->rows : 1, 1, 1, sizeof(float)),
-                              ra::rows_of("stats", d_stats, s->rows, 4, 4, sizeof(float)),
+                              {"stats", d_stats, static_cast<uint64_t>(ra::stats_bytes(*s))},
                               ra::rows_of("the gradient", d_grad, s->rows, s->classes, s->classes, ra::size_of(s->dtype)),
                               {"the workspace", d_workspace, static_cast<uint64_t>(need)}},
                              d_logits, d_teacher, d_ids, d_labels, {"factor", d_factor, sizeof(float)}, {}));
@@ -1004,7 +1014,7 @@ ra_status ra_distill_backward(const ra_distill_shape* s, const void* d_logits, c
     RA_TRY(ra::refuse_shared(*s, {ra::rows_of("the gradient", d_grad, s->rows, s->classes, s->classes, ra::size_of(s->dtype))}, d_logits,
                              d_teacher, d_ids, d_labels,
                              ra::rows_of("grad_loss", d_grad_loss, s->reduction == RA_REDUCE_NONE ? s->rows : 1, 1, 1, sizeof(float)),
-                             ra::rows_of("stats", d_stats, s->rows, 4, 4, sizeof(float))));
+                             {"stats", d_stats, static_cast<uint64_t>(ra::stats_bytes(*s))}));
     ra::DistillArgs a = ra::args_of(*s, d_logits, d_teacher, d_ids, d_labels);
     a.kept_stats = d_stats;
     a.up = d_grad_loss;

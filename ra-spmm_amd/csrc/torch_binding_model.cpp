@@ -195,6 +195,12 @@ DistillCall distill_call(const Tensor& logits, const Tensor& teacher, const Tens
     return c;
 }
 
+int64_t distill_stats_rows(const DistillCall& c) {
+    int64_t bytes = 0;
+    check(ra_distill_stats_bytes(&c.shape, &bytes), "distill_loss");
+    return bytes / 16;
+}
+
 // (loss, stats or nothing, gradient or nothing)
 std::tuple<Tensor, OptTensor, OptTensor> run_distill(Tensor logits, Tensor teacher, Tensor ids, double temperature,
                                                      OptTensor labels, double hard, std::string reduction, bool with_stats,
@@ -207,7 +213,7 @@ std::tuple<Tensor, OptTensor, OptTensor> run_distill(Tensor logits, Tensor teach
     const auto f32 = logits.options().dtype(torch::kFloat32);
     auto loss = c.shape.reduction == RA_REDUCE_NONE ? torch::empty({logits.size(0)}, f32) : torch::empty({}, f32);
     OptTensor stats, grad;
-    if (with_stats) stats = torch::empty({logits.size(0), 4}, f32);
+    if (with_stats) stats = torch::empty({distill_stats_rows(c), 4}, f32);
     if (with_grad) grad = torch::empty(logits.sizes(), logits.options());
     int64_t bytes = 0;
     check(ra_distill_workspace(&c.shape, &bytes), "distill_loss");
@@ -224,7 +230,7 @@ Tensor run_distill_backward(Tensor logits, Tensor teacher, Tensor ids, double te
     const DistillCall c = distill_call(logits, teacher, ids, temperature, labels, hard, reduction);
     check_on(stats, "stats", logits.device());
     TORCH_CHECK(stats.scalar_type() == torch::kFloat32 && stats.is_contiguous() && stats.dim() == 2 &&
-                    stats.size(0) == logits.size(0) && stats.size(1) == 4,
+                    stats.size(0) == distill_stats_rows(c) && stats.size(1) == 4,
                 "stats must be what run_distill returned for these inputs");
     const int64_t n = c.shape.reduction == RA_REDUCE_NONE ? logits.size(0) : 1;
     grad_loss = grad_loss.reshape({-1});  // a copy of it has to live until the launch

@@ -34,7 +34,7 @@ EXPORTED = [
     "ra_pack8", "ra_relu_pack8", "ra_unpack8", "ra_relu_grad8", "ra_weight_grad8_workspace", "ra_weight_grad8",
     "ra_embed", "ra_embed_workspace", "ra_embed_backward",
     "ra_layer_norm", "ra_layer_norm_workspace", "ra_layer_norm_backward",
-    "ra_distill_workspace", "ra_distill_loss", "ra_distill_backward",
+    "ra_distill_stats_bytes", "ra_distill_workspace", "ra_distill_loss", "ra_distill_backward",
 ]
 
 
@@ -227,6 +227,7 @@ def load():
         "ra_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormShape)] + [P] * 8),
         "ra_layer_norm_workspace": (ctypes.c_int, [ctypes.POINTER(LayerNormShape), ctypes.POINTER(I64)]),
         "ra_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormShape)] + [P] * 9 + [I64, P]),
+        "ra_distill_stats_bytes": (ctypes.c_int, [ctypes.POINTER(DistillShape), ctypes.POINTER(I64)]),
         "ra_distill_workspace": (ctypes.c_int, [ctypes.POINTER(DistillShape), ctypes.POINTER(I64)]),
         "ra_distill_loss": (ctypes.c_int, [ctypes.POINTER(DistillShape)] + [P] * 9 + [I64, P]),
         "ra_distill_backward": (ctypes.c_int, [ctypes.POINTER(DistillShape)] + [P] * 8),
