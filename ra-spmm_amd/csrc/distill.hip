@@ -211,8 +211,9 @@ __device__ __forceinline__ float class_amount(const Targets& t, int n, int e, bo
 // each; its gradient takes its place in LDS and goes out the same way.
 // SHIFT: lanes_shift, or -1 where it is only known at run time; HARD: labels count.  Both are
 // constants because the choices they leave would stand at every element and every sum.
-// Up to 10 classes a lane five workgroups fit a CU, in 16 bits with up to ten registers spilled
-// (769,230 x 65 in fp32 with labels 169 us, with four workgroups 195; in bf16 twice as many 279, 298).
+// Up to 10 classes a lane five workgroups fit a CU, with labels and up to eleven registers spilled (fp32: three)
+// (769,230 x 65 in fp32 with labels 169 us, with four workgroups 195; in bf16 twice as many 279, 298).  With 16
+// classes, labels and 16 bits up to four are spilled at four workgroups.
 template <typename T, int K, int SHIFT, bool HARD>
 __global__ __launch_bounds__(kThreads, K <= 10 ? 5 : 4) void distill_short(const DistillArgs args) {
     DistillArgs a = args;

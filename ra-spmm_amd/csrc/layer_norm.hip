@@ -18,7 +18,8 @@
 //
 // Measured, forward, backward and the last sum: 1e6 x 256 in bf16 with a residual 398 us (5.2 TB/s), 406
 // (5.0) and 6; 4,096 x 8,192 in fp32 with a residual 91 (5.9: the inputs of a repeated pass are partly
-// cached), 117 (4.6) and 8; 150,000 x 147 in fp16 26 (3.4), 37 (3.6) and 5.  A large copy: 4.75 TB/s.
+// cached), 117 (4.6) and 8; 2,048 x 16,384 in fp32 with a residual 100 (5.4), 140 (3.8: up to 13 registers spilled) and
+// 13; 150,000 x 147 in fp16 26 (3.4), 37 (3.6) and 5.  A large copy: 4.75 TB/s.
 #include <algorithm>
 #include <type_traits>
 
