@@ -101,12 +101,13 @@ __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const 
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) id[u] = id_at(a, min(i0 + u * groups, count - 1));
         const T* from[kAhead];
-        float add[kAhead];  // scale * v + add: -0 leaves the product, NaN is for ids outside; v is 0 without a row
+        float by[kAhead], add[kAhead];  // by * v + add: -0 leaves the product; without a row 0 * 0 + 0, or NaN for ids outside
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const bool padding = is_padding(a, id[u]), inside = !padding && (uint64_t)id[u] < (uint64_t)a.rows;
             from[u] = inside ? static_cast<const T*>(a.from) + (uint64_t)(uint32_t)id[u] * (uint32_t)a.ld : nullptr;
-            add[u] = inside || padding ? -0.f : __builtin_nanf("");
+            by[u] = inside ? a.scale : 0.f;  // a scale that is not finite makes no padding of its own
+            add[u] = inside ? -0.f : padding ? 0.f : __builtin_nanf("");
         }
         T* const to = static_cast<T*>(a.to) + (uint64_t)i0 * (uint32_t)a.dim;
         for (uint32_t d0 = lane * P; d0 < (uint32_t)a.dim; d0 += P << shift) {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kThreads) void embed_rows(const EmbedArgs a, const 
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
-                for (int e = 0; e < P; ++e) v[u][e] = (T)fmaf(a.scale, (float)v[u][e], add[u]);
+                for (int e = 0; e < P; ++e) v[u][e] = (T)fmaf(by[u], (float)v[u][e], add[u]);
                 if (i0 + u * groups >= count) continue;
                 vec* const at = reinterpret_cast<vec*>(to + (uint64_t)(u * groups) * (uint32_t)a.dim + d);
                 if constexpr (AROUND) __builtin_nontemporal_store(v[u], at);

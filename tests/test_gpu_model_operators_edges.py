@@ -164,3 +164,15 @@ def test_an_incoming_gradient_that_has_to_be_copied():
     assert not up.is_contiguous()
     for _ in range(5):
         assert torch.equal(back(up), want)
+
+
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan, -2.0, 0.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_padding_is_zero_whatever_the_scale_is(dtype, scale):
+    """Positive zeros, as of a tensor of zeros; rows and ids outside keep their values."""
+    table = torch.ones(5, 11, device="cuda", dtype=dtype).requires_grad_(True)
+    out = ra_spmm.embed(torch.tensor([3, -1, 7, 2], device="cuda"), table, scale, padding=-1)
+    assert not out[1].any() and not out[1].signbit().any() and out[2].isnan().all()
+    assert torch.equal(out[0], torch.full_like(out[0], scale)) or math.isnan(scale) and out[0].isnan().all()
+    grad, = torch.autograd.grad(out, table, torch.ones_like(out))
+    assert not grad[[0, 1, 4]].any() and torch.equal(grad[2].isnan(), out[0].isnan())
