@@ -23,6 +23,17 @@ int64_t matrix_stride(const Tensor& t, const char* name) {
     return row_stride(t, name);
 }
 
+// t itself where only its rows are strided, else a contiguous copy.
+Tensor with_rows(const Tensor& t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();
+    int64_t run = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        if (t.size(d) > 1 && t.stride(d) != run) return t.contiguous();
+        run *= t.size(d);
+    }
+    return t.dim() == 0 || t.size(0) <= 1 || t.stride(0) >= run ? t : t.contiguous();
+}
+
 // ------------------------------------------------------------ embedding lookup
 ra_embed_shape embed_shape(const Tensor& ids, int64_t rows, int64_t dim, const Tensor& values, double scale,
                            c10::optional<int64_t> padding) {
@@ -41,6 +52,8 @@ ra_embed_shape embed_shape(const Tensor& ids, int64_t rows, int64_t dim, const T
 }
 
 Tensor run_embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
+    check_no_tangents({{table, "table"}});
+    check_no_proxies("table");
     TORCH_CHECK(ids.is_cuda(), "ids must be a CUDA tensor");
     const auto dev = ids.device();
     check_on(table, "table", dev);
@@ -206,6 +219,11 @@ std::tuple<Tensor, OptTensor, OptTensor> run_distill(Tensor logits, Tensor teach
                                                      OptTensor labels, double hard, std::string reduction, bool with_stats,
                                                      bool with_grad, OptTensor factor) {
     check_no_tracer("distill_loss");
+    check_no_tangents({{logits, "logits"}, {teacher, "teacher"}});
+    logits = with_rows(logits);
+    teacher = with_rows(teacher);
+    ids = with_rows(ids);
+    if (labels.has_value()) labels = labels->contiguous();
     const DistillCall c = distill_call(logits, teacher, ids, temperature, labels, hard, reduction);
     if (factor.has_value()) factor = factor->reshape({-1});
     const float* const up = factor.has_value() ? f32_vector(*factor, "factor", 1, logits.device()) : nullptr;
@@ -246,17 +264,6 @@ Tensor run_distill_backward(Tensor logits, Tensor teacher, Tensor ids, double te
 // --------------------------------------------------------------------- autograd
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-// t itself where only its rows are strided, else a contiguous copy.
-Tensor with_rows(const Tensor& t) {
-    if (t.is_neg()) return t.resolve_neg().contiguous();
-    int64_t run = 1;
-    for (int64_t d = t.dim() - 1; d > 0; --d) {
-        if (t.size(d) > 1 && t.stride(d) != run) return t.contiguous();
-        run *= t.size(d);
-    }
-    return t.dim() == 0 || t.size(0) <= 1 || t.stride(0) >= run ? t : t.contiguous();
-}
 
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     if (!torch::GradMode::is_enabled()) return false;
@@ -306,8 +313,6 @@ struct EmbedNode : torch::autograd::Function<EmbedNode> {
 
 Tensor embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
     check_no_tracer("embed");
-    check_no_tangent(table, "table");
-    check_no_proxies("table");
     ids = ids.contiguous();
     table = with_rows(table);
     return wants_grad({&table}) ? EmbedNode::apply(ids, table, scale, padding) : run_embed(ids, table, scale, padding);
@@ -359,10 +364,7 @@ std::tuple<Tensor, OptTensor> layer_norm(Tensor x, OptTensor residual, OptTensor
     x = with_rows(x);
     if (residual.has_value()) residual = with_rows(*residual);
     const Tensor r = raw(residual), w = raw(weight), b = raw(bias);
-    check_no_tangent(x, "x");
-    check_no_tangent(r, "residual");
-    check_no_tangent(w, "weight");
-    check_no_tangent(b, "bias");
+    check_no_tangents({{x, "x"}, {r, "residual"}, {w, "weight"}, {b, "bias"}});
     if (wants_grad({&x, &r, &w, &b})) {
         const variable_list out = LayerNormNode::apply(x, residual, weight, bias, eps);
         return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
@@ -397,15 +399,13 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
 
 Tensor distill_loss(Tensor logits, Tensor teacher, Tensor ids, double temperature, OptTensor labels, double hard,
                     std::string reduction) {
-    check_no_tracer("distill_loss");
-    check_no_tangent(logits, "logits");
-    check_no_tangent(teacher, "teacher");
-    logits = with_rows(logits);
+    if (!wants_grad({&logits}))
+        return std::get<0>(run_distill(logits, teacher, ids, temperature, labels, hard, reduction, false, false, OptTensor()));
+    logits = with_rows(logits);  // as they are kept for the backward pass
     teacher = with_rows(teacher);
     ids = with_rows(ids);
     if (labels.has_value()) labels = labels->contiguous();
-    if (wants_grad({&logits})) return DistillNode::apply(logits, teacher, ids, labels, temperature, hard, reduction);
-    return std::get<0>(run_distill(logits, teacher, ids, temperature, labels, hard, reduction, false, false, OptTensor()));
+    return DistillNode::apply(logits, teacher, ids, labels, temperature, hard, reduction);
 }
 
 }  // namespace

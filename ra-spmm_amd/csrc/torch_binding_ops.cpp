@@ -9,6 +9,7 @@
 #include <memory>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "torch_checks.hpp"
 
@@ -69,6 +70,7 @@ struct AttentionCall {
 AttentionCall attention_call(int64_t M, int64_t K, int64_t nnz, const torch::Device& dev, const Tensor& q,
                              const Tensor& k, const Tensor& v, const Tensor& lam, c10::optional<double> scale,
                              const OptTensor& bias) {
+    check_cuda(q, "q");
     check_on(q, "q", dev);
     check_on(k, "k", dev);
     check_on(v, "v", dev);
@@ -377,6 +379,16 @@ Tensor weight_grad8(Tensor grad, Tensor codes, Tensor scales, int64_t cols, bool
 
 void bind_operators(pybind11::module_& m) {
     namespace py = pybind11;
+    m.def("through_node",
+          [](const std::vector<OptTensor>& of) {
+              bool any = torch::jit::tracer::isTracing();
+              if (!any && torch::GradMode::is_enabled())
+                  for (const OptTensor& t : of) any = any || (t.has_value() && t->requires_grad());
+              return any;
+          },
+          "Whether a call goes by its autograd node: where a gradient is recorded, and under torch.jit.trace, which records the node as a "
+          "whole and sees no launch outside of it",
+          py::arg("tensors"));
     py::class_<AttentionPlan, AttentionPlanPtr>(m, "RAAttentionPlan")
         .def_property_readonly("M", [](const AttentionPlan& w) { return w.info.M; })
         .def_property_readonly("K", [](const AttentionPlan& w) { return w.info.K; })

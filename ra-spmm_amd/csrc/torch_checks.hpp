@@ -33,9 +33,15 @@ inline int dtype_of(const Tensor& t, const char* name) {
 
 // A tensor with a tangent need not require a gradient: without this check the result would be
 // one whose tangent is missing.
-inline void check_no_tangent(const Tensor& t, const char* name) {
-    TORCH_CHECK(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
-                " carries a forward-mode tangent, this operator has reverse-mode derivatives only");
+struct Named {
+    const Tensor& t;
+    const char* name;
+};
+inline void check_no_tangents(std::initializer_list<Named> of) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Named& n : of)
+        TORCH_CHECK(!n.t.defined() || !n.t._fw_grad(0).defined(), n.name,
+                    " carries a forward-mode tangent, this operator has reverse-mode derivatives only");
 }
 
 // Tracers record torch's own operations: of a call here they would keep the outputs' allocation
@@ -46,19 +52,24 @@ inline void check_no_tracer(const char* what) {
 inline void check_no_proxies(const char* name) {
     using c10::impl::TorchDispatchModeKey;
     using c10::impl::TorchDispatchModeTLS;
+    if (!TorchDispatchModeTLS::any_modes_set()) return;
     TORCH_CHECK(!TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE),
                 name, ": this operator cannot be traced (make_fx, torch.export or fake tensors)");
 }
 
-inline void check_cuda(const Tensor& t, const char* name) {
-    check_no_tangent(t, name);
-    check_no_proxies(name);
+inline void check_values(const Tensor& t, const char* name) {
+    check_no_tangents({{t, name}});
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(!t.is_neg(), name, " is a view of the negated values (resolve_neg() gives them)");
 }
 
+// A call's first tensor, and the others.
+inline void check_cuda(const Tensor& t, const char* name) {
+    check_no_proxies(name);
+    check_values(t, name);
+}
 inline void check_on(const Tensor& t, const char* name, const torch::Device& dev) {
-    check_cuda(t, name);
+    check_values(t, name);
     TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", is on ", t.device());
 }
 

@@ -30,12 +30,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.size(0) <= 1 or t.stride(0) >= run else t.contiguous()
 
 
-def _through_node(*tensors) -> bool:
-    """Whether a call goes through its autograd node: where a gradient is recorded, and under torch.jit.trace, which records
-    the node as a whole and sees no launch outside of it."""
-    return torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
-
-
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, q, k, v, lam, scale, bias):
@@ -65,7 +59,7 @@ def diff_attention(plan, q, k, v, lam, scale=None, bias=None) -> torch.Tensor:
     if q.dim() == 4 and lam.numel() == 1:
         lam = lam.reshape(1).expand(q.size(1))
     lam = lam.contiguous()
-    if _through_node(q, k, v, lam):
+    if _C.through_node((q, k, v, lam)):
         return _DiffAttention.apply(plan, q, k, v, lam, scale, bias)
     return _C.run_attention_plan(plan, q, k, v, lam, scale, bias)
 
@@ -111,6 +105,6 @@ def head_norm_rotate(q, k, wq, wk, table=None, positions=None, eps: float = 1e-6
     of the table gives NaN.  Differentiable in q, k, wq and wk."""
     q = _rows(q)
     k = None if k is None else _rows(k)
-    if _through_node(q, k, wq, wk):
+    if _C.through_node((q, k, wq, wk)):
         return _HeadNorm.apply(q, k, wq, wk, table, positions, eps, layout)
     return _C.run_head_norm(q, k, wq, wk, table, positions, eps, layout)

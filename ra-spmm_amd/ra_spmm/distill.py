@@ -17,7 +17,6 @@ from typing import Optional, Union
 import torch
 
 from . import _C
-from .attention import _rows
 
 
 def _check_teacher(name, teacher):
@@ -44,7 +43,6 @@ def distill_loss_grad(logits: torch.Tensor, teacher: torch.Tensor, ids: torch.Te
     The gradient is that of factor * loss (factor: a number, or one float32 value on the logits' device, such as a loss
     scale; None: 1), for logits.backward(gradient); the loss is without the factor."""
     _check_teacher("distill_loss_grad", teacher)
-    logits, teacher, ids, labels = _rows(logits), _rows(teacher), _rows(ids), None if labels is None else labels.contiguous()
     if factor is not None and not isinstance(factor, torch.Tensor):
         factor = torch.full((1,), float(factor), dtype=torch.float32, device=logits.device)
     with torch.no_grad():
