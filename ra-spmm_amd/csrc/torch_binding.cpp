@@ -20,6 +20,7 @@
 #include <string>
 
 #include "../../include/ra_spmm.h"
+#include "torch_memory.hpp"
 
 void bind_operators(pybind11::module_& m);        // torch_binding_ops.cpp
 void bind_model_operators(pybind11::module_& m);  // torch_binding_model.cpp
@@ -27,6 +28,7 @@ void bind_model_operators(pybind11::module_& m);  // torch_binding_model.cpp
 namespace {
 
 ra_stream_t current_stream() {
+    check_launch();
     return reinterpret_cast<ra_stream_t>(c10::hip::getCurrentHIPStream().stream());
 }
 
@@ -36,6 +38,7 @@ void check(ra_status s, const char* what) {
 
 // bindings/ra_bindings.cpp:288-306
 void check_gpu_tensor(const torch::Tensor& t, const char* name) {
+    check_memory(t, name);
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
@@ -70,6 +73,8 @@ void check_plan_device(int plan_device, const torch::Tensor& B) {
 // each buffer is reused only after the copy that last read it (on whichever
 // device) has completed.  The source may be freed as soon as this returns.
 torch::Tensor upload(const torch::Tensor& t, torch::ScalarType dtype, const torch::Device& dev) {
+    check_memory(t, "tensor");
+    check_launch();
     if (t.is_cuda()) return t.to(dev, dtype).contiguous();
     const torch::Tensor h = t.contiguous().to(dtype);
     constexpr int64_t kStage = int64_t{16} << 20;
@@ -109,8 +114,16 @@ torch::Tensor upload(const torch::Tensor& t, torch::ScalarType dtype, const torc
     return out;
 }
 
-torch::Tensor host_i32(const torch::Tensor& t) { return t.cpu().contiguous().to(torch::kInt32); }
-torch::Tensor host_f32(const torch::Tensor& t) { return t.cpu().contiguous().to(torch::kFloat32); }
+torch::Tensor host_i32(const torch::Tensor& t) {
+    check_memory(t, "tensor");
+    check_launch();
+    return t.cpu().contiguous().to(torch::kInt32);
+}
+torch::Tensor host_f32(const torch::Tensor& t) {
+    check_memory(t, "tensor");
+    check_launch();
+    return t.cpu().contiguous().to(torch::kFloat32);
+}
 
 // ------------------------------------------------------------ CSR_DIRECT
 torch::Tensor spmm_csr_direct(torch::Tensor rowptr, torch::Tensor colind, torch::Tensor vals,
@@ -217,6 +230,7 @@ torch::Tensor run_cusparse_plan(std::shared_ptr<BaselinePlan> p, torch::Tensor B
 // ------------------------------------------------------------- features
 ra_features features_of(const torch::Tensor& rowptr, int M, int K, int N, const char** backend) {
     ra_features f{};
+    check_memory(rowptr, "rowptr");
     TORCH_CHECK(rowptr.numel() >= M + 1, "rowptr has fewer than M+1 entries");
     if (rowptr.is_cuda()) {
         TORCH_CHECK(rowptr.scalar_type() == torch::kInt32 && rowptr.is_contiguous(),

@@ -54,6 +54,8 @@ ra_embed_shape embed_shape(const Tensor& ids, int64_t rows, int64_t dim, const T
 Tensor run_embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> padding) {
     check_no_tangents({{table, "table"}});
     check_no_proxies("table");
+    check_memory(table, "table");
+    check_memory(ids, "ids");
     TORCH_CHECK(ids.is_cuda(), "ids must be a CUDA tensor");
     const auto dev = ids.device();
     check_on(table, "table", dev);
@@ -69,6 +71,7 @@ Tensor run_embed(Tensor ids, Tensor table, double scale, c10::optional<int64_t> 
 }
 
 Tensor run_embed_backward(Tensor ids, Tensor grad, int64_t rows, double scale, c10::optional<int64_t> padding) {
+    check_memory(ids, "ids");
     TORCH_CHECK(ids.is_cuda(), "ids must be a CUDA tensor");
     const auto dev = ids.device();
     check_on(grad, "grad", dev);

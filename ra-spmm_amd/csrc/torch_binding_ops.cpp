@@ -25,6 +25,8 @@ struct AttentionPlan {
 using AttentionPlanPtr = std::shared_ptr<AttentionPlan>;
 
 void check_lists(const Tensor& rowptr, const Tensor& colind) {
+    check_memory(rowptr, "rowptr");
+    check_memory(colind, "colind");
     TORCH_CHECK(rowptr.is_cuda() && colind.is_cuda(), "rowptr and colind must be CUDA tensors");
     TORCH_CHECK(rowptr.device() == colind.device(), "rowptr and colind must be on the same device");
     TORCH_CHECK(rowptr.scalar_type() == torch::kInt32 && colind.scalar_type() == torch::kInt32,
@@ -35,6 +37,9 @@ void check_lists(const Tensor& rowptr, const Tensor& colind) {
 }
 
 AttentionPlanPtr make_attention_plan(Tensor rowptr, Tensor colind, int64_t M, int64_t K, bool backward) {
+    check_memory(rowptr, "rowptr");
+    check_memory(colind, "colind");
+    check_launch();
     if (!rowptr.is_cuda() && !colind.is_cuda()) {  // a host CSR is uploaded, as the other plan builders do
         const torch::Device dev(torch::kCUDA, c10::hip::current_device());
         rowptr = rowptr.to(dev, torch::kInt32).contiguous();
@@ -297,6 +302,8 @@ int64_t check_matrix(const Tensor& x, const char* name) {
 }
 
 void check_packed(const Tensor& codes, const Tensor& scales, int64_t cols) {
+    check_memory(codes, "codes");
+    check_memory(scales, "scales");
     TORCH_CHECK(codes.is_cuda() && scales.is_cuda() && codes.device() == scales.device(),
                 "codes and scales must be CUDA tensors on the same device");
     TORCH_CHECK(codes.scalar_type() == torch::kUInt8 && codes.is_contiguous() && codes.dim() == 2 && cols > 0 &&

@@ -9,6 +9,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/ra_spmm.h"
+#include "torch_memory.hpp"
 
 namespace {
 
@@ -16,6 +17,7 @@ using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
 inline ra_stream_t current_stream() {
+    check_launch();
     return reinterpret_cast<ra_stream_t>(c10::hip::getCurrentHIPStream().stream());
 }
 
@@ -59,6 +61,7 @@ inline void check_no_proxies(const char* name) {
 
 inline void check_values(const Tensor& t, const char* name) {
     check_no_tangents({{t, name}});
+    check_memory(t, name);
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(!t.is_neg(), name, " is a view of the negated values (resolve_neg() gives them)");
 }

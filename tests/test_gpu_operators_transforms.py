@@ -102,3 +102,35 @@ def test_views_of_negated_values(name):
         assert "negated" in str(e)
     else:
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("inside", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_transformations_of_torch_func_are_refused(name, inside):
+    """Of an argument, and around a call on tensors from outside, whose outputs would have no memory."""
+    at, f = operators(*inputs())[name]
+
+    for transform in (torch.func.functionalize, torch.func.grad, torch.func.vmap):
+        def call(x):
+            with pytest.raises(RuntimeError, match=None if transform is torch.func.vmap else "functional wrapper|torch.func|functorch|storage"):
+                f(at if inside else x)
+            return (x * 2).sum()
+
+        transform(call)(at)
+
+
+def test_products_inside_of_transformations_are_refused():
+    rowptr, colind = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    vals, B = torch.ones(2, device="cuda"), torch.ones(2, 4, device="cuda")
+    plan = ra_spmm._C.make_zero_overhead_plan(rowptr, 2, 2)
+
+    def call(x):
+        for f in (lambda: ra_spmm._C.spmm_csr_direct(rowptr, colind, vals, B), lambda: ra_spmm._C.spmm_cusparse(rowptr, colind, vals, B),
+                  lambda: ra_spmm._C.run_zero_overhead_plan(plan, rowptr, colind, vals, B)):
+            with pytest.raises(RuntimeError, match="torch.func"):
+                f()
+        return (x * 2).sum()
+
+    for transform in (torch.func.functionalize, torch.func.grad, torch.func.vmap):
+        transform(call)(B)
+    assert torch.equal(ra_spmm._C.spmm_csr_direct(rowptr, colind, vals, B), B)

@@ -63,3 +63,44 @@ def test_proxies_are_refused(n, mode):
         return x + 1
 
     make_fx(f, tracing_mode=mode)(X.clone())
+
+
+@pytest.mark.parametrize("n", [0, 1, 5, 6, 8, 9, 10, 11])
+def test_functional_wrappers_are_refused(n):
+    """Their storage is empty: the address of a view is its offset, which must not reach a launch."""
+    def f(x):
+        view = torch.cat([x, x])[4:]
+        assert 0 < view.data_ptr() < 4096
+        with pytest.raises(RuntimeError, match="functional wrapper"):
+            list(calls(lambda t: view if t is X else t))[n]()
+        return x + 1
+
+    torch.func.functionalize(f)(X.clone())
+
+
+def test_functional_wrappers_of_a_matrix_are_refused():
+    rowptr, colind, vals = torch.tensor([0, 1, 2], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32), torch.ones(2)
+
+    def f(rowptr, colind, vals, B):
+        for call in (lambda: _C.spmm_csr_direct(rowptr, colind, vals, B), lambda: _C.spmm_cusparse(rowptr, colind, vals, B),
+                     lambda: _C.make_attention_plan(rowptr, colind, 2, 2), lambda: _C.compute_features(rowptr, 2, 2, 4),
+                     lambda: _C.analyze_matrix(rowptr, colind, 2, 2, 4), lambda: _C.make_zero_overhead_plan(rowptr, 2, 2, "host")):
+            with pytest.raises(RuntimeError, match="functional wrapper"):
+                call()
+        return B + 1
+
+    torch.func.functionalize(f)(rowptr, colind, vals, torch.ones(2, 4))
+
+
+@pytest.mark.parametrize("transform", [torch.func.functionalize, torch.func.grad, torch.func.vmap])
+def test_host_calls_inside_of_transformations_are_refused(transform):
+    """On tensors from outside of it: what is allocated inside has no memory."""
+    rowptr, colind = torch.tensor([0, 1, 2], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+
+    def f(x):
+        with pytest.raises(RuntimeError, match="torch.func"):
+            _C.analyze_matrix(rowptr, colind, 2, 2, 4)
+        return (x + 1).sum()
+
+    transform(f)(torch.ones(3))
+    assert _C.analyze_matrix(rowptr, colind, 2, 2, 4)
